@@ -1,8 +1,8 @@
 /*
  * inferno_hip.h -- C ABI of the MI355X (gfx950) K-quant matvec library.
  *
- * This is the whole boundary: plain pointers, sizes and status codes, no
- * HIP or torch types.  It replaces the native library behind Inferno.jl's
+ * This is the whole boundary: plain pointers, sizes, status codes and two plain
+ * structs of them, no HIP or torch types.  It replaces the native library behind Inferno.jl's
  * QuantizedKernels / FusedKernels / Dequant call surface (paths relative to
  * the Inferno.jl checkout):
  *
@@ -375,6 +375,154 @@ int ihip_gemv_q8k_dev(int ggml_type, const void *w, const void *q8, float *out, 
  * must not overlap. */
 int ihip_gemv_q8k_x_dev(int ggml_type, const void *w, const float *x, float *out, void *q8,
                         int inner, int outer, ihip_stream stream);
+
+/* ---- attention over a paged cache ---------------------------------------- */
+/* What a decoder layer does between wq/wk/wv and wo (src/ModelCPU.jl:789-885:
+ * q and k norms, rotary positions, append to the KV cache, grouped-query
+ * attention; src/FlashAttention.jl:19-84), for a batch of sequences whose
+ * cache lies in pages.  GGML type ids of values that are not quantized: */
+#define IHIP_F32 0
+#define IHIP_F16 1
+#define IHIP_BF16 30
+
+/* Bits or-ed into *flags (a device uint32 or NULL).  These calls never clear
+ * it: the caller does.  A batch whose device arrays hold values that do not
+ * fit its sizes reads and writes nothing outside the buffers; what does not
+ * fit is cut (lengths, row ranges) or left out (pages). */
+#define IHIP_FLAG_KV_PAGE 8u    /* a page id outside the pool; a list of copies that mix */
+#define IHIP_FLAG_KV_LENGTH 16u /* a length or row range that does not fit, more new tokens than tokens */
+#define IHIP_FLAG_KV_FULL 32u   /* no free page was left */
+
+/* One layer's cache: `pages` pages of page_size tokens (a power of two, 16 or
+ * more) of kv_heads heads of head_dim values (a multiple of 8, at most 256).
+ * Element (page, head, slot, i) of k and of v is at page * page_stride +
+ * (head * page_size + slot) * head_dim + i, with page_stride (elements, a
+ * multiple of 8) at least kv_heads * page_size * head_dim.  k and v: 16-byte
+ * aligned device memory. */
+typedef struct ihip_kv_cache {
+    void *k, *v;
+    int type; /* IHIP_F16 or IHIP_BF16 */
+    int pages, page_size, kv_heads, head_dim;
+    int64_t page_stride;
+} ihip_kv_cache;
+
+/* The sequences of a call, in device memory (only the sizes are read on the
+ * host, so a captured call replays with new contents).  Sequence s has the new
+ * tokens q_starts[s] .. q_starts[s+1] - 1 (rows of q; q_starts does not
+ * decrease) and kv_lens[s] tokens in all, the new ones last: row i of n is at
+ * cache position kv_lens[s] - n + i, whose page is page_table[s *
+ * table_stride + position / page_size].  Rows behind the last sequence's (a
+ * padded batch) are neither read nor written.  Sequences may share pages that
+ * hold only earlier tokens. */
+typedef struct ihip_kv_batch {
+    const int32_t *q_starts;   /* sequences + 1 */
+    const int32_t *kv_lens;    /* sequences */
+    const int32_t *page_table; /* sequences x table_stride */
+    int sequences, table_stride;
+    int tokens; /* rows of q, out and positions */
+} ihip_kv_batch;
+
+/* Turns per position (angle / 2 pi, in 64 bits) of the rot_dim / 2 rotated
+ * pairs into turns (host memory; the caller uploads it once), and the factor
+ * on the rotated values into *mscale.  With f_i = base^(-2 i / rot_dim):
+ *   IHIP_ROPE_NONE    f_i
+ *   IHIP_ROPE_LINEAR  f_i / factor
+ *   IHIP_ROPE_NTK     f_i of the base times factor^(rot_dim / (rot_dim - 2))
+ *   IHIP_ROPE_YARN    f_i / factor for pairs that make fewer than `low` turns
+ *                     in `original` positions, f_i for more than `high`, a
+ *                     ramp over the pairs between; mscale 0.1 ln(factor) + 1
+ *   IHIP_ROPE_BANDS   the same two, with a ramp over the number of turns;
+ *                     mscale 1
+ * low and high (low < high) and original are read by the last two only.  Needs
+ * no device. */
+#define IHIP_ROPE_NONE 0
+#define IHIP_ROPE_LINEAR 1
+#define IHIP_ROPE_NTK 2
+#define IHIP_ROPE_YARN 3
+#define IHIP_ROPE_BANDS 4
+int ihip_rope_turns(int scaling, int rot_dim, double base, double factor, int original, double low,
+                    double high, double *turns, float *mscale);
+
+/* Pairs of a rotated head: (i, i + rot_dim / 2) or (2 i, 2 i + 1). */
+#define IHIP_ROPE_HALF 0
+#define IHIP_ROPE_INTERLEAVED 1
+/* One launch from the projections' fp32 outputs to the attention's inputs:
+ *   q_out[t, h] = rope(norm(q[t, h])), rounded to q_type (F32, F16 or BF16);
+ *   the cache at t's position: k <- rope(norm(k[t, h])), v <- v[t, h].
+ * Row t of q is q_heads * head_dim floats at q + t * q_stride (floats), of k
+ * and v kv_heads * head_dim floats alike, so that one grouped wq/wk/wv GEMV's
+ * output is passed as three offsets into it.  norm is rmsnorm over a head
+ * (as ihip_rmsnorm_dev) with q_norm / k_norm (head_dim floats) or nothing where
+ * NULL.  turns: rot_dim / 2 doubles on the device, rot_dim even and at most
+ * head_dim (the rest of a head is not rotated).  positions: `tokens` int32 on
+ * the device, or NULL for the cache positions.  k and v NULL: q alone (a layer
+ * that reads another's cache).  q_out (tokens x q_heads x head_dim) may be q
+ * (F32, q_stride = q_heads * head_dim) but not overlap q, k or v otherwise.
+ * Everything is 16-byte aligned, strides multiples of 4.  A page that a batch
+ * appends to belongs to one sequence only. */
+int ihip_rope_kv_dev(const float *q, int64_t q_stride, const float *k, int64_t k_stride,
+                     const float *v, int64_t v_stride, int q_heads, const float *q_norm,
+                     const float *k_norm, float eps, const double *turns, int rot_dim, int layout,
+                     float mscale, const int32_t *positions, void *q_out, int q_type,
+                     const ihip_kv_cache *cache, const ihip_kv_batch *batch, uint32_t *flags,
+                     ihip_stream stream);
+
+/* out[t, h] = softmax over the keys that t sees of the scores with q[t, h],
+ * times their values: one token a sequence (decode), a few (drafted tokens) or
+ * a chunk of a prompt, in one batch.  q and out: tokens x q_heads x head_dim of
+ * q_type, which is F32 or the cache's type; q_heads a multiple of kv_heads,
+ * head h reading KV head h / (q_heads / kv_heads).  A row at position p sees
+ * the keys j <= p and, with prefix_lens (one a sequence, or NULL), every j <
+ * prefix_lens[s]; with window > 0 only those with p - j < window.  The score is
+ * scale * q.k, then softcap * tanh(score / softcap) where softcap > 0, then
+ * minus slopes[h] * |p - j| (q_heads floats, or NULL).  A row that sees no key
+ * gives 0, and what hidden keys or unfilled slots hold has no influence.
+ * F32: scores and outputs carry fp32's accuracy.  F16 / BF16: the softmax
+ * weights are rounded to that type (the sums stay fp32).
+ * workspace: ihip_attn_paged_scratch_bytes bytes, 16-byte aligned, NULL where
+ * that is 0; calls that share it must not overlap on the GPU. */
+int ihip_attn_paged_dev(const void *q, int q_type, void *out, int q_heads, float scale,
+                        float softcap, int window, const int32_t *prefix_lens, const float *slopes,
+                        const ihip_kv_cache *cache, const ihip_kv_batch *batch, uint32_t *flags,
+                        void *workspace, size_t workspace_bytes, ihip_stream stream);
+/* From the sizes alone: never more for other contents of the batch's arrays. */
+size_t ihip_attn_paged_scratch_bytes(int q_type, int q_heads, const ihip_kv_cache *cache,
+                                     const ihip_kv_batch *batch);
+
+/* The page tables of the next step.  Child c goes on from parents[c] (a row of
+ * table and lens; -1: an empty sequence) with room for `room` more tokens:
+ * lens_out[c] = the parent's length, table_out[c] (table_stride entries, -1
+ * behind the last page) its pages.  A parent's first child takes over all of
+ * its pages; a later one shares the full ones and gets a page of its own for a
+ * last one that is partly filled, to be copied: copies[2 c], copies[2 c + 1] =
+ * the page to copy and its copy, or -1, -1.  The pages of a parent without a
+ * child go back.  refs[p], the number of tables that hold page p, is kept up to
+ * date; missing pages are taken from those with refs 0 (after what went back),
+ * the lowest first, in order of child and place.  Where none is left the entry
+ * is -1 and IHIP_FLAG_KV_FULL is set.  table and table_out must not overlap;
+ * scratch: children ints.  All arrays are int32 in device memory.  Freeing,
+ * reordering, extending and forking sequences are all this call. */
+int ihip_kv_fork_dev(const int32_t *table, const int32_t *lens, int sequences,
+                     const int32_t *parents, int children, int room, int table_stride,
+                     int page_size, int pages, int32_t *refs, int32_t *table_out,
+                     int32_t *lens_out, int32_t *copies, int32_t *scratch, uint32_t *flags,
+                     ihip_stream stream);
+/* The used pages (refs > 0) moved to the indices 0 .. used - 1: those behind
+ * go, in order, to the free ones before, in order.  copies (pages / 2 pairs)
+ * receives the moves, then -1; *moved their number; refs and the tables'
+ * entries (any number of them, -1 where empty) are changed in place.  scratch:
+ * pages ints. */
+int ihip_kv_compact_dev(int32_t *table, int64_t entries, int32_t *refs, int pages, int32_t *copies,
+                        int32_t *moved, int32_t *scratch, uint32_t *flags, ihip_stream stream);
+/* Copies the pages copies[2 i] -> copies[2 i + 1], i < n (or < *count, a device
+ * int, where count is not NULL), of k and v in `layers` layers whose pools lie
+ * layer_stride elements apart (cache: the first layer's; layer_stride a
+ * multiple of 8).  Pairs with a negative entry are skipped.  No page may be
+ * written twice or both read and written (the two calls above give no such
+ * list); flags, where given, report it. */
+int ihip_kv_copy_dev(const ihip_kv_cache *cache, int layers, int64_t layer_stride,
+                     const int32_t *copies, int n, const int32_t *count, uint32_t *flags,
+                     ihip_stream stream);
 
 #ifdef __cplusplus
 }

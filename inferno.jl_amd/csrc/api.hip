@@ -10,7 +10,9 @@
 #include "kq_common.h"
 #include "kq_launch.h"
 #include "kq_sdig_plan.h"
+#include "kv_launch.h"
 
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
@@ -637,6 +639,61 @@ int host_vec_dot_q8k(int type, const void *x, const void *y, int nb, float *s)
     RET_IF(copy_out(c.y, s, sizeof(float)));
     return finish_locked();
 }
+
+// ---- the paged cache ---------------------------------------------------------
+int value_bytes(int type) { return type == kF32 ? 4 : type == kF16 || type == kBF16 ? 2 : 0; }
+
+int check_cache(const ihip_kv_cache *c, KvCache *out)
+{
+    if (!c || !c->k || !c->v)
+        return fail(IHIP_ERR_INVALID, "null cache");
+    if (c->type != kF16 && c->type != kBF16)
+        return fail(IHIP_ERR_INVALID, "cache type %d is neither F16 nor BF16", c->type);
+    if (c->head_dim <= 0 || c->head_dim % 8 || c->head_dim > kMaxHeadDim)
+        return fail(IHIP_ERR_INVALID, "head_dim=%d is not a multiple of 8 up to %d", c->head_dim, kMaxHeadDim);
+    if (c->pages <= 0 || c->kv_heads <= 0 || c->kv_heads > 4096)
+        return fail(IHIP_ERR_INVALID, "pages=%d, kv_heads=%d", c->pages, c->kv_heads);
+    if (c->page_size < kMinPage || c->page_size > 65536 || (c->page_size & (c->page_size - 1)))
+        return fail(IHIP_ERR_INVALID, "page_size=%d is not a power of two from %d to 65536", c->page_size, kMinPage);
+    const int64_t page = (int64_t)c->kv_heads * c->page_size * c->head_dim;
+    if (page > INT32_MAX)
+        return fail(IHIP_ERR_INVALID, "a page of %lld values passes 2^31", (long long)page);
+    if (c->page_stride < page || c->page_stride % 8 || c->page_stride > INT64_MAX / 4 / c->pages)
+        return fail(IHIP_ERR_INVALID, "page_stride=%lld does not hold a page of %lld values",
+                    (long long)c->page_stride, (long long)page);
+    if (!al16(c->k) || !al16(c->v))
+        return fail(IHIP_ERR_INVALID, "k and v must be 16-byte aligned");
+    *out = KvCache{c->k, c->v, c->type, c->pages, __builtin_ctz((unsigned)c->page_size), c->kv_heads, c->head_dim,
+                   c->page_stride};
+    return IHIP_OK;
+}
+
+int check_batch(const ihip_kv_batch *b, KvBatch *out)
+{
+    if (!b)
+        return fail(IHIP_ERR_INVALID, "null batch");
+    if (b->sequences < 0 || b->tokens < 0 || b->table_stride < 0)
+        return fail(IHIP_ERR_INVALID, "sequences=%d, tokens=%d, table_stride=%d", b->sequences, b->tokens,
+                    b->table_stride);
+    if (b->sequences && (!b->q_starts || !b->kv_lens || (b->table_stride && !b->page_table)))
+        return fail(IHIP_ERR_INVALID, "null pointer in the batch");
+    *out = KvBatch{b->q_starts, b->kv_lens, b->page_table, b->sequences, b->table_stride, b->tokens};
+    return IHIP_OK;
+}
+
+// Bytes that the pools of a cache reach over.
+size_t pool_bytes(const KvCache &c)
+{
+    return 2 * (size_t)((int64_t)(c.pages - 1) * c.page_stride + ((int64_t)c.heads * c.dim << c.page_shift));
+}
+
+bool in_pools(const KvCache &c, const void *p, size_t bytes)
+{
+    return overlap(p, bytes, c.k, pool_bytes(c)) || overlap(p, bytes, c.v, pool_bytes(c));
+}
+
+// A launch of `units` workgroups fits a grid.
+bool grid_fits(int64_t units) { return units <= (int64_t)INT32_MAX; }
 
 } // namespace
 
@@ -1455,6 +1512,264 @@ int ihip_lm_head_argmax_norm_dev(int ggml_type, const void *w, const float *norm
         return fail(IHIP_ERR_HIP, "rmsnorm launch failed: %s", hipGetErrorString(e));
     return lm_head_dev_locked(ggml_type, w, xn, logits, token, flags, hidden, vocab, workspace,
                               (hipStream_t)stream);
+}
+
+// ---- attention over a paged cache -------------------------------------------
+
+int ihip_rope_turns(int scaling, int rot_dim, double base, double factor, int original, double low,
+                    double high, double *turns, float *mscale)
+{
+    if (!turns || !mscale)
+        return fail(IHIP_ERR_INVALID, "null pointer");
+    if (scaling < IHIP_ROPE_NONE || scaling > IHIP_ROPE_BANDS)
+        return fail(IHIP_ERR_INVALID, "unknown scaling %d", scaling);
+    if (rot_dim <= 0 || rot_dim % 2 || rot_dim > kMaxHeadDim)
+        return fail(IHIP_ERR_INVALID, "rot_dim=%d is not an even number up to %d", rot_dim, kMaxHeadDim);
+    if (!(base > 0.0) || !(factor > 0.0) || !std::isfinite(base) || !std::isfinite(factor))
+        return fail(IHIP_ERR_INVALID, "base=%g, factor=%g", base, factor);
+    const bool ramp = scaling == IHIP_ROPE_YARN || scaling == IHIP_ROPE_BANDS;
+    if (ramp && (original <= 0 || !(low > 0.0) || !(low < high) || !std::isfinite(high)))
+        return fail(IHIP_ERR_INVALID, "original=%d, low=%g, high=%g", original, low, high);
+    if (scaling == IHIP_ROPE_YARN && !(base > 1.0))
+        return fail(IHIP_ERR_INVALID, "base=%g must pass 1", base);
+    if (scaling == IHIP_ROPE_NTK && rot_dim == 2)
+        return fail(IHIP_ERR_INVALID, "one pair has no base to scale");
+    const double pi2 = 6.283185307179586476925, n = rot_dim;
+    if (scaling == IHIP_ROPE_NTK)
+        base *= std::pow(factor, n / (n - 2.0));
+    // the pairs (as real numbers) that make `high` and `low` turns in `original` positions
+    double from = 0.0, to = 0.0;
+    if (scaling == IHIP_ROPE_YARN) {
+        from = std::fmax(std::floor(n * std::log(original / (high * pi2)) / (2.0 * std::log(base))), 0.0);
+        to = std::fmin(std::ceil(n * std::log(original / (low * pi2)) / (2.0 * std::log(base))), n - 1.0);
+    }
+    for (int i = 0; i < rot_dim / 2; ++i) {
+        double f = std::pow(base, -2.0 * i / n), keep = 1.0; // the share of f that is not scaled
+        if (scaling == IHIP_ROPE_LINEAR)
+            keep = 0.0;
+        else if (scaling == IHIP_ROPE_YARN)
+            keep = 1.0 - std::fmin(std::fmax((i - from) / std::fmax(to - from, 0.001), 0.0), 1.0);
+        else if (scaling == IHIP_ROPE_BANDS)
+            keep = std::fmin(std::fmax((original * f / pi2 - low) / (high - low), 0.0), 1.0);
+        turns[i] = (f / factor * (1.0 - keep) + f * keep) / pi2;
+    }
+    *mscale = scaling == IHIP_ROPE_YARN ? (float)(0.1 * std::log(factor) + 1.0) : 1.0f;
+    return IHIP_OK;
+}
+
+int ihip_rope_kv_dev(const float *q, int64_t q_stride, const float *k, int64_t k_stride,
+                     const float *v, int64_t v_stride, int q_heads, const float *q_norm,
+                     const float *k_norm, float eps, const double *turns, int rot_dim, int layout,
+                     float mscale, const int32_t *positions, void *q_out, int q_type,
+                     const ihip_kv_cache *cache, const ihip_kv_batch *batch, uint32_t *flags,
+                     ihip_stream stream)
+{
+    std::lock_guard<std::recursive_mutex> lk(ctx().mu);
+    if (disabled())
+        return fail(IHIP_ERR_DISABLED, "IHIP_DISABLE is set");
+    RopeArgs a{};
+    RET_IF(check_cache(cache, &a.cache));
+    RET_IF(check_batch(batch, &a.batch));
+    const int D = a.cache.dim;
+    if (!q || !q_out || (!k) != (!v) || (rot_dim && !turns))
+        return fail(IHIP_ERR_INVALID, "null pointer");
+    if (q_heads <= 0 || q_heads > 65536)
+        return fail(IHIP_ERR_INVALID, "q_heads=%d", q_heads);
+    if (!value_bytes(q_type))
+        return fail(IHIP_ERR_INVALID, "q_type=%d is none of F32, F16, BF16", q_type);
+    if (rot_dim < 0 || rot_dim % 2 || rot_dim > D)
+        return fail(IHIP_ERR_INVALID, "rot_dim=%d is not an even number up to head_dim=%d", rot_dim, D);
+    if (layout != IHIP_ROPE_HALF && layout != IHIP_ROPE_INTERLEAVED)
+        return fail(IHIP_ERR_INVALID, "unknown layout %d", layout);
+    const int64_t qw = (int64_t)q_heads * D, kw = (int64_t)a.cache.heads * D;
+    if (q_stride < qw || q_stride % 4 || (k && (k_stride < kw || k_stride % 4 || v_stride < kw || v_stride % 4)))
+        return fail(IHIP_ERR_INVALID, "a stride is no multiple of 4 that holds a token's heads");
+    if (!al16(q) || !al16(k) || !al16(v) || !al16(q_norm) || !al16(k_norm) || !al16(q_out) || ((uintptr_t)turns & 7))
+        return fail(IHIP_ERR_INVALID, "a pointer is not 16-byte aligned");
+    const int64_t T = a.batch.tokens;
+    if (T == 0 || a.batch.sequences == 0)
+        return IHIP_OK;
+    if (!grid_fits(T * (q_heads + 2 * a.cache.heads)) || q_stride > INT64_MAX / 8 / T ||
+        (k && (k_stride > INT64_MAX / 8 / T || v_stride > INT64_MAX / 8 / T)))
+        return fail(IHIP_ERR_INVALID, "%lld tokens of %d heads are too many for one call", (long long)T, q_heads);
+    const size_t ob = (size_t)(T * qw) * (size_t)value_bytes(q_type);
+    const size_t qb = 4 * (size_t)((T - 1) * q_stride + qw);
+    const size_t kb = k ? 4 * (size_t)((T - 1) * k_stride + kw) : 0, vb = k ? 4 * (size_t)((T - 1) * v_stride + kw) : 0;
+    const bool inplace = q_out == q && q_type == kF32 && q_stride == qw;
+    if ((!inplace && overlap(q, qb, q_out, ob)) || (k && (overlap(k, kb, q_out, ob) || overlap(v, vb, q_out, ob))))
+        return fail(IHIP_ERR_INVALID, "q, k or v overlaps q_out");
+    if (in_pools(a.cache, q_out, ob) || (k && (in_pools(a.cache, q, qb) || in_pools(a.cache, k, kb) || in_pools(a.cache, v, vb))))
+        return fail(IHIP_ERR_INVALID, "q, k, v or q_out overlaps the cache");
+    a.q = q, a.k = k, a.v = v;
+    a.q_step = q_stride, a.k_step = k_stride, a.v_step = v_stride;
+    a.q_heads = q_heads, a.kv_heads = k ? a.cache.heads : 0, a.dim = D;
+    a.q_norm = q_norm, a.k_norm = k_norm, a.eps = eps;
+    a.turns = turns, a.rot = rot_dim, a.interleaved = layout == IHIP_ROPE_INTERLEAVED, a.mscale = mscale;
+    a.positions = positions, a.out = q_out, a.out_type = q_type, a.flags = flags;
+    hipError_t e = launch_rope_kv(a, (hipStream_t)stream);
+    if (e != hipSuccess)
+        return fail(IHIP_ERR_HIP, "rope launch failed: %s", hipGetErrorString(e));
+    return IHIP_OK;
+}
+
+size_t ihip_attn_paged_scratch_bytes(int q_type, int q_heads, const ihip_kv_cache *cache,
+                                     const ihip_kv_batch *batch)
+{
+    KvCache c;
+    KvBatch b;
+    if (check_cache(cache, &c) != IHIP_OK || check_batch(batch, &b) != IHIP_OK || q_heads <= 0 ||
+        q_heads % c.heads || (q_type != kF32 && q_type != c.type) || b.tokens == 0 || b.sequences == 0)
+        return 0;
+    return attn_plan(q_type, c.type, q_heads, c.heads, c.dim, b.sequences, b.tokens, (int64_t)b.stride << c.page_shift).bytes;
+}
+
+int ihip_attn_paged_dev(const void *q, int q_type, void *out, int q_heads, float scale,
+                        float softcap, int window, const int32_t *prefix_lens, const float *slopes,
+                        const ihip_kv_cache *cache, const ihip_kv_batch *batch, uint32_t *flags,
+                        void *workspace, size_t workspace_bytes, ihip_stream stream)
+{
+    std::lock_guard<std::recursive_mutex> lk(ctx().mu);
+    if (disabled())
+        return fail(IHIP_ERR_DISABLED, "IHIP_DISABLE is set");
+    AttnArgs a{};
+    RET_IF(check_cache(cache, &a.cache));
+    RET_IF(check_batch(batch, &a.batch));
+    if (!q || !out)
+        return fail(IHIP_ERR_INVALID, "null pointer");
+    if (q_heads <= 0 || q_heads % a.cache.heads)
+        return fail(IHIP_ERR_INVALID, "q_heads=%d is not a multiple of kv_heads=%d", q_heads, a.cache.heads);
+    if (q_type != kF32 && q_type != a.cache.type)
+        return fail(IHIP_ERR_INVALID, "q_type=%d is neither F32 nor the cache's type %d", q_type, a.cache.type);
+    if (window < 0 || !std::isfinite(scale) || !std::isfinite(softcap) || softcap < 0.0f)
+        return fail(IHIP_ERR_INVALID, "window=%d, scale=%g, softcap=%g", window, scale, softcap);
+    if (!al16(q) || !al16(out))
+        return fail(IHIP_ERR_INVALID, "q and out must be 16-byte aligned");
+    const int64_t T = a.batch.tokens, rows = T * q_heads;
+    if (T == 0 || a.batch.sequences == 0)
+        return IHIP_OK;
+    const int64_t capacity = (int64_t)a.batch.stride << a.cache.page_shift;
+    if (!grid_fits(capacity) || !grid_fits(rows))
+        return fail(IHIP_ERR_INVALID, "%lld rows or %lld table tokens pass 2^31", (long long)rows, (long long)capacity);
+    const size_t bytes = (size_t)rows * (size_t)a.cache.dim * (size_t)value_bytes(q_type);
+    if (overlap(q, bytes, out, bytes))
+        return fail(IHIP_ERR_INVALID, "q overlaps out");
+    if (in_pools(a.cache, out, bytes))
+        return fail(IHIP_ERR_INVALID, "out overlaps the cache");
+    const AttnPlan p = attn_plan(q_type, a.cache.type, q_heads, a.cache.heads, a.cache.dim, a.batch.sequences,
+                                 a.batch.tokens, capacity);
+    if (!grid_fits((int64_t)p.tiles * a.cache.heads * p.splits))
+        return fail(IHIP_ERR_INVALID, "%lld rows are too many for one call", (long long)rows);
+    if (p.bytes) {
+        if (!workspace || workspace_bytes < p.bytes || !al16(workspace))
+            return fail(IHIP_ERR_INVALID, "the workspace needs %zu bytes, 16-byte aligned", p.bytes);
+        if (overlap(workspace, p.bytes, q, bytes) || overlap(workspace, p.bytes, out, bytes) ||
+            in_pools(a.cache, workspace, p.bytes))
+            return fail(IHIP_ERR_INVALID, "the workspace overlaps q, out or the cache");
+    }
+    a.q = q, a.out = out, a.act = q_type, a.q_heads = q_heads, a.group = q_heads / a.cache.heads;
+    a.scale = scale, a.cap = softcap, a.window = window, a.prefix = prefix_lens, a.slopes = slopes;
+    a.flags = flags, a.part = (float *)workspace;
+    hipError_t e = launch_attn(a, p, (hipStream_t)stream);
+    if (e != hipSuccess)
+        return fail(IHIP_ERR_HIP, "attention launch failed: %s", hipGetErrorString(e));
+    return IHIP_OK;
+}
+
+int ihip_kv_fork_dev(const int32_t *table, const int32_t *lens, int sequences,
+                     const int32_t *parents, int children, int room, int table_stride,
+                     int page_size, int pages, int32_t *refs, int32_t *table_out,
+                     int32_t *lens_out, int32_t *copies, int32_t *scratch, uint32_t *flags,
+                     ihip_stream stream)
+{
+    std::lock_guard<std::recursive_mutex> lk(ctx().mu);
+    if (disabled())
+        return fail(IHIP_ERR_DISABLED, "IHIP_DISABLE is set");
+    if (sequences < 0 || children < 0 || room < 0 || table_stride <= 0 || pages <= 0)
+        return fail(IHIP_ERR_INVALID, "sequences=%d, children=%d, room=%d, table_stride=%d, pages=%d", sequences,
+                    children, room, table_stride, pages);
+    if (page_size <= 0)
+        return fail(IHIP_ERR_INVALID, "page_size=%d must be positive", page_size);
+    if (sequences == 0 && children == 0)
+        return IHIP_OK;
+    if (!refs || (sequences && (!table || !lens)) || (children && (!parents || !table_out || !lens_out || !copies || !scratch)))
+        return fail(IHIP_ERR_INVALID, "null pointer");
+    if (!grid_fits((int64_t)sequences + children) || !grid_fits((int64_t)children * table_stride) ||
+        !grid_fits((int64_t)table_stride * page_size))
+        return fail(IHIP_ERR_INVALID, "%d children of %d pages are too many for one call", children, table_stride);
+    const size_t tb = 4 * (size_t)sequences * (size_t)table_stride, lb = 4 * (size_t)sequences;
+    const size_t cb = 4 * (size_t)children, ob = cb * (size_t)table_stride;
+    struct Span {
+        const void *p;
+        size_t n;
+    };
+    // what is written may be nothing else that is read or written
+    const Span ins[] = {{table, tb}, {lens, lb}, {parents, cb}};
+    const Span outs[] = {{refs, 4 * (size_t)pages}, {table_out, ob}, {lens_out, cb}, {copies, 2 * cb}, {scratch, cb}};
+    for (int i = 0; i < 5; ++i) {
+        for (const Span &r : ins)
+            if (r.n && outs[i].n && overlap(r.p, r.n, outs[i].p, outs[i].n))
+                return fail(IHIP_ERR_INVALID, "an output overlaps table, lens or parents");
+        for (int j = 0; j < i; ++j)
+            if (outs[i].n && outs[j].n && overlap(outs[i].p, outs[i].n, outs[j].p, outs[j].n))
+                return fail(IHIP_ERR_INVALID, "two outputs overlap");
+    }
+    ForkArgs a{table, lens, parents, sequences, children, table_stride, page_size, room, pages,
+               refs, table_out, lens_out, copies, scratch, flags};
+    hipError_t e = launch_kv_fork(a, (hipStream_t)stream);
+    if (e != hipSuccess)
+        return fail(IHIP_ERR_HIP, "fork launch failed: %s", hipGetErrorString(e));
+    return IHIP_OK;
+}
+
+int ihip_kv_compact_dev(int32_t *table, int64_t entries, int32_t *refs, int pages, int32_t *copies,
+                        int32_t *moved, int32_t *scratch, uint32_t *flags, ihip_stream stream)
+{
+    std::lock_guard<std::recursive_mutex> lk(ctx().mu);
+    if (disabled())
+        return fail(IHIP_ERR_DISABLED, "IHIP_DISABLE is set");
+    if (entries < 0 || pages <= 0)
+        return fail(IHIP_ERR_INVALID, "entries=%lld, pages=%d", (long long)entries, pages);
+    if (!refs || !moved || !scratch || (pages > 1 && !copies) || (entries && !table))
+        return fail(IHIP_ERR_INVALID, "null pointer");
+    if (!grid_fits((int64_t)pages + 4096) || entries > INT64_MAX / 8)
+        return fail(IHIP_ERR_INVALID, "%d pages are too many", pages);
+    const size_t pb = 4 * (size_t)pages, eb = 4 * (size_t)entries, cb = 8 * (size_t)(pages / 2);
+    if ((entries && (overlap(table, eb, refs, pb) || overlap(table, eb, scratch, pb) ||
+                     (cb && overlap(table, eb, copies, cb)))) ||
+        overlap(refs, pb, scratch, pb) || (cb && (overlap(copies, cb, refs, pb) || overlap(copies, cb, scratch, pb))) ||
+        overlap(moved, 4, refs, pb) || overlap(moved, 4, scratch, pb) || (cb && overlap(moved, 4, copies, cb)) ||
+        (entries && overlap(moved, 4, table, eb)))
+        return fail(IHIP_ERR_INVALID, "two of the arrays overlap");
+    CompactArgs a{table, entries, refs, pages, copies, moved, scratch, flags};
+    hipError_t e = launch_kv_compact(a, (hipStream_t)stream);
+    if (e != hipSuccess)
+        return fail(IHIP_ERR_HIP, "compact launch failed: %s", hipGetErrorString(e));
+    return IHIP_OK;
+}
+
+int ihip_kv_copy_dev(const ihip_kv_cache *cache, int layers, int64_t layer_stride,
+                     const int32_t *copies, int n, const int32_t *count, uint32_t *flags,
+                     ihip_stream stream)
+{
+    std::lock_guard<std::recursive_mutex> lk(ctx().mu);
+    if (disabled())
+        return fail(IHIP_ERR_DISABLED, "IHIP_DISABLE is set");
+    KvCache c;
+    RET_IF(check_cache(cache, &c));
+    if (layers <= 0 || n < 0 || layer_stride < 0 || layer_stride % 8 || layer_stride > INT64_MAX / 4 / layers)
+        return fail(IHIP_ERR_INVALID, "layers=%d, layer_stride=%lld, n=%d", layers, (long long)layer_stride, n);
+    if (layers > 1 && 2 * (size_t)layer_stride < 2 * (size_t)c.page_stride)
+        return fail(IHIP_ERR_INVALID, "layer_stride=%lld does not hold a page", (long long)layer_stride);
+    if (n == 0)
+        return IHIP_OK;
+    if (!copies)
+        return fail(IHIP_ERR_INVALID, "null pointer");
+    const int64_t page = 2 * ((int64_t)c.heads * c.dim << c.page_shift);
+    hipError_t e = launch_kv_copy(c.k, c.v, page, 2 * c.page_stride, 2 * layer_stride, layers, c.pages, copies, n, count,
+                                  flags, (hipStream_t)stream);
+    if (e != hipSuccess)
+        return fail(IHIP_ERR_HIP, "copy launch failed: %s", hipGetErrorString(e));
+    return IHIP_OK;
 }
 
 } // extern "C"

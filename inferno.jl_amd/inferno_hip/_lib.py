@@ -32,6 +32,11 @@ FLAG_NAN, FLAG_POSINF, FLAG_ALL_NEGINF = 1, 2, 4
 ARGMAX_WS_BYTES = 262144
 Q8_K_BYTES = 292
 
+F32, F16, BF16 = 0, 1, 30
+FLAG_KV_PAGE, FLAG_KV_LENGTH, FLAG_KV_FULL = 8, 16, 32
+ROPE_SCALING = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3, "bands": 4}
+ROPE_LAYOUT = {"half": 0, "interleaved": 1}
+
 
 class LibraryNotBuilt(RuntimeError):
     pass
@@ -49,6 +54,23 @@ class IHIPArgumentError(IHIPError, ValueError):
 
 
 _vp, _i, _i64, _sz, _u64 = C.c_void_p, C.c_int, C.c_int64, C.c_size_t, C.c_uint64
+
+
+
+class KVCacheStruct(C.Structure):
+    """ihip_kv_cache"""
+    _fields_ = [("k", _vp), ("v", _vp), ("type", _i), ("pages", _i), ("page_size", _i),
+                ("kv_heads", _i), ("head_dim", _i), ("page_stride", _i64)]
+
+
+class KVBatchStruct(C.Structure):
+    """ihip_kv_batch"""
+    _fields_ = [("q_starts", _vp), ("kv_lens", _vp), ("page_table", _vp), ("sequences", _i),
+                ("table_stride", _i), ("tokens", _i)]
+
+
+_f, _d = C.c_float, C.c_double
+_cache_p, _batch_p = C.POINTER(KVCacheStruct), C.POINTER(KVBatchStruct)
 
 SIGNATURES = {
     "ihip_last_error": ([], C.c_char_p),
@@ -114,6 +136,14 @@ SIGNATURES = {
     "ihip_quantize_row_q8_k_dev": ([_vp, _vp, _i64, _vp], _i),
     "ihip_gemv_q8k_dev": ([_i, _vp, _vp, _vp, _i, _i, _vp], _i),
     "ihip_gemv_q8k_x_dev": ([_i, _vp, _vp, _vp, _vp, _i, _i, _vp], _i),
+    "ihip_rope_turns": ([_i, _i, _d, _d, _i, _d, _d, C.POINTER(_d), C.POINTER(_f)], _i),
+    "ihip_rope_kv_dev": ([_vp, _i64, _vp, _i64, _vp, _i64, _i, _vp, _vp, _f, _vp, _i, _i, _f, _vp, _vp, _i,
+                          _cache_p, _batch_p, _vp, _vp], _i),
+    "ihip_attn_paged_dev": ([_vp, _i, _vp, _i, _f, _f, _i, _vp, _vp, _cache_p, _batch_p, _vp, _vp, _sz, _vp], _i),
+    "ihip_attn_paged_scratch_bytes": ([_i, _i, _cache_p, _batch_p], _sz),
+    "ihip_kv_fork_dev": ([_vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp], _i),
+    "ihip_kv_compact_dev": ([_vp, _i64, _vp, _i, _vp, _vp, _vp, _vp, _vp], _i),
+    "ihip_kv_copy_dev": ([_cache_p, _i, _i64, _vp, _i, _vp, _vp, _vp], _i),
 }
 
 _lib = None

@@ -363,3 +363,264 @@ def lm_head_argmax_norm(w: DeviceWeight, norm_w: torch.Tensor, eps: float, x: to
         None if logits is None else _ptr(logits, torch.float32, "logits"),
         ws.token.data_ptr(), ws.flags.data_ptr(), w.inner, w.outer, ws.ws.data_ptr(), _stream(stream)))
     return xn
+
+
+# ---- attention over a paged cache ---------------------------------------------
+_KV_TYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+_ACT_TYPES = {torch.float32: _lib.F32, **_KV_TYPES}
+
+
+def _invalid(msg: str):
+    return IHIPArgumentError(_lib.IHIP_ERR_INVALID, msg)
+
+
+def _opt(t, dtype, what, least=0):
+    """Pointer of an optional contiguous device tensor of at least `least` values."""
+    if t is None:
+        return None
+    p = _ptr(t, dtype, what)
+    if t.numel() < least:
+        raise _invalid(f"{what} holds {t.numel()} values, needs {least}")
+    return p
+
+
+class _on:
+    """The device of `t` made current for a call (the library launches on the
+    current device); free where it is already."""
+
+    def __init__(self, t: torch.Tensor):
+        self.guard = None if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _same_device(ref: torch.Tensor, *others):
+    for t in others:
+        if t is not None and t.device != ref.device:
+            raise _invalid(f"tensors on {ref.device} and {t.device}")
+
+
+def _held(stream, *tensors):
+    """Tensors allocated here, on the current stream, and used on `stream`."""
+    if stream is not None:
+        for t in tensors:
+            t.record_stream(stream)
+
+
+class KVCache:
+    """The paged cache of one layer (k, v: pages x kv_heads x page_size x
+    head_dim) or of several (layers in front): device tensors of fp16 or bf16
+    whose pages are contiguous; layer and page strides are the tensors' own, so
+    k and v may be two halves of one tensor."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor):
+        for t, what in ((k, "k"), (v, "v")):
+            if not t.is_cuda or t.dtype not in _KV_TYPES:
+                raise _invalid(f"{what} must be an fp16 or bf16 device tensor")
+            if t.dim() not in (4, 5):
+                raise _invalid(f"{what} must be [layers x] pages x kv_heads x page_size x head_dim")
+            if t.numel() == 0:
+                raise _invalid(f"{what} is empty")
+            _, heads, page, dim = t.shape[-4:]
+            if t.stride()[-3:] != (page * dim, dim, 1):
+                raise _invalid(f"a page of {what} must be contiguous")
+        if k.shape != v.shape or k.dtype != v.dtype or k.stride()[:-3] != v.stride()[:-3]:
+            raise _invalid("k and v differ in shape, type or strides")
+        _same_device(k, v)
+        self.k, self.v = k, v
+        self.layers = k.shape[0] if k.dim() == 5 else 1
+        self.layer_stride = k.stride(0) if k.dim() == 5 else 0
+        self.pages, self.kv_heads, self.page_size, self.head_dim = k.shape[-4:]
+        self.dtype, self.device = k.dtype, k.device
+        stride = k.stride(-4) if self.pages > 1 else self.kv_heads * self.page_size * self.head_dim
+        self.struct = _lib.KVCacheStruct(k.data_ptr(), v.data_ptr(), _KV_TYPES[k.dtype], self.pages, self.page_size,
+                                         self.kv_heads, self.head_dim, stride)
+        self.ref = C.byref(self.struct)
+
+    def layer(self, i: int) -> "KVCache":
+        """Layer i's cache, which rope_kv and attn_paged take."""
+        return KVCache(self.k[i], self.v[i]) if self.k.dim() == 5 else self
+
+
+class KVBatch:
+    """The sequences of a call (ihip_kv_batch): int32 device tensors q_starts
+    (sequences + 1), kv_lens (sequences), page_table (sequences x pages), and the
+    rows of q.  Their contents may change between calls, also under a captured
+    graph."""
+
+    def __init__(self, q_starts: torch.Tensor, kv_lens: torch.Tensor, page_table: torch.Tensor, tokens: int):
+        n = kv_lens.numel()
+        for t, what in ((q_starts, "q_starts"), (kv_lens, "kv_lens"), (page_table, "page_table")):
+            _ptr(t, torch.int32, what)
+        if q_starts.numel() != n + 1 or page_table.dim() != 2 or page_table.shape[0] != n:
+            raise _invalid("q_starts has sequences + 1 entries, page_table a row a sequence")
+        _same_device(q_starts, kv_lens, page_table)
+        self.q_starts, self.kv_lens, self.page_table, self.tokens = q_starts, kv_lens, page_table, tokens
+        self.device = kv_lens.device
+        self.struct = _lib.KVBatchStruct(q_starts.data_ptr(), kv_lens.data_ptr(), page_table.data_ptr(), n,
+                                         page_table.shape[1], tokens)
+        self.ref = C.byref(self.struct)
+
+
+def rope_turns(rot_dim: int, base: float, scaling: str = "none", factor: float = 1.0, original: int = 0,
+               low: float = 1.0, high: float = 32.0, device="cuda"):
+    """(turns, mscale) of ihip_rope_turns: rot_dim / 2 doubles on the device, laid
+    out once per model, and the factor on the rotated values."""
+    if scaling not in _lib.ROPE_SCALING:
+        raise _invalid(f"unknown scaling {scaling}")
+    host = (C.c_double * max(1, rot_dim // 2))()
+    m = C.c_float(1.0)
+    check(lib().ihip_rope_turns(_lib.ROPE_SCALING[scaling], rot_dim, base, factor, original, low, high, host,
+                                C.byref(m)))
+    return torch.tensor(list(host), dtype=torch.float64).to(device), m.value
+
+
+def _heads(t: torch.Tensor, what, tokens, heads, dim):
+    """Row stride of a tokens x heads x dim view whose rows are contiguous."""
+    if not t.is_cuda or t.dtype != torch.float32:
+        raise _invalid(f"{what} must be a float32 device tensor")
+    if t.dim() != 3 or t.shape[0] != tokens or t.shape[2] != dim or (heads is not None and t.shape[1] != heads):
+        raise _invalid(f"{what} is {tuple(t.shape)}, not {tokens} x {heads} x {dim}")
+    if t.shape[1] == 0:
+        raise _invalid(f"{what} has no heads")
+    if tokens and (t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != dim)):
+        raise _invalid(f"the heads of a token of {what} must be contiguous")
+    return t.stride(0) if tokens > 1 else t.shape[1] * dim
+
+
+def rope_kv(q: torch.Tensor, k, v, turns: torch.Tensor, cache: KVCache, batch: KVBatch, layout: str = "half",
+            mscale: float = 1.0, q_norm=None, k_norm=None, eps: float = 1e-6, positions=None,
+            out: torch.Tensor = None, out_dtype=None, flags=None, stream=None) -> torch.Tensor:
+    """The q and k norms, the rotary positions and the append to the cache
+    (ihip_rope_kv_dev).  q, k, v: tokens x heads x head_dim fp32, slices of a
+    grouped projection's rows as they are; k and v None for q alone.  The rotated
+    part of a head is 2 * turns.numel() values.  Returns q (out_dtype, default
+    fp32)."""
+    T, D = batch.tokens, cache.head_dim
+    if cache.k.dim() != 4:
+        raise _invalid("pass one layer of the cache (cache.layer(i))")
+    if layout not in _lib.ROPE_LAYOUT:
+        raise _invalid(f"unknown layout {layout}")
+    if (k is None) != (v is None):
+        raise _invalid("k and v go together")
+    qs = _heads(q, "q", T, None, D)
+    ks = _heads(k, "k", T, cache.kv_heads, D) if k is not None else 0
+    vs = _heads(v, "v", T, cache.kv_heads, D) if v is not None else 0
+    _same_device(q, k, v, turns, cache, batch, q_norm, k_norm, positions, out, flags)
+    with _on(q):
+        if out is None:
+            out = torch.empty(q.shape, dtype=out_dtype or torch.float32, device=q.device)
+            _held(stream, out)
+        if out.dtype not in _ACT_TYPES or out.shape != q.shape or (out_dtype is not None and out.dtype != out_dtype):
+            raise _invalid("out must have q's shape and be fp32, fp16 or bf16")
+        check(lib().ihip_rope_kv_dev(
+            q.data_ptr(), qs, None if k is None else k.data_ptr(), ks, None if v is None else v.data_ptr(), vs,
+            q.shape[1], _opt(q_norm, torch.float32, "q_norm", D), _opt(k_norm, torch.float32, "k_norm", D), eps,
+            _ptr(turns, torch.float64, "turns"), 2 * turns.numel(), _lib.ROPE_LAYOUT[layout], mscale,
+            _opt(positions, torch.int32, "positions", T), _ptr(out, None, "out"), _ACT_TYPES[out.dtype], cache.ref,
+            batch.ref, _opt(flags, torch.int32, "flags", 1), _stream(stream)))
+    return out
+
+
+def attn_workspace(q_heads: int, cache: KVCache, batch: KVBatch, dtype=torch.float32):
+    """The workspace of attn_paged for a batch of these sizes (for q of `dtype`),
+    or None where it needs none.  Calls that share one must not overlap."""
+    n = lib().ihip_attn_paged_scratch_bytes(_ACT_TYPES[dtype], q_heads, cache.ref, batch.ref)
+    return torch.empty(n, dtype=torch.uint8, device=cache.device) if n else None
+
+
+def attn_paged(q: torch.Tensor, cache: KVCache, batch: KVBatch, scale: float = None, softcap: float = 0.0,
+               window: int = 0, prefix_lens=None, slopes=None, out: torch.Tensor = None, workspace=None, flags=None,
+               stream=None) -> torch.Tensor:
+    """Attention of the batch's new tokens over their pages (ihip_attn_paged_dev).
+    q: tokens x q_heads x head_dim, fp32 or the cache's type, which out has too;
+    scale defaults to head_dim ** -0.5.  Rows of out behind the last sequence's
+    are not written."""
+    D = cache.head_dim
+    if cache.k.dim() != 4:
+        raise _invalid("pass one layer of the cache (cache.layer(i))")
+    if q.dim() != 3 or q.shape[0] != batch.tokens or q.shape[2] != D:
+        raise _invalid(f"q is {tuple(q.shape)}, not {batch.tokens} x heads x {D}")
+    if q.dtype not in _ACT_TYPES:
+        raise _invalid(f"q must be fp32, fp16 or bf16, got {q.dtype}")
+    H = q.shape[1]
+    _same_device(q, cache, batch, prefix_lens, slopes, out, workspace, flags)
+    with _on(q):
+        if out is None:
+            out = torch.empty_like(q)
+            _held(stream, out)
+        elif out.dtype != q.dtype or out.shape != q.shape:
+            raise _invalid("out must have q's shape and type")
+        if workspace is None:
+            workspace = attn_workspace(H, cache, batch, q.dtype)
+            if workspace is not None:
+                _held(stream, workspace)
+        check(lib().ihip_attn_paged_dev(
+            _ptr(q, None, "q"), _ACT_TYPES[q.dtype], _ptr(out, None, "out"), H, D ** -0.5 if scale is None else scale,
+            softcap, window, _opt(prefix_lens, torch.int32, "prefix_lens", batch.kv_lens.numel()),
+            _opt(slopes, torch.float32, "slopes", H), cache.ref, batch.ref, _opt(flags, torch.int32, "flags", 1),
+            None if workspace is None else _ptr(workspace, torch.uint8, "workspace"),
+            0 if workspace is None else workspace.numel(), _stream(stream)))
+    return out
+
+
+def kv_fork(table: torch.Tensor, lens: torch.Tensor, parents: torch.Tensor, refs: torch.Tensor, page_size: int,
+            room: int = 0, flags=None, stream=None):
+    """The page tables of the next step (ihip_kv_fork_dev): child c goes on from
+    parents[c] (-1: empty) with room for `room` more tokens.  Returns the new
+    table and lengths and the page copies that kv_copy has to make; refs is
+    updated in place."""
+    for t, what in ((table, "table"), (lens, "lens"), (parents, "parents"), (refs, "refs")):
+        _ptr(t, torch.int32, what)
+    if table.dim() != 2 or lens.numel() != table.shape[0]:
+        raise _invalid("table has a row and lens an entry a sequence")
+    _same_device(table, lens, parents, refs, flags)
+    n, width = parents.numel(), table.shape[1]
+    with _on(table):
+        new = torch.empty(n, width, dtype=torch.int32, device=table.device)
+        new_lens = torch.empty(n, dtype=torch.int32, device=table.device)
+        copies = torch.empty(n, 2, dtype=torch.int32, device=table.device)
+        scratch = torch.empty(n, dtype=torch.int32, device=table.device)
+        _held(stream, new, new_lens, copies, scratch)
+        check(lib().ihip_kv_fork_dev(table.data_ptr(), lens.data_ptr(), table.shape[0], parents.data_ptr(), n, room,
+                                     width, page_size, refs.numel(), refs.data_ptr(), new.data_ptr(),
+                                     new_lens.data_ptr(), copies.data_ptr(), scratch.data_ptr(),
+                                     _opt(flags, torch.int32, "flags", 1), _stream(stream)))
+    return new, new_lens, copies
+
+
+def kv_compact(table: torch.Tensor, refs: torch.Tensor, flags=None, stream=None):
+    """The used pages moved to the front of the pool (ihip_kv_compact_dev): table
+    and refs change in place; returns the moves (pages // 2 pairs, -1 behind the
+    last) and their number, both for kv_copy."""
+    _ptr(table, torch.int32, "table"), _ptr(refs, torch.int32, "refs")
+    _same_device(table, refs, flags)
+    pages = refs.numel()
+    with _on(table):
+        copies = torch.empty(pages // 2, 2, dtype=torch.int32, device=table.device)
+        moved = torch.empty(1, dtype=torch.int32, device=table.device)
+        scratch = torch.empty(pages, dtype=torch.int32, device=table.device)
+        _held(stream, copies, moved, scratch)
+        check(lib().ihip_kv_compact_dev(table.data_ptr(), table.numel(), refs.data_ptr(), pages, copies.data_ptr(),
+                                        moved.data_ptr(), scratch.data_ptr(), _opt(flags, torch.int32, "flags", 1),
+                                        _stream(stream)))
+    return copies, moved
+
+
+def kv_copy(cache: KVCache, copies: torch.Tensor, count: torch.Tensor = None, flags=None, stream=None):
+    """Copies pages copies[i, 0] -> copies[i, 1] in every layer of the cache
+    (ihip_kv_copy_dev); pairs with a negative entry are skipped, and those from
+    *count on."""
+    if copies.dim() != 2 or copies.shape[1] != 2:
+        raise _invalid("copies is pairs x 2")
+    _same_device(cache.k, copies, count, flags)
+    with _on(copies):
+        check(lib().ihip_kv_copy_dev(cache.ref, cache.layers, cache.layer_stride, _ptr(copies, torch.int32, "copies"),
+                                     copies.shape[0], _opt(count, torch.int32, "count", 1),
+                                     _opt(flags, torch.int32, "flags", 1), _stream(stream)))
