@@ -37,6 +37,7 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef __bf16 b2 __attribute__((ext_vector_type(2)));
 typedef __bf16 b4 __attribute__((ext_vector_type(4)));
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef float f16v __attribute__((ext_vector_type(16)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
@@ -54,6 +55,10 @@ struct Half {
     {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
     }
+    static __device__ __forceinline__ f16v mfma32(V8 a, V8 b, f16v c)
+    {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    }
 };
 struct BHalf {
     typedef __bf16 T;
@@ -66,12 +71,28 @@ struct BHalf {
     {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
     }
+    static __device__ __forceinline__ f16v mfma32(V8 a, V8 b, f16v c)
+    {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    }
 };
 
 template <typename V4>
 __device__ __forceinline__ V4 read_tr(const uint8_t *lds)
 {
     return __builtin_bit_cast(V4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)lds));
+}
+
+// The same by LDS byte address, and a plain read.
+template <typename V>
+__device__ __forceinline__ V read_lds(uint32_t at)
+{
+    return *(const __attribute__((address_space(3))) V *)at;
+}
+template <typename V4>
+__device__ __forceinline__ V4 read_tr_at(uint32_t at)
+{
+    return __builtin_bit_cast(V4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)at));
 }
 
 // Whether any of the 16-bit values in a dword is an infinity or a NaN.
@@ -111,6 +132,17 @@ __device__ __forceinline__ float groups_sum(float v)
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+__device__ __forceinline__ float halves_max(float v)
+{
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+__device__ __forceinline__ float halves_sum(float v)
+{
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+
 // What a workgroup works on: a tile of rows of one sequence and KV head, and
 // the part of its keys.
 struct Tile {
@@ -118,7 +150,7 @@ struct Tile {
     int start, row0, rows;   // the sequence's first token; the tile's first row in it; its rows
     int first, last;         // cache positions of the tile's first and last token
     int len, prefix;         // keys there are; keys every row sees
-    int lo, hi;              // keys to look at (lo a multiple of 32); lo >= hi: none
+    int lo, hi;              // keys to look at (lo a multiple of the step); lo >= hi: none
     int split;
     const int32_t *table;
 };
@@ -126,24 +158,22 @@ struct Tile {
 // Workgroup `bid`'s tile; false if there is none.  Tiles are counted over the
 // sequences in order; their number is only known here, the grid holds the most
 // there can be.
-template <int ROWS>
+template <int ROWS, int KEYS>
 __device__ __forceinline__ bool find_tile(const AttnArgs &a, int tiles, int least, int splits, int bid, Tile &t)
 {
     if (bid == 0 && a.flags)
         kv_report(a.batch, a.cache.page_shift, a.flags);
     t.head = bid % a.cache.heads;
     const int rest = bid / a.cache.heads;
-    const int want = rest % tiles;
+    // (a prompt's last rows have the most keys: they go first)
+    const int want = tiles - 1 - rest % tiles;
     t.split = rest / tiles;
     int first = 0;
-    const int s = kv_find(a.batch.sequences, want, first, [&](int i) {
-        const int b = kv_clamp(a.batch.starts[i], 0, a.batch.tokens);
-        const int n = kv_clamp(a.batch.starts[i + 1], b, a.batch.tokens) - b;
-        return (int)(((int64_t)n * a.group + ROWS - 1) / ROWS);
-    });
+    KvSeq q;
+    const int s = kv_find(a.batch, a.cache.page_shift, want, first, q,
+                          [&](int n) { return (int)(((int64_t)n * a.group + ROWS - 1) / ROWS); });
     if (s < 0)
         return false;
-    const KvSeq q = kv_seq(a.batch, a.cache.page_shift, s);
     t.start = q.start;
     t.row0 = (want - first) * ROWS;
     t.rows = min(ROWS, (int)((int64_t)q.n * a.group - t.row0));
@@ -152,7 +182,7 @@ __device__ __forceinline__ bool find_tile(const AttnArgs &a, int tiles, int leas
     t.last = q.len - q.n + (t.row0 + t.rows - 1) / a.group;
     t.prefix = a.prefix ? kv_clamp(a.prefix[s], 0, q.len) : 0;
     t.table = a.batch.table + (int64_t)s * a.batch.stride;
-    const int lo = a.window ? max(0, t.first - a.window + 1) & ~31 : 0;
+    const int lo = a.window ? max(0, t.first - a.window + 1) & ~(KEYS - 1) : 0;
     const int hi = max(t.last + 1, t.prefix);
     // the split's part of the keys: a fixed number, or more where the most
     // splits there may be would not reach the end
@@ -164,14 +194,41 @@ __device__ __forceinline__ bool find_tile(const AttnArgs &a, int tiles, int leas
     return true;
 }
 
-// Whether key j is seen from position p.
-__device__ __forceinline__ bool seen(const AttnArgs &a, const Tile &t, int p, int j)
+// The keys that position p sees: `from` .. `from` + count - 1.
+struct Seen {
+    int from;
+    uint32_t count;
+    __device__ __forceinline__ bool operator()(int j) const { return (uint32_t)(j - from) < count; }
+};
+__device__ __forceinline__ Seen seen_from(const AttnArgs &a, const Tile &t, int p)
 {
-    return (j <= p || j < t.prefix) && j < t.len && (a.window == 0 || p - j < a.window);
+    const int last = min(max(p, t.prefix - 1), t.len - 1);
+    const int from = a.window ? max(p - a.window + 1, 0) : 0;
+    return Seen{from, last >= from ? (uint32_t)(last - from) + 1u : 0u};
 }
 
-// q's part of a lane: KS chunks of 8 values (chunk 4 i + g of the row), in
-// PARTS parts.  Two fp16 parts are taken of q times a power of two that brings
+// Scores as powers of two, from q.k: `by` and the cap or the distance bias.
+// tanh x: the Taylor series to x^15 below 1/2 (the next term is under 2^-26 of
+// x), (e^2x - 1) / (e^2x + 1) from there.
+__device__ __forceinline__ float tanh_own(float x)
+{
+    const float y = x * x;
+    float p = -929569.0f / 638512875.0f;
+    p = fmaf(p, y, 21844.0f / 6081075.0f);
+    p = fmaf(p, y, -1382.0f / 155925.0f);
+    p = fmaf(p, y, 62.0f / 2835.0f);
+    p = fmaf(p, y, -17.0f / 315.0f);
+    p = fmaf(p, y, 2.0f / 15.0f);
+    p = fmaf(p, y, -1.0f / 3.0f);
+    const float small = fmaf(p * y, x, x);
+    const float e = exp2_fast(fminf(2.0f * kLog2e * fabsf(x), 64.0f));
+    const float large = copysignf((e - 1.0f) * __builtin_amdgcn_rcpf(e + 1.0f), x);
+    return y < 0.25f ? small : x == x ? large : x;
+}
+
+// q's part of a lane: KS chunks of 8 values (chunk step i + offset of the row),
+// in PARTS parts, with the sign of the scale (which then is positive, so that
+// the largest product gives the largest score; 0 makes q 0).  Two fp16 parts are taken of q times a power of two that brings
 // the row's largest value to [2^14, 2^15), undone (`undo`) on the scores.
 template <typename C, int PARTS, int KS>
 __device__ __forceinline__ void load_q(const AttnArgs &a, int64_t row, bool live, int step, int offset,
@@ -179,12 +236,17 @@ __device__ __forceinline__ void load_q(const AttnArgs &a, int64_t row, bool live
 {
     typedef typename C::V8 V8;
     undo = 1.0f;
+    const float sign = a.scale > 0.0f ? 1.0f : a.scale < 0.0f ? -1.0f : 0.0f;
     if constexpr (PARTS == 1) {
         const typename C::T *q = (const typename C::T *)a.q + row * a.cache.dim;
 #pragma unroll
         for (int i = 0; i < KS; ++i) {
             const int c = (step * i + offset) * 8;
             qf[0][i] = live && c < a.cache.dim ? *(const V8 *)(q + c) : V8{};
+            if (sign != 1.0f)
+#pragma unroll
+                for (int u = 0; u < 8; ++u)
+                    qf[0][i][u] = (typename C::T)((float)qf[0][i][u] * sign);
         }
     } else {
         const float *q = (const float *)a.q + row * a.cache.dim;
@@ -202,7 +264,7 @@ __device__ __forceinline__ void load_q(const AttnArgs &a, int64_t row, bool live
         }
         int up = 0;
         if constexpr (C::kShift != 0.0f) {
-            most = step == 4 ? groups_max(most) : fmaxf(most, __shfl_xor(most, 32));
+            most = step == 4 ? groups_max(most) : halves_max(most);
             const bool finite = most > 0.0f && most < __builtin_inff();
             up = finite ? 15 - __builtin_amdgcn_frexp_expf(most) : 0;
             undo = __builtin_ldexpf(1.0f, -up);
@@ -211,7 +273,7 @@ __device__ __forceinline__ void load_q(const AttnArgs &a, int64_t row, bool live
         for (int i = 0; i < KS; ++i)
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
-                float x = __builtin_ldexpf(v[2 * i + u / 4][u % 4], up);
+                float x = __builtin_ldexpf(v[2 * i + u / 4][u % 4] * sign, up);
 #pragma unroll
                 for (int part = 0; part < PARTS; ++part) {
                     const typename C::T y = (typename C::T)x;
@@ -226,6 +288,7 @@ __device__ __forceinline__ void load_q(const AttnArgs &a, int64_t row, bool live
 constexpr int AR_ROWS = 16;   // rows of a tile
 constexpr int AR_KEYS = 32;   // keys of a wave's step
 constexpr int AR_WAVES = 4;
+constexpr int AR_SPLITS = 128; // parts of a tile's keys at most
 
 // V's 16-byte chunk c of key row r lies at chunk c ^ swizzle(r): the four rows
 // (and both of their chunks) that a transposing read takes from then lie in
@@ -239,20 +302,22 @@ __device__ __forceinline__ int v_chunk(int r, int c)
 template <int DP>
 constexpr int ar_wave_lds()
 {
-    return AR_ROWS * (DP + 4) * 4 > AR_KEYS * DP * 2 ? AR_ROWS * (DP + 4) * 4 : AR_KEYS * DP * 2;
+    return AR_ROWS * (DP + 4) * 4 > 2 * AR_KEYS * DP * 2 ? AR_ROWS * (DP + 4) * 4 : 2 * AR_KEYS * DP * 2;
 }
 
 // A workgroup's 4 waves walk the keys of its part 32 at a time, each its own
-// steps (no shared data, no barrier), K from HBM into the matrix operand's
-// registers, V through 32 rows of LDS of the wave's own; the waves' sums are
-// joined at the end.  Loads run one step ahead.
+// steps (no shared data, no barrier): K from HBM into the matrix operand's
+// registers, V by direct copies into LDS of the wave's own, both one step
+// ahead and their page ids two; the waves' sums are joined at the end.
 template <typename C, int PARTS, int DP, bool GEN>
-__global__ void __launch_bounds__(64 * AR_WAVES) k_attn_rows(AttnArgs a, int tiles, int least, int splits)
+__global__ void __launch_bounds__(64 * AR_WAVES, DP == 256 ? 1 : 2)
+k_attn_rows(AttnArgs a, int tiles, int least, int splits)
 {
     typedef typename C::T T;
     typedef typename C::V8 V8;
     typedef typename C::V4 V4;
-    constexpr int KS = DP / 32, DT = DP / 16, NC = DP / 8, NV = AR_KEYS * NC / 64;
+    constexpr int KS = DP / 32, DT = DP / 16, NC = DP / 8, NI = DP / 32; // NI: copies of 1 KB for 16 keys
+    constexpr int TILE = AR_KEYS * DP * 2;
     __shared__ __attribute__((aligned(16))) uint8_t lds[AR_WAVES * ar_wave_lds<DP>()];
     __shared__ float lds_m[AR_WAVES][AR_ROWS], lds_l[AR_WAVES][AR_ROWS];
     const int tid = threadIdx.x, lane = tid & 63;
@@ -260,8 +325,64 @@ __global__ void __launch_bounds__(64 * AR_WAVES) k_attn_rows(AttnArgs a, int til
     const int col = lane & 15, g = lane >> 4;
     const int D = a.cache.dim;
     Tile t;
-    if (!find_tile<AR_ROWS>(a, tiles, least, splits, blockIdx.x, t))
+    if (!find_tile<AR_ROWS, AR_KEYS>(a, tiles, least, splits, blockIdx.x, t))
         return;
+
+    uint8_t *const mine = lds + wave * ar_wave_lds<DP>();
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)mine;
+    const int page_mask = (1 << a.cache.page_shift) - 1;
+    const int n_steps = (t.hi - t.lo + AR_KEYS - 1) / AR_KEYS;
+
+    // a lane's byte offsets in a run of 16 keys (chunks behind a head's end hold
+    // its last one: q is 0 there, and nothing reads those columns of the output)
+    uint32_t koff[KS], voff[NI];
+#pragma unroll
+    for (int i = 0; i < KS; ++i)
+        koff[i] = 2u * (uint32_t)(col * D + 8 * min(4 * i + g, D / 8 - 1));
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+        const int r = (64 * i + lane) / NC, c = (64 * i + lane) % NC;
+        voff[i] = 2u * (uint32_t)(r * D + 8 * min(v_chunk<NC>(r, c), D / 8 - 1));
+    }
+
+    V8 kf[2][KS];
+    int ids = -1;  // page ids of the next step's runs, in lanes 0 and 1
+    int ok = 0;    // bit u: run u's page is there
+    int64_t at[2]; // bytes from the pools' starts to the runs
+    auto page_of = [&](int step) {
+        const int j = t.lo + AR_KEYS * step + 16 * (lane & 1);
+        return step < n_steps && j < t.hi ? t.table[j >> a.cache.page_shift] : -1;
+    };
+    auto place = [&](int step) { // the runs of `step`, whose ids are here
+        ok = 0;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int j = t.lo + AR_KEYS * step + 16 * u;
+            const int id = __builtin_amdgcn_readlane(ids, u);
+            const bool in = (unsigned)id < (unsigned)a.cache.pages;
+            ok |= in << u;
+            at[u] = 2 * ((in ? (int64_t)id * a.cache.page_stride : 0) +
+                         (int64_t)((t.head << a.cache.page_shift) + (j & page_mask)) * D);
+            if (!in && j < t.hi && a.flags && lane == 0)
+                atomicOr(a.flags, kFlagKvPage);
+        }
+    };
+    auto copy_v = [&](int step) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+            if ((ok >> u) & 1)
+#pragma unroll
+                for (int i = 0; i < NI; ++i)
+                    lds_copy16_at((const uint8_t *)a.cache.v + at[u], voff[i],
+                                  lds0 + TILE * ((step / AR_WAVES) & 1) + 1024 * (NI * u + i));
+    };
+    auto load_k = [&]() { // (a run that is not there reads page 0, whose scores are masked)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int i = 0; i < KS; ++i)
+                kf[u][i] = *(const V8 *)((const uint8_t *)a.cache.k + at[u] + koff[i]);
+    };
 
     const int row = t.row0 + col; // the row of this lane's column
     const bool live = col < t.rows;
@@ -270,9 +391,22 @@ __global__ void __launch_bounds__(64 * AR_WAVES) k_attn_rows(AttnArgs a, int til
     const int pos = live ? t.first - t.row0 / a.group + row / a.group : t.first;
     V8 qf[PARTS][KS];
     float undo;
+    int step = wave;
+    if (step < n_steps)
+        ids = page_of(step);
     load_q<C, PARTS, KS>(a, qrow, live, 4, g, qf, undo);
-    const float slope = GEN && a.slopes ? a.slopes[qhead] * kLog2e : 0.0f;
-    const float by = GEN && a.cap > 0.0f ? a.scale * undo / a.cap : a.scale * undo * kLog2e;
+    if (step < n_steps) {
+        place(step);
+        ids = page_of(step + AR_WAVES);
+        load_k();
+        copy_v(step);
+    }
+    const float scale = (a.scale == 0.0f ? 1.0f : fabsf(a.scale)) * undo;
+    // scores become powers of two with the last factor, `by`; a cap takes the scale
+    // before, and the bias is added in units of `by`
+    const float by = GEN && a.cap > 0.0f ? a.cap * kLog2e : scale * kLog2e;
+    const float slope = GEN && a.slopes ? a.slopes[qhead] * kLog2e / by : 0.0f;
+    const Seen sees = seen_from(a, t, pos);
 
     float m = kNone, l = 0.0f;
     f4 o[DT];
@@ -280,61 +414,20 @@ __global__ void __launch_bounds__(64 * AR_WAVES) k_attn_rows(AttnArgs a, int til
     for (int d = 0; d < DT; ++d)
         o[d] = f4{};
 
-    uint8_t *const vt = lds + wave * ar_wave_lds<DP>();
-    V8 kf[2][KS];
-    u4 vf[NV];
-    int id[2];
-    bool ok[2];
-    const int page_mask = (1 << a.cache.page_shift) - 1;
-    const int n_steps = (t.hi - t.lo + AR_KEYS - 1) / AR_KEYS;
-
-    auto pages = [&](int key) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int j = key + 16 * u;
-            id[u] = j < t.hi ? __builtin_amdgcn_readfirstlane(t.table[j >> a.cache.page_shift]) : -1;
-            ok[u] = (unsigned)id[u] < (unsigned)a.cache.pages;
-            if (j < t.hi && !ok[u] && a.flags && lane == 0)
-                atomicOr(a.flags, kFlagKvPage);
-        }
-    };
-    auto base = [&](int key, int u) {
-        return (int64_t)id[u] * a.cache.page_stride +
-               ((int64_t)((t.head << a.cache.page_shift) + ((key + 16 * u) & page_mask))) * D;
-    };
-    auto load_k = [&](int key) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const T *k = (const T *)a.cache.k + (ok[u] ? base(key, u) : 0) + col * D;
-#pragma unroll
-            for (int i = 0; i < KS; ++i) {
-                const int c = (4 * i + g) * 8;
-                kf[u][i] = ok[u] && c < D ? *(const V8 *)(k + c) : V8{};
-            }
-        }
-    };
-    auto load_v = [&](int key) {
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int u = i / (NV / 2);
-            const int e = i * 64 + lane, r = e / NC - 16 * u, c = e % NC;
-            const T *v = (const T *)a.cache.v + (ok[u] ? base(key, u) : 0) + r * D + c * 8;
-            vf[i] = ok[u] && c * 8 < D ? *(const u4 *)v : u4{};
-        }
-    };
-
-    int step = wave;
-    if (step < n_steps) {
-        pages(t.lo + AR_KEYS * step);
-        load_k(t.lo + AR_KEYS * step);
-        load_v(t.lo + AR_KEYS * step);
-    }
     for (; step < n_steps; step += AR_WAVES) {
         const int key = t.lo + AR_KEYS * step;
-        const bool whole = ok[0] && ok[1] && key + AR_KEYS <= t.hi &&
+        const int here = ok;
+        const bool whole = here == 3 && key + AR_KEYS <= t.len &&
                            (key + AR_KEYS - 1 <= t.first || key + AR_KEYS <= t.prefix) &&
                            (a.window == 0 || t.last - key < a.window);
-        const bool ok0 = ok[0], ok1 = ok[1];
+        uint8_t *const vt = mine + TILE * ((step / AR_WAVES) & 1);
+        __builtin_amdgcn_s_waitcnt(0x0070); // vmcnt(0) lgkmcnt(0): V's copies, and the other half's reads
+        asm volatile("" ::: "memory");
+        const bool more = step + AR_WAVES < n_steps;
+        if (more) {
+            place(step + AR_WAVES);
+            copy_v(step + AR_WAVES);
+        }
         f4 s[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -345,32 +438,43 @@ __global__ void __launch_bounds__(64 * AR_WAVES) k_attn_rows(AttnArgs a, int til
                 for (int part = 0; part < PARTS; ++part)
                     s[u] = C::mfma16(kf[u][i], qf[part][i], s[u]);
         }
-        const bool more = step + AR_WAVES < n_steps;
         if (more) {
-            pages(key + AR_KEYS * AR_WAVES);
-            load_k(key + AR_KEYS * AR_WAVES);
+            ids = page_of(step + 2 * AR_WAVES);
+            load_k();
+        }
+        if (GEN) {
+            const float apart = (float)(pos - key - 4 * g);
+            if (a.cap > 0.0f)
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        s[u][i] = tanh_own(s[u][i] * (scale / a.cap));
+            if (a.slopes)
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        s[u][i] = fmaf(-slope, fabsf(apart - (float)(16 * u + i)), s[u][i]);
+        }
+        if (!whole) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    s[u][i] = ((here >> u) & 1) && sees(key + 16 * u + 4 * g + i) ? s[u][i] : kNone;
         }
         float mx = kNone;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float x = s[u][i] * by;
-                if (GEN && a.cap > 0.0f)
-                    x = a.cap * kLog2e * tanhf(x);
-                const int j = key + 16 * u + 4 * g + i;
-                if (GEN)
-                    x -= slope * fabsf((float)(pos - j));
-                if (!whole && !(seen(a, t, pos, j) && (u ? ok1 : ok0)))
-                    x = kNone;
-                s[u][i] = x;
-                mx = fmaxf(mx, x);
-            }
-        mx = fmaxf(groups_max(mx), m);
+            for (int i = 0; i < 4; ++i)
+                mx = fmaxf(mx, s[u][i]);
+        mx = fmaxf(groups_max(mx) * by, m);
         // (a row without a key yet keeps its sum 0 whatever is subtracted)
-        const float use = mx == kNone ? 0.0f : mx;
+        const float use = (mx == kNone ? 0.0f : mx) - C::kShift;
         if (__any(mx != m)) {
-            const float f = exp2_fast(m - use);
+            const float f = exp2_fast(m - use - C::kShift);
             l *= f;
 #pragma unroll
             for (int d = 0; d < DT; ++d)
@@ -383,7 +487,7 @@ __global__ void __launch_bounds__(64 * AR_WAVES) k_attn_rows(AttnArgs a, int til
         for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                float x = exp2_fast(s[u][i] - use + C::kShift);
+                float x = exp2_fast(fmaf(s[u][i], by, -use));
                 s[u][i] = x;
                 sum += x;
 #pragma unroll
@@ -395,25 +499,22 @@ __global__ void __launch_bounds__(64 * AR_WAVES) k_attn_rows(AttnArgs a, int til
             }
         l += sum;
 
-        // V's rows to LDS; of a step with hidden keys, the rows that no row of the
-        // tile sees as zeros (nothing may come from them, whatever they hold)
+        // of a step with hidden keys, the rows of V that no row of the tile sees are
+        // cleared (nothing may come from them, whatever they hold)
         bool odd = false;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int e = i * 64 + lane, r = e / NC, c = e % NC;
-            if (!whole) {
-                const int j = key + r;
-                if (!(j < t.len && (j <= t.last || j < t.prefix) && (a.window == 0 || t.first - j < a.window)))
-                    vf[i] = u4{};
-                odd |= odd_value<C>(vf[i].x) || odd_value<C>(vf[i].y) || odd_value<C>(vf[i].z) ||
-                       odd_value<C>(vf[i].w);
+        if (!whole)
+            for (int i = lane; i < AR_KEYS * NC; i += 64) {
+                const int r = i / NC, j = key + r;
+                if (((here >> (r >> 4)) & 1) && j < t.len && (j <= t.last || j < t.prefix) &&
+                    (a.window == 0 || t.first - j < a.window)) {
+                    const u4 w = *(const u4 *)(vt + 16 * i);
+                    odd |= odd_value<C>(w.x) || odd_value<C>(w.y) || odd_value<C>(w.z) || odd_value<C>(w.w);
+                } else {
+                    *(u4 *)(vt + 16 * i) = u4{};
+                }
             }
-            *(u4 *)(vt + r * (DP * 2) + v_chunk<NC>(r, c) * 16) = vf[i];
-        }
         asm volatile("" ::: "memory");
-        if (more)
-            load_v(key + AR_KEYS * AR_WAVES);
-        if (!whole && __any(odd)) {
+        if (__builtin_expect(!whole && __any(odd), 0)) {
             // infinities or NaNs that some rows of the tile see and others do not:
             // 0 times them must not reach the others.  They are added one key at a
             // time where a row has a weight for them, and the products take 0.
@@ -425,8 +526,7 @@ __global__ void __launch_bounds__(64 * AR_WAVES) k_attn_rows(AttnArgs a, int til
                 x = __shfl(x, col + 16 * ((j >> 2) & 3));
 #pragma unroll
                 for (int d = 0; d < DT; ++d) {
-                    const int e = 16 * d + 4 * g;
-                    const V4 v = *(const V4 *)(vt + j * (DP * 2) + v_chunk<NC>(j, e / 8) * 16 + (e % 8) * 2);
+                    const V4 v = *(const V4 *)(vt + j * (DP * 2) + v_chunk<NC>(j, 2 * d + (g >> 1)) * 16 + 8 * (g & 1));
 #pragma unroll
                     for (int q = 0; q < 4; ++q)
                         o[d][q] += x != 0.0f && !__builtin_isfinite((float)v[q]) ? x * (float)v[q] : 0.0f;
@@ -452,7 +552,8 @@ __global__ void __launch_bounds__(64 * AR_WAVES) k_attn_rows(AttnArgs a, int til
 
     // the waves' sums, in wave order
     l = groups_sum(l);
-    float *const ol = (float *)vt;
+    asm volatile("" ::: "memory");
+    float *const ol = (float *)mine;
 #pragma unroll
     for (int d = 0; d < DT; ++d)
         *(f4 *)(ol + col * (DP + 4) + 16 * d + 4 * g) = o[d];
@@ -498,90 +599,525 @@ __global__ void __launch_bounds__(64 * AR_WAVES) k_attn_rows(AttnArgs a, int til
     }
 }
 
-// The splits' partial rows joined, a wave a row: sum_i e^(m_i - m) o_i over
-// sum_i e^(m_i - m) l_i, in split order.
-template <typename C, int PARTS>
-__global__ void __launch_bounds__(256) k_attn_join(AttnArgs a, int splits)
+// ---- many rows: chunks of a prompt ---------------------------------------------
+constexpr int AC_ROWS = 128; // rows of a workgroup's tile, 32 a wave
+constexpr int AC_KEYS = 128; // keys of a step at most
+
+// Keys that a wave multiplies in a step: as many as leave its registers room
+// beside O^T and q (256 wide: 128 registers of O^T, 64 a part of q).
+constexpr int ac_half_keys(int) { return 64; }
+// Waves a SIMD: two, where a wave's operands fit 256 registers.
+constexpr int ac_waves(int parts, int dp) { return dp <= 64 || (dp <= 128 && parts <= 2) ? 2 : 1; }
+
+// Where 16-byte chunk c of key row r lies in its row of LDS: K's so that the 16
+// rows of a matrix operand's read lie in different banks, V's so that the four
+// rows and 64 bytes of a pair of transposing reads do.
+template <int NC>
+__device__ __forceinline__ int ac_k_chunk(int r, int c)
 {
-    const int lane = threadIdx.x & 63, D = a.cache.dim;
-    const int64_t rows = (int64_t)a.batch.tokens * a.q_heads;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= rows)
-        return;
-    int first = 0;
-    if (kv_find(a.batch.sequences, (int)(row / a.q_heads), first, [&](int i) {
-            const int b = kv_clamp(a.batch.starts[i], 0, a.batch.tokens);
-            return kv_clamp(a.batch.starts[i + 1], b, a.batch.tokens) - b;
-        }) < 0)
-        return; // a row behind the last sequence
-    const float *ml = a.part + (int64_t)splits * rows * D;
-    float top = kNone;
-    for (int i = lane; i < splits; i += 64)
-        top = fmaxf(top, ml[2 * (i * rows + row)]);
-    for (int d = 32; d; d /= 2)
-        top = fmaxf(top, __shfl_xor(top, d));
-    f4 v = f4{};
-    float sum = 0.0f;
-    for (int i = 0; i < splits; ++i) {
-        const float m = ml[2 * (i * rows + row)], l = ml[2 * (i * rows + row) + 1];
-        if (l == 0.0f)
-            continue; // no key was seen: nothing else was written
-        const float f = m == kNone ? 0.0f : exp2_fast(m - top);
-        sum += l * f;
-        if (4 * lane < D)
-            v += *(const f4 *)(a.part + (i * rows + row) * D + 4 * lane) * f;
-    }
-    if (4 * lane < D) {
-        v = sum == 0.0f ? f4{} : v * (1.0f / sum);
-        if constexpr (PARTS == 1)
-            *(typename C::V4 *)((typename C::T *)a.out + row * D + 4 * lane) = __builtin_convertvector(v, typename C::V4);
-        else
-            *(f4 *)((float *)a.out + row * D + 4 * lane) = v;
-    }
+    return NC == 8 ? c ^ ((r >> 1) & 7) : c ^ (r & 15);
+}
+template <int NC>
+__device__ __forceinline__ int ac_v_chunk(int r, int c)
+{
+    return NC == 8 ? c ^ (4 * ((r >> 1) & 1)) : c ^ (4 * (r & 3));
 }
 
-template <typename C, int PARTS, int DP>
+// Four waves hold 32 rows each; where HALVES is 2, a second four hold the same
+// rows for the second half of a step's keys, and the halves' sums are joined at
+// the end.  The keys come into LDS by direct copies one step ahead (each wave a
+// run of one page of K and of V) while the step before is multiplied; one barrier
+// a step.  S^T = K Q^T and O^T = V^T P^T in 32 x 32 x 16 products: a lane holds
+// half of the scores of its row and 16 of the 32 rows of each d tile.
+template <typename C, int PARTS, int DP, bool GEN, int HALVES>
+__global__ void __launch_bounds__(256 * HALVES, ac_waves(PARTS, DP))
+k_attn_chunk(AttnArgs a, int tiles, int least, int splits)
+{
+    typedef typename C::T T;
+    typedef typename C::V8 V8;
+    typedef typename C::V4 V4;
+    constexpr int WAVES = 4 * HALVES;
+    constexpr int HK = ac_half_keys(DP), KEYS = HK * HALVES, SU = HK / 32; // a half's keys of a step, and all
+    constexpr int RUN = HK / 4, NI = RUN * DP / 512; // keys that a wave copies, in NI copies of 1 KB
+    constexpr int KS = DP / 16, DT = DP / 32, NC = DP / 8;
+    constexpr int TILE = KEYS * DP * 2;
+    constexpr float kUp = C::kShift != 0.0f ? 8.0f : 0.0f; // p times 2^kUp, with room for kLate
+    constexpr float kLate = 7.0f; // the sums are scaled again when the maximum has grown by more than 2^kLate
+    __shared__ __attribute__((aligned(16))) uint8_t lds[4 * TILE]; // K, V of two steps
+    __shared__ int lds_odd;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = wave >> 2;
+    const int col = lane & 31, h = lane >> 5;
+    const int D = a.cache.dim;
+    Tile t;
+    if (!find_tile<AC_ROWS, KEYS>(a, tiles, least, splits, blockIdx.x, t))
+        return;
+    if (tid == 0)
+        lds_odd = -1;
+
+    const int wrow0 = t.row0 + 32 * (wave & 3);
+    const int wrows = min(32, t.row0 + t.rows - wrow0);
+    const int before = t.first - t.row0 / a.group; // position of the sequence's first new token
+    const int row = wrow0 + col;
+    const bool live = col < wrows;
+    const int qhead = t.head * a.group + (live ? row % a.group : 0);
+    const int64_t qrow = (int64_t)(t.start + (live ? row / a.group : 0)) * a.q_heads + qhead;
+    const int wfirst = before + wrow0 / a.group, wlast = before + (wrow0 + max(wrows, 1) - 1) / a.group;
+    const int pos = live ? before + row / a.group : wfirst;
+    V8 qf[PARTS][KS];
+    float undo;
+    load_q<C, PARTS, KS>(a, qrow, live, 2, h, qf, undo);
+    const float scale = (a.scale == 0.0f ? 1.0f : fabsf(a.scale)) * undo;
+    // scores become powers of two with the last factor, `by`; a cap takes the scale
+    // before, and the bias is added in units of `by`
+    const float by = GEN && a.cap > 0.0f ? a.cap * kLog2e : scale * kLog2e;
+    const float slope = GEN && a.slopes ? a.slopes[qhead] * kLog2e / by : 0.0f;
+    const Seen sees = seen_from(a, t, pos);
+
+    // a lane's part of the copies: RUN keys of one page
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds;
+    uint32_t koff[NI], voff[NI];
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+        const int r = (64 * i + lane) / NC, c = (64 * i + lane) % NC;
+        // (chunks behind a head's end hold its last one: nothing reads them with weight)
+        koff[i] = 2u * (uint32_t)(r * D + 8 * min(ac_k_chunk<NC>(RUN * wave + r, c), D / 8 - 1));
+        voff[i] = 2u * (uint32_t)(r * D + 8 * min(ac_v_chunk<NC>(RUN * wave + r, c), D / 8 - 1));
+    }
+    const int page_mask = (1 << a.cache.page_shift) - 1;
+    const int n_steps = (t.hi - t.lo + KEYS - 1) / KEYS;
+    // page ids of a step's runs of 16 keys, in the first lanes
+    auto page_of = [&](int step) {
+        const int j = t.lo + KEYS * step + 16 * (lane & (KEYS / 16 - 1));
+        return j < t.hi ? t.table[j >> a.cache.page_shift] : -1;
+    };
+    // the runs of a step that name no page of the pool
+    auto bad_runs = [&](int step, int ids) {
+        const bool bad = lane < KEYS / 16 && t.lo + KEYS * step + 16 * lane < t.hi &&
+                         (unsigned)ids >= (unsigned)a.cache.pages;
+        return (int)__ballot(bad);
+    };
+    auto copy = [&](int step, int ids) {
+        const int id = __builtin_amdgcn_readlane(ids, RUN * wave / 16);
+        if ((unsigned)id >= (unsigned)a.cache.pages)
+            return; // (no such key, or reported: its rows of V are cleared before use)
+        const int j = t.lo + KEYS * step + RUN * wave;
+        const int64_t at = (int64_t)id * a.cache.page_stride +
+                           ((int64_t)((t.head << a.cache.page_shift) + (j & page_mask))) * D;
+        const T *k = (const T *)a.cache.k + at, *v = (const T *)a.cache.v + at;
+        const uint32_t to = lds0 + 2 * TILE * (step & 1) + 1024 * NI * wave;
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+            lds_copy16_at(k, koff[i], to + 1024 * i);
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+            lds_copy16_at(v, voff[i], to + TILE + 1024 * i);
+    };
+
+    // every wave, when all have read the step's values
+    auto clear_odd = [&](int step) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        lds_barrier();
+        uint32_t *const v = (uint32_t *)(lds + 2 * TILE * (step & 1) + TILE);
+        for (int i = tid; i < TILE / 4; i += 64 * WAVES)
+            v[i] = without_odd<C>(v[i]);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        lds_barrier();
+    };
+
+    // a lane's places in a tile: K's operand (row col, chunk 2 i + h), V^T's (rows
+    // 4 h + q, columns of the 16-lane group).  The chunks of the other products lie
+    // at these addresses with the number of the chunk xor-ed in, which is formed
+    // anew each step: the registers that the addresses would take are needed.
+    const int l16 = lane & 15, vrow = 4 * h + (l16 >> 2);
+    const uint32_t kat = (uint32_t)(col * DP * 2 + 16 * ac_k_chunk<NC>(col, h));
+    const uint32_t vat = (uint32_t)(vrow * DP * 2 +
+                                    16 * ac_v_chunk<NC>(vrow, 2 * ((lane >> 4) & 1) + ((l16 & 3) >> 1)) + 8 * (l16 & 1));
+
+    float m = kNone, l = 0.0f;
+    f16v o[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+        o[d] = f16v{};
+
+    int ids = -1, ids_next = -1;
+    if (n_steps > 0) {
+        ids = page_of(0);
+        copy(0, ids);
+        ids_next = page_of(1);
+    }
+    for (int step = 0; step < n_steps; ++step) {
+        const int key0 = t.lo + KEYS * step, key = key0 + HK * half;
+        __builtin_amdgcn_s_waitcnt(0x0070); // vmcnt(0) lgkmcnt(0): this wave's copies, and its reads of the other buffer
+        lds_barrier();
+        const int bad_all = bad_runs(step, ids), bad = bad_all >> (HK / 16 * half) & ((1 << HK / 16) - 1);
+        if (bad_all && a.flags && tid == 0)
+            atomicOr(a.flags, kFlagKvPage);
+        if (step + 1 < n_steps) {
+            copy(step + 1, ids_next);
+            ids = ids_next;
+            ids_next = page_of(step + 2);
+        }
+        uint8_t *const vt = lds + 2 * TILE * (step & 1) + TILE + HK * half * (DP * 2);
+        // a step that the whole tile does not see whole: rows of V that no row sees
+        // are cleared, and an infinity or NaN among the others is looked for
+        const bool edge = bad_all || key0 + KEYS > t.len || !(key0 + KEYS - 1 <= t.first || key0 + KEYS <= t.prefix) ||
+                          !(a.window == 0 || t.last - key0 < a.window);
+        bool odd = false;
+        if (__builtin_expect(edge, 0)) {
+            uint8_t *const all = lds + 2 * TILE * (step & 1) + TILE;
+            for (int i = tid; i < KEYS * NC; i += 64 * WAVES) {
+                const int r = i / NC, j = key0 + r;
+                if (!(j < t.len && (j <= t.last || j < t.prefix) && (a.window == 0 || t.first - j < a.window)) ||
+                    ((bad_all >> (r >> 4)) & 1)) {
+                    *(u4 *)(all + 16 * i) = u4{};
+                } else {
+                    const u4 w = *(const u4 *)(all + 16 * i);
+                    odd |= odd_value<C>(w.x) || odd_value<C>(w.y) || odd_value<C>(w.z) || odd_value<C>(w.w);
+                }
+            }
+            if (odd)
+                lds_odd = step;
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            lds_barrier();
+            odd = __builtin_amdgcn_readfirstlane(lds_odd) == step;
+        }
+        // keys that none of the wave's rows sees
+        if (wrows <= 0 || key >= t.hi || (key > wlast && key >= t.prefix) ||
+            (a.window && wfirst - (key + HK - 1) >= a.window)) {
+            if (odd)
+                clear_odd(step);
+            continue;
+        }
+        const bool whole = !bad && key + HK <= t.len && (key + HK - 1 <= wfirst || key + HK <= t.prefix) &&
+                           (a.window == 0 || wlast - key < a.window);
+
+        const uint32_t k_here = lds0 + 2 * TILE * (step & 1) + HK * half * (DP * 2) + kat;
+        const uint32_t v_here = lds0 + 2 * TILE * (step & 1) + HK * half * (DP * 2) + TILE + vat;
+        f16v s[SU];
+#pragma unroll
+        for (int u = 0; u < SU; ++u) {
+            s[u] = f16v{};
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+                // (256 wide: chunks 16 and up lie 256 bytes on)
+                const V8 kf = read_lds<V8>((k_here ^ (32 * (i & 7))) + 32 * u * (DP * 2) + (i >> 3) * 256);
+#pragma unroll
+                for (int part = 0; part < PARTS; ++part)
+                    s[u] = C::mfma32(kf, qf[part][i], s[u]);
+                if (DP == 256 && i % 8 == 7)
+                    __builtin_amdgcn_sched_barrier(0); // (operands further ahead would not fit the registers)
+            }
+        }
+        if (GEN) {
+            const float apart = (float)(pos - key - 4 * h);
+            if (a.cap > 0.0f)
+#pragma unroll
+                for (int u = 0; u < SU; ++u)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        s[u][i] = tanh_own(s[u][i] * (scale / a.cap));
+            if (a.slopes)
+#pragma unroll
+                for (int u = 0; u < SU; ++u)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        s[u][i] = fmaf(-slope, fabsf(apart - (float)(32 * u + 8 * (i >> 2) + (i & 3))), s[u][i]);
+        }
+        if (__builtin_expect(!whole, 0)) {
+#pragma unroll
+            for (int u = 0; u < SU; ++u)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    s[u][i] = sees(key + 32 * u + 8 * (i >> 2) + 4 * h + (i & 3)) ? s[u][i] : kNone;
+            if (__builtin_expect(bad, 0))
+#pragma unroll
+                for (int u = 0; u < SU; ++u)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        s[u][i] = (bad >> (2 * u + (i >> 3))) & 1 ? kNone : s[u][i];
+        }
+        float mx = kNone;
+#pragma unroll
+        for (int u = 0; u < SU; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                mx = fmaxf(mx, s[u][i]);
+        mx = halves_max(mx) * by;
+        if (__any(mx > m + kLate || (m == kNone && mx != kNone))) {
+            const float top = fmaxf(mx, m);
+            const float f = top == kNone ? 1.0f : exp2_fast(m - top);
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+                o[d] *= f;
+            m = top;
+        }
+        const float use = (m == kNone ? 0.0f : m) - kUp;
+        if (__builtin_expect(odd, 0)) {
+            // infinities or NaNs that some rows of the tile see and others do not:
+            // they are added one key at a time where a row has a weight for them,
+            // then the products take 0 (see k_attn_rows)
+#pragma unroll 1
+            for (int j = 0; j < HK; ++j) {
+                const int i = 4 * ((j & 31) >> 3) + (j & 3);
+                float x = kNone;
+#pragma unroll
+                for (int u = 0; u < SU; ++u)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        x = i == e && u == j >> 5 ? s[u][e] : x;
+                x = __shfl(exp2_fast(fmaf(x, by, -use)), col + 32 * ((j >> 2) & 1));
+                const uint8_t *const vj = vt + j * (DP * 2) + 8 * h;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4) {
+                        const V4 v = *(const V4 *)(vj + ac_v_chunk<NC>(j, 4 * d + e / 4) * 16);
+#pragma unroll
+                        for (int q = 0; q < 4; ++q)
+                            o[d][e + q] += x != 0.0f && !__builtin_isfinite((float)v[q]) ? x * (float)v[q] : 0.0f;
+                    }
+                    __builtin_amdgcn_sched_barrier(0); // (rare: no registers for loads ahead)
+                }
+            }
+            clear_odd(step);
+        }
+        // 32 keys at a time: their weights, then their products
+#pragma unroll
+        for (int u = 0; u < SU; ++u) {
+            V8 pf[PARTS][2];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                float x = exp2_fast(fmaf(s[u][i], by, -use));
+                s[u][i] = x;
+                l += x;
+#pragma unroll
+                for (int part = 0; part < PARTS; ++part) {
+                    const T y = (T)x;
+                    pf[part][i >> 3][i & 7] = y;
+                    x -= (float)y;
+                }
+            }
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                if (DP == 256 && d % 2 == 0)
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const uint32_t at = (v_here ^ (64 * (d & 3))) + (32 * u + 16 * k) * (DP * 2) + (d >> 2) * 256;
+                    const V4 lo = read_tr_at<V4>(at), hi = read_tr_at<V4>(at + 8 * (DP * 2));
+                    const V8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+                    for (int part = 0; part < PARTS; ++part)
+                        o[d] = C::mfma32(v, pf[part][k], o[d]);
+                }
+            }
+        }
+    }
+    __builtin_amdgcn_s_waitcnt(0x0070); // no copy is in flight when the workgroup ends
+
+    if constexpr (HALVES == 2) {
+        // the second half's maxima, sums and rows to the first, by lane
+        lds_barrier(); // nobody reads the keys any more
+        float *const to = (float *)lds + (DT * 16 + 2) * 64 * (wave & 3) + lane;
+        if (half) {
+            to[0] = m;
+            to[64] = l;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    to[64 * (2 + 16 * d + e)] = o[d][e];
+        }
+        __syncthreads();
+        if (half)
+            return;
+        const float m2 = to[0], l2 = to[64], top = fmaxf(m, m2);
+        const float f = m == kNone ? 0.0f : exp2_fast(m - top), f2 = m2 == kNone ? 0.0f : exp2_fast(m2 - top);
+        // (a half without keys has only zeros; NaN stays)
+        l = l * f + l2 * f2;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                o[d][e] = o[d][e] * f + to[64 * (2 + 16 * d + e)] * f2;
+        m = top;
+    }
+
+    if (!live)
+        return;
+    l = halves_sum(l);
+    const int64_t rows_all = (int64_t)a.batch.tokens * a.q_heads;
+    if (splits > 1) {
+        if (h == 0)
+            *(f2 *)(a.part + (int64_t)splits * rows_all * D + 2 * (t.split * rows_all + qrow)) = f2{m, l};
+        if (l == 0.0f)
+            return;
+    }
+    const float f = splits > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            const int at = 32 * d + 2 * e + 4 * h;
+            if (at >= D)
+                continue;
+            f4 v = f4{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]};
+            v = l == 0.0f ? f4{} : v * f;
+            if (splits > 1)
+                *(f4 *)(a.part + (t.split * rows_all + qrow) * D + at) = v;
+            else if constexpr (PARTS == 1)
+                *(V4 *)((T *)a.out + qrow * D + at) = __builtin_convertvector(v, V4);
+            else
+                *(f4 *)((float *)a.out + qrow * D + at) = v;
+        }
+}
+
+// The splits' partial rows joined, N threads a row: sum_i e^(m_i - m) o_i over
+// sum_i e^(m_i - m) l_i.  A split is read by one group of dim / 4 threads, the
+// groups' sums are added in their order.  Few splits of many rows take a wave a
+// row, many splits a workgroup.
+template <typename C, int PARTS, int N>
+__global__ void __launch_bounds__(256) k_attn_join(AttnArgs a, int splits)
+{
+    __shared__ float weight[256 / N][AR_SPLITS], lds_l[256 / N];
+    __shared__ __attribute__((aligned(16))) float lds_o[256 * 4];
+    const int tid = threadIdx.x % N, mine = threadIdx.x / N, lane = threadIdx.x & 63, D = a.cache.dim;
+    const int64_t rows = (int64_t)a.batch.tokens * a.q_heads, row = (int64_t)blockIdx.x * (256 / N) + mine;
+    int first = 0;
+    KvSeq q;
+    // (a row behind the last sequence is left as it is)
+    const bool live = kv_find(a.batch, a.cache.page_shift, (int)min(row / a.q_heads, (int64_t)a.batch.tokens), first, q,
+                              [](int n) { return n; }) >= 0;
+    const f2 *ml = (const f2 *)(a.part + (int64_t)splits * rows * D);
+    if (live && tid < 64) {
+        f2 v[AR_SPLITS / 64];
+        float top = kNone, sum = 0.0f;
+#pragma unroll
+        for (int u = 0; u < AR_SPLITS / 64; ++u) {
+            const int i = lane + 64 * u;
+            v[u] = i < splits ? ml[i * rows + row] : f2{kNone, 0.0f};
+            top = fmaxf(top, v[u].x);
+        }
+#pragma unroll
+        for (int d = 32; d; d /= 2)
+            top = fmaxf(top, __shfl_xor(top, d));
+#pragma unroll
+        for (int u = 0; u < AR_SPLITS / 64; ++u) {
+            // (sum 0: no key was seen and nothing else was written; NaN stays)
+            const float f = v[u].x == kNone ? 0.0f : exp2_fast(v[u].x - top);
+            sum += v[u].y * f;
+            weight[mine][lane + 64 * u] = v[u].y == 0.0f ? -1.0f : f;
+        }
+#pragma unroll
+        for (int d = 32; d; d /= 2)
+            sum += __shfl_xor(sum, d);
+        if (lane == 0)
+            lds_l[mine] = sum;
+    }
+    __syncthreads();
+    const int per = D / 4, groups = N / per, at = tid / per, d = 4 * (tid - at * per);
+    f4 v = f4{};
+    if (live && at < groups) {
+#pragma unroll 4
+        for (int i = at; i < splits; i += groups) {
+            const float f = weight[mine][i];
+            if (f >= 0.0f)
+                v += *(const f4 *)(a.part + (i * rows + row) * D + d) * f;
+        }
+        *(f4 *)(lds_o + 4 * threadIdx.x) = v;
+    }
+    __syncthreads();
+    if (!live || tid >= per)
+        return;
+    for (int i = 1; i < groups; ++i)
+        v += *(const f4 *)(lds_o + 4 * (threadIdx.x + i * per));
+    const float sum = lds_l[mine];
+    v = sum == 0.0f ? f4{} : v * (1.0f / sum);
+    if constexpr (PARTS == 1)
+        *(typename C::V4 *)((typename C::T *)a.out + row * D + d) = __builtin_convertvector(v, typename C::V4);
+    else
+        *(f4 *)((float *)a.out + row * D + d) = v;
+}
+
+template <typename C, int PARTS, int DP, bool GEN>
 void start(const AttnArgs &a, const AttnPlan &p, hipStream_t s)
 {
     const dim3 grid((uint32_t)((int64_t)p.tiles * a.cache.heads * p.splits));
-    if (a.cap > 0.0f || a.slopes)
-        hipLaunchKernelGGL((k_attn_rows<C, PARTS, DP, true>), grid, dim3(64 * AR_WAVES), 0, s, a, p.tiles, p.least, p.splits);
+    if (p.rows == AR_ROWS) {
+        hipLaunchKernelGGL((k_attn_rows<C, PARTS, DP, GEN>), grid, dim3(64 * AR_WAVES), 0, s, a, p.tiles, p.least, p.splits);
+        return;
+    }
+    if constexpr (ac_waves(PARTS, DP) == 2 && DP <= 128) {
+        if (p.halves) {
+            hipLaunchKernelGGL((k_attn_chunk<C, PARTS, DP, GEN, 2>), grid, dim3(512), 0, s, a, p.tiles, p.least, p.splits);
+            return;
+        }
+    }
+    hipLaunchKernelGGL((k_attn_chunk<C, PARTS, DP, GEN, 1>), grid, dim3(256), 0, s, a, p.tiles, p.least, p.splits);
+}
+
+template <typename C, int PARTS, bool GEN>
+void start_gen(const AttnArgs &a, const AttnPlan &p, hipStream_t s)
+{
+    if (a.cache.dim <= 64)
+        start<C, PARTS, 64, GEN>(a, p, s);
+    else if (a.cache.dim <= 128)
+        start<C, PARTS, 128, GEN>(a, p, s);
     else
-        hipLaunchKernelGGL((k_attn_rows<C, PARTS, DP, false>), grid, dim3(64 * AR_WAVES), 0, s, a, p.tiles, p.least, p.splits);
+        start<C, PARTS, 256, GEN>(a, p, s);
 }
 
 template <typename C, int PARTS>
 hipError_t start_dim(const AttnArgs &a, const AttnPlan &p, hipStream_t s)
 {
-    if (a.cache.dim <= 64)
-        start<C, PARTS, 64>(a, p, s);
-    else if (a.cache.dim <= 128)
-        start<C, PARTS, 128>(a, p, s);
+    if (a.cap > 0.0f || a.slopes)
+        start_gen<C, PARTS, true>(a, p, s);
     else
-        start<C, PARTS, 256>(a, p, s);
+        start_gen<C, PARTS, false>(a, p, s);
     if (p.splits > 1) {
         const int64_t rows = (int64_t)a.batch.tokens * a.q_heads;
-        hipLaunchKernelGGL((k_attn_join<C, PARTS>), dim3((uint32_t)((rows + 3) / 4)), dim3(256), 0, s, a, p.splits);
+        if (p.splits <= 16)
+            hipLaunchKernelGGL((k_attn_join<C, PARTS, 64>), dim3((uint32_t)((rows + 3) / 4)), dim3(256), 0, s, a, p.splits);
+        else
+            hipLaunchKernelGGL((k_attn_join<C, PARTS, 256>), dim3((uint32_t)rows), dim3(256), 0, s, a, p.splits);
     }
     return hipGetLastError();
 }
 
 } // namespace
 
-AttnPlan attn_plan(int act, int kv_type, int q_heads, int kv_heads, int dim, int sequences, int tokens,
-                   int64_t capacity)
+AttnPlan attn_plan(int q_heads, int kv_heads, int dim, int sequences, int tokens, int64_t capacity, int window)
 {
-    (void)act;
-    (void)kv_type;
     AttnPlan p;
     const int group = q_heads / kv_heads;
-    p.rows = AR_ROWS;
-    p.tiles = (int)(((int64_t)tokens * group + AR_ROWS - 1) / AR_ROWS) + sequences;
-    // enough workgroups to fill the chip twice over, of at least `least` keys
-    p.least = sequences == 1 ? 128 : 512;
-    const int64_t most = (capacity + p.least - 1) / p.least;
-    const int64_t want = (4 * 512 + (int64_t)p.tiles * kv_heads - 1) / ((int64_t)p.tiles * kv_heads);
-    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(most, want), 128));
+    // p.tiles: the sum of ceil(rows of a sequence / p.rows) at most
+    const int64_t rows = (int64_t)tokens * group, some = std::min(sequences, tokens);
+    // a batch whose sequences have more than a tile of few rows on average takes the
+    // tiles of many
+    p.rows = rows > (int64_t)AR_ROWS * some ? AC_ROWS : AR_ROWS;
+    p.tiles = (int)((rows - some) / p.rows + some);
+    const int64_t units = (int64_t)p.tiles * kv_heads;
+    int64_t want;
+    if (p.rows == AR_ROWS) {
+        // a sequence alone fills the chip once; of many, of which some are longer
+        // than others, the parts stay short enough to even out
+        p.least = units <= 32 ? 128 : units <= 64 ? 256 : 512;
+        want = (256 * std::min<int64_t>(some, 16) + units - 1) / units;
+    } else {
+        // tiles that fill the chip are not split: joining would cost more
+        p.least = 256;
+        want = units >= 256 ? 1 : (512 * std::min<int64_t>(some, 2) + units - 1) / units;
+    }
+    // (a window, where there is one, ends a tile's keys: no part would lie behind)
+    const int64_t reach = window ? std::min(capacity, (int64_t)window + p.rows + AC_KEYS) : capacity;
+    const int64_t most = (reach + p.least - 1) / p.least;
+    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(most, want), AR_SPLITS));
+    // Few tiles: two halves of a workgroup each, which end a long tile sooner
+    // (512 tiles of a 2048-token prompt: 65 us against 77); of many, two
+    // workgroups a CU come further (4096 tokens: 174 us against 200).
+    p.halves = units * p.splits <= 512;
     p.bytes = p.splits > 1 ? (size_t)p.splits * tokens * q_heads * (dim + 2) * 4 : 0;
     return p;
 }

@@ -64,19 +64,23 @@ __device__ __forceinline__ void kv_report(const KvBatch &b, int page_shift, uint
     }
 }
 
-// The sequence of unit `want` where sequence s has units(s) of them (its rows,
-// or its tiles of rows): the lanes of a wave look at 64 sequences at a time.
-// Returns -1 if the batch has no such unit, else leaves in `first` the units
-// of the sequences before.  All lanes of the wave must be active.
+// The sequence that unit `want` lies in, where a sequence of n rows has
+// units(n) of them (its rows, or tiles of them): the lanes of a wave look at 64
+// sequences at a time, so that a batch of up to 64 costs one round of loads.
+// Returns its index (-1: the batch has no such unit), the units of those before
+// it in `first` and the sequence itself in `q`.  All lanes must be active.
 template <typename F>
-__device__ __forceinline__ int kv_find(int sequences, int want, int &first, F units)
+__device__ __forceinline__ int kv_find(const KvBatch &b, int page_shift, int want, int &first, KvSeq &q, F units)
 {
     const int lane = threadIdx.x & 63;
     int before = 0;
-    for (int s0 = 0; s0 < sequences; s0 += 64) {
+    for (int s0 = 0; s0 < b.sequences; s0 += 64) {
         const int s = s0 + lane;
-        int sum = s < sequences ? units(s) : 0;
-        const int own = sum;
+        KvSeq mine{0, 0, 0};
+        if (s < b.sequences)
+            mine = kv_seq(b, page_shift, s);
+        const int own = units(mine.n);
+        int sum = own;
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) {
             const int up = __shfl_up(sum, d);
@@ -86,6 +90,9 @@ __device__ __forceinline__ int kv_find(int sequences, int want, int &first, F un
         if (past) {
             const int at = __builtin_ctzll(past);
             first = before + __builtin_amdgcn_readlane(sum - own, at);
+            q.start = __builtin_amdgcn_readlane(mine.start, at);
+            q.n = __builtin_amdgcn_readlane(mine.n, at);
+            q.len = __builtin_amdgcn_readlane(mine.len, at);
             return s0 + at;
         }
         before += __builtin_amdgcn_readlane(sum, 63);

@@ -48,10 +48,12 @@ struct AttnPlan {
     int tiles;   // tiles at most, over all sequences
     int splits;  // parts of a tile's keys at most
     int least;   // keys of a part at least
+    bool halves; // whether two halves of a workgroup share a tile's keys
     size_t bytes; // workspace
 };
-AttnPlan attn_plan(int act, int kv_type, int q_heads, int kv_heads, int dim, int sequences, int tokens,
-                   int64_t capacity);
+// window: the window where there is one and no prefix reaches behind it, else 0
+// (which never needs less workspace).
+AttnPlan attn_plan(int q_heads, int kv_heads, int dim, int sequences, int tokens, int64_t capacity, int window);
 hipError_t launch_attn(const AttnArgs &a, const AttnPlan &p, hipStream_t s);
 
 // kv_pages.hip

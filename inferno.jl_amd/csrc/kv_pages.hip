@@ -290,6 +290,7 @@ __global__ void __launch_bounds__(256) k_compact_tables(CompactArgs a)
     }
 }
 
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 constexpr int COPY_THREADS = 256;
 constexpr int COPY_PER = 4;                                // 16-byte loads in flight a thread
 constexpr int COPY_BYTES = COPY_THREADS * COPY_PER * 16;   // a workgroup's item
@@ -334,21 +335,17 @@ __global__ void __launch_bounds__(COPY_THREADS) k_kv_copy(CopyArgs a)
         }
         uint8_t *pool = (r < a.pieces ? a.k : a.v) + layer * a.layer_stride;
         const int64_t off = (r < a.pieces ? r : r - a.pieces) * COPY_BYTES;
-        const uint8_t *from = pool + src * a.page_stride;
-        uint8_t *to = pool + dst * a.page_stride;
-        uint4 v[COPY_PER];
+        const uint8_t *from = pool + src * a.page_stride + off + 16 * tid;
+        uint8_t *to = pool + dst * a.page_stride + off + 16 * tid;
+        const int64_t left = a.page_bytes - off - 16 * tid; // bytes from this thread's first on
+        u4 v[COPY_PER];
 #pragma unroll
-        for (int u = 0; u < COPY_PER; ++u) {
-            const int64_t b = off + 16 * (tid + COPY_THREADS * u);
-            if (b < a.page_bytes)
-                v[u] = *(const uint4 *)(from + b);
-        }
+        for (int u = 0; u < COPY_PER; ++u)
+            v[u] = left > 16 * COPY_THREADS * u ? *(const u4 *)(from + 16 * COPY_THREADS * u) : u4{};
 #pragma unroll
-        for (int u = 0; u < COPY_PER; ++u) {
-            const int64_t b = off + 16 * (tid + COPY_THREADS * u);
-            if (b < a.page_bytes)
-                *(uint4 *)(to + b) = v[u];
-        }
+        for (int u = 0; u < COPY_PER; ++u)
+            if (left > 16 * COPY_THREADS * u)
+                *(u4 *)(to + 16 * COPY_THREADS * u) = v[u];
     }
 }
 

@@ -21,6 +21,7 @@ constexpr int ROPE_THREADS = 256;
 constexpr int ROPE_FLOATS = 4096; // head values a workgroup holds
 constexpr int ROPE_HEADS = 16;    // heads a workgroup holds (16 lanes each sum a norm)
 
+typedef float f4 __attribute__((ext_vector_type(4)));
 typedef float float8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bhalf8 __attribute__((ext_vector_type(8)));
@@ -53,29 +54,27 @@ __global__ void __launch_bounds__(ROPE_THREADS) k_rope_kv(RopeArgs a)
 
     // the values are on their way while the token's place is looked up
     const int n4 = heads * D / 4;
-    float4 val[ROPE_FLOATS / 4 / ROPE_THREADS];
+    f4 val[ROPE_FLOATS / 4 / ROPE_THREADS];
 #pragma unroll
     for (int j = 0; j < ROPE_FLOATS / 4 / ROPE_THREADS; ++j) {
         const int i = tid + ROPE_THREADS * j;
+        val[j] = f4{};
         if (i < n4) {
             const int h = h0 + 4 * i / D, e = 4 * i % D;
             const float *src = h < knob ? a.q + token * a.q_step + h * D
                              : h < vnob ? a.k + token * a.k_step + (h - knob) * D
                                         : a.v + token * a.v_step + (h - vnob) * D;
-            val[j] = *(const float4 *)(src + e);
+            val[j] = *(const f4 *)(src + e);
         }
     }
 
     if (blockIdx.x == 0 && a.flags)
         kv_report(a.batch, a.cache.page_shift, a.flags);
     int first = 0;
-    const int s = kv_find(a.batch.sequences, token, first, [&](int i) {
-        const int b = kv_clamp(a.batch.starts[i], 0, a.batch.tokens);
-        return kv_clamp(a.batch.starts[i + 1], b, a.batch.tokens) - b;
-    });
+    KvSeq seq;
+    const int s = kv_find(a.batch, a.cache.page_shift, token, first, seq, [](int n) { return n; });
     if (s < 0)
         return; // a row behind the last sequence
-    const KvSeq seq = kv_seq(a.batch, a.cache.page_shift, s);
     const int at = seq.len - seq.n + (token - first);
     const int pos = a.positions ? a.positions[token] : at;
 
@@ -90,7 +89,7 @@ __global__ void __launch_bounds__(ROPE_THREADS) k_rope_kv(RopeArgs a)
     for (int j = 0; j < ROPE_FLOATS / 4 / ROPE_THREADS; ++j) {
         const int i = tid + ROPE_THREADS * j;
         if (i < n4)
-            *(float4 *)(x + 4 * i) = val[j];
+            *(f4 *)(x + 4 * i) = val[j];
     }
     __syncthreads();
     if (a.q_norm || a.k_norm) {
@@ -99,7 +98,7 @@ __global__ void __launch_bounds__(ROPE_THREADS) k_rope_kv(RopeArgs a)
         if (h < heads) {
             float sum = 0.0f;
             for (int e = 4 * (tid & 15); e < D; e += 64) {
-                const float4 v = *(const float4 *)(x + h * D + e);
+                const f4 v = *(const f4 *)(x + h * D + e);
                 sum += (v.x * v.x + v.y * v.y) + (v.z * v.z + v.w * v.w);
             }
             sum = dpp_add<0xb1, 0xf>(sum);  // quad_perm [1,0,3,2]
@@ -156,16 +155,16 @@ __global__ void __launch_bounds__(ROPE_THREADS) k_rope_kv(RopeArgs a)
                 } else {
 #pragma unroll
                     for (int u = 0; u < 8; ++u) {
-                        const int e = e0 + u;
-                        if (e >= a.rot)
-                            continue;
+                        // (behind the rotated part: the first pair's partner, not used)
+                        const bool in = e0 + u < a.rot;
+                        const int e = in ? e0 + u : 0;
                         const bool left = a.interleaved ? e % 2 == 0 : e < R2;
                         const int other = a.interleaved ? e ^ 1 : left ? e + R2 : e - R2;
                         const float2 c = cs[a.interleaved ? e / 2 : left ? e : e - R2];
                         float z = xh[other];
                         if (w)
                             z = z * f * w[other];
-                        y[u] = y[u] * c.x + (left ? -z : z) * c.y;
+                        y[u] = in ? y[u] * c.x + (left ? -z : z) * c.y : y[u];
                     }
                 }
             }

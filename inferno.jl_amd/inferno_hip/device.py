@@ -384,26 +384,23 @@ def _opt(t, dtype, what, least=0):
     return p
 
 
-class _on:
-    """The device of `t` made current for a call (the library launches on the
-    current device); free where it is already."""
-
-    def __init__(self, t: torch.Tensor):
-        self.guard = None if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
-def _same_device(ref: torch.Tensor, *others):
+def _launch(device: int, stream, fn, *args):
+    """fn(*args, stream) with the tensors' device current (the library launches
+    there), on `stream` or that device's current one."""
+    if device == _current_device():
+        check(fn(*args, _stream(stream)))
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, _stream(stream)))
+
+
+def _same_device(index: int, *others):
     for t in others:
-        if t is not None and t.device != ref.device:
-            raise _invalid(f"tensors on {ref.device} and {t.device}")
+        if t is not None and t.get_device() != index:
+            raise _invalid(f"tensors on devices {index} and {t.get_device()}")
 
 
 def _held(stream, *tensors):
@@ -432,16 +429,20 @@ class KVCache:
                 raise _invalid(f"a page of {what} must be contiguous")
         if k.shape != v.shape or k.dtype != v.dtype or k.stride()[:-3] != v.stride()[:-3]:
             raise _invalid("k and v differ in shape, type or strides")
-        _same_device(k, v)
+        _same_device(k.get_device(), v)
         self.k, self.v = k, v
+        self.layers_dim = k.dim() == 5
         self.layers = k.shape[0] if k.dim() == 5 else 1
         self.layer_stride = k.stride(0) if k.dim() == 5 else 0
         self.pages, self.kv_heads, self.page_size, self.head_dim = k.shape[-4:]
-        self.dtype, self.device = k.dtype, k.device
+        self.dtype, self.device, self.index = k.dtype, k.device, k.get_device()
         stride = k.stride(-4) if self.pages > 1 else self.kv_heads * self.page_size * self.head_dim
         self.struct = _lib.KVCacheStruct(k.data_ptr(), v.data_ptr(), _KV_TYPES[k.dtype], self.pages, self.page_size,
                                          self.kv_heads, self.head_dim, stride)
         self.ref = C.byref(self.struct)
+
+    def get_device(self) -> int:
+        return self.index
 
     def layer(self, i: int) -> "KVCache":
         """Layer i's cache, which rope_kv and attn_paged take."""
@@ -460,12 +461,16 @@ class KVBatch:
             _ptr(t, torch.int32, what)
         if q_starts.numel() != n + 1 or page_table.dim() != 2 or page_table.shape[0] != n:
             raise _invalid("q_starts has sequences + 1 entries, page_table a row a sequence")
-        _same_device(q_starts, kv_lens, page_table)
+        self.index = kv_lens.get_device()
+        _same_device(self.index, q_starts, page_table)
         self.q_starts, self.kv_lens, self.page_table, self.tokens = q_starts, kv_lens, page_table, tokens
-        self.device = kv_lens.device
+        self.sequences = n
         self.struct = _lib.KVBatchStruct(q_starts.data_ptr(), kv_lens.data_ptr(), page_table.data_ptr(), n,
                                          page_table.shape[1], tokens)
         self.ref = C.byref(self.struct)
+
+    def get_device(self) -> int:
+        return self.index
 
 
 def rope_turns(rot_dim: int, base: float, scaling: str = "none", factor: float = 1.0, original: int = 0,
@@ -485,13 +490,13 @@ def _heads(t: torch.Tensor, what, tokens, heads, dim):
     """Row stride of a tokens x heads x dim view whose rows are contiguous."""
     if not t.is_cuda or t.dtype != torch.float32:
         raise _invalid(f"{what} must be a float32 device tensor")
-    if t.dim() != 3 or t.shape[0] != tokens or t.shape[2] != dim or (heads is not None and t.shape[1] != heads):
-        raise _invalid(f"{what} is {tuple(t.shape)}, not {tokens} x {heads} x {dim}")
-    if t.shape[1] == 0:
-        raise _invalid(f"{what} has no heads")
-    if tokens and (t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != dim)):
+    shape = t.shape
+    if len(shape) != 3 or shape[0] != tokens or shape[2] != dim or shape[1] != (heads or shape[1]) or shape[1] == 0:
+        raise _invalid(f"{what} is {tuple(shape)}, not {tokens} x {heads or 'heads'} x {dim}")
+    step, head, one = t.stride()
+    if tokens and (one != 1 or (head != dim and shape[1] > 1)):
         raise _invalid(f"the heads of a token of {what} must be contiguous")
-    return t.stride(0) if tokens > 1 else t.shape[1] * dim
+    return step if tokens > 1 else shape[1] * dim
 
 
 def rope_kv(q: torch.Tensor, k, v, turns: torch.Tensor, cache: KVCache, batch: KVBatch, layout: str = "half",
@@ -503,28 +508,29 @@ def rope_kv(q: torch.Tensor, k, v, turns: torch.Tensor, cache: KVCache, batch: K
     part of a head is 2 * turns.numel() values.  Returns q (out_dtype, default
     fp32)."""
     T, D = batch.tokens, cache.head_dim
-    if cache.k.dim() != 4:
+    if cache.layers_dim:
         raise _invalid("pass one layer of the cache (cache.layer(i))")
     if layout not in _lib.ROPE_LAYOUT:
         raise _invalid(f"unknown layout {layout}")
     if (k is None) != (v is None):
         raise _invalid("k and v go together")
-    qs = _heads(q, "q", T, None, D)
-    ks = _heads(k, "k", T, cache.kv_heads, D) if k is not None else 0
-    vs = _heads(v, "v", T, cache.kv_heads, D) if v is not None else 0
-    _same_device(q, k, v, turns, cache, batch, q_norm, k_norm, positions, out, flags)
-    with _on(q):
-        if out is None:
-            out = torch.empty(q.shape, dtype=out_dtype or torch.float32, device=q.device)
-            _held(stream, out)
-        if out.dtype not in _ACT_TYPES or out.shape != q.shape or (out_dtype is not None and out.dtype != out_dtype):
-            raise _invalid("out must have q's shape and be fp32, fp16 or bf16")
-        check(lib().ihip_rope_kv_dev(
-            q.data_ptr(), qs, None if k is None else k.data_ptr(), ks, None if v is None else v.data_ptr(), vs,
-            q.shape[1], _opt(q_norm, torch.float32, "q_norm", D), _opt(k_norm, torch.float32, "k_norm", D), eps,
+    qs, kp, ks, vp, vs = _heads(q, "q", T, None, D), None, 0, None, 0
+    if k is not None:
+        kp, ks, vp, vs = k.data_ptr(), _heads(k, "k", T, cache.kv_heads, D), v.data_ptr(), _heads(v, "v", T, cache.kv_heads, D)
+    dev = q.get_device()
+    _same_device(dev, k, v, turns, cache, batch, q_norm, k_norm, positions, out, flags)
+    if out is None:
+        out = torch.empty(q.shape, dtype=out_dtype or torch.float32, device=q.device)
+        _held(stream, out)
+    elif out.shape != q.shape or out.dtype != (out_dtype or out.dtype):
+        raise _invalid("out must have q's shape and the type asked for")
+    if out.dtype not in _ACT_TYPES:
+        raise _invalid("out must be fp32, fp16 or bf16")
+    _launch(dev, stream, lib().ihip_rope_kv_dev, q.data_ptr(), qs, kp, ks, vp, vs, q.shape[1],
+            _opt(q_norm, torch.float32, "q_norm", D), _opt(k_norm, torch.float32, "k_norm", D), eps,
             _ptr(turns, torch.float64, "turns"), 2 * turns.numel(), _lib.ROPE_LAYOUT[layout], mscale,
             _opt(positions, torch.int32, "positions", T), _ptr(out, None, "out"), _ACT_TYPES[out.dtype], cache.ref,
-            batch.ref, _opt(flags, torch.int32, "flags", 1), _stream(stream)))
+            batch.ref, _opt(flags, torch.int32, "flags", 1))
     return out
 
 
@@ -542,31 +548,30 @@ def attn_paged(q: torch.Tensor, cache: KVCache, batch: KVBatch, scale: float = N
     q: tokens x q_heads x head_dim, fp32 or the cache's type, which out has too;
     scale defaults to head_dim ** -0.5.  Rows of out behind the last sequence's
     are not written."""
-    D = cache.head_dim
-    if cache.k.dim() != 4:
+    T, D = batch.tokens, cache.head_dim
+    if cache.layers_dim:
         raise _invalid("pass one layer of the cache (cache.layer(i))")
-    if q.dim() != 3 or q.shape[0] != batch.tokens or q.shape[2] != D:
-        raise _invalid(f"q is {tuple(q.shape)}, not {batch.tokens} x heads x {D}")
-    if q.dtype not in _ACT_TYPES:
+    shape, act = q.shape, _ACT_TYPES.get(q.dtype)
+    if len(shape) != 3 or shape[0] != T or shape[2] != D:
+        raise _invalid(f"q is {tuple(shape)}, not {T} x heads x {D}")
+    if act is None:
         raise _invalid(f"q must be fp32, fp16 or bf16, got {q.dtype}")
-    H = q.shape[1]
-    _same_device(q, cache, batch, prefix_lens, slopes, out, workspace, flags)
-    with _on(q):
-        if out is None:
-            out = torch.empty_like(q)
-            _held(stream, out)
-        elif out.dtype != q.dtype or out.shape != q.shape:
-            raise _invalid("out must have q's shape and type")
-        if workspace is None:
-            workspace = attn_workspace(H, cache, batch, q.dtype)
-            if workspace is not None:
-                _held(stream, workspace)
-        check(lib().ihip_attn_paged_dev(
-            _ptr(q, None, "q"), _ACT_TYPES[q.dtype], _ptr(out, None, "out"), H, D ** -0.5 if scale is None else scale,
-            softcap, window, _opt(prefix_lens, torch.int32, "prefix_lens", batch.kv_lens.numel()),
-            _opt(slopes, torch.float32, "slopes", H), cache.ref, batch.ref, _opt(flags, torch.int32, "flags", 1),
-            None if workspace is None else _ptr(workspace, torch.uint8, "workspace"),
-            0 if workspace is None else workspace.numel(), _stream(stream)))
+    H, dev = shape[1], q.get_device()
+    _same_device(dev, cache, batch, prefix_lens, slopes, out, workspace, flags)
+    if out is None:
+        out = torch.empty_like(q)
+        _held(stream, out)
+    elif out.dtype != q.dtype or out.shape != shape:
+        raise _invalid("out must have q's shape and type")
+    if workspace is None:
+        workspace = attn_workspace(H, cache, batch, q.dtype)
+        if workspace is not None:
+            _held(stream, workspace)
+    _launch(dev, stream, lib().ihip_attn_paged_dev, _ptr(q, None, "q"), act, _ptr(out, None, "out"), H,
+            D ** -0.5 if scale is None else scale, softcap, window,
+            _opt(prefix_lens, torch.int32, "prefix_lens", batch.sequences), _opt(slopes, torch.float32, "slopes", H),
+            cache.ref, batch.ref, _opt(flags, torch.int32, "flags", 1), _opt(workspace, torch.uint8, "workspace"),
+            0 if workspace is None else workspace.numel())
     return out
 
 
@@ -580,19 +585,18 @@ def kv_fork(table: torch.Tensor, lens: torch.Tensor, parents: torch.Tensor, refs
         _ptr(t, torch.int32, what)
     if table.dim() != 2 or lens.numel() != table.shape[0]:
         raise _invalid("table has a row and lens an entry a sequence")
-    _same_device(table, lens, parents, refs, flags)
+    dev = table.get_device()
+    _same_device(dev, lens, parents, refs, flags)
     n, width = parents.numel(), table.shape[1]
-    with _on(table):
-        new = torch.empty(n, width, dtype=torch.int32, device=table.device)
-        new_lens = torch.empty(n, dtype=torch.int32, device=table.device)
-        copies = torch.empty(n, 2, dtype=torch.int32, device=table.device)
-        scratch = torch.empty(n, dtype=torch.int32, device=table.device)
-        _held(stream, new, new_lens, copies, scratch)
-        check(lib().ihip_kv_fork_dev(table.data_ptr(), lens.data_ptr(), table.shape[0], parents.data_ptr(), n, room,
-                                     width, page_size, refs.numel(), refs.data_ptr(), new.data_ptr(),
-                                     new_lens.data_ptr(), copies.data_ptr(), scratch.data_ptr(),
-                                     _opt(flags, torch.int32, "flags", 1), _stream(stream)))
-    return new, new_lens, copies
+    # the tables, their lengths, the copies and the scratch
+    new, ints = (torch.empty(n, width, dtype=torch.int32, device=table.device),
+                 torch.empty(4 * n, dtype=torch.int32, device=table.device))
+    _held(stream, new, ints)
+    p = ints.data_ptr()
+    _launch(dev, stream, lib().ihip_kv_fork_dev, table.data_ptr(), lens.data_ptr(), table.shape[0], parents.data_ptr(), n,
+            room, width, page_size, refs.numel(), refs.data_ptr(), new.data_ptr(), p, p + 4 * n, p + 12 * n,
+            _opt(flags, torch.int32, "flags", 1))
+    return new, ints[:n], ints[n:3 * n].view(n, 2)
 
 
 def kv_compact(table: torch.Tensor, refs: torch.Tensor, flags=None, stream=None):
@@ -600,17 +604,16 @@ def kv_compact(table: torch.Tensor, refs: torch.Tensor, flags=None, stream=None)
     and refs change in place; returns the moves (pages // 2 pairs, -1 behind the
     last) and their number, both for kv_copy."""
     _ptr(table, torch.int32, "table"), _ptr(refs, torch.int32, "refs")
-    _same_device(table, refs, flags)
-    pages = refs.numel()
-    with _on(table):
-        copies = torch.empty(pages // 2, 2, dtype=torch.int32, device=table.device)
-        moved = torch.empty(1, dtype=torch.int32, device=table.device)
-        scratch = torch.empty(pages, dtype=torch.int32, device=table.device)
-        _held(stream, copies, moved, scratch)
-        check(lib().ihip_kv_compact_dev(table.data_ptr(), table.numel(), refs.data_ptr(), pages, copies.data_ptr(),
-                                        moved.data_ptr(), scratch.data_ptr(), _opt(flags, torch.int32, "flags", 1),
-                                        _stream(stream)))
-    return copies, moved
+    dev, pages = table.get_device(), refs.numel()
+    _same_device(dev, refs, flags)
+    n = pages // 2
+    # the moves, the scratch and the moves' number
+    ints = torch.empty(2 * n + pages + 1, dtype=torch.int32, device=table.device)
+    _held(stream, ints)
+    p = ints.data_ptr()
+    _launch(dev, stream, lib().ihip_kv_compact_dev, table.data_ptr(), table.numel(), refs.data_ptr(), pages, p,
+            p + 4 * (2 * n + pages), p + 8 * n, _opt(flags, torch.int32, "flags", 1))
+    return ints[:2 * n].view(n, 2), ints[2 * n + pages:]
 
 
 def kv_copy(cache: KVCache, copies: torch.Tensor, count: torch.Tensor = None, flags=None, stream=None):
@@ -619,8 +622,8 @@ def kv_copy(cache: KVCache, copies: torch.Tensor, count: torch.Tensor = None, fl
     *count on."""
     if copies.dim() != 2 or copies.shape[1] != 2:
         raise _invalid("copies is pairs x 2")
-    _same_device(cache.k, copies, count, flags)
-    with _on(copies):
-        check(lib().ihip_kv_copy_dev(cache.ref, cache.layers, cache.layer_stride, _ptr(copies, torch.int32, "copies"),
-                                     copies.shape[0], _opt(count, torch.int32, "count", 1),
-                                     _opt(flags, torch.int32, "flags", 1), _stream(stream)))
+    dev = copies.get_device()
+    _same_device(dev, cache, count, flags)
+    _launch(dev, stream, lib().ihip_kv_copy_dev, cache.ref, cache.layers, cache.layer_stride,
+            _ptr(copies, torch.int32, "copies"), copies.shape[0], _opt(count, torch.int32, "count", 1),
+            _opt(flags, torch.int32, "flags", 1))
