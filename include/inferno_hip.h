@@ -480,7 +480,11 @@ int ihip_rope_kv_dev(const float *q, int64_t q_stride, const float *k, int64_t k
  * F32: scores and outputs carry fp32's accuracy.  F16 / BF16: the softmax
  * weights are rounded to that type (the sums stay fp32).
  * workspace: ihip_attn_paged_scratch_bytes bytes, 16-byte aligned, NULL where
- * that is 0; calls that share it must not overlap on the GPU. */
+ * that is 0.  The caller fills its first IHIP_ATTN_COUNT_BYTES with zeros once,
+ * before its first call; every call leaves them zero again, so that it serves any
+ * number of calls of any sizes that it is large enough for.  Calls that share it
+ * must not overlap on the GPU. */
+#define IHIP_ATTN_COUNT_BYTES 16384
 int ihip_attn_paged_dev(const void *q, int q_type, void *out, int q_heads, float scale,
                         float softcap, int window, const int32_t *prefix_lens, const float *slopes,
                         const ihip_kv_cache *cache, const ihip_kv_batch *batch, uint32_t *flags,

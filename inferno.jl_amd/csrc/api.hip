@@ -1668,7 +1668,7 @@ int ihip_attn_paged_dev(const void *q, int q_type, void *out, int q_heads, float
     }
     a.q = q, a.out = out, a.act = q_type, a.q_heads = q_heads, a.group = q_heads / a.cache.heads;
     a.scale = scale, a.cap = softcap, a.window = window, a.prefix = prefix_lens, a.slopes = slopes;
-    a.flags = flags, a.part = (float *)workspace;
+    a.flags = flags, a.count = (uint32_t *)workspace, a.part = (float *)workspace + kAttnCounts;
     hipError_t e = launch_attn(a, p, (hipStream_t)stream);
     if (e != hipSuccess)
         return fail(IHIP_ERR_HIP, "attention launch failed: %s", hipGetErrorString(e));

@@ -143,6 +143,19 @@ __device__ __forceinline__ float halves_sum(float v)
     return __uint_as_float(a[0]) + __uint_as_float(a[1]);
 }
 
+// Two floats passed between workgroups of different XCDs, whose caches do not
+// follow each other: relaxed atomics of the whole device, which go to memory.
+__device__ __forceinline__ void put_shared(uint64_t *p, float a, float b)
+{
+    __hip_atomic_store(p, (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a), __ATOMIC_RELAXED,
+                       __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ f2 get_shared(const uint64_t *p)
+{
+    const uint64_t v = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return f2{__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32))};
+}
+
 // What a workgroup works on: a tile of rows of one sequence and KV head, and
 // the part of its keys.
 struct Tile {
@@ -151,7 +164,8 @@ struct Tile {
     int first, last;         // cache positions of the tile's first and last token
     int len, prefix;         // keys there are; keys every row sees
     int lo, hi;              // keys to look at (lo a multiple of the step); lo >= hi: none
-    int split;
+    int split, parts;        // the part of its keys, of how many that have any (1 at least)
+    int index;               // its place among all tiles and heads
     const int32_t *table;
 };
 
@@ -188,6 +202,8 @@ __device__ __forceinline__ bool find_tile(const AttnArgs &a, int tiles, int leas
     // splits there may be would not reach the end
     const int keys = max(0, hi - lo);
     const int per = max(least, (int)(((int64_t)keys + splits - 1) / splits + 127) & ~127);
+    t.parts = max(1, (int)(((int64_t)keys + per - 1) / per));
+    t.index = want * a.cache.heads + t.head;
     const int64_t from = (int64_t)lo + (int64_t)t.split * per;
     t.lo = (int)min(from, (int64_t)hi);
     t.hi = (int)min(from + per, (int64_t)hi);
@@ -308,7 +324,8 @@ constexpr int ar_wave_lds()
 // A workgroup's 4 waves walk the keys of its part 32 at a time, each its own
 // steps (no shared data, no barrier): K from HBM into the matrix operand's
 // registers, V by direct copies into LDS of the wave's own, both one step
-// ahead and their page ids two; the waves' sums are joined at the end.
+// ahead and their page ids two; the waves' sums are joined at the end, and the
+// parts' by the workgroup that ends last.
 template <typename C, int PARTS, int DP, bool GEN>
 __global__ void __launch_bounds__(64 * AR_WAVES, DP == 256 ? 1 : 2)
 k_attn_rows(AttnArgs a, int tiles, int least, int splits)
@@ -320,12 +337,13 @@ k_attn_rows(AttnArgs a, int tiles, int least, int splits)
     constexpr int TILE = AR_KEYS * DP * 2;
     __shared__ __attribute__((aligned(16))) uint8_t lds[AR_WAVES * ar_wave_lds<DP>()];
     __shared__ float lds_m[AR_WAVES][AR_ROWS], lds_l[AR_WAVES][AR_ROWS];
+    __shared__ int lds_last;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, g = lane >> 4;
     const int D = a.cache.dim;
     Tile t;
-    if (!find_tile<AR_ROWS, AR_KEYS>(a, tiles, least, splits, blockIdx.x, t))
+    if (!find_tile<AR_ROWS, AR_KEYS>(a, tiles, least, splits, blockIdx.x, t) || t.split >= t.parts)
         return;
 
     uint8_t *const mine = lds + wave * ar_wave_lds<DP>();
@@ -563,8 +581,22 @@ k_attn_rows(AttnArgs a, int tiles, int least, int splits)
     }
     __syncthreads();
     const int64_t rows_all = (int64_t)a.batch.tokens * a.q_heads;
-    float *const ml = a.part + (int64_t)splits * rows_all * D;
-    for (int e = tid; e < t.rows * (D / 4); e += 64 * AR_WAVES) {
+    auto row_of = [&](int r) {
+        const int rr = t.row0 + r;
+        return (int64_t)(t.start + rr / a.group) * a.q_heads + t.head * a.group + rr % a.group;
+    };
+    auto finish = [&](int r, int d, f4 v, float sum) {
+        v = sum == 0.0f ? f4{} : v * (1.0f / sum);
+        if constexpr (PARTS == 1)
+            *(V4 *)((T *)a.out + row_of(r) * D + d) = __builtin_convertvector(v, V4);
+        else
+            *(f4 *)((float *)a.out + row_of(r) * D + d) = v;
+    };
+    // a part's rows lie in a.part, their maxima and sums behind
+    uint64_t *const part_o = (uint64_t *)a.part;
+    uint64_t *const part_ml = part_o + (int64_t)splits * rows_all * D / 2;
+    const int items = t.rows * (D / 4);
+    for (int e = tid; e < items; e += 64 * AR_WAVES) {
         const int r = e / (D / 4), d = 4 * (e % (D / 4));
         float top = kNone;
 #pragma unroll
@@ -579,23 +611,90 @@ k_attn_rows(AttnArgs a, int tiles, int least, int splits)
             sum += lds_l[w][r] * f;
             v += x * f;
         }
-        const int rr = t.row0 + r;
-        const int64_t to = (int64_t)(t.start + rr / a.group) * a.q_heads + t.head * a.group + rr % a.group;
-        if (splits > 1) {
-            if (sum != 0.0f) // (NaN too; a part without keys is its sum alone)
-                *(f4 *)(a.part + ((int64_t)t.split * rows_all + to) * D + d) = v;
-            if (d == 0) {
-                ml[2 * (t.split * rows_all + to)] = top;
-                ml[2 * (t.split * rows_all + to) + 1] = sum;
-            }
+        if (t.parts == 1) {
+            finish(r, d, v, sum);
         } else {
-            const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
-            v = sum == 0.0f ? f4{} : v * f;
-            if constexpr (PARTS == 1)
-                *(V4 *)((T *)a.out + to * D + d) = __builtin_convertvector(v, V4);
-            else
-                *(f4 *)((float *)a.out + to * D + d) = v;
+            const int64_t to = t.split * rows_all + row_of(r);
+            put_shared(part_o + (to * D + d) / 2, v.x, v.y);
+            put_shared(part_o + (to * D + d) / 2 + 1, v.z, v.w);
+            if (d == 0)
+                put_shared(part_ml + to, top, sum);
         }
+    }
+    if (t.parts == 1)
+        return;
+
+    // The workgroup that is the last of its tile's to come here joins the parts, in
+    // their order.  Everything that passes between workgroups goes through memory
+    // that all of the chip sees (put_shared, get_shared); a workgroup counts itself
+    // when its stores have arrived, and the last one sets the count to 0 again.
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (tid == 0)
+        lds_last = atomicInc(a.count + t.index, (uint32_t)t.parts - 1) == (uint32_t)t.parts - 1;
+    __syncthreads();
+    if (!lds_last)
+        return;
+    // four values of a row a thread, eight parts at a time with their maxima and
+    // sums; few rows: the parts are shared among groups of threads, which are joined
+    // in the groups' order
+    constexpr int AT_ONCE = 8;
+    const int groups = max(1, 64 * AR_WAVES / items);
+    float *const lds_g = (float *)lds;
+    for (int e0 = 0; e0 < items; e0 += 64 * AR_WAVES) {
+        const int group = groups > 1 ? tid / items : 0;
+        const int e = groups > 1 ? tid - group * items : e0 + tid;
+        const bool in = group < groups && e < items;
+        const int r = in ? e / (D / 4) : 0, d = in ? 4 * (e % (D / 4)) : 0;
+        const uint64_t *const from_o = part_o + (row_of(r) * D + d) / 2, *const from_ml = part_ml + row_of(r);
+        float top = kNone, sum = 0.0f;
+        f4 v = f4{};
+        for (int p0 = AT_ONCE * group; in && p0 < t.parts; p0 += AT_ONCE * groups) {
+            f2 w[AT_ONCE], x[AT_ONCE], y[AT_ONCE];
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; ++u) {
+                const int64_t p = min(p0 + u, t.parts - 1) * rows_all;
+                w[u] = get_shared(from_ml + p);
+                x[u] = get_shared(from_o + p * D / 2);
+                y[u] = get_shared(from_o + p * D / 2 + 1);
+            }
+            float up = top;
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; ++u)
+                up = p0 + u < t.parts ? fmaxf(up, w[u].x) : up;
+            const float f = top == kNone ? 0.0f : exp2_fast(top - up);
+            sum *= f;
+            v *= f;
+            top = up;
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; ++u) {
+                const float g = p0 + u >= t.parts || w[u].x == kNone ? 0.0f : exp2_fast(w[u].x - up);
+                if (p0 + u < t.parts) { // (a weight 0 times NaN stays NaN)
+                    sum += w[u].y * g;
+                    v += f4{x[u].x, x[u].y, y[u].x, y[u].y} * g;
+                }
+            }
+        }
+        if (groups > 1) {
+            if (in && group > 0) {
+                *(f4 *)(lds_g + 8 * tid) = v;
+                *(f2 *)(lds_g + 8 * tid + 4) = f2{top, sum};
+            }
+            __syncthreads();
+            if (!in || group > 0)
+                return;
+            for (int q = 1; q < groups; ++q) {
+                const f4 v2 = *(const f4 *)(lds_g + 8 * (tid + q * items));
+                const f2 w2 = *(const f2 *)(lds_g + 8 * (tid + q * items) + 4);
+                const float up = fmaxf(top, w2.x);
+                const float f = top == kNone ? 0.0f : exp2_fast(top - up), g = w2.x == kNone ? 0.0f : exp2_fast(w2.x - up);
+                sum = sum * f + w2.y * g;
+                v = v * f + v2 * g;
+                top = up;
+            }
+        }
+        if (in)
+            finish(r, d, v, sum);
     }
 }
 
@@ -1076,7 +1175,7 @@ hipError_t start_dim(const AttnArgs &a, const AttnPlan &p, hipStream_t s)
         start_gen<C, PARTS, true>(a, p, s);
     else
         start_gen<C, PARTS, false>(a, p, s);
-    if (p.splits > 1) {
+    if (p.splits > 1 && p.rows == AC_ROWS) {
         const int64_t rows = (int64_t)a.batch.tokens * a.q_heads;
         if (p.splits <= 16)
             hipLaunchKernelGGL((k_attn_join<C, PARTS, 64>), dim3((uint32_t)((rows + 3) / 4)), dim3(256), 0, s, a, p.splits);
@@ -1103,8 +1202,8 @@ AttnPlan attn_plan(int q_heads, int kv_heads, int dim, int sequences, int tokens
     if (p.rows == AR_ROWS) {
         // a sequence alone fills the chip once; of many, of which some are longer
         // than others, the parts stay short enough to even out
-        p.least = units <= 32 ? 128 : units <= 64 ? 256 : 512;
-        want = (256 * std::min<int64_t>(some, 16) + units - 1) / units;
+        p.least = units <= 32 ? 128 : units <= 128 ? 256 : 512;
+        want = units >= kAttnCounts ? 1 : (256 * std::min<int64_t>(some, 16) + units - 1) / units;
     } else {
         // tiles that fill the chip are not split: joining would cost more
         p.least = 256;
@@ -1118,7 +1217,8 @@ AttnPlan attn_plan(int q_heads, int kv_heads, int dim, int sequences, int tokens
     // (512 tiles of a 2048-token prompt: 65 us against 77); of many, two
     // workgroups a CU come further (4096 tokens: 174 us against 200).
     p.halves = units * p.splits <= 512;
-    p.bytes = p.splits > 1 ? (size_t)p.splits * tokens * q_heads * (dim + 2) * 4 : 0;
+    // (with 4096 tiles and heads or more nothing is split: their counts are enough)
+    p.bytes = p.splits > 1 ? 4 * (size_t)kAttnCounts + (size_t)p.splits * tokens * q_heads * (dim + 2) * 4 : 0;
     return p;
 }
 

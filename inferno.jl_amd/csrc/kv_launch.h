@@ -39,8 +39,12 @@ struct AttnArgs {
     KvCache cache;
     KvBatch batch;
     uint32_t *flags;
+    uint32_t *count; // parts of each tile that have ended (0 between calls)
     float *part; // partial rows, then their maxima and sums, of every split
 };
+// Counts in front of the workspace, for calls of all sizes: its place does not
+// depend on a call's.
+constexpr int kAttnCounts = 4096;
 // How a batch of these sizes is launched: it depends on nothing else, so that
 // the workspace can be sized before the lengths are known.
 struct AttnPlan {
@@ -49,7 +53,7 @@ struct AttnPlan {
     int splits;  // parts of a tile's keys at most
     int least;   // keys of a part at least
     bool halves; // whether two halves of a workgroup share a tile's keys
-    size_t bytes; // workspace
+    size_t bytes; // workspace: the counts, then the parts
 };
 // window: the window where there is one and no prefix reaches behind it, else 0
 // (which never needs less workspace).

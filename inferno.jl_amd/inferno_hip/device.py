@@ -536,9 +536,10 @@ def rope_kv(q: torch.Tensor, k, v, turns: torch.Tensor, cache: KVCache, batch: K
 
 def attn_workspace(q_heads: int, cache: KVCache, batch: KVBatch, dtype=torch.float32):
     """The workspace of attn_paged for a batch of these sizes (for q of `dtype`),
-    or None where it needs none.  Calls that share one must not overlap."""
+    or None where it needs none.  It starts as zeros, and every call leaves what
+    has to be zero so.  Calls that share one must not overlap."""
     n = lib().ihip_attn_paged_scratch_bytes(_ACT_TYPES[dtype], q_heads, cache.ref, batch.ref)
-    return torch.empty(n, dtype=torch.uint8, device=cache.device) if n else None
+    return torch.zeros(n, dtype=torch.uint8, device=cache.device) if n else None
 
 
 def attn_paged(q: torch.Tensor, cache: KVCache, batch: KVBatch, scale: float = None, softcap: float = 0.0,

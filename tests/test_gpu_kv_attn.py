@@ -267,3 +267,22 @@ def test_offsets_past_32_bits():
     got = D.attn_paged(q.cuda(), D.KVCache(kk, vv), D.KVBatch(ints(starts), ints(lens), ints([far]), 1))
     # (another capacity may split the keys otherwise: the same to rounding)
     assert float((got.cpu() - want).abs().max()) < 1e-5
+
+
+def test_one_workspace_serves_calls_of_all_sizes():
+    """The counts in its front are zero again after every call, whatever the next one's sizes."""
+    from inferno_hip import device as D
+    from inferno_hip import _lib
+    cases = [build(20, [1], [3000], 8, 2, 64, 16, F32, F16), build(21, [1] * 9, [900] * 9, 8, 8, 64, 16, F32, F16),
+             build(22, [40], [700], 8, 2, 64, 16, F32, F16), build(23, [2], [2000], 4, 1, 64, 16, F32, F16)]
+    made = []
+    for q, k, v, starts, lens, table in cases:
+        cache = D.KVCache(k.cuda(), v.cuda())
+        batch = D.KVBatch(ints(starts), ints(lens), ints(table), q.shape[0])
+        made.append((q.cuda(), cache, batch, D.attn_paged(q.cuda(), cache, batch)))
+    n = max(_lib.lib().ihip_attn_paged_scratch_bytes(_lib.F32, q.shape[1], c.ref, b.ref) for q, c, b, _ in made)
+    ws = torch.zeros(n, dtype=torch.uint8, device="cuda")
+    for i in (0, 1, 2, 3, 1, 0, 3, 2, 0):
+        q, cache, batch, want = made[i]
+        assert torch.equal(D.attn_paged(q, cache, batch, workspace=ws), want)
+        assert not bool(ws[:16384].any())
