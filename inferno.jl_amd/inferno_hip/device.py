@@ -374,33 +374,40 @@ def _invalid(msg: str):
     return IHIPArgumentError(_lib.IHIP_ERR_INVALID, msg)
 
 
-def _opt(t, dtype, what, least=0):
-    """Pointer of an optional contiguous device tensor of at least `least` values."""
+def _at(t, dtype, what, dev, least=0):
+    """Pointer of a contiguous tensor of `dtype` and at least `least` values on device
+    `dev` (None: none)."""
     if t is None:
         return None
-    p = _ptr(t, dtype, what)
-    if t.numel() < least:
+    if t.get_device() != dev:
+        raise _invalid(f"{what} must be on device {dev}, not {t.device}")
+    if t.dtype != dtype or not t.is_contiguous():
+        raise _invalid(f"{what} must be contiguous {dtype}, got {t.dtype}")
+    if least and t.numel() < least:
         raise _invalid(f"{what} holds {t.numel()} values, needs {least}")
-    return p
+    return t.data_ptr()
 
 
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
-def _launch(device: int, stream, fn, *args):
+def _launch(dev: int, stream, fn, *args):
     """fn(*args, stream) with the tensors' device current (the library launches
     there), on `stream` or that device's current one."""
-    if device == _current_device():
-        check(fn(*args, _stream(stream)))
+    if dev == _current_device():
+        rc = fn(*args, stream.cuda_stream if stream is not None else _raw_current_stream(dev) if _raw_current_stream
+                else torch.cuda.current_stream().cuda_stream)
     else:
-        with torch.cuda.device(device):
-            check(fn(*args, _stream(stream)))
+        with torch.cuda.device(dev):
+            rc = fn(*args, _stream(stream))
+    if rc:
+        check(rc)
 
 
-def _same_device(index: int, *others):
+def _same_device(dev: int, *others):
     for t in others:
-        if t is not None and t.get_device() != index:
-            raise _invalid(f"tensors on devices {index} and {t.get_device()}")
+        if t.index != dev:
+            raise _invalid(f"a cache or batch on device {t.index}, tensors on {dev}")
 
 
 def _held(stream, *tensors):
@@ -429,7 +436,8 @@ class KVCache:
                 raise _invalid(f"a page of {what} must be contiguous")
         if k.shape != v.shape or k.dtype != v.dtype or k.stride()[:-3] != v.stride()[:-3]:
             raise _invalid("k and v differ in shape, type or strides")
-        _same_device(k.get_device(), v)
+        if k.device != v.device:
+            raise _invalid("k and v are on different devices")
         self.k, self.v = k, v
         self.layers_dim = k.dim() == 5
         self.layers = k.shape[0] if k.dim() == 5 else 1
@@ -440,9 +448,6 @@ class KVCache:
         self.struct = _lib.KVCacheStruct(k.data_ptr(), v.data_ptr(), _KV_TYPES[k.dtype], self.pages, self.page_size,
                                          self.kv_heads, self.head_dim, stride)
         self.ref = C.byref(self.struct)
-
-    def get_device(self) -> int:
-        return self.index
 
     def layer(self, i: int) -> "KVCache":
         """Layer i's cache, which rope_kv and attn_paged take."""
@@ -456,21 +461,16 @@ class KVBatch:
     graph."""
 
     def __init__(self, q_starts: torch.Tensor, kv_lens: torch.Tensor, page_table: torch.Tensor, tokens: int):
-        n = kv_lens.numel()
-        for t, what in ((q_starts, "q_starts"), (kv_lens, "kv_lens"), (page_table, "page_table")):
-            _ptr(t, torch.int32, what)
+        n, self.index = kv_lens.numel(), kv_lens.get_device()
+        for t, what in ((kv_lens, "kv_lens"), (q_starts, "q_starts"), (page_table, "page_table")):
+            _ptr(t, torch.int32, what), _at(t, torch.int32, what, self.index)
         if q_starts.numel() != n + 1 or page_table.dim() != 2 or page_table.shape[0] != n:
             raise _invalid("q_starts has sequences + 1 entries, page_table a row a sequence")
-        self.index = kv_lens.get_device()
-        _same_device(self.index, q_starts, page_table)
         self.q_starts, self.kv_lens, self.page_table, self.tokens = q_starts, kv_lens, page_table, tokens
         self.sequences = n
         self.struct = _lib.KVBatchStruct(q_starts.data_ptr(), kv_lens.data_ptr(), page_table.data_ptr(), n,
                                          page_table.shape[1], tokens)
         self.ref = C.byref(self.struct)
-
-    def get_device(self) -> int:
-        return self.index
 
 
 def rope_turns(rot_dim: int, base: float, scaling: str = "none", factor: float = 1.0, original: int = 0,
@@ -486,17 +486,20 @@ def rope_turns(rot_dim: int, base: float, scaling: str = "none", factor: float =
     return torch.tensor(list(host), dtype=torch.float64).to(device), m.value
 
 
-def _heads(t: torch.Tensor, what, tokens, heads, dim):
-    """Row stride of a tokens x heads x dim view whose rows are contiguous."""
-    if not t.is_cuda or t.dtype != torch.float32:
-        raise _invalid(f"{what} must be a float32 device tensor")
-    shape = t.shape
-    if len(shape) != 3 or shape[0] != tokens or shape[2] != dim or shape[1] != (heads or shape[1]) or shape[1] == 0:
+def _heads(t: torch.Tensor, what, dev, tokens, heads, dim):
+    """Pointer, row stride and heads of a tokens x heads x dim fp32 view whose rows
+    are contiguous."""
+    if t.dtype != torch.float32 or t.get_device() != dev or dev < 0:
+        raise _invalid(f"{what} must be float32 on device {dev}")
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3:
+        raise _invalid(f"{what} is not tokens x heads x head_dim")
+    n, h, d = shape
+    if n != tokens or d != dim or h != (heads or h) or h == 0:
         raise _invalid(f"{what} is {tuple(shape)}, not {tokens} x {heads or 'heads'} x {dim}")
-    step, head, one = t.stride()
-    if tokens and (one != 1 or (head != dim and shape[1] > 1)):
+    if n and (stride[2] != 1 or (stride[1] != d and h > 1)):
         raise _invalid(f"the heads of a token of {what} must be contiguous")
-    return step if tokens > 1 else shape[1] * dim
+    return t.data_ptr(), stride[0] if n > 1 else h * d, h
 
 
 def rope_kv(q: torch.Tensor, k, v, turns: torch.Tensor, cache: KVCache, batch: KVBatch, layout: str = "half",
@@ -510,27 +513,32 @@ def rope_kv(q: torch.Tensor, k, v, turns: torch.Tensor, cache: KVCache, batch: K
     T, D = batch.tokens, cache.head_dim
     if cache.layers_dim:
         raise _invalid("pass one layer of the cache (cache.layer(i))")
-    if layout not in _lib.ROPE_LAYOUT:
+    how = _lib.ROPE_LAYOUT.get(layout)
+    if how is None:
         raise _invalid(f"unknown layout {layout}")
     if (k is None) != (v is None):
         raise _invalid("k and v go together")
-    qs, kp, ks, vp, vs = _heads(q, "q", T, None, D), None, 0, None, 0
-    if k is not None:
-        kp, ks, vp, vs = k.data_ptr(), _heads(k, "k", T, cache.kv_heads, D), v.data_ptr(), _heads(v, "v", T, cache.kv_heads, D)
     dev = q.get_device()
-    _same_device(dev, k, v, turns, cache, batch, q_norm, k_norm, positions, out, flags)
+    _same_device(dev, cache, batch)
+    qp, qs, H = _heads(q, "q", dev, T, None, D)
+    kp, ks, vp, vs = None, 0, None, 0
+    if k is not None:
+        kp, ks, _ = _heads(k, "k", dev, T, cache.kv_heads, D)
+        vp, vs, _ = _heads(v, "v", dev, T, cache.kv_heads, D)
     if out is None:
         out = torch.empty(q.shape, dtype=out_dtype or torch.float32, device=q.device)
         _held(stream, out)
-    elif out.shape != q.shape or out.dtype != (out_dtype or out.dtype):
-        raise _invalid("out must have q's shape and the type asked for")
-    if out.dtype not in _ACT_TYPES:
-        raise _invalid("out must be fp32, fp16 or bf16")
-    _launch(dev, stream, lib().ihip_rope_kv_dev, q.data_ptr(), qs, kp, ks, vp, vs, q.shape[1],
-            _opt(q_norm, torch.float32, "q_norm", D), _opt(k_norm, torch.float32, "k_norm", D), eps,
-            _ptr(turns, torch.float64, "turns"), 2 * turns.numel(), _lib.ROPE_LAYOUT[layout], mscale,
-            _opt(positions, torch.int32, "positions", T), _ptr(out, None, "out"), _ACT_TYPES[out.dtype], cache.ref,
-            batch.ref, _opt(flags, torch.int32, "flags", 1))
+    elif out.shape != q.shape:
+        raise _invalid("out must have q's shape")
+    kind = out.dtype
+    act = _ACT_TYPES.get(kind)
+    if act is None or (out_dtype is not None and kind != out_dtype):
+        raise _invalid("out must be fp32, fp16 or bf16, and the type asked for")
+    _launch(dev, stream, lib().ihip_rope_kv_dev, qp, qs, kp, ks, vp, vs, H,
+            _at(q_norm, torch.float32, "q_norm", dev, D), _at(k_norm, torch.float32, "k_norm", dev, D), eps,
+            _at(turns, torch.float64, "turns", dev), 2 * turns.numel(), how, mscale,
+            _at(positions, torch.int32, "positions", dev, T), _at(out, kind, "out", dev), act, cache.ref, batch.ref,
+            _at(flags, torch.int32, "flags", dev, 1))
     return out
 
 
@@ -558,21 +566,21 @@ def attn_paged(q: torch.Tensor, cache: KVCache, batch: KVBatch, scale: float = N
     if act is None:
         raise _invalid(f"q must be fp32, fp16 or bf16, got {q.dtype}")
     H, dev = shape[1], q.get_device()
-    _same_device(dev, cache, batch, prefix_lens, slopes, out, workspace, flags)
+    _same_device(dev, cache, batch)
     if out is None:
         out = torch.empty_like(q)
         _held(stream, out)
-    elif out.dtype != q.dtype or out.shape != shape:
+    elif out.shape != shape:
         raise _invalid("out must have q's shape and type")
     if workspace is None:
         workspace = attn_workspace(H, cache, batch, q.dtype)
         if workspace is not None:
             _held(stream, workspace)
-    _launch(dev, stream, lib().ihip_attn_paged_dev, _ptr(q, None, "q"), act, _ptr(out, None, "out"), H,
+    _launch(dev, stream, lib().ihip_attn_paged_dev, _at(q, q.dtype, "q", dev), act, _at(out, q.dtype, "out", dev), H,
             D ** -0.5 if scale is None else scale, softcap, window,
-            _opt(prefix_lens, torch.int32, "prefix_lens", batch.sequences), _opt(slopes, torch.float32, "slopes", H),
-            cache.ref, batch.ref, _opt(flags, torch.int32, "flags", 1), _opt(workspace, torch.uint8, "workspace"),
-            0 if workspace is None else workspace.numel())
+            _at(prefix_lens, torch.int32, "prefix_lens", dev, batch.sequences),
+            _at(slopes, torch.float32, "slopes", dev, H), cache.ref, batch.ref, _at(flags, torch.int32, "flags", dev, 1),
+            _at(workspace, torch.uint8, "workspace", dev), 0 if workspace is None else workspace.numel())
     return out
 
 
@@ -582,21 +590,20 @@ def kv_fork(table: torch.Tensor, lens: torch.Tensor, parents: torch.Tensor, refs
     parents[c] (-1: empty) with room for `room` more tokens.  Returns the new
     table and lengths and the page copies that kv_copy has to make; refs is
     updated in place."""
-    for t, what in ((table, "table"), (lens, "lens"), (parents, "parents"), (refs, "refs")):
-        _ptr(t, torch.int32, what)
+    dev = table.get_device()
+    tp = _ptr(table, torch.int32, "table")
     if table.dim() != 2 or lens.numel() != table.shape[0]:
         raise _invalid("table has a row and lens an entry a sequence")
-    dev = table.get_device()
-    _same_device(dev, lens, parents, refs, flags)
-    n, width = parents.numel(), table.shape[1]
-    # the tables, their lengths, the copies and the scratch
-    new, ints = (torch.empty(n, width, dtype=torch.int32, device=table.device),
-                 torch.empty(4 * n, dtype=torch.int32, device=table.device))
+    sequences, width = table.shape
+    n, where = parents.numel(), table.device
+    # the new table; its lengths, the copies and the scratch
+    new, ints = (torch.empty(n, width, dtype=torch.int32, device=where), torch.empty(4 * n, dtype=torch.int32, device=where))
     _held(stream, new, ints)
     p = ints.data_ptr()
-    _launch(dev, stream, lib().ihip_kv_fork_dev, table.data_ptr(), lens.data_ptr(), table.shape[0], parents.data_ptr(), n,
-            room, width, page_size, refs.numel(), refs.data_ptr(), new.data_ptr(), p, p + 4 * n, p + 12 * n,
-            _opt(flags, torch.int32, "flags", 1))
+    _launch(dev, stream, lib().ihip_kv_fork_dev, tp, _at(lens, torch.int32, "lens", dev), sequences,
+            _at(parents, torch.int32, "parents", dev), n, room, width, page_size, refs.numel(),
+            _at(refs, torch.int32, "refs", dev), new.data_ptr(), p, p + 4 * n, p + 12 * n,
+            _at(flags, torch.int32, "flags", dev, 1))
     return new, ints[:n], ints[n:3 * n].view(n, 2)
 
 
@@ -604,16 +611,14 @@ def kv_compact(table: torch.Tensor, refs: torch.Tensor, flags=None, stream=None)
     """The used pages moved to the front of the pool (ihip_kv_compact_dev): table
     and refs change in place; returns the moves (pages // 2 pairs, -1 behind the
     last) and their number, both for kv_copy."""
-    _ptr(table, torch.int32, "table"), _ptr(refs, torch.int32, "refs")
     dev, pages = table.get_device(), refs.numel()
-    _same_device(dev, refs, flags)
-    n = pages // 2
+    tp, n = _ptr(table, torch.int32, "table"), pages // 2
     # the moves, the scratch and the moves' number
     ints = torch.empty(2 * n + pages + 1, dtype=torch.int32, device=table.device)
     _held(stream, ints)
     p = ints.data_ptr()
-    _launch(dev, stream, lib().ihip_kv_compact_dev, table.data_ptr(), table.numel(), refs.data_ptr(), pages, p,
-            p + 4 * (2 * n + pages), p + 8 * n, _opt(flags, torch.int32, "flags", 1))
+    _launch(dev, stream, lib().ihip_kv_compact_dev, tp, table.numel(), _at(refs, torch.int32, "refs", dev), pages, p,
+            p + 4 * (2 * n + pages), p + 8 * n, _at(flags, torch.int32, "flags", dev, 1))
     return ints[:2 * n].view(n, 2), ints[2 * n + pages:]
 
 
@@ -623,8 +628,7 @@ def kv_copy(cache: KVCache, copies: torch.Tensor, count: torch.Tensor = None, fl
     *count on."""
     if copies.dim() != 2 or copies.shape[1] != 2:
         raise _invalid("copies is pairs x 2")
-    dev = copies.get_device()
-    _same_device(dev, cache, count, flags)
+    dev = cache.index
     _launch(dev, stream, lib().ihip_kv_copy_dev, cache.ref, cache.layers, cache.layer_stride,
-            _ptr(copies, torch.int32, "copies"), copies.shape[0], _opt(count, torch.int32, "count", 1),
-            _opt(flags, torch.int32, "flags", 1))
+            _at(copies, torch.int32, "copies", dev), copies.shape[0], _at(count, torch.int32, "count", dev, 1),
+            _at(flags, torch.int32, "flags", dev, 1))
