@@ -156,6 +156,54 @@ __device__ __forceinline__ f2 get_shared(const uint64_t *p)
     return f2{__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32))};
 }
 
+// Four values of a row over its parts `from`, `from` + `by`, ... of n: their sum
+// (relative to `top`, as `sum` is), eight parts at a time with their maxima and
+// sums; `rows` rows lie between a row's parts.
+struct Joined {
+    float top, sum;
+    f4 v;
+    __device__ __forceinline__ void add(float top2, float sum2, f4 v2)
+    {
+        const float up = fmaxf(top, top2);
+        const float f = top == kNone ? 0.0f : exp2_fast(top - up), g = top2 == kNone ? 0.0f : exp2_fast(top2 - up);
+        sum = sum * f + sum2 * g;
+        v = v * f + v2 * g;
+        top = up;
+    }
+};
+__device__ __forceinline__ Joined join_parts(const uint64_t *o, const uint64_t *ml, int64_t rows, int dim, int from,
+                                             int by, int n)
+{
+    constexpr int AT_ONCE = 8;
+    Joined j{kNone, 0.0f, f4{}};
+    for (int p0 = AT_ONCE * from; p0 < n; p0 += AT_ONCE * by) {
+        f2 w[AT_ONCE], x[AT_ONCE], y[AT_ONCE];
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u) {
+            const int64_t p = min(p0 + u, n - 1) * rows;
+            w[u] = get_shared(ml + p);
+            x[u] = get_shared(o + p * dim / 2);
+            y[u] = get_shared(o + p * dim / 2 + 1);
+        }
+        float up = j.top;
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u)
+            up = p0 + u < n ? fmaxf(up, w[u].x) : up;
+        const float f = j.top == kNone ? 0.0f : exp2_fast(j.top - up);
+        j.sum *= f;
+        j.v *= f;
+        j.top = up;
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u)
+            if (p0 + u < n && w[u].y != 0.0f) { // (sum 0: a part without keys has written nothing else; NaN stays)
+                const float g = w[u].x == kNone ? 0.0f : exp2_fast(w[u].x - up);
+                j.sum += w[u].y * g;
+                j.v += f4{x[u].x, x[u].y, y[u].x, y[u].y} * g;
+            }
+    }
+    return j;
+}
+
 // What a workgroup works on: a tile of rows of one sequence and KV head, and
 // the part of its keys.
 struct Tile {
@@ -635,72 +683,35 @@ k_attn_rows(AttnArgs a, int tiles, int least, int splits)
     __syncthreads();
     if (!lds_last)
         return;
-    // four values of a row a thread, eight parts at a time with their maxima and
-    // sums; few rows: the parts are shared among groups of threads, which are joined
-    // in the groups' order
-    constexpr int AT_ONCE = 8;
+    // four values of a row a thread; few rows: the parts are shared among groups of
+    // threads, which are joined in the groups' order
     const int groups = max(1, 64 * AR_WAVES / items);
-    float *const lds_g = (float *)lds;
+    Joined *const lds_g = (Joined *)lds;
     for (int e0 = 0; e0 < items; e0 += 64 * AR_WAVES) {
         const int group = groups > 1 ? tid / items : 0;
         const int e = groups > 1 ? tid - group * items : e0 + tid;
         const bool in = group < groups && e < items;
         const int r = in ? e / (D / 4) : 0, d = in ? 4 * (e % (D / 4)) : 0;
-        const uint64_t *const from_o = part_o + (row_of(r) * D + d) / 2, *const from_ml = part_ml + row_of(r);
-        float top = kNone, sum = 0.0f;
-        f4 v = f4{};
-        for (int p0 = AT_ONCE * group; in && p0 < t.parts; p0 += AT_ONCE * groups) {
-            f2 w[AT_ONCE], x[AT_ONCE], y[AT_ONCE];
-#pragma unroll
-            for (int u = 0; u < AT_ONCE; ++u) {
-                const int64_t p = min(p0 + u, t.parts - 1) * rows_all;
-                w[u] = get_shared(from_ml + p);
-                x[u] = get_shared(from_o + p * D / 2);
-                y[u] = get_shared(from_o + p * D / 2 + 1);
-            }
-            float up = top;
-#pragma unroll
-            for (int u = 0; u < AT_ONCE; ++u)
-                up = p0 + u < t.parts ? fmaxf(up, w[u].x) : up;
-            const float f = top == kNone ? 0.0f : exp2_fast(top - up);
-            sum *= f;
-            v *= f;
-            top = up;
-#pragma unroll
-            for (int u = 0; u < AT_ONCE; ++u) {
-                const float g = p0 + u >= t.parts || w[u].x == kNone ? 0.0f : exp2_fast(w[u].x - up);
-                if (p0 + u < t.parts) { // (a weight 0 times NaN stays NaN)
-                    sum += w[u].y * g;
-                    v += f4{x[u].x, x[u].y, y[u].x, y[u].y} * g;
-                }
-            }
-        }
+        Joined j = join_parts(part_o + (row_of(r) * D + d) / 2, part_ml + row_of(r), rows_all, D, group, groups,
+                              in ? t.parts : 0);
         if (groups > 1) {
-            if (in && group > 0) {
-                *(f4 *)(lds_g + 8 * tid) = v;
-                *(f2 *)(lds_g + 8 * tid + 4) = f2{top, sum};
-            }
+            if (in && group > 0)
+                lds_g[tid] = j;
             __syncthreads();
             if (!in || group > 0)
                 return;
-            for (int q = 1; q < groups; ++q) {
-                const f4 v2 = *(const f4 *)(lds_g + 8 * (tid + q * items));
-                const f2 w2 = *(const f2 *)(lds_g + 8 * (tid + q * items) + 4);
-                const float up = fmaxf(top, w2.x);
-                const float f = top == kNone ? 0.0f : exp2_fast(top - up), g = w2.x == kNone ? 0.0f : exp2_fast(w2.x - up);
-                sum = sum * f + w2.y * g;
-                v = v * f + v2 * g;
-                top = up;
-            }
+            for (int q = 1; q < groups; ++q)
+                j.add(lds_g[tid + q * items].top, lds_g[tid + q * items].sum, lds_g[tid + q * items].v);
         }
         if (in)
-            finish(r, d, v, sum);
+            finish(r, d, j.v, j.sum);
     }
 }
 
 // ---- many rows: chunks of a prompt ---------------------------------------------
 constexpr int AC_ROWS = 128; // rows of a workgroup's tile, 32 a wave
 constexpr int AC_KEYS = 128; // keys of a step at most
+constexpr int AC_FEW_SPLITS = 16; // splits that one thread joins alone
 
 // Keys that a wave multiplies in a step: as many as leave its registers room
 // beside O^T and q (256 wide: 128 registers of O^T, 64 a part of q).
@@ -1073,67 +1084,34 @@ k_attn_chunk(AttnArgs a, int tiles, int least, int splits)
         }
 }
 
-// The splits' partial rows joined, N threads a row: sum_i e^(m_i - m) o_i over
-// sum_i e^(m_i - m) l_i.  A split is read by one group of dim / 4 threads, the
-// groups' sums are added in their order.  Few splits of many rows take a wave a
-// row, many splits a workgroup.
-template <typename C, int PARTS, int N>
+// The splits' partial rows joined, four values a thread: sum_i e^(m_i - m) o_i
+// over sum_i e^(m_i - m) l_i.  Few splits: several rows a workgroup; many: one,
+// its splits shared among groups of threads, which are joined in their order.
+template <typename C, int PARTS>
 __global__ void __launch_bounds__(256) k_attn_join(AttnArgs a, int splits)
 {
-    __shared__ float weight[256 / N][AR_SPLITS], lds_l[256 / N];
-    __shared__ __attribute__((aligned(16))) float lds_o[256 * 4];
-    const int tid = threadIdx.x % N, mine = threadIdx.x / N, lane = threadIdx.x & 63, D = a.cache.dim;
-    const int64_t rows = (int64_t)a.batch.tokens * a.q_heads, row = (int64_t)blockIdx.x * (256 / N) + mine;
-    int first = 0;
-    KvSeq q;
-    // (a row behind the last sequence is left as it is)
-    const bool live = kv_find(a.batch, a.cache.page_shift, (int)min(row / a.q_heads, (int64_t)a.batch.tokens), first, q,
-                              [](int n) { return n; }) >= 0;
-    const f2 *ml = (const f2 *)(a.part + (int64_t)splits * rows * D);
-    if (live && tid < 64) {
-        f2 v[AR_SPLITS / 64];
-        float top = kNone, sum = 0.0f;
-#pragma unroll
-        for (int u = 0; u < AR_SPLITS / 64; ++u) {
-            const int i = lane + 64 * u;
-            v[u] = i < splits ? ml[i * rows + row] : f2{kNone, 0.0f};
-            top = fmaxf(top, v[u].x);
-        }
-#pragma unroll
-        for (int d = 32; d; d /= 2)
-            top = fmaxf(top, __shfl_xor(top, d));
-#pragma unroll
-        for (int u = 0; u < AR_SPLITS / 64; ++u) {
-            // (sum 0: no key was seen and nothing else was written; NaN stays)
-            const float f = v[u].x == kNone ? 0.0f : exp2_fast(v[u].x - top);
-            sum += v[u].y * f;
-            weight[mine][lane + 64 * u] = v[u].y == 0.0f ? -1.0f : f;
-        }
-#pragma unroll
-        for (int d = 32; d; d /= 2)
-            sum += __shfl_xor(sum, d);
-        if (lane == 0)
-            lds_l[mine] = sum;
+    __shared__ Joined lds_g[256];
+    const int D = a.cache.dim, per = D / 4, slots = 256 / per, slot = threadIdx.x / per, d = 4 * (threadIdx.x - slot * per);
+    const bool many = splits > AC_FEW_SPLITS;
+    const int64_t rows = (int64_t)a.batch.tokens * a.q_heads;
+    const int64_t row = many ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * slots + slot;
+    // (a row of no sequence is left as it is)
+    const int token = (int)(row / a.q_heads);
+    const bool live = slot < slots && row < rows && token >= a.batch.starts[0] && token < a.batch.starts[a.batch.sequences];
+    const int64_t at = live ? row : 0;
+    const uint64_t *const o = (const uint64_t *)a.part, *const ml = o + (int64_t)splits * rows * D / 2;
+    Joined j = join_parts(o + (at * D + d) / 2, ml + at, rows, D, many ? slot : 0, many ? slots : 1, live ? splits : 0);
+    if (many) {
+        lds_g[threadIdx.x] = j;
+        __syncthreads();
+        if (slot > 0)
+            return;
+        for (int q = 1; q < slots; ++q)
+            j.add(lds_g[threadIdx.x + q * per].top, lds_g[threadIdx.x + q * per].sum, lds_g[threadIdx.x + q * per].v);
     }
-    __syncthreads();
-    const int per = D / 4, groups = N / per, at = tid / per, d = 4 * (tid - at * per);
-    f4 v = f4{};
-    if (live && at < groups) {
-#pragma unroll 4
-        for (int i = at; i < splits; i += groups) {
-            const float f = weight[mine][i];
-            if (f >= 0.0f)
-                v += *(const f4 *)(a.part + (i * rows + row) * D + d) * f;
-        }
-        *(f4 *)(lds_o + 4 * threadIdx.x) = v;
-    }
-    __syncthreads();
-    if (!live || tid >= per)
+    if (!live)
         return;
-    for (int i = 1; i < groups; ++i)
-        v += *(const f4 *)(lds_o + 4 * (threadIdx.x + i * per));
-    const float sum = lds_l[mine];
-    v = sum == 0.0f ? f4{} : v * (1.0f / sum);
+    const f4 v = j.sum == 0.0f ? f4{} : j.v * (1.0f / j.sum);
     if constexpr (PARTS == 1)
         *(typename C::V4 *)((typename C::T *)a.out + row * D + d) = __builtin_convertvector(v, typename C::V4);
     else
@@ -1177,10 +1155,8 @@ hipError_t start_dim(const AttnArgs &a, const AttnPlan &p, hipStream_t s)
         start_gen<C, PARTS, false>(a, p, s);
     if (p.splits > 1 && p.rows == AC_ROWS) {
         const int64_t rows = (int64_t)a.batch.tokens * a.q_heads;
-        if (p.splits <= 16)
-            hipLaunchKernelGGL((k_attn_join<C, PARTS, 64>), dim3((uint32_t)((rows + 3) / 4)), dim3(256), 0, s, a, p.splits);
-        else
-            hipLaunchKernelGGL((k_attn_join<C, PARTS, 256>), dim3((uint32_t)rows), dim3(256), 0, s, a, p.splits);
+        const int slots = p.splits > AC_FEW_SPLITS ? 1 : 256 / (a.cache.dim / 4);
+        hipLaunchKernelGGL((k_attn_join<C, PARTS>), dim3((uint32_t)((rows + slots - 1) / slots)), dim3(256), 0, s, a, p.splits);
     }
     return hipGetLastError();
 }
