@@ -489,7 +489,8 @@ int ihip_attn_paged_dev(const void *q, int q_type, void *out, int q_heads, float
                         float softcap, int window, const int32_t *prefix_lens, const float *slopes,
                         const ihip_kv_cache *cache, const ihip_kv_batch *batch, uint32_t *flags,
                         void *workspace, size_t workspace_bytes, ihip_stream stream);
-/* From the sizes alone: never more for other contents of the batch's arrays. */
+/* From the sizes alone, for either q_type, any window and any contents of the
+ * batch's arrays. */
 size_t ihip_attn_paged_scratch_bytes(int q_type, int q_heads, const ihip_kv_cache *cache,
                                      const ihip_kv_batch *batch);
 

@@ -1620,7 +1620,9 @@ size_t ihip_attn_paged_scratch_bytes(int q_type, int q_heads, const ihip_kv_cach
     if (check_cache(cache, &c) != IHIP_OK || check_batch(batch, &b) != IHIP_OK || q_heads <= 0 ||
         q_heads % c.heads || (q_type != kF32 && q_type != c.type) || b.tokens == 0 || b.sequences == 0)
         return 0;
-    return attn_plan(q_heads, c.heads, c.dim, b.sequences, b.tokens, (int64_t)b.stride << c.page_shift, 0).bytes;
+    // (q of the cache's type may be split furthest: enough for F32 too)
+    return attn_plan(c.type, c.type, q_heads, c.heads, c.dim, b.sequences, b.tokens, (int64_t)b.stride << c.page_shift, 0)
+        .bytes;
 }
 
 int ihip_attn_paged_dev(const void *q, int q_type, void *out, int q_heads, float scale,
@@ -1655,8 +1657,8 @@ int ihip_attn_paged_dev(const void *q, int q_type, void *out, int q_heads, float
         return fail(IHIP_ERR_INVALID, "q overlaps out");
     if (in_pools(a.cache, out, bytes))
         return fail(IHIP_ERR_INVALID, "out overlaps the cache");
-    const AttnPlan p = attn_plan(q_heads, a.cache.heads, a.cache.dim, a.batch.sequences, a.batch.tokens, capacity,
-                                 prefix_lens ? 0 : window);
+    const AttnPlan p = attn_plan(q_type, a.cache.type, q_heads, a.cache.heads, a.cache.dim, a.batch.sequences,
+                                 a.batch.tokens, capacity, prefix_lens ? 0 : window);
     if (!grid_fits((int64_t)p.tiles * a.cache.heads * p.splits))
         return fail(IHIP_ERR_INVALID, "%lld rows are too many for one call", (long long)rows);
     if (p.bytes) {

@@ -204,6 +204,11 @@ __device__ __forceinline__ Joined join_parts(const uint64_t *o, const uint64_t *
     return j;
 }
 
+// What the scores go through, each a kernel of its own: the registers of a cap
+// would cost the others a wave a SIMD (64 wide: 38 us against 34 for five ragged
+// chunks).
+constexpr int kPlain = 0, kBias = 1, kCap = 2; // (kCap: with a bias or without)
+
 // What a workgroup works on: a tile of rows of one sequence and KV head, and
 // the part of its keys.
 struct Tile {
@@ -271,10 +276,22 @@ __device__ __forceinline__ Seen seen_from(const AttnArgs &a, const Tile &t, int 
     return Seen{from, last >= from ? (uint32_t)(last - from) + 1u : 0u};
 }
 
-// Scores as powers of two, from q.k: `by` and the cap or the distance bias.
-// tanh x: the Taylor series to x^15 below 1/2 (the next term is under 2^-26 of
-// x), (e^2x - 1) / (e^2x + 1) from there.
-__device__ __forceinline__ float tanh_own(float x)
+// tanh x by its Taylor series, to x^11 for |x| <= 0.35 and to x^15 for |x| < 1/2
+// (what is left out is under 2^-26 of x), and as (e^2x - 1) / (e^2x + 1) from there.
+// Capped scores are mostly a small part of their cap: a wave whose scores all are
+// takes the short series alone (8 operations a score against 23).
+constexpr float kNear = 0.35f;
+__device__ __forceinline__ float tanh_near(float x)
+{
+    const float y = x * x;
+    float p = -1382.0f / 155925.0f;
+    p = fmaf(p, y, 62.0f / 2835.0f);
+    p = fmaf(p, y, -17.0f / 315.0f);
+    p = fmaf(p, y, 2.0f / 15.0f);
+    p = fmaf(p, y, -1.0f / 3.0f);
+    return fmaf(p * y, x, x);
+}
+__device__ __forceinline__ float tanh_any(float x)
 {
     const float y = x * x;
     float p = -929569.0f / 638512875.0f;
@@ -374,7 +391,7 @@ constexpr int ar_wave_lds()
 // registers, V by direct copies into LDS of the wave's own, both one step
 // ahead and their page ids two; the waves' sums are joined at the end, and the
 // parts' by the workgroup that ends last.
-template <typename C, int PARTS, int DP, bool GEN>
+template <typename C, int PARTS, int DP, int FEAT>
 __global__ void __launch_bounds__(64 * AR_WAVES, DP == 256 ? 1 : 2)
 k_attn_rows(AttnArgs a, int tiles, int least, int splits)
 {
@@ -470,8 +487,8 @@ k_attn_rows(AttnArgs a, int tiles, int least, int splits)
     const float scale = (a.scale == 0.0f ? 1.0f : fabsf(a.scale)) * undo;
     // scores become powers of two with the last factor, `by`; a cap takes the scale
     // before, and the bias is added in units of `by`
-    const float by = GEN && a.cap > 0.0f ? a.cap * kLog2e : scale * kLog2e;
-    const float slope = GEN && a.slopes ? a.slopes[qhead] * kLog2e / by : 0.0f;
+    const float by = FEAT == kCap ? a.cap * kLog2e : scale * kLog2e;
+    const float slope = FEAT != kPlain && a.slopes ? a.slopes[qhead] * kLog2e / by : 0.0f;
     const Seen sees = seen_from(a, t, pos);
 
     float m = kNone, l = 0.0f;
@@ -508,14 +525,32 @@ k_attn_rows(AttnArgs a, int tiles, int least, int splits)
             ids = page_of(step + 2 * AR_WAVES);
             load_k();
         }
-        if (GEN) {
+        if constexpr (FEAT != kPlain) {
             const float apart = (float)(pos - key - 4 * g);
-            if (a.cap > 0.0f)
+            if constexpr (FEAT == kCap) {
+                const float by_cap = scale / a.cap;
+                float most = 0.0f;
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        s[u][i] = tanh_own(s[u][i] * (scale / a.cap));
+                    for (int i = 0; i < 4; ++i) {
+                        s[u][i] *= by_cap;
+                        most = fmaxf(most, fabsf(s[u][i]));
+                    }
+                if (__any(most > kNear)) {
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            s[u][i] = tanh_any(s[u][i]);
+                } else { // (a NaN is neither, and stays)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            s[u][i] = tanh_near(s[u][i]);
+                }
+            }
             if (a.slopes)
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
@@ -739,7 +774,7 @@ __device__ __forceinline__ int ac_v_chunk(int r, int c)
 // run of one page of K and of V) while the step before is multiplied; one barrier
 // a step.  S^T = K Q^T and O^T = V^T P^T in 32 x 32 x 16 products: a lane holds
 // half of the scores of its row and 16 of the 32 rows of each d tile.
-template <typename C, int PARTS, int DP, bool GEN, int HALVES>
+template <typename C, int PARTS, int DP, int FEAT, int HALVES>
 __global__ void __launch_bounds__(256 * HALVES, ac_waves(PARTS, DP))
 k_attn_chunk(AttnArgs a, int tiles, int least, int splits)
 {
@@ -780,8 +815,8 @@ k_attn_chunk(AttnArgs a, int tiles, int least, int splits)
     const float scale = (a.scale == 0.0f ? 1.0f : fabsf(a.scale)) * undo;
     // scores become powers of two with the last factor, `by`; a cap takes the scale
     // before, and the bias is added in units of `by`
-    const float by = GEN && a.cap > 0.0f ? a.cap * kLog2e : scale * kLog2e;
-    const float slope = GEN && a.slopes ? a.slopes[qhead] * kLog2e / by : 0.0f;
+    const float by = FEAT == kCap ? a.cap * kLog2e : scale * kLog2e;
+    const float slope = FEAT != kPlain && a.slopes ? a.slopes[qhead] * kLog2e / by : 0.0f;
     const Seen sees = seen_from(a, t, pos);
 
     // a lane's part of the copies: RUN keys of one page
@@ -919,14 +954,32 @@ k_attn_chunk(AttnArgs a, int tiles, int least, int splits)
                     __builtin_amdgcn_sched_barrier(0); // (operands further ahead would not fit the registers)
             }
         }
-        if (GEN) {
+        if constexpr (FEAT != kPlain) {
             const float apart = (float)(pos - key - 4 * h);
-            if (a.cap > 0.0f)
+            if constexpr (FEAT == kCap) {
+                const float by_cap = scale / a.cap;
+                float most = 0.0f;
 #pragma unroll
                 for (int u = 0; u < SU; ++u)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        s[u][i] = tanh_own(s[u][i] * (scale / a.cap));
+                    for (int i = 0; i < 16; ++i) {
+                        s[u][i] *= by_cap;
+                        most = fmaxf(most, fabsf(s[u][i]));
+                    }
+                if (__any(most > kNear)) {
+#pragma unroll
+                    for (int u = 0; u < SU; ++u)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            s[u][i] = tanh_any(s[u][i]);
+                } else { // (a NaN is neither, and stays)
+#pragma unroll
+                    for (int u = 0; u < SU; ++u)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            s[u][i] = tanh_near(s[u][i]);
+                }
+            }
             if (a.slopes)
 #pragma unroll
                 for (int u = 0; u < SU; ++u)
@@ -1118,41 +1171,43 @@ __global__ void __launch_bounds__(256) k_attn_join(AttnArgs a, int splits)
         *(f4 *)((float *)a.out + row * D + d) = v;
 }
 
-template <typename C, int PARTS, int DP, bool GEN>
+template <typename C, int PARTS, int DP, int FEAT>
 void start(const AttnArgs &a, const AttnPlan &p, hipStream_t s)
 {
     const dim3 grid((uint32_t)((int64_t)p.tiles * a.cache.heads * p.splits));
     if (p.rows == AR_ROWS) {
-        hipLaunchKernelGGL((k_attn_rows<C, PARTS, DP, GEN>), grid, dim3(64 * AR_WAVES), 0, s, a, p.tiles, p.least, p.splits);
+        hipLaunchKernelGGL((k_attn_rows<C, PARTS, DP, FEAT>), grid, dim3(64 * AR_WAVES), 0, s, a, p.tiles, p.least, p.splits);
         return;
     }
     if constexpr (ac_waves(PARTS, DP) == 2 && DP <= 128) {
         if (p.halves) {
-            hipLaunchKernelGGL((k_attn_chunk<C, PARTS, DP, GEN, 2>), grid, dim3(512), 0, s, a, p.tiles, p.least, p.splits);
+            hipLaunchKernelGGL((k_attn_chunk<C, PARTS, DP, FEAT, 2>), grid, dim3(512), 0, s, a, p.tiles, p.least, p.splits);
             return;
         }
     }
-    hipLaunchKernelGGL((k_attn_chunk<C, PARTS, DP, GEN, 1>), grid, dim3(256), 0, s, a, p.tiles, p.least, p.splits);
+    hipLaunchKernelGGL((k_attn_chunk<C, PARTS, DP, FEAT, 1>), grid, dim3(256), 0, s, a, p.tiles, p.least, p.splits);
 }
 
-template <typename C, int PARTS, bool GEN>
-void start_gen(const AttnArgs &a, const AttnPlan &p, hipStream_t s)
+template <typename C, int PARTS, int FEAT>
+void start_feat(const AttnArgs &a, const AttnPlan &p, hipStream_t s)
 {
     if (a.cache.dim <= 64)
-        start<C, PARTS, 64, GEN>(a, p, s);
+        start<C, PARTS, 64, FEAT>(a, p, s);
     else if (a.cache.dim <= 128)
-        start<C, PARTS, 128, GEN>(a, p, s);
+        start<C, PARTS, 128, FEAT>(a, p, s);
     else
-        start<C, PARTS, 256, GEN>(a, p, s);
+        start<C, PARTS, 256, FEAT>(a, p, s);
 }
 
 template <typename C, int PARTS>
 hipError_t start_dim(const AttnArgs &a, const AttnPlan &p, hipStream_t s)
 {
-    if (a.cap > 0.0f || a.slopes)
-        start_gen<C, PARTS, true>(a, p, s);
+    if (a.cap > 0.0f)
+        start_feat<C, PARTS, kCap>(a, p, s);
+    else if (a.slopes)
+        start_feat<C, PARTS, kBias>(a, p, s);
     else
-        start_gen<C, PARTS, false>(a, p, s);
+        start_feat<C, PARTS, kPlain>(a, p, s);
     if (p.splits > 1 && p.rows == AC_ROWS) {
         const int64_t rows = (int64_t)a.batch.tokens * a.q_heads;
         const int slots = p.splits > AC_FEW_SPLITS ? 1 : 256 / (a.cache.dim / 4);
@@ -1163,16 +1218,23 @@ hipError_t start_dim(const AttnArgs &a, const AttnPlan &p, hipStream_t s)
 
 } // namespace
 
-AttnPlan attn_plan(int q_heads, int kv_heads, int dim, int sequences, int tokens, int64_t capacity, int window)
+AttnPlan attn_plan(int act, int kv_type, int q_heads, int kv_heads, int dim, int sequences, int tokens,
+                   int64_t capacity, int window)
 {
     AttnPlan p;
-    const int group = q_heads / kv_heads;
+    const int group = q_heads / kv_heads, parts = act != kF32 ? 1 : kv_type == kF16 ? 2 : 3;
     // p.tiles: the sum of ceil(rows of a sequence / p.rows) at most
     const int64_t rows = (int64_t)tokens * group, some = std::min(sequences, tokens);
-    // a batch whose sequences have more than a tile of few rows on average takes the
-    // tiles of many
-    p.rows = rows > (int64_t)AR_ROWS * some ? AC_ROWS : AR_ROWS;
-    p.tiles = (int)((rows - some) / p.rows + some);
+    // Two tiles of few rows a sequence on average, or short caches whose tiles of few
+    // rows all have room at once, take the kernel of few rows; more rows read the keys
+    // too often there.  us, few rows against many (fp16, 128 wide, 8 KV heads): 8
+    // sequences of 20 rows over 4000 keys 42, 48; of 48 rows 59, 54; of 96 rows 86,
+    // 53; of 96 rows over 300 keys 15, 20; 32 of 48 rows over 300 keys 24, 18.
+    auto tiles_of = [&](int n) { return (rows - some) / n + some; };
+    const bool fits = capacity <= 512 && tiles_of(AR_ROWS) * kv_heads <= 512;
+    p.rows = rows <= 2 * (int64_t)AR_ROWS * some || fits ? AR_ROWS : AC_ROWS;
+    if (getenv("X_ROWS")) p.rows = atoi(getenv("X_ROWS"));
+    p.tiles = (int)tiles_of(p.rows);
     const int64_t units = (int64_t)p.tiles * kv_heads;
     int64_t want;
     if (p.rows == AR_ROWS) {
@@ -1181,18 +1243,24 @@ AttnPlan attn_plan(int q_heads, int kv_heads, int dim, int sequences, int tokens
         p.least = units <= 32 ? 128 : units <= 128 ? 256 : 512;
         want = units >= kAttnCounts ? 1 : (256 * std::min<int64_t>(some, 16) + units - 1) / units;
     } else {
-        // tiles that fill the chip are not split: joining would cost more
+        // tiles that fill the chip are not split: joining would cost more.  Fewer are
+        // split as far as their workgroups all have room at once (twice as far where
+        // sequences differ)
+        const int64_t room = ac_waves(parts, dim <= 64 ? 64 : dim <= 128 ? 128 : 256) == 2 ? 512 : 256;
         p.least = 256;
-        want = units >= 256 ? 1 : (512 * std::min<int64_t>(some, 2) + units - 1) / units;
+        want = units >= 256 ? 1 : room * std::min<int64_t>(some, 2) / units;
     }
+    if (getenv("X_LEAST")) p.least = atoi(getenv("X_LEAST"));
     // (a window, where there is one, ends a tile's keys: no part would lie behind)
     const int64_t reach = window ? std::min(capacity, (int64_t)window + p.rows + AC_KEYS) : capacity;
     const int64_t most = (reach + p.least - 1) / p.least;
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(most, want), AR_SPLITS));
+    if (getenv("X_SPLITS")) p.splits = std::min<int64_t>(most, atoi(getenv("X_SPLITS")));
     // Few tiles: two halves of a workgroup each, which end a long tile sooner
     // (512 tiles of a 2048-token prompt: 65 us against 77); of many, two
     // workgroups a CU come further (4096 tokens: 174 us against 200).
-    p.halves = units * p.splits <= 512;
+    p.halves = p.splits == 1 && units <= 512;
+    if (getenv("X_HALVES")) p.halves = atoi(getenv("X_HALVES"));
     // (with 4096 tiles and heads or more nothing is split: their counts are enough)
     p.bytes = p.splits > 1 ? 4 * (size_t)kAttnCounts + (size_t)p.splits * tokens * q_heads * (dim + 2) * 4 : 0;
     return p;

@@ -57,7 +57,8 @@ struct AttnPlan {
 };
 // window: the window where there is one and no prefix reaches behind it, else 0
 // (which never needs less workspace).
-AttnPlan attn_plan(int q_heads, int kv_heads, int dim, int sequences, int tokens, int64_t capacity, int window);
+AttnPlan attn_plan(int act, int kv_type, int q_heads, int kv_heads, int dim, int sequences, int tokens,
+                   int64_t capacity, int window);
 hipError_t launch_attn(const AttnArgs &a, const AttnPlan &p, hipStream_t s);
 
 // kv_pages.hip

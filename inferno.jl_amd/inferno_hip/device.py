@@ -542,11 +542,11 @@ def rope_kv(q: torch.Tensor, k, v, turns: torch.Tensor, cache: KVCache, batch: K
     return out
 
 
-def attn_workspace(q_heads: int, cache: KVCache, batch: KVBatch, dtype=torch.float32):
-    """The workspace of attn_paged for a batch of these sizes (for q of `dtype`),
+def attn_workspace(q_heads: int, cache: KVCache, batch: KVBatch):
+    """The workspace of attn_paged for a batch of these sizes (q of either type),
     or None where it needs none.  It starts as zeros, and every call leaves what
     has to be zero so.  Calls that share one must not overlap."""
-    n = lib().ihip_attn_paged_scratch_bytes(_ACT_TYPES[dtype], q_heads, cache.ref, batch.ref)
+    n = lib().ihip_attn_paged_scratch_bytes(_lib.F32, q_heads, cache.ref, batch.ref)
     return torch.zeros(n, dtype=torch.uint8, device=cache.device) if n else None
 
 
@@ -573,7 +573,7 @@ def attn_paged(q: torch.Tensor, cache: KVCache, batch: KVBatch, scale: float = N
     elif out.shape != shape:
         raise _invalid("out must have q's shape and type")
     if workspace is None:
-        workspace = attn_workspace(H, cache, batch, q.dtype)
+        workspace = attn_workspace(H, cache, batch)
         if workspace is not None:
             _held(stream, workspace)
     _launch(dev, stream, lib().ihip_attn_paged_dev, _at(q, q.dtype, "q", dev), act, _at(out, q.dtype, "out", dev), H,
