@@ -750,7 +750,7 @@ constexpr int AC_FEW_SPLITS = 16; // splits that one thread joins alone
 
 // Keys that a wave multiplies in a step: as many as leave its registers room
 // beside O^T and q (256 wide: 128 registers of O^T, 64 a part of q).
-constexpr int ac_half_keys(int) { return 64; }
+constexpr int ac_half_keys(int parts, int dp) { return dp == 256 && parts == 3 ? 32 : 64; }
 // Waves a SIMD: two, where a wave's operands fit 256 registers.
 constexpr int ac_waves(int parts, int dp) { return dp <= 64 || (dp <= 128 && parts <= 2) ? 2 : 1; }
 
@@ -782,7 +782,7 @@ k_attn_chunk(AttnArgs a, int tiles, int least, int splits)
     typedef typename C::V8 V8;
     typedef typename C::V4 V4;
     constexpr int WAVES = 4 * HALVES;
-    constexpr int HK = ac_half_keys(DP), KEYS = HK * HALVES, SU = HK / 32; // a half's keys of a step, and all
+    constexpr int HK = ac_half_keys(PARTS, DP), KEYS = HK * HALVES, SU = HK / 32; // a half's keys of a step, and all
     constexpr int RUN = HK / 4, NI = RUN * DP / 512; // keys that a wave copies, in NI copies of 1 KB
     constexpr int KS = DP / 16, DT = DP / 32, NC = DP / 8;
     constexpr int TILE = KEYS * DP * 2;
