@@ -476,9 +476,11 @@ int ihip_rope_kv_dev(const float *q, int64_t q_stride, const float *k, int64_t k
  * prefix_lens[s]; with window > 0 only those with p - j < window.  The score is
  * scale * q.k, then softcap * tanh(score / softcap) where softcap > 0, then
  * minus slopes[h] * |p - j| (q_heads floats, or NULL).  A row that sees no key
- * gives 0, and what hidden keys or unfilled slots hold has no influence.
+ * gives 0, and what hidden keys or unfilled slots hold has no influence.  scale
+ * and softcap are 0 or at least 1e-12 in magnitude.
  * F32: scores and outputs carry fp32's accuracy.  F16 / BF16: the softmax
- * weights are rounded to that type (the sums stay fp32).
+ * weights are rounded to that type (the sums stay fp32).  A row that sees an
+ * infinity in k may be NaN (q is multiplied in parts, and padded with zeros).
  * workspace: ihip_attn_paged_scratch_bytes bytes, 16-byte aligned, NULL where
  * that is 0.  The caller fills its first IHIP_ATTN_COUNT_BYTES with zeros once,
  * before its first call; every call leaves them zero again, so that it serves any

@@ -1642,7 +1642,9 @@ int ihip_attn_paged_dev(const void *q, int q_type, void *out, int q_heads, float
         return fail(IHIP_ERR_INVALID, "q_heads=%d is not a multiple of kv_heads=%d", q_heads, a.cache.heads);
     if (q_type != kF32 && q_type != a.cache.type)
         return fail(IHIP_ERR_INVALID, "q_type=%d is neither F32 nor the cache's type %d", q_type, a.cache.type);
-    if (window < 0 || !std::isfinite(scale) || !std::isfinite(softcap) || softcap < 0.0f)
+    // (a scale or a cap so small that a ratio of the two, or of a slope, could pass fp32)
+    if (window < 0 || !std::isfinite(scale) || !std::isfinite(softcap) || softcap < 0.0f ||
+        (scale != 0.0f && std::fabs(scale) < 1e-12f) || (softcap > 0.0f && softcap < 1e-12f))
         return fail(IHIP_ERR_INVALID, "window=%d, scale=%g, softcap=%g", window, scale, softcap);
     if (!al16(q) || !al16(out))
         return fail(IHIP_ERR_INVALID, "q and out must be 16-byte aligned");
@@ -1650,8 +1652,11 @@ int ihip_attn_paged_dev(const void *q, int q_type, void *out, int q_heads, float
     if (T == 0 || a.batch.sequences == 0)
         return IHIP_OK;
     const int64_t capacity = (int64_t)a.batch.stride << a.cache.page_shift;
-    if (!grid_fits(capacity) || !grid_fits(rows))
-        return fail(IHIP_ERR_INVALID, "%lld rows or %lld table tokens pass 2^31", (long long)rows, (long long)capacity);
+    if (capacity > 1 << 30 || T > 1 << 30 || !grid_fits(rows))
+        return fail(IHIP_ERR_INVALID, "%lld rows pass 2^31 or %lld table tokens 2^30", (long long)rows,
+                    (long long)capacity);
+    if (window >= capacity)
+        window = 0; // hides nothing
     const size_t bytes = (size_t)rows * (size_t)a.cache.dim * (size_t)value_bytes(q_type);
     if (overlap(q, bytes, out, bytes))
         return fail(IHIP_ERR_INVALID, "q overlaps out");
@@ -1696,7 +1701,7 @@ int ihip_kv_fork_dev(const int32_t *table, const int32_t *lens, int sequences,
     if (!refs || (sequences && (!table || !lens)) || (children && (!parents || !table_out || !lens_out || !copies || !scratch)))
         return fail(IHIP_ERR_INVALID, "null pointer");
     if (!grid_fits((int64_t)sequences + children) || !grid_fits((int64_t)children * table_stride) ||
-        !grid_fits((int64_t)table_stride * page_size))
+        !grid_fits((int64_t)table_stride * page_size) || !grid_fits((int64_t)pages + 4096))
         return fail(IHIP_ERR_INVALID, "%d children of %d pages are too many for one call", children, table_stride);
     const size_t tb = 4 * (size_t)sequences * (size_t)table_stride, lb = 4 * (size_t)sequences;
     const size_t cb = 4 * (size_t)children, ob = cb * (size_t)table_stride;
@@ -1760,7 +1765,7 @@ int ihip_kv_copy_dev(const ihip_kv_cache *cache, int layers, int64_t layer_strid
     RET_IF(check_cache(cache, &c));
     if (layers <= 0 || n < 0 || layer_stride < 0 || layer_stride % 8 || layer_stride > INT64_MAX / 4 / layers)
         return fail(IHIP_ERR_INVALID, "layers=%d, layer_stride=%lld, n=%d", layers, (long long)layer_stride, n);
-    if (layers > 1 && 2 * (size_t)layer_stride < 2 * (size_t)c.page_stride)
+    if (layers > 1 && layer_stride < ((int64_t)c.heads * c.dim << c.page_shift))
         return fail(IHIP_ERR_INVALID, "layer_stride=%lld does not hold a page", (long long)layer_stride);
     if (n == 0)
         return IHIP_OK;

@@ -347,7 +347,8 @@ __device__ __forceinline__ void load_q(const AttnArgs &a, int64_t row, bool live
         if constexpr (C::kShift != 0.0f) {
             most = step == 4 ? groups_max(most) : halves_max(most);
             const bool finite = most > 0.0f && most < __builtin_inff();
-            up = finite ? 15 - __builtin_amdgcn_frexp_expf(most) : 0;
+            // (rows under 2^-45 lose bits that no score would show)
+            up = finite ? min(15 - __builtin_amdgcn_frexp_expf(most), 60) : 0;
             undo = __builtin_ldexpf(1.0f, -up);
         }
 #pragma unroll

@@ -160,12 +160,53 @@ def test_hidden_keys_have_no_influence_whatever_they_hold(act, kv, bad):
         assert bool(torch.isfinite(torch.cat((last[:, :5], last[:, 6:]), 1)).all())
 
 
+@pytest.mark.parametrize("dim", [8, 72, 80, 128, 200])
+def test_an_infinite_score_stays_in_the_rows_that_see_it(dim):
+    """An infinity in a key's last value, beside which a narrower head's kernel has zeros of q: rows that see it
+    may be NaN, as the interface says; where they are not, the key has no weight.  No other row changes."""
+    for act, kv in TYPES:
+        for new, lens in (([1], [70]), ([40], [77])):
+            case = build(30, new, lens, 4, 1, dim, 16, act, kv)
+            q, k, v, starts, _, table = case
+            q[..., -1] = q[..., -1].abs() + 0.5
+            clean, _ = run(case)
+            k[table[0][2], :, 8, -1] = -float("inf")  # token 40: rows 3 .. 39 of 40 see it, or the only one
+            got, _ = run(case)
+            before = 3 if len(got) > 1 else 0
+            assert torch.equal(got[:before], clean[:before])
+            m = lens[0]
+            keep = [j for j in range(m) if j != 40]
+            z = q[-1, 2].double() @ kv_plain.gathered(k, table[0], m, 0)[keep].T * dim ** -0.5
+            want = torch.softmax(z, 0) @ kv_plain.gathered(v, table[0], m, 0)[keep]
+            if bool(torch.isfinite(got[-1, 2].float()).all()):
+                # half a step of the weights and of the output, of values under 4
+                assert float((got[-1, 2].double() - want).abs().max()) < 2 * 4 * kv_plain.HALF_STEP[act]
+            else:
+                assert bool(torch.isnan(got[-1, 2].float()).all()) and (act == F32 or dim not in (64, 128))
+
+
+@pytest.mark.parametrize("act,kv", TYPES)
+def test_windows_and_scales_at_their_limits(act, kv):
+    case = build(31, [1, 30], [50, 64], 4, 2, 64, 16, act, kv)
+    plain, _ = run(case)
+    assert torch.equal(run(case, window=2 ** 31 - 1)[0], plain)
+    check(case, scale=0.0)
+    check(case, scale=-0.2)
+    check(case, scale=1e-12, slopes=[0.5, 0.25, 0.125, 0.0])
+    check(case, softcap=1e-3)
+    case = build(31, [30], [9], 4, 2, 64, 16, act, kv)  # rows before position 0
+    assert torch.equal(run(case, window=2 ** 31 - 1)[0], run(case)[0])
+
+
 def test_extreme_queries_keep_fp32_accuracy():
     """fp32 rows whose values fp16 could not hold: far over its largest, far under its smallest."""
     case = list(build(11, [1, 5], [90, 40], 4, 2, 128, 16, F32, F16))
     case[0][0] *= 1e7
     case[0][1:] *= 1e-7
     check(tuple(case), scale=1e-6)
+    check(tuple(case), slopes=[0.5, 0.25, 0.125, 0.0625], scale=1e-6)
+    case[0] *= 1e-25
+    check(tuple(case), slopes=[0.5, 0.25, 0.125, 0.0625])
     case[0].zero_()
     check(tuple(case))
 

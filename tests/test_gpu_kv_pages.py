@@ -167,6 +167,18 @@ def test_copies(layers, heads, page, dim, dtype):
         assert int(flags.item()) == 8
 
 
+def test_copies_of_layers_within_pages():
+    """All layers of a page together: the layer stride is the smaller one."""
+    from inferno_hip import device as D
+    both = torch.randn(9, 3, 2, 2, 16, 64, device="cuda").half()  # pages, layers, k and v
+    want = both.clone()
+    want[7] = both[2]
+    k, v = both[:, :, 0].transpose(0, 1), both[:, :, 1].transpose(0, 1)
+    D.kv_copy(D.KVCache(k, v), ints([[2, 7]]))
+    torch.cuda.synchronize()
+    assert torch.equal(both, want)
+
+
 def test_wrapper_refusals():
     from inferno_hip import device as D
     t, n, r = ints([[0, 1]]), ints([20]), ints([1, 1, 0])

@@ -65,15 +65,16 @@ def test_a_batch_that_does_not_hold_together_is_refused(bad):
 
 @pytest.mark.parametrize("bad", [
     dict(q=None), dict(out=None), dict(heads=3), dict(heads=0), dict(type=_lib.BF16), dict(type=8), dict(window=-1),
-    dict(scale=math.nan), dict(scale=math.inf), dict(cap=-1.0), dict(cap=math.nan), dict(q=FAR[5] + 2),
+    dict(scale=math.nan), dict(scale=math.inf), dict(cap=-1.0), dict(cap=math.nan), dict(cap=1e-20), dict(scale=1e-30), dict(q=FAR[5] + 2),
     dict(out=FAR[9] + 8), dict(out=FAR[5]), dict(out=FAR[5] + 6 * 4 * 64 * 2 - 16), dict(out=FAR[0] + 16)])
 def test_attention_arguments_are_refused(bad):
     assert attn(**bad) == _lib.IHIP_ERR_INVALID, said()
 
 
 def test_attention_sizes_past_the_index_ranges_are_refused():
-    assert attn(b=batch(table_stride=1 << 30)) == _lib.IHIP_ERR_INVALID
-    assert b"2^31" in said()
+    for stride in (1 << 30, (1 << 26) + 1):  # 2^30 + 16 tokens
+        assert attn(b=batch(table_stride=stride)) == _lib.IHIP_ERR_INVALID
+        assert b"2^30" in said()
     assert attn(b=batch(tokens=1 << 30)) == _lib.IHIP_ERR_INVALID
 
 
@@ -118,7 +119,7 @@ def fork(**kw):
     dict(sequences=-1), dict(children=-1), dict(room=-1), dict(stride=0), dict(page=0), dict(pages=0), dict(table=None),
     dict(lens=None), dict(parents=None), dict(refs=None), dict(table_out=None), dict(lens_out=None), dict(copies=None),
     dict(scratch=None), dict(table_out=FAR[10] + 16), dict(lens_out=FAR[12]), dict(copies=FAR[14]), dict(refs=FAR[11]),
-    dict(scratch=FAR[16] + 8), dict(children=1 << 20, stride=1 << 20), dict(stride=1 << 28)])
+    dict(scratch=FAR[16] + 8), dict(pages=2 ** 31 - 1), dict(children=1 << 20, stride=1 << 20), dict(stride=1 << 28)])
 def test_fork_arguments_are_refused(bad):
     assert fork(**bad) == _lib.IHIP_ERR_INVALID, said()
 
