@@ -507,7 +507,7 @@ size_t ihip_attn_paged_scratch_bytes(int q_type, int q_heads, const ihip_kv_cach
  * date; missing pages are taken from those with refs 0 (after what went back),
  * the lowest first, in order of child and place.  Where none is left the entry
  * is -1 and IHIP_FLAG_KV_FULL is set.  table and table_out must not overlap;
- * scratch: children ints.  All arrays are int32 in device memory.  Freeing,
+ * scratch: 2 * children ints.  All arrays are int32 in device memory.  Freeing,
  * reordering, extending and forking sequences are all this call. */
 int ihip_kv_fork_dev(const int32_t *table, const int32_t *lens, int sequences,
                      const int32_t *parents, int children, int room, int table_stride,

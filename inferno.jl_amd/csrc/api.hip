@@ -1711,7 +1711,7 @@ int ihip_kv_fork_dev(const int32_t *table, const int32_t *lens, int sequences,
     };
     // what is written may be nothing else that is read or written
     const Span ins[] = {{table, tb}, {lens, lb}, {parents, cb}};
-    const Span outs[] = {{refs, 4 * (size_t)pages}, {table_out, ob}, {lens_out, cb}, {copies, 2 * cb}, {scratch, cb}};
+    const Span outs[] = {{refs, 4 * (size_t)pages}, {table_out, ob}, {lens_out, cb}, {copies, 2 * cb}, {scratch, 2 * cb}};
     for (int i = 0; i < 5; ++i) {
         for (const Span &r : ins)
             if (r.n && outs[i].n && overlap(r.p, r.n, outs[i].p, outs[i].n))

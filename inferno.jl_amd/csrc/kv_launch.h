@@ -66,7 +66,7 @@ struct ForkArgs {
     const int32_t *table, *lens, *parents;
     int sequences, children, stride, page_size, room, pages;
     int32_t *refs, *table_out, *lens_out, *copies;
-    int32_t *fresh; // children ints of scratch: pages each child is missing
+    int32_t *fresh; // 2 x children ints of scratch: pages each child is missing, and from where
     uint32_t *flags;
 };
 hipError_t launch_kv_fork(const ForkArgs &a, hipStream_t s);

@@ -26,22 +26,19 @@ __device__ __forceinline__ int wave_find(const int32_t *v, int n, int want)
     return n;
 }
 
-constexpr int FORK_THREADS = 256;
-
-// One workgroup a child, then one a parent.  A child's row takes over the pages
-// of its parent's: the first child of a parent all of them (no count changes),
-// a later one the full pages (their counts rise).  What a later child lacks,
-// and what a longer child lacks at its end, is left to k_fork_take as `fresh`.
-// A parent without a child gives its pages back.
-__global__ void __launch_bounds__(FORK_THREADS) k_fork_rows(ForkArgs a)
+// A wave's work on child i, or on parent i - children.  A child's row takes over
+// the pages of its parent's: the first child of a parent all of them (no count
+// changes), a later one the full pages (their counts rise).  What a later child
+// lacks, and what a longer child lacks at its end, is left to fork_take as
+// `fresh`.  A parent without a child gives its pages back.
+__device__ __forceinline__ void fork_row(const ForkArgs &a, int i)
 {
-    __shared__ int n_fresh, copied;
-    const int tid = threadIdx.x;
-    if (blockIdx.x >= a.children) {
-        const int p = blockIdx.x - a.children;
+    const int lane = threadIdx.x & 63;
+    if (i >= a.children) {
+        const int p = i - a.children;
         if (wave_find(a.parents, a.children, p) < a.children)
             return;
-        for (int j = tid; j < a.stride; j += FORK_THREADS) {
+        for (int j = lane; j < a.stride; j += 64) {
             const int id = a.table[(int64_t)p * a.stride + j];
             if ((unsigned)id < (unsigned)a.pages)
                 atomicSub(&a.refs[id], 1);
@@ -50,7 +47,7 @@ __global__ void __launch_bounds__(FORK_THREADS) k_fork_rows(ForkArgs a)
         }
         return;
     }
-    const int c = blockIdx.x, p = a.parents[c];
+    const int c = i, p = a.parents[c];
     const bool alive = (unsigned)p < (unsigned)a.sequences;
     const bool first = alive && wave_find(a.parents, a.children, p) == c;
     const int64_t cap = (int64_t)a.stride * a.page_size;
@@ -59,17 +56,11 @@ __global__ void __launch_bounds__(FORK_THREADS) k_fork_rows(ForkArgs a)
     const int full = len / a.page_size;
     const int64_t longer = ((int64_t)len + a.room + a.page_size - 1) / a.page_size;
     const int need = longer > a.stride ? a.stride : (int)longer;
-    if (tid == 0) {
-        n_fresh = 0;
-        copied = -1;
-        a.lens_out[c] = len;
-        if (a.flags && (told != len || longer > a.stride || p >= a.sequences))
-            atomicOr(a.flags, kFlagKvLength);
-    }
-    __syncthreads();
-    int mine = 0;
-    for (int j = tid; j < a.stride; j += FORK_THREADS) {
-        int id = alive ? a.table[(int64_t)p * a.stride + j] : -1;
+    int fresh = 0, copied = -1, from = a.stride;
+    for (int j0 = 0; j0 < a.stride; j0 += 64) {
+        const int j = j0 + lane;
+        const bool in = j < a.stride;
+        int id = in && alive ? a.table[(int64_t)p * a.stride + j] : -1;
         if (id >= a.pages) {
             if (a.flags)
                 atomicOr(a.flags, kFlagKvPage);
@@ -78,22 +69,38 @@ __global__ void __launch_bounds__(FORK_THREADS) k_fork_rows(ForkArgs a)
         const bool keep = id >= 0 && (first || j < full);
         if (keep && !first)
             atomicAdd(&a.refs[id], 1);
-        // -2: a page that k_fork_take is to find
-        const bool lacks = !keep && j < need;
-        mine += lacks;
-        a.table_out[(int64_t)c * a.stride + j] = keep ? id : lacks ? -2 : -1;
+        // -2: a page that fork_take is to find
+        const bool lacks = in && !keep && j < need;
+        const uint64_t lack = __ballot(lacks);
+        if (lack && !fresh)
+            from = j0;
+        fresh += __popcll(lack);
+        if (in)
+            a.table_out[(int64_t)c * a.stride + j] = keep ? id : lacks ? -2 : -1;
         // the page that this child shares no longer: copied into the one it gets
-        if (lacks && !first && id >= 0 && j == full && len % a.page_size)
-            copied = id;
+        const uint64_t part = __ballot(lacks && !first && id >= 0 && j == full && len % a.page_size);
+        if (part)
+            copied = __builtin_amdgcn_readlane(id, __builtin_ctzll(part));
     }
-    if (mine)
-        atomicAdd(&n_fresh, mine);
-    __syncthreads();
-    if (tid == 0) {
-        a.fresh[c] = n_fresh;
+    if (lane == 0) {
+        a.fresh[c] = fresh;
+        a.fresh[a.children + c] = from; // no entry before this place is missing
+        a.lens_out[c] = len;
         a.copies[2 * c] = copied;
         a.copies[2 * c + 1] = -1;
+        if (a.flags && (told != len || longer > a.stride || p >= a.sequences))
+            atomicOr(a.flags, kFlagKvLength);
     }
+}
+
+constexpr int FORK_THREADS = 256;
+constexpr int FORK_ROWS = 64, FORK_ENTRIES = 1 << 14; // tables that one workgroup takes
+
+__global__ void __launch_bounds__(FORK_THREADS) k_fork_rows(ForkArgs a)
+{
+    const int i = blockIdx.x * (FORK_THREADS / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (i < a.children + a.sequences)
+        fork_row(a, i);
 }
 
 constexpr int TAKE_THREADS = 1024;
@@ -128,7 +135,7 @@ __device__ __forceinline__ int block_scan(int v, int *part, int &total)
 // One workgroup: free pages are found 4096 counts at a time and each step hands
 // out what it found; the search ends with the last entry, so that it reads the
 // counts only up to there.
-__global__ void __launch_bounds__(TAKE_THREADS) k_fork_take(ForkArgs a)
+__device__ __forceinline__ void fork_take(const ForkArgs &a)
 {
     __shared__ int part[TAKE_THREADS / 64];
     __shared__ int found[TAKE_THREADS * TAKE_PER];
@@ -172,7 +179,7 @@ __global__ void __launch_bounds__(TAKE_THREADS) k_fork_take(ForkArgs a)
             // entries that an earlier step filled are no longer -2: the count
             // starts behind them
             int rank = max(lo, given);
-            for (int j0 = 0; j0 < a.stride; j0 += 64) {
+            for (int j0 = a.fresh[a.children + c]; j0 < a.stride && rank < min(hi, last); j0 += 64) {
                 const int j = j0 + lane;
                 const bool lacks = j < a.stride && row[j] == -2;
                 const uint64_t all = __ballot(lacks);
@@ -201,6 +208,17 @@ __global__ void __launch_bounds__(TAKE_THREADS) k_fork_take(ForkArgs a)
             if (a.copies[2 * c + 1] < 0)
                 a.copies[2 * c] = -1;
     }
+}
+
+__global__ void __launch_bounds__(TAKE_THREADS) k_fork_take(ForkArgs a) { fork_take(a); }
+
+// Both for small tables, as one launch.
+__global__ void __launch_bounds__(TAKE_THREADS) k_fork(ForkArgs a)
+{
+    for (int i = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); i < a.children + a.sequences; i += TAKE_THREADS / 64)
+        fork_row(a, i);
+    __syncthreads(); // (the counts' atomics and the rows are in L2, and no wave has read them before)
+    fork_take(a);
 }
 
 // The used pages at or behind index `used` (their number), in order, to the
@@ -353,7 +371,13 @@ __global__ void __launch_bounds__(COPY_THREADS) k_kv_copy(CopyArgs a)
 
 hipError_t launch_kv_fork(const ForkArgs &a, hipStream_t s)
 {
-    hipLaunchKernelGGL(k_fork_rows, dim3(a.children + a.sequences), dim3(FORK_THREADS), 0, s, a);
+    const int64_t rows = (int64_t)a.children + a.sequences;
+    if (a.children > 0 && rows <= FORK_ROWS && rows * a.stride <= FORK_ENTRIES) {
+        hipLaunchKernelGGL(k_fork, dim3(1), dim3(TAKE_THREADS), 0, s, a);
+        return hipGetLastError();
+    }
+    hipLaunchKernelGGL(k_fork_rows, dim3((uint32_t)((rows + FORK_THREADS / 64 - 1) / (FORK_THREADS / 64))), dim3(FORK_THREADS),
+                       0, s, a);
     if (a.children > 0)
         hipLaunchKernelGGL(k_fork_take, dim3(1), dim3(TAKE_THREADS), 0, s, a);
     return hipGetLastError();

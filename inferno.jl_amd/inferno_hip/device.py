@@ -597,7 +597,7 @@ def kv_fork(table: torch.Tensor, lens: torch.Tensor, parents: torch.Tensor, refs
     sequences, width = table.shape
     n, where = parents.numel(), table.device
     # the new table; its lengths, the copies and the scratch
-    new, ints = (torch.empty(n, width, dtype=torch.int32, device=where), torch.empty(4 * n, dtype=torch.int32, device=where))
+    new, ints = (torch.empty(n, width, dtype=torch.int32, device=where), torch.empty(5 * n, dtype=torch.int32, device=where))
     _held(stream, new, ints)
     p = ints.data_ptr()
     _launch(dev, stream, lib().ihip_kv_fork_dev, tp, _at(lens, torch.int32, "lens", dev), sequences,
