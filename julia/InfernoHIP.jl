@@ -600,6 +600,7 @@ module Device
 # pointers to GGML blocks (e.g. `GGUF.upload`).
 export gemv!, gemv_add!, gemv_norm!, dequantize!, rmsnorm!, gate_up_swiglu!, lm_head_argmax_norm!
 export register_group, weight_bytes
+export rope_turns, rope_kv!, attn_paged!, attn_paged_scratch_bytes, kv_fork!, kv_compact!, kv_copy!
 
 import ..InfernoHIP: LIBIHIP, check, require, ArgmaxWorkspace, token_ptr, flags_ptr, read_token
 
@@ -767,6 +768,171 @@ function register_group(datas::Vector{Vector{UInt8}}, w_type::Integer, inner::In
     p = Ref{Ptr{Cvoid}}(C_NULL)
     check(ccall((:ihip_weight_device_ptr, LIBIHIP), Cint, (UInt64, Ref{Ptr{Cvoid}}), h[], p))
     return h[], p[]
+end
+
+# ---- attention over a paged cache (src/ModelCPU.jl:789-885) -------------------
+const F32, F16, BF16 = 0, 1, 30 # GGML type ids
+const ROPE_SCALINGS = (none = 0, linear = 1, ntk = 2, yarn = 3, bands = 4)
+
+"""
+One layer's paged cache (`ihip_kv_cache`): device pools of `pages` pages of
+`page_size` tokens x `kv_heads` x `head_dim` values of type F16 or BF16; Julia
+arrays of size (head_dim, page_size, kv_heads, pages) have this layout with
+`page_stride = head_dim * page_size * kv_heads`.
+"""
+struct KVCache
+    k::Ptr{Cvoid}
+    v::Ptr{Cvoid}
+    type::Cint
+    pages::Cint
+    page_size::Cint
+    kv_heads::Cint
+    head_dim::Cint
+    page_stride::Int64
+end
+
+"""
+The sequences of a call (`ihip_kv_batch`): device arrays of Int32 -- `q_starts`
+(sequences + 1 row offsets from 0), `kv_lens` and `page_table` (`table_stride`
+page ids from 0 a sequence) -- and the rows of q.
+"""
+struct KVBatch
+    q_starts::Ptr{Int32}
+    kv_lens::Ptr{Int32}
+    page_table::Ptr{Int32}
+    sequences::Cint
+    table_stride::Cint
+    tokens::Cint
+end
+
+"""
+    rope_turns(rot_dim, base; scaling, factor, original, low, high) -> (turns, mscale)
+
+Turns per position of the rot_dim / 2 rotated pairs, in 64 bits (upload once),
+and the factor on the rotated values.  `scaling` is one of :none, :linear, :ntk,
+:yarn, :bands.
+"""
+function rope_turns(rot_dim::Integer, base::Real; scaling::Symbol = :none, factor::Real = 1.0,
+                    original::Integer = 0, low::Real = 1.0, high::Real = 32.0)
+    turns = Vector{Float64}(undef, rot_dim ÷ 2)
+    m = Ref{Cfloat}(1)
+    check(ccall((:ihip_rope_turns, LIBIHIP), Cint,
+                (Cint, Cint, Cdouble, Cdouble, Cint, Cdouble, Cdouble, Ptr{Float64}, Ref{Cfloat}),
+                ROPE_SCALINGS[scaling], rot_dim, base, factor, original, low, high, turns, m))
+    return turns, m[]
+end
+
+"""
+    rope_kv!(q_out, q_type, q, q_stride, k, k_stride, v, v_stride, q_heads, turns, rot_dim,
+             cache, batch; q_norm, k_norm, eps, interleaved, mscale, positions, flags, stream)
+
+The q and k norms, the rotary positions and the append of k and v to the cache,
+in one launch from the projections' fp32 outputs (device pointers; strides in
+floats from token to token, so a grouped wq/wk/wv GEMV's output is passed as
+three offsets into it).
+"""
+function rope_kv!(q_out::Ptr{Cvoid}, q_type::Integer, q::Ptr{Float32}, q_stride::Integer,
+                  k::Ptr{Float32}, k_stride::Integer, v::Ptr{Float32}, v_stride::Integer,
+                  q_heads::Integer, turns::Ptr{Float64}, rot_dim::Integer, cache::KVCache,
+                  batch::KVBatch; q_norm::Ptr{Float32} = Ptr{Float32}(C_NULL),
+                  k_norm::Ptr{Float32} = Ptr{Float32}(C_NULL), eps::Real = 1f-6,
+                  interleaved::Bool = false, mscale::Real = 1f0,
+                  positions::Ptr{Int32} = Ptr{Int32}(C_NULL),
+                  flags::Ptr{UInt32} = Ptr{UInt32}(C_NULL), stream::Ptr{Cvoid} = C_NULL)
+    require()
+    check(ccall((:ihip_rope_kv_dev, LIBIHIP), Cint,
+                (Ptr{Float32}, Int64, Ptr{Float32}, Int64, Ptr{Float32}, Int64, Cint, Ptr{Float32},
+                 Ptr{Float32}, Cfloat, Ptr{Float64}, Cint, Cint, Cfloat, Ptr{Int32}, Ptr{Cvoid},
+                 Cint, Ref{KVCache}, Ref{KVBatch}, Ptr{UInt32}, Ptr{Cvoid}),
+                q, q_stride, k, k_stride, v, v_stride, q_heads, q_norm, k_norm, Float32(eps), turns,
+                rot_dim, interleaved ? 1 : 0, Float32(mscale), positions, q_out, q_type, Ref(cache),
+                Ref(batch), flags, stream))
+    return q_out
+end
+
+"""Workspace of `attn_paged!` for a batch of these sizes; its first 16384 bytes start as zeros."""
+attn_paged_scratch_bytes(q_type::Integer, q_heads::Integer, cache::KVCache, batch::KVBatch) =
+    Int(ccall((:ihip_attn_paged_scratch_bytes, LIBIHIP), Csize_t,
+              (Cint, Cint, Ref{KVCache}, Ref{KVBatch}), q_type, q_heads, Ref(cache), Ref(batch)))
+
+"""
+    attn_paged!(out, q, q_type, q_heads, scale, cache, batch; softcap, window, prefix_lens,
+                slopes, flags, workspace, workspace_bytes, stream)
+
+Grouped-query attention of the batch's new tokens over their pages
+(src/ModelCPU.jl:761-887, src/FlashAttention.jl:19-84): causal, optionally in a
+window, with a prefix that sees itself whole, capped scores and a bias that
+grows with the distance.  q and out: tokens x q_heads x head_dim of q_type (F32
+or the cache's type).
+"""
+function attn_paged!(out::Ptr{Cvoid}, q::Ptr{Cvoid}, q_type::Integer, q_heads::Integer, scale::Real,
+                     cache::KVCache, batch::KVBatch; softcap::Real = 0f0, window::Integer = 0,
+                     prefix_lens::Ptr{Int32} = Ptr{Int32}(C_NULL),
+                     slopes::Ptr{Float32} = Ptr{Float32}(C_NULL),
+                     flags::Ptr{UInt32} = Ptr{UInt32}(C_NULL), workspace::Ptr{Cvoid} = C_NULL,
+                     workspace_bytes::Integer = 0, stream::Ptr{Cvoid} = C_NULL)
+    require()
+    check(ccall((:ihip_attn_paged_dev, LIBIHIP), Cint,
+                (Ptr{Cvoid}, Cint, Ptr{Cvoid}, Cint, Cfloat, Cfloat, Cint, Ptr{Int32}, Ptr{Float32},
+                 Ref{KVCache}, Ref{KVBatch}, Ptr{UInt32}, Ptr{Cvoid}, Csize_t, Ptr{Cvoid}),
+                q, q_type, out, q_heads, Float32(scale), Float32(softcap), window, prefix_lens, slopes,
+                Ref(cache), Ref(batch), flags, workspace, workspace_bytes, stream))
+    return out
+end
+
+"""
+    kv_fork!(table_out, lens_out, copies, table, lens, sequences, parents, children, room,
+             table_stride, page_size, pages, refs, scratch; flags, stream)
+
+The page tables of the next step from the parents that were picked (device
+arrays of Int32, sequences and pages counted from 0): forks, reorders, extends
+and frees sequences; `copies` names the pages that `kv_copy!` has to copy.
+"""
+function kv_fork!(table_out::Ptr{Int32}, lens_out::Ptr{Int32}, copies::Ptr{Int32}, table::Ptr{Int32},
+                  lens::Ptr{Int32}, sequences::Integer, parents::Ptr{Int32}, children::Integer,
+                  room::Integer, table_stride::Integer, page_size::Integer, pages::Integer,
+                  refs::Ptr{Int32}, scratch::Ptr{Int32}; flags::Ptr{UInt32} = Ptr{UInt32}(C_NULL),
+                  stream::Ptr{Cvoid} = C_NULL)
+    require()
+    check(ccall((:ihip_kv_fork_dev, LIBIHIP), Cint,
+                (Ptr{Int32}, Ptr{Int32}, Cint, Ptr{Int32}, Cint, Cint, Cint, Cint, Cint, Ptr{Int32},
+                 Ptr{Int32}, Ptr{Int32}, Ptr{Int32}, Ptr{Int32}, Ptr{UInt32}, Ptr{Cvoid}),
+                table, lens, sequences, parents, children, room, table_stride, page_size, pages, refs,
+                table_out, lens_out, copies, scratch, flags, stream))
+    return nothing
+end
+
+"""
+    kv_compact!(table, entries, refs, pages, copies, moved, scratch; flags, stream)
+
+The used pages moved to the front of the pool: `table` and `refs` change in
+place, `copies` and `moved` are for `kv_copy!`.
+"""
+function kv_compact!(table::Ptr{Int32}, entries::Integer, refs::Ptr{Int32}, pages::Integer,
+                     copies::Ptr{Int32}, moved::Ptr{Int32}, scratch::Ptr{Int32};
+                     flags::Ptr{UInt32} = Ptr{UInt32}(C_NULL), stream::Ptr{Cvoid} = C_NULL)
+    require()
+    check(ccall((:ihip_kv_compact_dev, LIBIHIP), Cint,
+                (Ptr{Int32}, Int64, Ptr{Int32}, Cint, Ptr{Int32}, Ptr{Int32}, Ptr{Int32}, Ptr{UInt32},
+                 Ptr{Cvoid}),
+                table, entries, refs, pages, copies, moved, scratch, flags, stream))
+    return nothing
+end
+
+"""
+    kv_copy!(cache, copies, n; layers, layer_stride, count, flags, stream)
+
+Copies pages `copies[2i] -> copies[2i+1]` (pairs from 0, negative entries
+skipped) in every layer of the cache.
+"""
+function kv_copy!(cache::KVCache, copies::Ptr{Int32}, n::Integer; layers::Integer = 1,
+                  layer_stride::Integer = 0, count::Ptr{Int32} = Ptr{Int32}(C_NULL),
+                  flags::Ptr{UInt32} = Ptr{UInt32}(C_NULL), stream::Ptr{Cvoid} = C_NULL)
+    require()
+    check(ccall((:ihip_kv_copy_dev, LIBIHIP), Cint,
+                (Ref{KVCache}, Cint, Int64, Ptr{Int32}, Cint, Ptr{Int32}, Ptr{UInt32}, Ptr{Cvoid}),
+                Ref(cache), layers, layer_stride, copies, n, count, flags, stream))
+    return nothing
 end
 
 end # module Device
