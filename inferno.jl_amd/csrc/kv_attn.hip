@@ -1234,7 +1234,6 @@ AttnPlan attn_plan(int act, int kv_type, int q_heads, int kv_heads, int dim, int
     auto tiles_of = [&](int n) { return (rows - some) / n + some; };
     const bool fits = capacity <= 512 && tiles_of(AR_ROWS) * kv_heads <= 512;
     p.rows = rows <= 2 * (int64_t)AR_ROWS * some || fits ? AR_ROWS : AC_ROWS;
-    if (getenv("X_ROWS")) p.rows = atoi(getenv("X_ROWS"));
     p.tiles = (int)tiles_of(p.rows);
     const int64_t units = (int64_t)p.tiles * kv_heads;
     int64_t want;
@@ -1251,17 +1250,14 @@ AttnPlan attn_plan(int act, int kv_type, int q_heads, int kv_heads, int dim, int
         p.least = 256;
         want = units >= 256 ? 1 : room * std::min<int64_t>(some, 2) / units;
     }
-    if (getenv("X_LEAST")) p.least = atoi(getenv("X_LEAST"));
     // (a window, where there is one, ends a tile's keys: no part would lie behind)
     const int64_t reach = window ? std::min(capacity, (int64_t)window + p.rows + AC_KEYS) : capacity;
     const int64_t most = (reach + p.least - 1) / p.least;
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(most, want), AR_SPLITS));
-    if (getenv("X_SPLITS")) p.splits = std::min<int64_t>(most, atoi(getenv("X_SPLITS")));
     // Few tiles: two halves of a workgroup each, which end a long tile sooner
     // (512 tiles of a 2048-token prompt: 65 us against 77); of many, two
     // workgroups a CU come further (4096 tokens: 174 us against 200).
     p.halves = p.splits == 1 && units <= 512;
-    if (getenv("X_HALVES")) p.halves = atoi(getenv("X_HALVES"));
     // (with 4096 tiles and heads or more nothing is split: their counts are enough)
     p.bytes = p.splits > 1 ? 4 * (size_t)kAttnCounts + (size_t)p.splits * tokens * q_heads * (dim + 2) * 4 : 0;
     return p;
