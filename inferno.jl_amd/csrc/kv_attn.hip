@@ -755,6 +755,12 @@ constexpr int ac_half_keys(int parts, int dp) { return dp == 256 && parts == 3 ?
 // Waves a SIMD: two, where a wave's operands fit 256 registers.
 constexpr int ac_waves(int parts, int dp) { return dp <= 64 || (dp <= 128 && parts <= 2) ? 2 : 1; }
 
+// Operands read from LDS a set of products ahead, where the registers allow it (a
+// cap's would spill).  us, ahead against not, 2048 rows of 32 heads over 8192 keys,
+// bf16: 128 wide 281, 294, with a bias 310, 325, with a cap 457, 370; 64 wide 190,
+// 205, with a cap 268, 273.
+constexpr bool ac_ahead(int parts, int dp, int feat) { return parts == 1 && (dp <= 64 || (dp <= 128 && feat != kCap)); }
+
 // Where 16-byte chunk c of key row r lies in its row of LDS: K's so that the 16
 // rows of a matrix operand's read lie in different banks, V's so that the four
 // rows and 64 bytes of a pair of transposing reads do.
@@ -787,6 +793,7 @@ k_attn_chunk(AttnArgs a, int tiles, int least, int splits)
     constexpr int RUN = HK / 4, NI = RUN * DP / 512; // keys that a wave copies, in NI copies of 1 KB
     constexpr int KS = DP / 16, DT = DP / 32, NC = DP / 8;
     constexpr int TILE = KEYS * DP * 2;
+    constexpr bool AHEAD = ac_ahead(PARTS, DP, FEAT);
     constexpr float kUp = C::kShift != 0.0f ? 8.0f : 0.0f; // p times 2^kUp, with room for kLate
     constexpr float kLate = 7.0f; // the sums are scaled again when the maximum has grown by more than 2^kLate
     __shared__ __attribute__((aligned(16))) uint8_t lds[4 * TILE]; // K, V of two steps
@@ -940,19 +947,61 @@ k_attn_chunk(AttnArgs a, int tiles, int least, int splits)
 
         const uint32_t k_here = lds0 + 2 * TILE * (step & 1) + HK * half * (DP * 2) + kat;
         const uint32_t v_here = lds0 + 2 * TILE * (step & 1) + HK * half * (DP * 2) + TILE + vat;
+        auto read_k = [&](int u, int i) { // (256 wide: chunks 16 and up lie 256 bytes on)
+            return read_lds<V8>((k_here ^ (32 * (i & 7))) + 32 * u * (DP * 2) + (i >> 3) * 256);
+        };
+        auto read_v = [&](int u, int d, int k) {
+            const uint32_t at = (v_here ^ (64 * (d & 3))) + (32 * u + 16 * k) * (DP * 2) + (d >> 2) * 256;
+            const V4 lo = read_tr_at<V4>(at), hi = read_tr_at<V4>(at + 8 * (DP * 2));
+            return (V8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        };
         f16v s[SU];
+        V8 vf[AHEAD ? DT : 1][2];
+        if constexpr (AHEAD) {
+            V8 kf[SU][KS];
 #pragma unroll
-        for (int u = 0; u < SU; ++u) {
-            s[u] = f16v{};
+            for (int i = 0; i < KS; ++i)
+                kf[0][i] = read_k(0, i);
+#pragma unroll
+            for (int u = 0; u < SU; ++u) {
+                s[u] = f16v{};
+#pragma unroll
+                for (int i = 0; i < KS; ++i) {
+                    if (u + 1 < SU)
+                        kf[u + 1][i] = read_k(u + 1, i);
+                    s[u] = C::mfma32(kf[u][i], qf[0][i], s[u]);
+                }
+            }
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+                    vf[d][k] = read_v(0, d, k);
+            // (in this order: LDS reads 0x100, products 8)
+            __builtin_amdgcn_sched_group_barrier(0x100, KS, 0);
 #pragma unroll
             for (int i = 0; i < KS; ++i) {
-                // (256 wide: chunks 16 and up lie 256 bytes on)
-                const V8 kf = read_lds<V8>((k_here ^ (32 * (i & 7))) + 32 * u * (DP * 2) + (i >> 3) * 256);
+                __builtin_amdgcn_sched_group_barrier(8, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            }
 #pragma unroll
-                for (int part = 0; part < PARTS; ++part)
-                    s[u] = C::mfma32(kf, qf[part][i], s[u]);
-                if (DP == 256 && i % 8 == 7)
-                    __builtin_amdgcn_sched_barrier(0); // (operands further ahead would not fit the registers)
+            for (int i = 0; i < KS; ++i) {
+                __builtin_amdgcn_sched_group_barrier(8, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 4 * DT / KS, 0);
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < SU; ++u) {
+                s[u] = f16v{};
+#pragma unroll
+                for (int i = 0; i < KS; ++i) {
+                    const V8 kf = read_k(u, i);
+#pragma unroll
+                    for (int part = 0; part < PARTS; ++part)
+                        s[u] = C::mfma32(kf, qf[part][i], s[u]);
+                    if (DP == 256 && i % 8 == 7)
+                        __builtin_amdgcn_sched_barrier(0); // (operands further ahead would not fit the registers)
+                }
             }
         }
         if constexpr (FEAT != kPlain) {
@@ -1046,6 +1095,12 @@ k_attn_chunk(AttnArgs a, int tiles, int least, int splits)
                 }
             }
             clear_odd(step);
+            if constexpr (AHEAD)
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+                        vf[d][k] = read_v(0, d, k);
         }
         // 32 keys at a time: their weights, then their products
 #pragma unroll
@@ -1069,12 +1124,16 @@ k_attn_chunk(AttnArgs a, int tiles, int least, int splits)
                     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
-                    const uint32_t at = (v_here ^ (64 * (d & 3))) + (32 * u + 16 * k) * (DP * 2) + (d >> 2) * 256;
-                    const V4 lo = read_tr_at<V4>(at), hi = read_tr_at<V4>(at + 8 * (DP * 2));
-                    const V8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                    if constexpr (AHEAD) {
+                        o[d] = C::mfma32(vf[d][k], pf[0][k], o[d]);
+                        if (u + 1 < SU)
+                            vf[d][k] = read_v(u + 1, d, k);
+                    } else {
+                        const V8 v = read_v(u, d, k);
 #pragma unroll
-                    for (int part = 0; part < PARTS; ++part)
-                        o[d] = C::mfma32(v, pf[part][k], o[d]);
+                        for (int part = 0; part < PARTS; ++part)
+                            o[d] = C::mfma32(v, pf[part][k], o[d]);
+                    }
                 }
             }
         }
