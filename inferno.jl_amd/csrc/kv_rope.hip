@@ -38,9 +38,11 @@ __device__ __forceinline__ void store8(void *base, int64_t at, int type, float8 
 }
 
 // A workgroup takes `hb` of one token's q_heads + 2 kv heads.  Bound by bytes
-// for a prompt, by its launch for a decode step.  The heads go through LDS:
-// the two values of a pair lie rot/2 apart or side by side, and either way a
-// thread then writes 8 neighbours at once.
+// for a prompt (8192 tokens of 32 + 16 heads, 128 wide: 302 MB in 67 us, 4.5 TB/s;
+// 113 with the values in indexed arrays), by its launch and three loads that wait
+// for each other for a decode step (4.6 us).  The heads go through LDS: the two
+// values of a pair lie rot/2 apart or side by side, and either way a thread then
+// writes 8 neighbours at once.
 __global__ void __launch_bounds__(ROPE_THREADS) k_rope_kv(RopeArgs a)
 {
     __shared__ __attribute__((aligned(16))) float x[ROPE_FLOATS];
@@ -184,7 +186,8 @@ hipError_t launch_rope_kv(RopeArgs a, hipStream_t s)
 {
     const int heads = a.q_heads + 2 * a.kv_heads;
     int hb = ROPE_FLOATS / a.dim < ROPE_HEADS ? ROPE_FLOATS / a.dim : ROPE_HEADS;
-    // few tokens: one 16-byte load a thread, spread over more workgroups
+    // few tokens: one 16-byte load a thread, spread over more workgroups (us, spread
+    // against not: 1 token 4.6, 4.9; 61 5.0, 5.9; 128 4.7, 4.6; 1000 14.7, 11.0)
     const int small = ROPE_THREADS * 4 / a.dim;
     if ((int64_t)a.batch.tokens * ((heads + hb - 1) / hb) < 2 * device_cus())
         hb = small < hb ? small : hb;
