@@ -768,11 +768,15 @@ constexpr int ac_half_keys(int parts, int dp) { return dp == 256 && parts == 3 ?
 // Waves a SIMD: two, where a wave's operands fit 256 registers.
 constexpr int ac_waves(int parts, int dp) { return dp <= 64 || (dp <= 128 && parts <= 2) ? 2 : 1; }
 
-// Operands read from LDS a set of products ahead, where the registers allow it (a
-// cap's would spill).  us, ahead against not, 2048 rows of 32 heads over 8192 keys,
-// bf16: 128 wide 281, 294, with a bias 310, 325, with a cap 457, 370; 64 wide 190,
-// 205, with a cap 268, 273.
-constexpr bool ac_ahead(int parts, int dp, int feat) { return parts == 1 && (dp <= 64 || (dp <= 128 && feat != kCap)); }
+// Operands read from LDS some products ahead, where the registers allow it.  us,
+// ahead against not, 2048 rows of 32 heads over 8192 keys, 1 part: 64 wide 190, 205;
+// 128 wide 281, 294, with a bias 310, 325, with a cap 457, 370 (it spills); 256 wide
+// 710, 830, with a bias 855, 972, with a cap 1409, 975.  Over 4096 keys, 3 parts,
+// 128 wide: 320, 329, with a cap 369, 395; 2 parts, 64 wide: 145, 149.
+constexpr bool ac_ahead(int parts, int dp, int feat)
+{
+    return parts == 1 ? dp <= 64 || feat != kCap : dp <= 64 || (parts == 3 && dp <= 128);
+}
 
 // Where 16-byte chunk c of key row r lies in its row of LDS: K's so that the 16
 // rows of a matrix operand's read lie in different banks, V's so that the four
@@ -990,7 +994,9 @@ k_attn_chunk(AttnArgs a, int tiles, int least, int splits)
                 for (int i = 0; i < KS; ++i) {
                     if (u + 1 < SU)
                         kf[u + 1][i] = read_k(u + 1, i);
-                    s[u] = C::mfma32(kf[u][i], qf[0][i], s[u]);
+#pragma unroll
+                    for (int part = 0; part < PARTS; ++part)
+                        s[u] = C::mfma32(kf[u][i], qf[part][i], s[u]);
                 }
             }
 #pragma unroll
@@ -999,16 +1005,17 @@ k_attn_chunk(AttnArgs a, int tiles, int least, int splits)
                 for (int k = 0; k < 2; ++k)
                     vf[d][k] = read_v(0, d, k);
             // (in this order: LDS reads 0x100, products 8)
-            __builtin_amdgcn_sched_group_barrier(0x100, KS, 0);
+            constexpr int FIRST = KS < 8 ? KS : 8;
+            __builtin_amdgcn_sched_group_barrier(0x100, FIRST, 0);
 #pragma unroll
-            for (int i = 0; i < KS; ++i) {
-                __builtin_amdgcn_sched_group_barrier(8, 1, 0);
+            for (int i = 0; i < SU * KS - FIRST; ++i) {
+                __builtin_amdgcn_sched_group_barrier(8, PARTS, 0);
                 __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             }
 #pragma unroll
-            for (int i = 0; i < KS; ++i) {
-                __builtin_amdgcn_sched_group_barrier(8, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x100, 4 * DT / KS, 0);
+            for (int i = 0; i < FIRST; ++i) {
+                __builtin_amdgcn_sched_group_barrier(8, PARTS, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 4 * DT / FIRST, 0);
             }
         } else {
 #pragma unroll
@@ -1141,12 +1148,14 @@ k_attn_chunk(AttnArgs a, int tiles, int least, int splits)
             }
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
-                if (DP == 256 && d % 2 == 0)
+                if (DP == 256 && !AHEAD && d % 2 == 0)
                     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
                     if constexpr (AHEAD) {
-                        o[d] = C::mfma32(vf[d][k], pf[0][k], o[d]);
+#pragma unroll
+                        for (int part = 0; part < PARTS; ++part)
+                            o[d] = C::mfma32(vf[d][k], pf[part][k], o[d]);
                         if (u + 1 < SU)
                             vf[d][k] = read_v(u + 1, d, k);
                     } else {
