@@ -410,11 +410,16 @@ def _same_device(dev: int, *others):
             raise _invalid(f"a cache or batch on device {t.index}, tensors on {dev}")
 
 
-def _held(stream, *tensors):
-    """Tensors allocated here, on the current stream, and used on `stream`."""
-    if stream is not None:
-        for t in tensors:
-            t.record_stream(stream)
+def _fresh(stream, make):
+    """make()'s tensor for a call on `stream`: allocated (and filled) there, since
+    work that the current stream still has ahead of it may use the same memory, and
+    kept from other uses while the current stream reads it."""
+    if stream is None:
+        return make()
+    with torch.cuda.stream(stream):
+        t = make()
+    t.record_stream(torch.cuda.current_stream(t.device))
+    return t
 
 
 class KVCache:
@@ -526,8 +531,7 @@ def rope_kv(q: torch.Tensor, k, v, turns: torch.Tensor, cache: KVCache, batch: K
         kp, ks, _ = _heads(k, "k", dev, T, cache.kv_heads, D)
         vp, vs, _ = _heads(v, "v", dev, T, cache.kv_heads, D)
     if out is None:
-        out = torch.empty(q.shape, dtype=out_dtype or torch.float32, device=q.device)
-        _held(stream, out)
+        out = _fresh(stream, lambda: torch.empty(q.shape, dtype=out_dtype or torch.float32, device=q.device))
     elif out.shape != q.shape:
         raise _invalid("out must have q's shape")
     kind = out.dtype
@@ -544,8 +548,9 @@ def rope_kv(q: torch.Tensor, k, v, turns: torch.Tensor, cache: KVCache, batch: K
 
 def attn_workspace(q_heads: int, cache: KVCache, batch: KVBatch):
     """The workspace of attn_paged for a batch of these sizes (q of either type),
-    or None where it needs none.  It starts as zeros, and every call leaves what
-    has to be zero so.  Calls that share one must not overlap."""
+    or None where it needs none.  It starts as zeros, written on the current stream,
+    and every call leaves what has to be zero so.  Calls that share one must not
+    overlap."""
     n = lib().ihip_attn_paged_scratch_bytes(_lib.F32, q_heads, cache.ref, batch.ref)
     return torch.zeros(n, dtype=torch.uint8, device=cache.device) if n else None
 
@@ -568,14 +573,13 @@ def attn_paged(q: torch.Tensor, cache: KVCache, batch: KVBatch, scale: float = N
     H, dev = shape[1], q.get_device()
     _same_device(dev, cache, batch)
     if out is None:
-        out = torch.empty_like(q)
-        _held(stream, out)
+        out = _fresh(stream, lambda: torch.empty_like(q))
     elif out.shape != shape:
         raise _invalid("out must have q's shape and type")
     if workspace is None:
-        workspace = attn_workspace(H, cache, batch)
-        if workspace is not None:
-            _held(stream, workspace)
+        n = lib().ihip_attn_paged_scratch_bytes(_lib.F32, H, cache.ref, batch.ref)
+        if n:
+            workspace = _fresh(stream, lambda: torch.zeros(n, dtype=torch.uint8, device=q.device))
     _launch(dev, stream, lib().ihip_attn_paged_dev, _at(q, q.dtype, "q", dev), act, _at(out, q.dtype, "out", dev), H,
             D ** -0.5 if scale is None else scale, softcap, window,
             _at(prefix_lens, torch.int32, "prefix_lens", dev, batch.sequences),
@@ -597,8 +601,8 @@ def kv_fork(table: torch.Tensor, lens: torch.Tensor, parents: torch.Tensor, refs
     sequences, width = table.shape
     n, where = parents.numel(), table.device
     # the new table; its lengths, the copies and the scratch
-    new, ints = (torch.empty(n, width, dtype=torch.int32, device=where), torch.empty(5 * n, dtype=torch.int32, device=where))
-    _held(stream, new, ints)
+    new = _fresh(stream, lambda: torch.empty(n, width, dtype=torch.int32, device=where))
+    ints = _fresh(stream, lambda: torch.empty(5 * n, dtype=torch.int32, device=where))
     p = ints.data_ptr()
     _launch(dev, stream, lib().ihip_kv_fork_dev, tp, _at(lens, torch.int32, "lens", dev), sequences,
             _at(parents, torch.int32, "parents", dev), n, room, width, page_size, refs.numel(),
@@ -614,8 +618,7 @@ def kv_compact(table: torch.Tensor, refs: torch.Tensor, flags=None, stream=None)
     dev, pages = table.get_device(), refs.numel()
     tp, n = _ptr(table, torch.int32, "table"), pages // 2
     # the moves, the scratch and the moves' number
-    ints = torch.empty(2 * n + pages + 1, dtype=torch.int32, device=table.device)
-    _held(stream, ints)
+    ints = _fresh(stream, lambda: torch.empty(2 * n + pages + 1, dtype=torch.int32, device=table.device))
     p = ints.data_ptr()
     _launch(dev, stream, lib().ihip_kv_compact_dev, tp, table.numel(), _at(refs, torch.int32, "refs", dev), pages, p,
             p + 4 * (2 * n + pages), p + 8 * n, _at(flags, torch.int32, "flags", dev, 1))
