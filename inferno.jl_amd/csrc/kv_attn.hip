@@ -772,11 +772,15 @@ constexpr int ac_waves(int parts, int dp) { return dp <= 64 || (dp <= 128 && par
 // ahead against not, 2048 rows of 32 heads over 8192 keys, 1 part: 64 wide 190, 205;
 // 128 wide 281, 294, with a bias 310, 325, with a cap 457, 370 (it spills); 256 wide
 // 710, 830, with a bias 855, 972, with a cap 1409, 975.  Over 4096 keys, 3 parts,
-// 128 wide: 320, 329, with a cap 369, 395; 2 parts, 64 wide: 145, 149.
+// 128 wide: 320, 329, with a cap 369, 395; 2 parts, 64 wide: 145, 149; 128 wide 208,
+// 213, with a cap 355, 246.
 constexpr bool ac_ahead(int parts, int dp, int feat)
 {
-    return parts == 1 ? dp <= 64 || feat != kCap : dp <= 64 || (parts == 3 && dp <= 128);
+    return dp <= 64 || (feat == kCap ? parts == 3 && dp <= 128 : parts == 1 || dp <= 128);
 }
+// K's operands on their way before the first product (2 parts, 128 wide: a
+// 2048-token prompt 97 us with 2, 98 with 8; the others have the room).
+constexpr int ac_first(int parts, int dp) { return parts == 2 && dp == 128 ? 2 : dp <= 64 ? dp / 16 : 8; }
 
 // Where 16-byte chunk c of key row r lies in its row of LDS: K's so that the 16
 // rows of a matrix operand's read lie in different banks, V's so that the four
@@ -1005,7 +1009,7 @@ k_attn_chunk(AttnArgs a, int tiles, int least, int splits)
                 for (int k = 0; k < 2; ++k)
                     vf[d][k] = read_v(0, d, k);
             // (in this order: LDS reads 0x100, products 8)
-            constexpr int FIRST = KS < 8 ? KS : 8;
+            constexpr int FIRST = ac_first(PARTS, DP);
             __builtin_amdgcn_sched_group_barrier(0x100, FIRST, 0);
 #pragma unroll
             for (int i = 0; i < SU * KS - FIRST; ++i) {
