@@ -411,9 +411,9 @@ typedef struct ihip_kv_cache {
  * tokens q_starts[s] .. q_starts[s+1] - 1 (rows of q; q_starts does not
  * decrease) and kv_lens[s] tokens in all, the new ones last: row i of n is at
  * cache position kv_lens[s] - n + i, whose page is page_table[s *
- * table_stride + position / page_size].  Rows behind the last sequence's (a
- * padded batch) are neither read nor written.  Sequences may share pages that
- * hold only earlier tokens. */
+ * table_stride + position / page_size].  Rows before the first sequence's and
+ * behind the last one's (a padded batch, a part of one) have no influence and
+ * are not written.  Sequences may share pages that hold only earlier tokens. */
 typedef struct ihip_kv_batch {
     const int32_t *q_starts;   /* sequences + 1 */
     const int32_t *kv_lens;    /* sequences */

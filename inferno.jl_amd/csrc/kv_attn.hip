@@ -233,11 +233,11 @@ __device__ __forceinline__ bool find_tile(const AttnArgs &a, int tiles, int leas
     t.head = bid % a.cache.heads;
     const int rest = bid / a.cache.heads;
     // (a prompt's last rows have the most keys: they go first)
-    const int want = tiles - 1 - rest % tiles;
+    int want = tiles - 1 - rest % tiles;
     t.split = rest / tiles;
     int first = 0;
     KvSeq q;
-    const int s = kv_find(a.batch, a.cache.page_shift, want, first, q,
+    const int s = kv_find<false>(a.batch, a.cache.page_shift, want, first, q,
                           [&](int n) { return (int)(((int64_t)n * a.group + ROWS - 1) / ROWS); });
     if (s < 0)
         return false;

@@ -69,8 +69,10 @@ __device__ __forceinline__ void kv_report(const KvBatch &b, int page_shift, uint
 // sequences at a time, so that a batch of up to 64 costs one round of loads.
 // Returns its index (-1: the batch has no such unit), the units of those before
 // it in `first` and the sequence itself in `q`.  All lanes must be active.
-template <typename F>
-__device__ __forceinline__ int kv_find(const KvBatch &b, int page_shift, int want, int &first, KvSeq &q, F units)
+// ROW: units are rows, and `want` comes as a row of q and is made the unit that
+// it is, counted from the first sequence's first row (which need not be row 0).
+template <bool ROW, typename F>
+__device__ __forceinline__ int kv_find(const KvBatch &b, int page_shift, int &want, int &first, KvSeq &q, F units)
 {
     const int lane = threadIdx.x & 63;
     int before = 0;
@@ -79,6 +81,11 @@ __device__ __forceinline__ int kv_find(const KvBatch &b, int page_shift, int wan
         KvSeq mine{0, 0, 0};
         if (s < b.sequences)
             mine = kv_seq(b, page_shift, s);
+        if (ROW && s0 == 0) {
+            want -= __builtin_amdgcn_readlane(mine.start, 0);
+            if (want < 0)
+                return -1;
+        }
         const int own = units(mine.n);
         int sum = own;
 #pragma unroll

@@ -74,10 +74,11 @@ __global__ void __launch_bounds__(ROPE_THREADS) k_rope_kv(RopeArgs a)
         kv_report(a.batch, a.cache.page_shift, a.flags);
     int first = 0;
     KvSeq seq;
-    const int s = kv_find(a.batch, a.cache.page_shift, token, first, seq, [](int n) { return n; });
+    int row = token;
+    const int s = kv_find<true>(a.batch, a.cache.page_shift, row, first, seq, [](int n) { return n; });
     if (s < 0)
-        return; // a row behind the last sequence
-    const int at = seq.len - seq.n + (token - first);
+        return; // a row before the first sequence or behind the last
+    const int at = seq.len - seq.n + (row - first);
     const int pos = a.positions ? a.positions[token] : at;
 
     for (int i = tid; i < a.rot / 2; i += ROPE_THREADS) {

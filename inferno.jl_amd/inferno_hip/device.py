@@ -560,8 +560,8 @@ def attn_paged(q: torch.Tensor, cache: KVCache, batch: KVBatch, scale: float = N
                stream=None) -> torch.Tensor:
     """Attention of the batch's new tokens over their pages (ihip_attn_paged_dev).
     q: tokens x q_heads x head_dim, fp32 or the cache's type, which out has too;
-    scale defaults to head_dim ** -0.5.  Rows of out behind the last sequence's
-    are not written."""
+    scale defaults to head_dim ** -0.5.  Rows of out before the first
+    sequence's and behind the last one's are not written."""
     T, D = batch.tokens, cache.head_dim
     if cache.layers_dim:
         raise _invalid("pass one layer of the cache (cache.layer(i))")
