@@ -11,6 +11,14 @@
 // sees no key gives 0.  The rows of a tile are those of one KV head's group of
 // q heads, token by token, so that a key that is read serves all of them.
 //
+// The weights are powers of two, 2^((s_j - m) by): m is kept in the units of the
+// products, and only differences are multiplied, so that scores of any size give
+// the weights that their differences say.  (fma(s_j, by, -m by) is one operation a
+// score less, but from scores of 2e7 on it rounds m by more than the room that p
+// has in fp16, and gives NaN or wrong weights.  us, this against that: 4096 tokens
+// over 32768 keys 2398, 2318; 2048 over 8192, 64 wide 199, 189, 128 wide 292, 284;
+// a 2048-token prompt of fp32 rows 95.6, 94.2; one token the same.)
+//
 // Both products run on the matrix cores, transposed: S^T = K Q^T puts a row's
 // scores in the lanes of one column, so that maxima and sums stay in a lane but
 // for one exchange between lane groups, and leaves P^T in the registers that
@@ -47,8 +55,8 @@ struct Half {
     typedef h2 V2;
     typedef h4 V4;
     typedef h8 V8;
-    // p = e^(s - m) is carried times 2^14: what fp16 keeps of small ones reaches
-    // down to 2^-38 of the largest
+    // p = e^(s - m) is carried times 2^14 by k_attn_rows: what fp16 keeps of small
+    // ones reaches down to 2^-38 of the largest (k_attn_chunk: see kUp there)
     static constexpr float kShift = 14.0f;
     static constexpr uint32_t kExp = 0x7c007c00u;
     static __device__ __forceinline__ f4 mfma16(V8 a, V8 b, f4 c)
@@ -158,25 +166,27 @@ __device__ __forceinline__ f2 get_shared(const uint64_t *p)
 
 // Four values of a row over its parts `from`, `from` + `by`, ... of n: their sum
 // (relative to `top`, as `sum` is), eight parts at a time with their maxima and
-// sums; `rows` rows lie between a row's parts.
+// sums; `rows` rows lie between a row's parts; `by` makes a difference of maxima a
+// power of two.
 struct Joined {
     float top, sum;
     f4 v;
-    __device__ __forceinline__ void add(float top2, float sum2, f4 v2)
+    __device__ __forceinline__ void add(float top2, float sum2, f4 v2, float by)
     {
         const float up = fmaxf(top, top2);
-        const float f = top == kNone ? 0.0f : exp2_fast(top - up), g = top2 == kNone ? 0.0f : exp2_fast(top2 - up);
+        const float f = top == kNone ? 0.0f : exp2_fast((top - up) * by);
+        const float g = top2 == kNone ? 0.0f : exp2_fast((top2 - up) * by);
         sum = sum * f + sum2 * g;
         v = v * f + v2 * g;
         top = up;
     }
 };
 __device__ __forceinline__ Joined join_parts(const uint64_t *o, const uint64_t *ml, int64_t rows, int dim, int from,
-                                             int by, int n)
+                                             int step, int n, float by)
 {
     constexpr int AT_ONCE = 8;
     Joined j{kNone, 0.0f, f4{}};
-    for (int p0 = AT_ONCE * from; p0 < n; p0 += AT_ONCE * by) {
+    for (int p0 = AT_ONCE * from; p0 < n; p0 += AT_ONCE * step) {
         f2 w[AT_ONCE], x[AT_ONCE], y[AT_ONCE];
 #pragma unroll
         for (int u = 0; u < AT_ONCE; ++u) {
@@ -189,14 +199,14 @@ __device__ __forceinline__ Joined join_parts(const uint64_t *o, const uint64_t *
 #pragma unroll
         for (int u = 0; u < AT_ONCE; ++u)
             up = p0 + u < n ? fmaxf(up, w[u].x) : up;
-        const float f = j.top == kNone ? 0.0f : exp2_fast(j.top - up);
+        const float f = j.top == kNone ? 0.0f : exp2_fast((j.top - up) * by);
         j.sum *= f;
         j.v *= f;
         j.top = up;
 #pragma unroll
         for (int u = 0; u < AT_ONCE; ++u)
             if (p0 + u < n && w[u].y != 0.0f) { // (sum 0: a part without keys has written nothing else; NaN stays)
-                const float g = w[u].x == kNone ? 0.0f : exp2_fast(w[u].x - up);
+                const float g = w[u].x == kNone ? 0.0f : exp2_fast((w[u].x - up) * by);
                 j.sum += w[u].y * g;
                 j.v += f4{x[u].x, x[u].y, y[u].x, y[u].y} * g;
             }
@@ -493,10 +503,10 @@ k_attn_rows(AttnArgs a, int tiles, int least, int splits)
         load_k();
         copy_v(step);
     }
-    const float scale = (a.scale == 0.0f ? 1.0f : fabsf(a.scale)) * undo;
     // scores become powers of two with the last factor, `by`; a cap takes the scale
-    // before, and the bias is added in units of `by`
-    const float by = FEAT == kCap ? a.cap * kLog2e : scale * kLog2e;
+    // before, and the bias is added in units of `by`.  `unit`, a power of two (the
+    // row's and the scale's), brings the maxima of a row's parts to one unit.
+    const float unit = FEAT == kCap ? 1.0f : __builtin_ldexpf(undo, a.scale_exp), by = a.by * unit;
     const float slope = FEAT != kPlain && a.slopes ? a.slopes[qhead] * kLog2e / by : 0.0f;
     const Seen sees = seen_from(a, t, pos);
 
@@ -537,7 +547,7 @@ k_attn_rows(AttnArgs a, int tiles, int least, int splits)
         if constexpr (FEAT != kPlain) {
             const float apart = (float)(pos - key - 4 * g);
             if constexpr (FEAT == kCap) {
-                const float by_cap = scale / a.cap;
+                const float by_cap = (a.scale == 0.0f ? 1.0f : fabsf(a.scale)) * undo / a.cap;
                 float most = 0.0f;
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
@@ -580,11 +590,11 @@ k_attn_rows(AttnArgs a, int tiles, int least, int splits)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 mx = fmaxf(mx, s[u][i]);
-        mx = fmaxf(groups_max(mx) * by, m);
+        mx = fmaxf(groups_max(mx), m);
         // (a row without a key yet keeps its sum 0 whatever is subtracted)
-        const float use = (mx == kNone ? 0.0f : mx) - C::kShift;
+        const float use = mx == kNone ? 0.0f : mx;
         if (__any(mx != m)) {
-            const float f = exp2_fast(m - use - C::kShift);
+            const float f = exp2_fast((m - use) * by);
             l *= f;
 #pragma unroll
             for (int d = 0; d < DT; ++d)
@@ -597,7 +607,7 @@ k_attn_rows(AttnArgs a, int tiles, int least, int splits)
         for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                float x = exp2_fast(fmaf(s[u][i], by, -use));
+                float x = exp2_fast(fmaf(s[u][i] - use, by, C::kShift));
                 s[u][i] = x;
                 sum += x;
 #pragma unroll
@@ -668,7 +678,7 @@ k_attn_rows(AttnArgs a, int tiles, int least, int splits)
     for (int d = 0; d < DT; ++d)
         *(f4 *)(ol + col * (DP + 4) + 16 * d + 4 * g) = o[d];
     if (g == 0) {
-        lds_m[wave][col] = m;
+        lds_m[wave][col] = m * unit;
         lds_l[wave][col] = l;
     }
     __syncthreads();
@@ -698,7 +708,7 @@ k_attn_rows(AttnArgs a, int tiles, int least, int splits)
         f4 v = f4{};
 #pragma unroll
         for (int w = 0; w < AR_WAVES; ++w) {
-            const float f = lds_m[w][r] == kNone ? 0.0f : exp2_fast(lds_m[w][r] - top);
+            const float f = lds_m[w][r] == kNone ? 0.0f : exp2_fast((lds_m[w][r] - top) * a.by);
             const f4 x = *(const f4 *)(lds + w * ar_wave_lds<DP>() + 4 * (r * (DP + 4) + d));
             sum += lds_l[w][r] * f;
             v += x * f;
@@ -737,7 +747,7 @@ k_attn_rows(AttnArgs a, int tiles, int least, int splits)
         const bool in = group < groups && e < items;
         const int r = in ? e / (D / 4) : 0, d = in ? 4 * (e % (D / 4)) : 0;
         Joined j = join_parts(part_o + (row_of(r) * D + d) / 2, part_ml + row_of(r), rows_all, D, group, groups,
-                              in ? t.parts : 0);
+                              in ? t.parts : 0, a.by);
         if (groups > 1) {
             if (in && group > 0)
                 lds_g[tid] = j;
@@ -745,7 +755,7 @@ k_attn_rows(AttnArgs a, int tiles, int least, int splits)
             if (!in || group > 0)
                 return;
             for (int q = 1; q < groups; ++q)
-                j.add(lds_g[tid + q * items].top, lds_g[tid + q * items].sum, lds_g[tid + q * items].v);
+                j.add(lds_g[tid + q * items].top, lds_g[tid + q * items].sum, lds_g[tid + q * items].v, a.by);
         }
         if (in)
             finish(r, d, j.v, j.sum);
@@ -823,8 +833,10 @@ k_attn_chunk(AttnArgs a, int tiles, int least, int splits)
     constexpr int KS = DP / 16, DT = DP / 32, NC = DP / 8;
     constexpr int TILE = KEYS * DP * 2;
     constexpr bool AHEAD = ac_ahead(PARTS, DP, FEAT);
-    constexpr float kUp = C::kShift != 0.0f ? 8.0f : 0.0f; // p times 2^kUp, with room for kLate
-    constexpr float kLate = 7.0f; // the sums are scaled again when the maximum has grown by more than 2^kLate
+    // p times 2^kUp, with room for 2^kLate below fp16's 2^16: kept down to 2^-32 of
+    // the largest; the sums are scaled again when the maximum has grown by 2^kLate
+    constexpr float kUp = C::kShift != 0.0f ? 8.0f : 0.0f;
+    constexpr float kLate = 7.0f;
     __shared__ __attribute__((aligned(16))) uint8_t lds[4 * TILE]; // K, V of two steps
     __shared__ int lds_odd;
     const int tid = threadIdx.x, lane = tid & 63;
@@ -849,10 +861,10 @@ k_attn_chunk(AttnArgs a, int tiles, int least, int splits)
     V8 qf[PARTS][KS];
     float undo;
     load_q<C, PARTS, KS>(a, qrow, live, 2, h, qf, undo);
-    const float scale = (a.scale == 0.0f ? 1.0f : fabsf(a.scale)) * undo;
     // scores become powers of two with the last factor, `by`; a cap takes the scale
-    // before, and the bias is added in units of `by`
-    const float by = FEAT == kCap ? a.cap * kLog2e : scale * kLog2e;
+    // before, and the bias is added in units of `by`.  by / a.by, a power of two (the
+    // row's and the scale's), brings the maxima of a row's parts to one unit.
+    const float by = FEAT == kCap ? a.by : a.by * __builtin_ldexpf(undo, a.scale_exp);
     const float slope = FEAT != kPlain && a.slopes ? a.slopes[qhead] * kLog2e / by : 0.0f;
     const Seen sees = seen_from(a, t, pos);
 
@@ -1039,7 +1051,7 @@ k_attn_chunk(AttnArgs a, int tiles, int least, int splits)
         if constexpr (FEAT != kPlain) {
             const float apart = (float)(pos - key - 4 * h);
             if constexpr (FEAT == kCap) {
-                const float by_cap = scale / a.cap;
+                const float by_cap = (a.scale == 0.0f ? 1.0f : fabsf(a.scale)) * undo / a.cap;
                 float most = 0.0f;
 #pragma unroll
                 for (int u = 0; u < SU; ++u)
@@ -1088,17 +1100,17 @@ k_attn_chunk(AttnArgs a, int tiles, int least, int splits)
 #pragma unroll
             for (int i = 0; i < 16; ++i)
                 mx = fmaxf(mx, s[u][i]);
-        mx = halves_max(mx) * by;
-        if (__any(mx > m + kLate || (m == kNone && mx != kNone))) {
+        mx = halves_max(mx);
+        if (__any((mx - m) * by > kLate)) { // (a row's first key: by an infinity; without one: NaN, no)
             const float top = fmaxf(mx, m);
-            const float f = top == kNone ? 1.0f : exp2_fast(m - top);
+            const float f = top == kNone ? 1.0f : exp2_fast((m - top) * by);
             l *= f;
 #pragma unroll
             for (int d = 0; d < DT; ++d)
                 o[d] *= f;
             m = top;
         }
-        const float use = (m == kNone ? 0.0f : m) - kUp;
+        const float use = m == kNone ? 0.0f : m;
         if (__builtin_expect(odd, 0)) {
             // infinities or NaNs that some rows of the tile see and others do not:
             // they are added one key at a time where a row has a weight for them,
@@ -1112,7 +1124,7 @@ k_attn_chunk(AttnArgs a, int tiles, int least, int splits)
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
                         x = i == e && u == j >> 5 ? s[u][e] : x;
-                x = __shfl(exp2_fast(fmaf(x, by, -use)), col + 32 * ((j >> 2) & 1));
+                x = __shfl(exp2_fast(fmaf(x - use, by, kUp)), col + 32 * ((j >> 2) & 1));
                 const uint8_t *const vj = vt + j * (DP * 2) + 8 * h;
 #pragma unroll
                 for (int d = 0; d < DT; ++d) {
@@ -1140,7 +1152,7 @@ k_attn_chunk(AttnArgs a, int tiles, int least, int splits)
             V8 pf[PARTS][2];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                float x = exp2_fast(fmaf(s[u][i], by, -use));
+                float x = exp2_fast(fmaf(s[u][i] - use, by, kUp));
                 s[u][i] = x;
                 l += x;
 #pragma unroll
@@ -1191,7 +1203,8 @@ k_attn_chunk(AttnArgs a, int tiles, int least, int splits)
         if (half)
             return;
         const float m2 = to[0], l2 = to[64], top = fmaxf(m, m2);
-        const float f = m == kNone ? 0.0f : exp2_fast(m - top), f2 = m2 == kNone ? 0.0f : exp2_fast(m2 - top);
+        const float f = m == kNone ? 0.0f : exp2_fast((m - top) * by);
+        const float f2 = m2 == kNone ? 0.0f : exp2_fast((m2 - top) * by);
         // (a half without keys has only zeros; NaN stays)
         l = l * f + l2 * f2;
 #pragma unroll
@@ -1208,7 +1221,7 @@ k_attn_chunk(AttnArgs a, int tiles, int least, int splits)
     const int64_t rows_all = (int64_t)a.batch.tokens * a.q_heads;
     if (splits > 1) {
         if (h == 0)
-            *(f2 *)(a.part + (int64_t)splits * rows_all * D + 2 * (t.split * rows_all + qrow)) = f2{m, l};
+            *(f2 *)(a.part + (int64_t)splits * rows_all * D + 2 * (t.split * rows_all + qrow)) = f2{m * (by / a.by), l};
         if (l == 0.0f)
             return;
     }
@@ -1249,14 +1262,16 @@ __global__ void __launch_bounds__(256) k_attn_join(AttnArgs a, int splits)
     const bool live = slot < slots && row < rows && token >= a.batch.starts[0] && token < a.batch.starts[a.batch.sequences];
     const int64_t at = live ? row : 0;
     const uint64_t *const o = (const uint64_t *)a.part, *const ml = o + (int64_t)splits * rows * D / 2;
-    Joined j = join_parts(o + (at * D + d) / 2, ml + at, rows, D, many ? slot : 0, many ? slots : 1, live ? splits : 0);
+    Joined j = join_parts(o + (at * D + d) / 2, ml + at, rows, D, many ? slot : 0, many ? slots : 1, live ? splits : 0,
+                          a.by);
     if (many) {
         lds_g[threadIdx.x] = j;
         __syncthreads();
         if (slot > 0)
             return;
         for (int q = 1; q < slots; ++q)
-            j.add(lds_g[threadIdx.x + q * per].top, lds_g[threadIdx.x + q * per].sum, lds_g[threadIdx.x + q * per].v);
+            j.add(lds_g[threadIdx.x + q * per].top, lds_g[threadIdx.x + q * per].sum, lds_g[threadIdx.x + q * per].v,
+                  a.by);
     }
     if (!live)
         return;
@@ -1358,8 +1373,11 @@ AttnPlan attn_plan(int act, int kv_type, int q_heads, int kv_heads, int dim, int
     return p;
 }
 
-hipError_t launch_attn(const AttnArgs &a, const AttnPlan &p, hipStream_t s)
+hipError_t launch_attn(AttnArgs a, const AttnPlan &p, hipStream_t s)
 {
+    a.scale_exp = 0;
+    a.by = a.cap > 0.0f ? a.cap * kLog2e
+                        : std::frexp(a.scale == 0.0f ? 1.0f : std::fabs(a.scale), &a.scale_exp) * kLog2e;
     if (a.cache.type == kF16)
         return a.act == kF32 ? start_dim<Half, 2>(a, p, s) : start_dim<Half, 1>(a, p, s);
     return a.act == kF32 ? start_dim<BHalf, 3>(a, p, s) : start_dim<BHalf, 1>(a, p, s);

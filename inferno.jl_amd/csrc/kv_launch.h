@@ -33,6 +33,8 @@ struct AttnArgs {
     void *out;
     int act, q_heads, group;
     float scale, cap;
+    float by;      // a score's factor to a power of two: the cap, or the scale without
+    int scale_exp; // its power of two, 2^scale_exp (both set by the launcher)
     int window;
     const int32_t *prefix;
     const float *slopes;
@@ -59,7 +61,7 @@ struct AttnPlan {
 // (which never needs less workspace).
 AttnPlan attn_plan(int act, int kv_type, int q_heads, int kv_heads, int dim, int sequences, int tokens,
                    int64_t capacity, int window);
-hipError_t launch_attn(const AttnArgs &a, const AttnPlan &p, hipStream_t s);
+hipError_t launch_attn(AttnArgs a, const AttnPlan &p, hipStream_t s);
 
 // kv_pages.hip
 struct ForkArgs {
