@@ -413,7 +413,9 @@ typedef struct ihip_kv_cache {
  * cache position kv_lens[s] - n + i, whose page is page_table[s *
  * table_stride + position / page_size].  Rows before the first sequence's and
  * behind the last one's (a padded batch, a part of one) have no influence and
- * are not written.  Sequences may share pages that hold only earlier tokens. */
+ * are not written.  Sequences may share pages that hold only earlier tokens.
+ * A batch without tokens or without sequences is nothing to do: its other sizes
+ * and types are checked, its buffers may be NULL. */
 typedef struct ihip_kv_batch {
     const int32_t *q_starts;   /* sequences + 1 */
     const int32_t *kv_lens;    /* sequences */

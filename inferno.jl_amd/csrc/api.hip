@@ -1571,8 +1571,6 @@ int ihip_rope_kv_dev(const float *q, int64_t q_stride, const float *k, int64_t k
     RET_IF(check_cache(cache, &a.cache));
     RET_IF(check_batch(batch, &a.batch));
     const int D = a.cache.dim;
-    if (!q || !q_out || (!k) != (!v) || (rot_dim && !turns))
-        return fail(IHIP_ERR_INVALID, "null pointer");
     if (q_heads <= 0 || q_heads > 65536)
         return fail(IHIP_ERR_INVALID, "q_heads=%d", q_heads);
     if (!value_bytes(q_type))
@@ -1581,14 +1579,16 @@ int ihip_rope_kv_dev(const float *q, int64_t q_stride, const float *k, int64_t k
         return fail(IHIP_ERR_INVALID, "rot_dim=%d is not an even number up to head_dim=%d", rot_dim, D);
     if (layout != IHIP_ROPE_HALF && layout != IHIP_ROPE_INTERLEAVED)
         return fail(IHIP_ERR_INVALID, "unknown layout %d", layout);
+    const int64_t T = a.batch.tokens;
+    if (T == 0 || a.batch.sequences == 0)
+        return IHIP_OK; // (an empty buffer has no address to check)
+    if (!q || !q_out || (!k) != (!v) || (rot_dim && !turns))
+        return fail(IHIP_ERR_INVALID, "null pointer");
     const int64_t qw = (int64_t)q_heads * D, kw = (int64_t)a.cache.heads * D;
     if (q_stride < qw || q_stride % 4 || (k && (k_stride < kw || k_stride % 4 || v_stride < kw || v_stride % 4)))
         return fail(IHIP_ERR_INVALID, "a stride is no multiple of 4 that holds a token's heads");
     if (!al16(q) || !al16(k) || !al16(v) || !al16(q_norm) || !al16(k_norm) || !al16(q_out) || ((uintptr_t)turns & 7))
         return fail(IHIP_ERR_INVALID, "a pointer is not 16-byte aligned");
-    const int64_t T = a.batch.tokens;
-    if (T == 0 || a.batch.sequences == 0)
-        return IHIP_OK;
     if (!grid_fits(T * (q_heads + 2 * a.cache.heads)) || q_stride > INT64_MAX / 8 / T ||
         (k && (k_stride > INT64_MAX / 8 / T || v_stride > INT64_MAX / 8 / T)))
         return fail(IHIP_ERR_INVALID, "%lld tokens of %d heads are too many for one call", (long long)T, q_heads);
@@ -1636,8 +1636,6 @@ int ihip_attn_paged_dev(const void *q, int q_type, void *out, int q_heads, float
     AttnArgs a{};
     RET_IF(check_cache(cache, &a.cache));
     RET_IF(check_batch(batch, &a.batch));
-    if (!q || !out)
-        return fail(IHIP_ERR_INVALID, "null pointer");
     if (q_heads <= 0 || q_heads % a.cache.heads)
         return fail(IHIP_ERR_INVALID, "q_heads=%d is not a multiple of kv_heads=%d", q_heads, a.cache.heads);
     if (q_type != kF32 && q_type != a.cache.type)
@@ -1646,11 +1644,13 @@ int ihip_attn_paged_dev(const void *q, int q_type, void *out, int q_heads, float
     if (window < 0 || !std::isfinite(scale) || !std::isfinite(softcap) || softcap < 0.0f ||
         (scale != 0.0f && std::fabs(scale) < 1e-12f) || (softcap > 0.0f && softcap < 1e-12f))
         return fail(IHIP_ERR_INVALID, "window=%d, scale=%g, softcap=%g", window, scale, softcap);
-    if (!al16(q) || !al16(out))
-        return fail(IHIP_ERR_INVALID, "q and out must be 16-byte aligned");
     const int64_t T = a.batch.tokens, rows = T * q_heads;
     if (T == 0 || a.batch.sequences == 0)
-        return IHIP_OK;
+        return IHIP_OK; // (an empty buffer has no address to check)
+    if (!q || !out)
+        return fail(IHIP_ERR_INVALID, "null pointer");
+    if (!al16(q) || !al16(out))
+        return fail(IHIP_ERR_INVALID, "q and out must be 16-byte aligned");
     const int64_t capacity = (int64_t)a.batch.stride << a.cache.page_shift;
     if (capacity > 1 << 30 || T > 1 << 30 || !grid_fits(rows))
         return fail(IHIP_ERR_INVALID, "%lld rows pass 2^31 or %lld table tokens 2^30", (long long)rows,
