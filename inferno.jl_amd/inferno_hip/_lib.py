@@ -33,6 +33,7 @@ ARGMAX_WS_BYTES = 262144
 Q8_K_BYTES = 292
 
 F32, F16, BF16 = 0, 1, 30
+ATTN_COUNT_BYTES = 16384
 FLAG_KV_PAGE, FLAG_KV_LENGTH, FLAG_KV_FULL = 8, 16, 32
 ROPE_SCALING = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3, "bands": 4}
 ROPE_LAYOUT = {"half": 0, "interleaved": 1}

@@ -546,13 +546,19 @@ def rope_kv(q: torch.Tensor, k, v, turns: torch.Tensor, cache: KVCache, batch: K
     return out
 
 
+def _counted(n: int, device):
+    """n bytes whose front, the counts of attn_paged's parts, is zero."""
+    t = torch.empty(n, dtype=torch.uint8, device=device)
+    t[:_lib.ATTN_COUNT_BYTES].zero_()
+    return t
+
+
 def attn_workspace(q_heads: int, cache: KVCache, batch: KVBatch):
     """The workspace of attn_paged for a batch of these sizes (q of either type),
-    or None where it needs none.  It starts as zeros, written on the current stream,
-    and every call leaves what has to be zero so.  Calls that share one must not
-    overlap."""
+    or None where it needs none.  Its counts start as zeros, written on the current
+    stream, and every call leaves them so.  Calls that share one must not overlap."""
     n = lib().ihip_attn_paged_scratch_bytes(_lib.F32, q_heads, cache.ref, batch.ref)
-    return torch.zeros(n, dtype=torch.uint8, device=cache.device) if n else None
+    return _counted(n, cache.device) if n else None
 
 
 def attn_paged(q: torch.Tensor, cache: KVCache, batch: KVBatch, scale: float = None, softcap: float = 0.0,
@@ -579,7 +585,7 @@ def attn_paged(q: torch.Tensor, cache: KVCache, batch: KVBatch, scale: float = N
     if workspace is None:
         n = lib().ihip_attn_paged_scratch_bytes(_lib.F32, H, cache.ref, batch.ref)
         if n:
-            workspace = _fresh(stream, lambda: torch.zeros(n, dtype=torch.uint8, device=q.device))
+            workspace = _fresh(stream, lambda: _counted(n, q.device))
     _launch(dev, stream, lib().ihip_attn_paged_dev, _at(q, q.dtype, "q", dev), act, _at(out, q.dtype, "out", dev), H,
             D ** -0.5 if scale is None else scale, softcap, window,
             _at(prefix_lens, torch.int32, "prefix_lens", dev, batch.sequences),
