@@ -3,6 +3,7 @@
 #pragma once
 
 #include "kq_launch.h"
+#include "kv_attn_plan.h"
 #include "kv_common.h"
 
 namespace ihip {
@@ -44,23 +45,6 @@ struct AttnArgs {
     uint32_t *count; // parts of each tile that have ended (0 between calls)
     float *part; // partial rows, then their maxima and sums, of every split
 };
-// Counts in front of the workspace, for calls of all sizes: its place does not
-// depend on a call's.
-constexpr int kAttnCounts = 4096;
-// How a batch of these sizes is launched: it depends on nothing else, so that
-// the workspace can be sized before the lengths are known.
-struct AttnPlan {
-    int rows;    // rows (tokens x heads of a group) of a tile
-    int tiles;   // tiles at most, over all sequences
-    int splits;  // parts of a tile's keys at most
-    int least;   // keys of a part at least
-    bool halves; // whether two halves of a workgroup share a tile's keys
-    size_t bytes; // workspace: the counts, then the parts
-};
-// window: the window where there is one and no prefix reaches behind it, else 0
-// (which never needs less workspace).
-AttnPlan attn_plan(int act, int kv_type, int q_heads, int kv_heads, int dim, int sequences, int tokens,
-                   int64_t capacity, int window);
 hipError_t launch_attn(AttnArgs a, const AttnPlan &p, hipStream_t s);
 
 // kv_pages.hip

@@ -110,7 +110,7 @@ def build_checks(verbose: bool = False) -> Path:
     return _hipcc(CHECK_LIB, [CHECKS / "sdig_check.hip", CHECKS / "prefill_check.hip",
                               CHECKS / "prefill_plan_check.hip",
                               CHECKS / "gemv_plan_check.hip", CHECKS / "mdig_check.hip",
-                              CHECKS / "prefill_copy_check.hip"], verbose)
+                              CHECKS / "prefill_copy_check.hip", CHECKS / "attn_plan_check.hip"], verbose)
 
 
 if __name__ == "__main__":
