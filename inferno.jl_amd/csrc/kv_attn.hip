@@ -317,16 +317,25 @@ __device__ __forceinline__ float tanh_any(float x)
     return y < 0.25f ? small : x == x ? large : x;
 }
 
+// A factor that may have passed the largest number: 0 times it stays 0.
+__device__ __forceinline__ float finite(float x)
+{
+    return __builtin_isinf(x) ? copysignf(3.402823466e38f, x) : x;
+}
+__device__ __forceinline__ float power_of_two(int e) { return finite(__builtin_ldexpf(1.0f, e)); }
+
 // q's part of a lane: KS chunks of 8 values (chunk step i + offset of the row),
 // in PARTS parts, with the sign of the scale (which then is positive, so that
-// the largest product gives the largest score; 0 makes q 0).  Two fp16 parts are taken of q times a power of two that brings
-// the row's largest value to [2^14, 2^15), undone (`undo`) on the scores.
+// the largest product gives the largest score; 0 makes q 0).  Parts are taken of q
+// times 2^up, which brings the row's largest value to [2^14, 2^15): fp16 holds it
+// then, and no part of either type is lost below the type's smallest numbers (rows
+// that the scale leaves under 2^-85 lose bits that no score would show).
 template <typename C, int PARTS, int KS>
 __device__ __forceinline__ void load_q(const AttnArgs &a, int64_t row, bool live, int step, int offset,
-                                       typename C::V8 (&qf)[PARTS][KS], float &undo)
+                                       typename C::V8 (&qf)[PARTS][KS], int &up)
 {
     typedef typename C::V8 V8;
-    undo = 1.0f;
+    up = 0;
     const float sign = a.scale > 0.0f ? 1.0f : a.scale < 0.0f ? -1.0f : 0.0f;
     if constexpr (PARTS == 1) {
         const typename C::T *q = (const typename C::T *)a.q + row * a.cache.dim;
@@ -353,14 +362,9 @@ __device__ __forceinline__ void load_q(const AttnArgs &a, int64_t row, bool live
             for (int u = 0; u < 4; ++u)
                 most = fmaxf(most, fmaxf(fabsf(v[2 * i][u]), fabsf(v[2 * i + 1][u])));
         }
-        int up = 0;
-        if constexpr (C::kShift != 0.0f) {
-            most = step == 4 ? groups_max(most) : halves_max(most);
-            const bool finite = most > 0.0f && most < __builtin_inff();
-            // (rows under 2^-45 lose bits that no score would show)
-            up = finite ? min(15 - __builtin_amdgcn_frexp_expf(most), 60) : 0;
-            undo = __builtin_ldexpf(1.0f, -up);
-        }
+        most = step == 4 ? groups_max(most) : halves_max(most);
+        if (most > 0.0f && most < __builtin_inff())
+            up = min(15 - __builtin_amdgcn_frexp_expf(most), a.scale_exp + 100);
 #pragma unroll
         for (int i = 0; i < KS; ++i)
 #pragma unroll
@@ -487,11 +491,11 @@ k_attn_rows(AttnArgs a, int tiles, int least, int splits)
     const int64_t qrow = (int64_t)(t.start + (live ? row / a.group : 0)) * a.q_heads + qhead;
     const int pos = live ? t.first - t.row0 / a.group + row / a.group : t.first;
     V8 qf[PARTS][KS];
-    float undo;
+    int up;
     int step = wave;
     if (step < n_steps)
         ids = page_of(step);
-    load_q<C, PARTS, KS>(a, qrow, live, 4, g, qf, undo);
+    load_q<C, PARTS, KS>(a, qrow, live, 4, g, qf, up);
     if (step < n_steps) {
         place(step);
         ids = page_of(step + AR_WAVES);
@@ -501,8 +505,8 @@ k_attn_rows(AttnArgs a, int tiles, int least, int splits)
     // scores become powers of two with the last factor, `by`; a cap takes the scale
     // before, and the bias is added in units of `by`.  `unit`, a power of two (the
     // row's and the scale's), brings the maxima of a row's parts to one unit.
-    const float unit = FEAT == kCap ? 1.0f : __builtin_ldexpf(undo, a.scale_exp), by = a.by * unit;
-    const float slope = FEAT != kPlain && a.slopes ? a.slopes[qhead] * kLog2e / by : 0.0f;
+    const float unit = FEAT == kCap ? 1.0f : power_of_two(a.scale_exp - up), by = finite(a.by * unit);
+    const float slope = FEAT != kPlain && a.slopes ? finite(a.slopes[qhead] * kLog2e / by) : 0.0f;
     const Seen sees = seen_from(a, t, pos);
 
     float m = kNone, l = 0.0f;
@@ -542,7 +546,7 @@ k_attn_rows(AttnArgs a, int tiles, int least, int splits)
         if constexpr (FEAT != kPlain) {
             const float apart = (float)(pos - key - 4 * g);
             if constexpr (FEAT == kCap) {
-                const float by_cap = (a.scale == 0.0f ? 1.0f : fabsf(a.scale)) * undo / a.cap;
+                const float by_cap = finite(__builtin_ldexpf(a.to_cap, a.scale_exp - up));
                 float most = 0.0f;
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
@@ -839,13 +843,13 @@ k_attn_chunk(AttnArgs a, int tiles, int least, int splits)
     const int wfirst = before + wrow0 / a.group, wlast = before + (wrow0 + max(wrows, 1) - 1) / a.group;
     const int pos = live ? before + row / a.group : wfirst;
     V8 qf[PARTS][KS];
-    float undo;
-    load_q<C, PARTS, KS>(a, qrow, live, 2, h, qf, undo);
+    int up;
+    load_q<C, PARTS, KS>(a, qrow, live, 2, h, qf, up);
     // scores become powers of two with the last factor, `by`; a cap takes the scale
     // before, and the bias is added in units of `by`.  by / a.by, a power of two (the
     // row's and the scale's), brings the maxima of a row's parts to one unit.
-    const float by = FEAT == kCap ? a.by : a.by * __builtin_ldexpf(undo, a.scale_exp);
-    const float slope = FEAT != kPlain && a.slopes ? a.slopes[qhead] * kLog2e / by : 0.0f;
+    const float by = FEAT == kCap ? a.by : finite(a.by * power_of_two(a.scale_exp - up));
+    const float slope = FEAT != kPlain && a.slopes ? finite(a.slopes[qhead] * kLog2e / by) : 0.0f;
     const Seen sees = seen_from(a, t, pos);
 
     // a lane's part of the copies: RUN keys of one page
@@ -1031,7 +1035,7 @@ k_attn_chunk(AttnArgs a, int tiles, int least, int splits)
         if constexpr (FEAT != kPlain) {
             const float apart = (float)(pos - key - 4 * h);
             if constexpr (FEAT == kCap) {
-                const float by_cap = (a.scale == 0.0f ? 1.0f : fabsf(a.scale)) * undo / a.cap;
+                const float by_cap = finite(__builtin_ldexpf(a.to_cap, a.scale_exp - up));
                 float most = 0.0f;
 #pragma unroll
                 for (int u = 0; u < SU; ++u)
@@ -1311,9 +1315,9 @@ hipError_t start_dim(const AttnArgs &a, const AttnPlan &p, hipStream_t s)
 
 hipError_t launch_attn(AttnArgs a, const AttnPlan &p, hipStream_t s)
 {
-    a.scale_exp = 0;
-    a.by = a.cap > 0.0f ? a.cap * kLog2e
-                        : std::frexp(a.scale == 0.0f ? 1.0f : std::fabs(a.scale), &a.scale_exp) * kLog2e;
+    const float scale = std::frexp(a.scale == 0.0f ? 1.0f : std::fabs(a.scale), &a.scale_exp);
+    a.by = a.cap > 0.0f ? std::fmin(a.cap * kLog2e, 3.402823466e38f) : scale * kLog2e;
+    a.to_cap = a.cap > 0.0f ? scale / a.cap : 0.0f;
     if (a.cache.type == kF16)
         return a.act == kF32 ? start_dim<Half, 2>(a, p, s) : start_dim<Half, 1>(a, p, s);
     return a.act == kF32 ? start_dim<BHalf, 3>(a, p, s) : start_dim<BHalf, 1>(a, p, s);

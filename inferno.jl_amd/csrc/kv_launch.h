@@ -34,8 +34,10 @@ struct AttnArgs {
     void *out;
     int act, q_heads, group;
     float scale, cap;
-    float by;      // a score's factor to a power of two: the cap, or the scale without
-    int scale_exp; // its power of two, 2^scale_exp (both set by the launcher)
+    // set by the launcher: the scale's power of two, and without that a score's
+    // factor to a power of two (with a cap: the cap's, and the score's to the cap)
+    int scale_exp;
+    float by, to_cap;
     int window;
     const int32_t *prefix;
     const float *slopes;
