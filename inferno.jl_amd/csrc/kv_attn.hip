@@ -1199,13 +1199,20 @@ k_attn_chunk(AttnArgs a, int tiles, int least, int splits)
         m = top;
     }
 
-    if (!live)
+    // the row's place, formed anew: kept, it takes registers that the loop spills for
+    // (us, formed anew against kept, 2048 fp32 rows over 8192 keys, 256 wide: bf16
+    // 1637, 2148, fp16 1253, 1273; elsewhere within 1 %)
+    int at_end = lane;
+    asm volatile("" : "+v"(at_end));
+    const int row_end = wrow0 + (at_end & 31);
+    if ((at_end & 31) >= wrows)
         return;
+    const int64_t qrow_end = (int64_t)(t.start + row_end / a.group) * a.q_heads + t.head * a.group + row_end % a.group;
     l = halves_sum(l);
     const int64_t rows_all = (int64_t)a.batch.tokens * a.q_heads;
     if (splits > 1) {
-        if (h == 0)
-            *(f2 *)(a.part + (int64_t)splits * rows_all * D + 2 * (t.split * rows_all + qrow)) = f2{m * (by / a.by), l};
+        if (at_end < 32)
+            *(f2 *)(a.part + (int64_t)splits * rows_all * D + 2 * (t.split * rows_all + qrow_end)) = f2{m * (by / a.by), l};
         if (l == 0.0f)
             return;
     }
@@ -1214,17 +1221,17 @@ k_attn_chunk(AttnArgs a, int tiles, int least, int splits)
     for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
-            const int at = 32 * d + 2 * e + 4 * h;
+            const int at = 32 * d + 2 * e + 4 * (at_end >> 5);
             if (at >= D)
                 continue;
             f4 v = f4{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]};
             v = l == 0.0f ? f4{} : v * f;
             if (splits > 1)
-                *(f4 *)(a.part + (t.split * rows_all + qrow) * D + at) = v;
+                *(f4 *)(a.part + (t.split * rows_all + qrow_end) * D + at) = v;
             else if constexpr (PARTS == 1)
-                *(V4 *)((T *)a.out + qrow * D + at) = __builtin_convertvector(v, V4);
+                *(V4 *)((T *)a.out + qrow_end * D + at) = __builtin_convertvector(v, V4);
             else
-                *(f4 *)((float *)a.out + qrow * D + at) = v;
+                *(f4 *)((float *)a.out + qrow_end * D + at) = v;
         }
 }
 
