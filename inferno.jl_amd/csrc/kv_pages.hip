@@ -27,7 +27,7 @@ __device__ __forceinline__ int wave_find(const int32_t *v, int n, int want)
 }
 
 // A fork is bound by its chain of dependent reads (table, counts, free pages), not
-// by bytes: 7 parents of up to 3000 tokens to 29 children take 9.3 us in one launch.
+// by bytes: 7 parents of up to 3000 tokens to 29 children take 8.6 us in one launch.
 //
 // A wave's work on child i, or on parent i - children.  A child's row takes over
 // the pages of its parent's: the first child of a parent all of them (no count
@@ -97,11 +97,13 @@ __device__ __forceinline__ void fork_row(const ForkArgs &a, int i)
 }
 
 constexpr int FORK_THREADS = 256;
-// Tables that one workgroup takes, in one launch: as fast as two for the GPU and
-// 2.5 to 4 us less for the host.  Beyond, its 16 waves take the rows in turns: us,
-// one launch against two, 24 parents to 90 children 21.5, 16.2; 48 to 180 58.8,
-// 35.8 (both before missing pages were looked for from the first one on).
-constexpr int FORK_ROWS = 64, FORK_ENTRIES = 1 << 14;
+// Tables that one workgroup takes, in one launch: its 16 waves take the rows in
+// turns, which costs the GPU what the second launch would cost the host.  us in a
+// graph and of host time, one launch against two: 1 parent to 3 children 4.6 and
+// 12.4, 5.5 and 15.1; 7 of up to 3000 tokens to 29 (6084 entries) 11.2 and 12.6, 8.9
+// and 15.0; 12 to 52 17.1, 10.6; 16 of up to 4000 to 48 21.9, 11.4; 4 of up to 16000
+// to 60 70, 19 (the host's times as before).
+constexpr int FORK_ROWS = 40, FORK_ENTRIES = 1 << 13;
 
 __global__ void __launch_bounds__(FORK_THREADS) k_fork_rows(ForkArgs a)
 {
