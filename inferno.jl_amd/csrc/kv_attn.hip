@@ -16,8 +16,8 @@
 // the weights that their differences say.  (fma(s_j, by, -m by) is one operation a
 // score less, but from scores of 2e7 on it rounds m by more than the room that p
 // has in fp16, and gives NaN or wrong weights.  us, this against that: 4096 tokens
-// over 32768 keys 2398, 2318; 2048 over 8192, 64 wide 199, 189, 128 wide 292, 284;
-// a 2048-token prompt of fp32 rows 95.6, 94.2; one token the same.)
+// over 32768 keys 2440, 2388; 2048 over 8192, 64 wide 200, 193, 128 wide 297, 289,
+// with a bias 328, 321; fp32 rows over bf16 730, 714; one token the same.)
 //
 // Both products run on the matrix cores, transposed: S^T = K Q^T puts a row's
 // scores in the lanes of one column, so that maxima and sums stay in a lane but
@@ -763,17 +763,18 @@ k_attn_rows(AttnArgs a, int tiles, int least, int splits)
 
 // ---- many rows: chunks of a prompt ---------------------------------------------
 // Operands read from LDS some products ahead, where the registers allow it.  us,
-// ahead against not, 2048 rows of 32 heads over 8192 keys, 1 part: 64 wide 190, 205;
-// 128 wide 281, 294, with a bias 310, 325, with a cap 457, 370 (it spills); 256 wide
-// 710, 830, with a bias 855, 972, with a cap 1409, 975.  Over 4096 keys, 3 parts,
-// 128 wide: 320, 329, with a cap 369, 395; 2 parts, 64 wide: 145, 149; 128 wide 208,
-// 213, with a cap 355, 246.
+// ahead against not, 2048 rows of 32 heads over 8192 keys, 1 part: 64 wide 200, 213,
+// with a bias 232, 243, with a cap 278, 280; 128 wide 296, 308, with a bias 328, 343,
+// with a cap 494, 384 (it spills); 256 wide 711, 867, with a bias 865, 997, with a
+// cap 1417, 996.  2 parts: 64 wide 291, 302; 128 wide 458, 466, with a cap 808, 545;
+// 256 wide 2126, 1263.  3 parts: 128 wide 730, 731, with a bias 819, 846, with a cap
+// 842, 897; 256 wide 3219, 1637.
 constexpr bool ac_ahead(int parts, int dp, int feat)
 {
     return dp <= 64 || (feat == kCap ? parts == 3 && dp <= 128 : parts == 1 || dp <= 128);
 }
 // K's operands on their way before the first product (2 parts, 128 wide: a
-// 2048-token prompt 97 us with 2, 98 with 8; the others have the room).
+// 2048-token prompt 96.4 us with 2, 97.7 with 8; the others have the room).
 constexpr int ac_first(int parts, int dp) { return parts == 2 && dp == 128 ? 2 : dp <= 64 ? dp / 16 : 8; }
 
 // Where 16-byte chunk c of key row r lies in its row of LDS: K's so that the 16
@@ -797,11 +798,12 @@ __device__ __forceinline__ int ac_v_chunk(int r, int c)
 // a step.  S^T = K Q^T and O^T = V^T P^T in 32 x 32 x 16 products: a lane holds
 // half of the scores of its row and 16 of the 32 rows of each d tile.
 //
-// 4096 tokens over 32768 keys, 32 heads on 8, 128 wide, bf16: 2350 us, 995
-// TFLOP/s, 83 % of what a large library product of this type reaches.  Counters of
-// that call: matrix cores busy 41 % of the cycles, vector work (exponentials,
-// maxima, rounding) 38 %, LDS 20 %, no bank conflicts; what is left is two waves a
-// SIMD waiting for each other's step, and 128 rows of registers allow no third.
+// 4096 tokens over 32768 keys, 32 heads on 8, 128 wide, bf16: 2440 us, 957 TFLOP/s,
+// 70 % of what a large library product of this type reaches.  Counters of that
+// call: matrix cores busy 44 % of the cycles, vector work (exponentials, maxima,
+// differences, rounding) 46 %, LDS 22 %, no bank conflicts, waves waiting 33 % of
+// theirs; what is left is two waves a SIMD waiting for each other's step, and 128
+// rows of registers allow no third.
 // 128 rows a tile so that a key read from HBM or L2 serves them all: 16-row tiles
 // took 11964 us.
 template <typename C, int PARTS, int DP, int FEAT, int HALVES>

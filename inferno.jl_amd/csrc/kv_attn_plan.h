@@ -20,14 +20,14 @@ constexpr int AR_SPLITS = 128; // parts of a tile's keys at most
 constexpr int AC_ROWS = 128; // rows of a workgroup's tile, 32 a wave
 constexpr int AC_KEYS = 128; // keys of a step at most
 // Splits that one thread joins alone; more are shared among a workgroup's.  us,
-// 256 tokens of 32 heads over 8000 keys in 8 splits 60 alone, 71 shared; 64 tokens
-// of 4 heads over 60000 keys in 128 splits 48, 32.
+// 256 tokens of 32 heads over 8000 keys in 8 splits 40 alone, 53 shared; 64 tokens
+// of 4 heads over 60000 keys in 128 splits 44, 27.
 constexpr int AC_FEW_SPLITS = 16;
 
 // Keys that a wave multiplies in a step: as many as leave its registers room
 // beside O^T and q (256 wide: 128 registers of O^T, 64 a part of q).  us, 32 keys
-// against 64, a prompt of 4096 tokens of 32 heads, 256 wide: 3 parts 994, 2272; 2
-// parts 825, 766.
+// against 64, a prompt of 4096 tokens of 32 heads, 256 wide: 3 parts 990, 2273; 2
+// parts 830, 769.
 constexpr int ac_half_keys(int parts, int dp) { return dp == 256 && parts == 3 ? 32 : 64; }
 // Waves a SIMD: two, where a wave's operands fit 256 registers.
 constexpr int ac_waves(int parts, int dp) { return dp <= 64 || (dp <= 128 && parts <= 2) ? 2 : 1; }
@@ -83,9 +83,11 @@ inline AttnPlan attn_plan(int act, int kv_type, int q_heads, int kv_heads, int d
     const int64_t reach = window ? std::min(capacity, (int64_t)window + p.rows + AC_KEYS) : capacity;
     const int64_t most = (reach + p.least - 1) / p.least;
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(most, want), AR_SPLITS));
-    // Few tiles: two halves of a workgroup each, which end a long tile sooner
-    // (512 tiles of a 2048-token prompt: 65 us against 77); of many, two
-    // workgroups a CU come further (4096 tokens: 174 us against 200).
+    // Few tiles: two halves of a workgroup each, which end a long tile sooner (us,
+    // halves against none, 128 wide, 512 tiles of a 2048-token prompt: fp16 43.5, 52,
+    // fp32 rows over fp16 96, 100; but 512 tiles of one length, 2048 tokens over 8192
+    // keys, 297, 279, which the sizes do not tell apart); of many, two workgroups a CU
+    // come further (4096 tokens, fp16: 132, 108).
     p.halves = p.splits == 1 && units <= 512;
     // (with 4096 tiles and heads or more nothing is split: their counts are enough)
     p.bytes = p.splits > 1 ? 4 * (size_t)kAttnCounts + (size_t)p.splits * tokens * q_heads * (dim + 2) * 4 : 0;
