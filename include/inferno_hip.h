@@ -1,7 +1,7 @@
 /*
  * inferno_hip.h -- C ABI of the MI355X (gfx950) K-quant matvec library.
  *
- * This is the whole boundary: plain pointers, sizes, status codes and two plain
+ * This is the whole boundary: plain pointers, sizes, status codes and a few plain
  * structs of them, no HIP or torch types.  It replaces the native library behind Inferno.jl's
  * QuantizedKernels / FusedKernels / Dequant call surface (paths relative to
  * the Inferno.jl checkout):
@@ -532,6 +532,120 @@ int ihip_kv_compact_dev(int32_t *table, int64_t entries, int32_t *refs, int page
 int ihip_kv_copy_dev(const ihip_kv_cache *cache, int layers, int64_t layer_stride,
                      const int32_t *copies, int n, const int32_t *count, uint32_t *flags,
                      ihip_stream stream);
+
+/* ---- layers that keep a state ---------------------------------------------- */
+/* What a recurrent layer does between its input and output projections
+ * (src/ModelCPU.jl:511-759: a short convolution over q, k and v, the gated delta
+ * rule, a gated norm), for a batch of sequences, each of which owns a slot of
+ * the layer's pools. */
+#define IHIP_FLAG_STATE_SLOT 64u /* a slot outside the pool, or an earlier sequence's */
+
+/* The sequences of a call, in device memory (only the sizes are read on the
+ * host, so a captured call replays with new contents).  Sequence s has the rows
+ * q_starts[s] .. q_starts[s+1] - 1 (q_starts does not decrease) and the state in
+ * slots[s].  It begins with this call (its slot is not read, and counts as zeros)
+ * where kv_lens[s], its tokens in all with the new ones, is their number; kv_lens
+ * NULL: every sequence goes on.  A sequence without new tokens is left as it is,
+ * whatever its slot.  One whose slot lies outside the pool, or is that of an
+ * earlier sequence with new tokens, is left out: its rows and its slot are not
+ * written.  Rows before the first sequence's and behind the last one's are not
+ * written either.  Flags as for the paged cache.
+ * most: the most new tokens that a sequence has, or 0 where that is not known.
+ * It only helps to choose kernels: results are right with any value. */
+typedef struct ihip_state_batch {
+    const int32_t *q_starts; /* sequences + 1 */
+    const int32_t *kv_lens;  /* sequences, or NULL */
+    const int32_t *slots;    /* sequences */
+    int sequences, tokens;
+    int most;
+} ihip_state_batch;
+
+/* out[t, c] = act(bias[c] + sum over j < width of w[c * width + j] *
+ * x[t - width + 1 + j, c]), act silu or nothing; the inputs before a sequence's
+ * first new token are its slot's, which then holds its last width - 1.  x: rows
+ * of `channels` (a multiple of 8) values of x_type, x_stride elements apart (a
+ * multiple of 8); w, bias (or NULL) fp32; state: `slots` slots of (width - 1) x
+ * channels floats, the oldest first, slot_stride floats apart (a multiple of 4);
+ * out: tokens x channels of out_type.  Types F32, F16 or BF16; width 2 .. 8; sums
+ * in 32 bits.  Buffers are 16-byte aligned and do not overlap. */
+int ihip_short_conv_dev(const void *x, int x_type, int64_t x_stride, const float *w,
+                        const float *bias, int channels, int width, int silu, float *state,
+                        int64_t slot_stride, int slots, void *out, int out_type,
+                        const ihip_state_batch *batch, uint32_t *flags, ihip_stream stream);
+
+/* A layer of the gated delta rule: k_heads heads of q and k, v_heads (a multiple
+ * of them) of v, head h reading q and k head h / (v_heads / k_heads); k_dim and
+ * v_dim multiples of 16, at most 128.  state: `slots` slots of v_heads x k_dim x
+ * v_dim floats, slot_stride floats apart (a multiple of 4).  decay (v_heads floats,
+ * at most 0, as a GGUF file's ssm_a; a higher one counts as 0), dt_bias (v_heads),
+ * norm_w (v_dim, or NULL: no norm). */
+typedef struct ihip_delta_layer {
+    float *state;
+    int64_t slot_stride;
+    int slots, k_heads, v_heads, k_dim, v_dim;
+    const float *decay, *dt_bias, *norm_w;
+    float norm_eps, l2_eps, scale;
+} ihip_delta_layer;
+
+/* For every new token of a sequence and every head, with S the head's state,
+ *   q^ = q / sqrt(|q|^2 + l2_eps), k^ alike,  beta = sigmoid(b),
+ *   S <- exp(decay * softplus(a + dt_bias)) S;  S <- S + beta k^ (v - k^T S)^T;
+ *   o = scale * q^T S
+ * and out = o, divided by sqrt(mean(o^2) + norm_eps) and times norm_w where that is
+ * given, then times silu(gate) where that is.  q, k, v: rows of a token's heads
+ * (F32, F16 or BF16), strides in elements, multiples of 8, so that the short
+ * convolution's output is passed as three offsets into it; a, b: rows of v_heads
+ * floats; gate: rows of v_heads * v_dim floats (stride a multiple of 4) or NULL; out:
+ * tokens x v_heads x v_dim of out_type, which is F32 or the type of q, k and v.
+ * States and F32 outputs carry fp32's accuracy; F16 and BF16 outputs are rounded once.
+ * A value that is not finite may reach every output of its head from 64 tokens before
+ * it on.  Buffers are 16-byte aligned (a and b 4), out overlaps no input.
+ * workspace: ihip_gated_delta_scratch_bytes bytes, 16-byte aligned, NULL where that
+ * is 0; its contents do not matter.  Calls that share it, or a slot, must not
+ * overlap on the GPU. */
+int ihip_gated_delta_dev(const void *q, int64_t q_stride, const void *k, int64_t k_stride,
+                         const void *v, int64_t v_stride, int type, const float *a,
+                         int64_t a_stride, const float *b, int64_t b_stride, const float *gate,
+                         int64_t gate_stride, void *out, int out_type,
+                         const ihip_delta_layer *layer, const ihip_state_batch *batch,
+                         uint32_t *flags, void *workspace, size_t workspace_bytes,
+                         ihip_stream stream);
+/* From the sizes alone (of the layer and the batch, `most` among them), for any
+ * contents of the batch's arrays. */
+size_t ihip_gated_delta_scratch_bytes(int type, const ihip_delta_layer *layer,
+                                      const ihip_state_batch *batch);
+
+/* ---- the choice of a token --------------------------------------------------- */
+/* tokens[r] = one of row r's `vocab` logits (F32, F16 or BF16, rows row_stride
+ * elements apart), chosen by the given number u[r] in [0, 1).  With T =
+ * temperature[r], w_i = exp((logit_i - max) / T) and the tokens in order of their
+ * logits (equal ones by index, the lowest first):
+ *   top_k[r] > 0 keeps the first top_k[r];
+ *   top_p[r] < 1 of those the shortest prefix (at least one) whose weights reach
+ *     top_p[r] times their sum;
+ *   min_p[r] > 0 of those the ones with w_i >= min_p[r] (the largest always);
+ * the token is the first, in order of index, at which the sum of the kept weights up
+ * to it passes u[r] times the sum of them all (the last kept one where none does),
+ * and logprobs[r] the logarithm of its share of that sum.  T = 0 (or below) is the
+ * greedy choice: the lowest index of the largest logit, with logprob 0.  temperature,
+ * top_k, top_p, min_p (one value a row) may be NULL: 1, and no filter; logprobs and
+ * flags may be NULL.  Weights and sums are formed in 64 bits.  A logit of -infinity
+ * is never chosen.  flags[r] = IHIP_FLAG_NAN / IHIP_FLAG_POSINF where the row holds
+ * such a value (the token is then 0 and the logprob NaN), IHIP_FLAG_ALL_NEGINF where
+ * every logit is -infinity (the token is 0), else 0.  Everything is device memory.
+ * workspace: ihip_sample_scratch_bytes bytes, 16-byte aligned.  The caller fills its
+ * first IHIP_SAMPLE_COUNT_BYTES with zeros once, before its first call; every call
+ * leaves them zero again, so that it serves any number of calls of any sizes that it
+ * is large enough for.  Calls that share it must not overlap on the GPU.  At most
+ * IHIP_SAMPLE_ROWS rows and 2^30 logits a row. */
+#define IHIP_SAMPLE_COUNT_BYTES 65536
+#define IHIP_SAMPLE_ROWS 16384
+int ihip_sample_dev(const void *logits, int type, int64_t row_stride, int rows, int vocab,
+                    const float *temperature, const int32_t *top_k, const float *top_p,
+                    const float *min_p, const float *u, int32_t *tokens, float *logprobs,
+                    uint32_t *flags, void *workspace, size_t workspace_bytes,
+                    ihip_stream stream);
+size_t ihip_sample_scratch_bytes(int rows, int vocab);
 
 #ifdef __cplusplus
 }

@@ -7,10 +7,12 @@
 // of Inferno.jl).  Unlike the reference they report failures through a
 // status code and ihip_last_error() instead of returning void.
 #include "inferno_hip.h"
+#include "gd_launch.h"
 #include "kq_common.h"
 #include "kq_launch.h"
 #include "kq_sdig_plan.h"
 #include "kv_launch.h"
+#include "sample_common.h"
 
 #include <cmath>
 #include <cstdarg>
@@ -694,6 +696,67 @@ bool in_pools(const KvCache &c, const void *p, size_t bytes)
 
 // A launch of `units` workgroups fits a grid.
 bool grid_fits(int64_t units) { return units <= (int64_t)INT32_MAX; }
+
+// ---- layers that keep a state ---------------------------------------------------
+int check_states(const ihip_state_batch *b, StateBatch *out)
+{
+    if (!b)
+        return fail(IHIP_ERR_INVALID, "null batch");
+    if (b->sequences < 0 || b->tokens < 0 || b->most < 0)
+        return fail(IHIP_ERR_INVALID, "sequences=%d, tokens=%d, most=%d", b->sequences, b->tokens, b->most);
+    if (!grid_fits((int64_t)b->tokens + b->sequences))
+        return fail(IHIP_ERR_INVALID, "%d sequences of %d tokens are too many for one call", b->sequences, b->tokens);
+    if (b->tokens && b->sequences && (!b->q_starts || !b->slots))
+        return fail(IHIP_ERR_INVALID, "null pointer in the batch");
+    *out = StateBatch{b->q_starts, b->kv_lens, b->slots, b->sequences, b->tokens};
+    return IHIP_OK;
+}
+
+// A buffer of a call: bytes from p on (none: NULL).
+struct Span {
+    const void *p;
+    size_t n;
+};
+
+// rows of `width` values of `bytes` bytes, `step` values apart
+Span rows_of(const void *p, int64_t rows, int64_t step, int64_t width, int bytes)
+{
+    return Span{p, p ? (size_t)bytes * (size_t)((rows - 1) * step + width) : 0};
+}
+
+bool apart(const Span &a, const Span &b)
+{
+    return !a.n || !b.n || !overlap(a.p, a.n, b.p, b.n);
+}
+
+// Row strides that hold a row, keep its alignment and stay far from 64 bits.
+bool step_fits(int64_t step, int64_t width, int64_t rows, int multiple)
+{
+    return step >= width && step % multiple == 0 && step <= INT64_MAX / 8 / (rows + 1);
+}
+
+int check_layer(const ihip_delta_layer *l, DeltaArgs *a)
+{
+    if (!l || !l->state || !l->decay || !l->dt_bias)
+        return fail(IHIP_ERR_INVALID, "null pointer in the layer");
+    if (l->k_heads <= 0 || l->v_heads <= 0 || l->v_heads % l->k_heads || l->v_heads > 4096)
+        return fail(IHIP_ERR_INVALID, "v_heads=%d is not a multiple of k_heads=%d, up to 4096", l->v_heads, l->k_heads);
+    if (l->k_dim <= 0 || l->k_dim % 16 || l->k_dim > kMaxDeltaDim || l->v_dim <= 0 || l->v_dim % 16 || l->v_dim > kMaxDeltaDim)
+        return fail(IHIP_ERR_INVALID, "k_dim=%d or v_dim=%d is not a multiple of 16 up to %d", l->k_dim, l->v_dim,
+                    kMaxDeltaDim);
+    if (l->slots <= 0 || !step_fits(l->slot_stride, (int64_t)l->v_heads * l->k_dim * l->v_dim, l->slots, 4))
+        return fail(IHIP_ERR_INVALID, "slots=%d, slot_stride=%lld", l->slots, (long long)l->slot_stride);
+    if (!std::isfinite(l->scale) || !(l->l2_eps >= 0.0f) || !(l->norm_eps >= 0.0f))
+        return fail(IHIP_ERR_INVALID, "scale=%g, l2_eps=%g, norm_eps=%g", l->scale, l->l2_eps, l->norm_eps);
+    if (!al16(l->state) || !al16(l->norm_w) || ((uintptr_t)l->decay & 3) || ((uintptr_t)l->dt_bias & 3))
+        return fail(IHIP_ERR_INVALID, "state and norm_w must be 16-byte aligned");
+    a->state = l->state, a->slot_step = l->slot_stride, a->pool = l->slots;
+    a->k_heads = l->k_heads, a->v_heads = l->v_heads, a->group = l->v_heads / l->k_heads;
+    a->k_dim = l->k_dim, a->v_dim = l->v_dim;
+    a->decay = l->decay, a->dt_bias = l->dt_bias, a->norm_w = l->norm_w;
+    a->norm_eps = l->norm_eps, a->l2_eps = l->l2_eps, a->scale = l->scale;
+    return IHIP_OK;
+}
 
 } // namespace
 
@@ -1705,10 +1768,6 @@ int ihip_kv_fork_dev(const int32_t *table, const int32_t *lens, int sequences,
         return fail(IHIP_ERR_INVALID, "%d children of %d pages are too many for one call", children, table_stride);
     const size_t tb = 4 * (size_t)sequences * (size_t)table_stride, lb = 4 * (size_t)sequences;
     const size_t cb = 4 * (size_t)children, ob = cb * (size_t)table_stride;
-    struct Span {
-        const void *p;
-        size_t n;
-    };
     // what is written may be nothing else that is read or written
     const Span ins[] = {{table, tb}, {lens, lb}, {parents, cb}};
     const Span outs[] = {{refs, 4 * (size_t)pages}, {table_out, ob}, {lens_out, cb}, {copies, 2 * cb}, {scratch, 2 * cb}};
@@ -1776,6 +1835,167 @@ int ihip_kv_copy_dev(const ihip_kv_cache *cache, int layers, int64_t layer_strid
                                   flags, (hipStream_t)stream);
     if (e != hipSuccess)
         return fail(IHIP_ERR_HIP, "copy launch failed: %s", hipGetErrorString(e));
+    return IHIP_OK;
+}
+
+// ---- layers that keep a state ---------------------------------------------------
+
+int ihip_short_conv_dev(const void *x, int x_type, int64_t x_stride, const float *w,
+                        const float *bias, int channels, int width, int silu, float *state,
+                        int64_t slot_stride, int slots, void *out, int out_type,
+                        const ihip_state_batch *batch, uint32_t *flags, ihip_stream stream)
+{
+    std::lock_guard<std::recursive_mutex> lk(ctx().mu);
+    if (disabled())
+        return fail(IHIP_ERR_DISABLED, "IHIP_DISABLE is set");
+    ConvArgs a{};
+    RET_IF(check_states(batch, &a.batch));
+    if (!value_bytes(x_type) || !value_bytes(out_type))
+        return fail(IHIP_ERR_INVALID, "x_type=%d or out_type=%d is none of F32, F16, BF16", x_type, out_type);
+    if (channels <= 0 || channels % 8 || channels > 1 << 24)
+        return fail(IHIP_ERR_INVALID, "channels=%d is not a multiple of 8 up to 2^24", channels);
+    if (width < 2 || width > 8)
+        return fail(IHIP_ERR_INVALID, "width=%d is not 2 to 8", width);
+    const int64_t kept = (int64_t)(width - 1) * channels, T = a.batch.tokens;
+    if (slots <= 0 || !step_fits(slot_stride, kept, slots, 4))
+        return fail(IHIP_ERR_INVALID, "slots=%d, slot_stride=%lld", slots, (long long)slot_stride);
+    if (T == 0 || a.batch.sequences == 0)
+        return IHIP_OK; // (an empty buffer has no address to check)
+    if (!x || !w || !state || !out)
+        return fail(IHIP_ERR_INVALID, "null pointer");
+    if (!step_fits(x_stride, channels, T, 8))
+        return fail(IHIP_ERR_INVALID, "x_stride=%lld is no multiple of 8 that holds %d channels", (long long)x_stride, channels);
+    if (!al16(x) || !al16(w) || !al16(bias) || !al16(state) || !al16(out))
+        return fail(IHIP_ERR_INVALID, "a pointer is not 16-byte aligned");
+    const Span in = rows_of(x, T, x_stride, channels, value_bytes(x_type));
+    const Span to = rows_of(out, T, channels, channels, value_bytes(out_type));
+    const Span held = rows_of(state, slots, slot_stride, kept, 4);
+    const Span taps{w, 4 * (size_t)width * (size_t)channels}, add{bias, bias ? 4 * (size_t)channels : 0};
+    if (!apart(in, to) || !apart(in, held) || !apart(to, held) || !apart(taps, to) || !apart(taps, held) ||
+        !apart(add, to) || !apart(add, held))
+        return fail(IHIP_ERR_INVALID, "out or state overlaps another buffer");
+    a.x = x, a.x_type = x_type, a.x_step = x_stride, a.w = w, a.bias = bias;
+    a.channels = channels, a.width = width, a.silu = silu;
+    a.state = state, a.slot_step = slot_stride, a.pool = slots;
+    a.out = out, a.out_type = out_type, a.flags = flags;
+    hipError_t e = launch_short_conv(a, (hipStream_t)stream);
+    if (e != hipSuccess)
+        return fail(IHIP_ERR_HIP, "convolution launch failed: %s", hipGetErrorString(e));
+    return IHIP_OK;
+}
+
+size_t ihip_gated_delta_scratch_bytes(int type, const ihip_delta_layer *layer,
+                                      const ihip_state_batch *batch)
+{
+    DeltaArgs a{};
+    if (check_layer(layer, &a) != IHIP_OK || check_states(batch, &a.batch) != IHIP_OK || !value_bytes(type) ||
+        a.batch.tokens == 0 || a.batch.sequences == 0)
+        return 0;
+    return 0;
+}
+
+int ihip_gated_delta_dev(const void *q, int64_t q_stride, const void *k, int64_t k_stride,
+                         const void *v, int64_t v_stride, int type, const float *a,
+                         int64_t a_stride, const float *b, int64_t b_stride, const float *gate,
+                         int64_t gate_stride, void *out, int out_type,
+                         const ihip_delta_layer *layer, const ihip_state_batch *batch,
+                         uint32_t *flags, void *workspace, size_t workspace_bytes,
+                         ihip_stream stream)
+{
+    std::lock_guard<std::recursive_mutex> lk(ctx().mu);
+    if (disabled())
+        return fail(IHIP_ERR_DISABLED, "IHIP_DISABLE is set");
+    DeltaArgs d{};
+    RET_IF(check_layer(layer, &d));
+    RET_IF(check_states(batch, &d.batch));
+    const int vb = value_bytes(type);
+    if (!vb || (out_type != kF32 && out_type != type))
+        return fail(IHIP_ERR_INVALID, "type=%d is none of F32, F16, BF16, or out_type=%d neither F32 nor that", type, out_type);
+    const int64_t T = d.batch.tokens, S = d.batch.sequences;
+    if (T == 0 || S == 0)
+        return IHIP_OK; // (an empty buffer has no address to check)
+    if (!q || !k || !v || !a || !b || !out)
+        return fail(IHIP_ERR_INVALID, "null pointer");
+    const int64_t kw = (int64_t)d.k_heads * d.k_dim, vw = (int64_t)d.v_heads * d.v_dim;
+    if (!step_fits(q_stride, kw, T, 8) || !step_fits(k_stride, kw, T, 8) || !step_fits(v_stride, vw, T, 8) ||
+        !step_fits(a_stride, d.v_heads, T, 1) || !step_fits(b_stride, d.v_heads, T, 1) ||
+        (gate && !step_fits(gate_stride, vw, T, 4)))
+        return fail(IHIP_ERR_INVALID, "a stride does not hold a token's heads, or is no multiple of 8 (q, k, v) or 4 (gate)");
+    if (!al16(q) || !al16(k) || !al16(v) || !al16(gate) || !al16(out) || ((uintptr_t)a & 3) || ((uintptr_t)b & 3))
+        return fail(IHIP_ERR_INVALID, "a pointer is not 16-byte aligned (a, b: 4)");
+    if (!grid_fits((T + S) * d.v_heads) || T * vw > INT64_MAX / 8)
+        return fail(IHIP_ERR_INVALID, "%lld tokens and %lld sequences of %d heads are too many for one call", (long long)T,
+                    (long long)S, d.v_heads);
+    const Span to = rows_of(out, T, vw, vw, value_bytes(out_type));
+    const Span held = rows_of(d.state, d.pool, d.slot_step, (int64_t)d.v_heads * d.k_dim * d.v_dim, 4);
+    const Span ins[] = {rows_of(q, T, q_stride, kw, vb), rows_of(k, T, k_stride, kw, vb), rows_of(v, T, v_stride, vw, vb),
+                        rows_of(a, T, a_stride, d.v_heads, 4), rows_of(b, T, b_stride, d.v_heads, 4),
+                        rows_of(gate, T, gate_stride, vw, 4), {d.decay, 4 * (size_t)d.v_heads},
+                        {d.dt_bias, 4 * (size_t)d.v_heads}, {d.norm_w, d.norm_w ? 4 * (size_t)d.v_dim : 0}};
+    if (!apart(to, held))
+        return fail(IHIP_ERR_INVALID, "out overlaps state");
+    for (const Span &in : ins)
+        if (!apart(in, to) || !apart(in, held))
+            return fail(IHIP_ERR_INVALID, "out or state overlaps another buffer");
+    (void)workspace, (void)workspace_bytes;
+    d.q = q, d.k = k, d.v = v, d.type = type, d.q_step = q_stride, d.k_step = k_stride, d.v_step = v_stride;
+    d.a = a, d.b = b, d.a_step = a_stride, d.b_step = b_stride, d.gate = gate, d.gate_step = gate_stride;
+    d.out = out, d.out_type = out_type, d.flags = flags;
+    hipError_t e = launch_delta_step(d, (hipStream_t)stream);
+    if (e != hipSuccess)
+        return fail(IHIP_ERR_HIP, "delta rule launch failed: %s", hipGetErrorString(e));
+    return IHIP_OK;
+}
+
+// ---- the choice of a token --------------------------------------------------------
+
+size_t ihip_sample_scratch_bytes(int rows, int vocab)
+{
+    return rows <= 0 || rows > IHIP_SAMPLE_ROWS || vocab <= 0 || vocab > 1 << 30 ? 0 : IHIP_SAMPLE_COUNT_BYTES;
+}
+
+int ihip_sample_dev(const void *logits, int type, int64_t row_stride, int rows, int vocab,
+                    const float *temperature, const int32_t *top_k, const float *top_p,
+                    const float *min_p, const float *u, int32_t *tokens, float *logprobs,
+                    uint32_t *flags, void *workspace, size_t workspace_bytes,
+                    ihip_stream stream)
+{
+    std::lock_guard<std::recursive_mutex> lk(ctx().mu);
+    if (disabled())
+        return fail(IHIP_ERR_DISABLED, "IHIP_DISABLE is set");
+    const int vb = value_bytes(type);
+    if (!vb)
+        return fail(IHIP_ERR_INVALID, "type=%d is none of F32, F16, BF16", type);
+    if (rows < 0 || rows > IHIP_SAMPLE_ROWS || vocab < 0 || vocab > 1 << 30)
+        return fail(IHIP_ERR_INVALID, "rows=%d (up to %d), vocab=%d (up to 2^30)", rows, IHIP_SAMPLE_ROWS, vocab);
+    if (rows == 0)
+        return IHIP_OK;
+    if (vocab == 0)
+        return fail(IHIP_ERR_EMPTY, "no logits to choose from");
+    if (!logits || !u || !tokens)
+        return fail(IHIP_ERR_INVALID, "null pointer");
+    if (row_stride < vocab || row_stride > INT64_MAX / 8 / rows)
+        return fail(IHIP_ERR_INVALID, "row_stride=%lld does not hold %d logits", (long long)row_stride, vocab);
+    if ((uintptr_t)logits & (uintptr_t)(vb - 1))
+        return fail(IHIP_ERR_INVALID, "logits are not aligned to their values");
+    const size_t need = ihip_sample_scratch_bytes(rows, vocab), n = 4 * (size_t)rows;
+    if (!workspace || workspace_bytes < need || !al16(workspace))
+        return fail(IHIP_ERR_INVALID, "the workspace needs %zu bytes, 16-byte aligned", need);
+    const Span ins[] = {rows_of(logits, rows, row_stride, vocab, vb), {temperature, temperature ? n : 0}, {top_k, top_k ? n : 0},
+                        {top_p, top_p ? n : 0}, {min_p, min_p ? n : 0}, {u, n}};
+    const Span outs[] = {{tokens, n}, {logprobs, logprobs ? n : 0}, {flags, flags ? n : 0}, {workspace, need}};
+    for (const Span &o : outs) {
+        for (const Span &i : ins)
+            if (!apart(i, o))
+                return fail(IHIP_ERR_INVALID, "an output or the workspace overlaps an input");
+        for (const Span &p : outs)
+            if (&p < &o && !apart(p, o))
+                return fail(IHIP_ERR_INVALID, "two outputs, or one and the workspace, overlap");
+    }
+    SampleArgs a{logits, type, rows, vocab, row_stride, temperature, top_k, top_p, min_p, u, tokens, logprobs, flags};
+    hipError_t e = launch_sample(a, (hipStream_t)stream);
+    if (e != hipSuccess)
+        return fail(IHIP_ERR_HIP, "sampling launch failed: %s", hipGetErrorString(e));
     return IHIP_OK;
 }
 

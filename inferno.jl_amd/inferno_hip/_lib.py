@@ -34,7 +34,8 @@ Q8_K_BYTES = 292
 
 F32, F16, BF16 = 0, 1, 30
 ATTN_COUNT_BYTES = 16384
-FLAG_KV_PAGE, FLAG_KV_LENGTH, FLAG_KV_FULL = 8, 16, 32
+FLAG_KV_PAGE, FLAG_KV_LENGTH, FLAG_KV_FULL, FLAG_STATE_SLOT = 8, 16, 32, 64
+SAMPLE_COUNT_BYTES = 65536
 ROPE_SCALING = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3, "bands": 4}
 ROPE_LAYOUT = {"half": 0, "interleaved": 1}
 
@@ -72,6 +73,21 @@ class KVBatchStruct(C.Structure):
 
 _f, _d = C.c_float, C.c_double
 _cache_p, _batch_p = C.POINTER(KVCacheStruct), C.POINTER(KVBatchStruct)
+
+
+class StateBatchStruct(C.Structure):
+    """ihip_state_batch"""
+    _fields_ = [("q_starts", _vp), ("kv_lens", _vp), ("slots", _vp), ("sequences", _i), ("tokens", _i), ("most", _i)]
+
+
+class DeltaLayerStruct(C.Structure):
+    """ihip_delta_layer"""
+    _fields_ = [("state", _vp), ("slot_stride", _i64), ("slots", _i), ("k_heads", _i), ("v_heads", _i), ("k_dim", _i),
+                ("v_dim", _i), ("decay", _vp), ("dt_bias", _vp), ("norm_w", _vp), ("norm_eps", _f), ("l2_eps", _f),
+                ("scale", _f)]
+
+
+_states_p, _layer_p = C.POINTER(StateBatchStruct), C.POINTER(DeltaLayerStruct)
 
 SIGNATURES = {
     "ihip_last_error": ([], C.c_char_p),
@@ -145,6 +161,12 @@ SIGNATURES = {
     "ihip_kv_fork_dev": ([_vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp], _i),
     "ihip_kv_compact_dev": ([_vp, _i64, _vp, _i, _vp, _vp, _vp, _vp, _vp], _i),
     "ihip_kv_copy_dev": ([_cache_p, _i, _i64, _vp, _i, _vp, _vp, _vp], _i),
+    "ihip_short_conv_dev": ([_vp, _i, _i64, _vp, _vp, _i, _i, _i, _vp, _i64, _i, _vp, _i, _states_p, _vp, _vp], _i),
+    "ihip_gated_delta_dev": ([_vp, _i64, _vp, _i64, _vp, _i64, _i, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i, _layer_p,
+                              _states_p, _vp, _vp, _sz, _vp], _i),
+    "ihip_gated_delta_scratch_bytes": ([_i, _layer_p, _states_p], _sz),
+    "ihip_sample_dev": ([_vp, _i, _i64, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp], _i),
+    "ihip_sample_scratch_bytes": ([_i, _i], _sz),
 }
 
 _lib = None

@@ -546,10 +546,10 @@ def rope_kv(q: torch.Tensor, k, v, turns: torch.Tensor, cache: KVCache, batch: K
     return out
 
 
-def _counted(n: int, device):
-    """n bytes whose front, the counts of attn_paged's parts, is zero."""
+def _counted(n: int, device, front: int = _lib.ATTN_COUNT_BYTES):
+    """n bytes whose front, the counts of a call's parts, is zero."""
     t = torch.empty(n, dtype=torch.uint8, device=device)
-    t[:_lib.ATTN_COUNT_BYTES].zero_()
+    t[:front].zero_()
     return t
 
 
@@ -641,3 +641,196 @@ def kv_copy(cache: KVCache, copies: torch.Tensor, count: torch.Tensor = None, fl
     _launch(dev, stream, lib().ihip_kv_copy_dev, cache.ref, cache.layers, cache.layer_stride,
             _at(copies, torch.int32, "copies", dev), copies.shape[0], _at(count, torch.int32, "count", dev, 1),
             _at(flags, torch.int32, "flags", dev, 1))
+
+
+# ---- layers that keep a state ---------------------------------------------------
+class StateBatch:
+    """The sequences of a call on layers that keep a state (ihip_state_batch): int32
+    device tensors q_starts (sequences + 1), slots (sequences) and, where some begin
+    with the call, kv_lens (sequences: all their tokens), and the rows of the call.
+    Their contents may change between calls, also under a captured graph.  most: the
+    most new tokens of a sequence (a help in the choice of kernels; 0: not known)."""
+
+    def __init__(self, q_starts: torch.Tensor, slots: torch.Tensor, tokens: int, kv_lens=None, most: int = 0):
+        n, self.index = slots.numel(), slots.get_device()
+        for t, what in ((slots, "slots"), (q_starts, "q_starts"), (kv_lens, "kv_lens")):
+            if t is not None:
+                _ptr(t, torch.int32, what), _at(t, torch.int32, what, self.index)
+        if q_starts.numel() != n + 1 or (kv_lens is not None and kv_lens.numel() != n):
+            raise _invalid("q_starts has sequences + 1 entries, kv_lens one a sequence")
+        self.q_starts, self.slots, self.kv_lens, self.tokens = q_starts, slots, kv_lens, tokens
+        self.sequences = n
+        self.struct = _lib.StateBatchStruct(q_starts.data_ptr(), None if kv_lens is None else kv_lens.data_ptr(),
+                                            slots.data_ptr(), n, tokens, most)
+        self.ref = C.byref(self.struct)
+
+
+def _slots(state: torch.Tensor, what: str, inner):
+    """Floats from one slot of a pool to the next: a float32 tensor slots x inner whose
+    slots are contiguous."""
+    if not state.is_cuda or state.dtype != torch.float32 or state.dim() != len(inner) + 1 or state.shape[0] == 0:
+        raise _invalid(f"{what} must be a float32 device tensor of slots x {' x '.join(inner)}")
+    want, n = [], 1
+    for d in reversed(state.shape[1:]):
+        want.insert(0, n)
+        n *= d
+    if n == 0 or state.stride()[1:] != tuple(want):
+        raise _invalid(f"a slot of {what} must be contiguous")
+    return state.stride(0) if state.shape[0] > 1 else n
+
+
+def _row_step(t: torch.Tensor, what, dev, dtype, tokens, *inner):
+    """Pointer and row stride of a tokens x inner view whose rows are contiguous."""
+    shape, stride = t.shape, t.stride()
+    if t.dtype != dtype or t.get_device() != dev:
+        raise _invalid(f"{what} must be {dtype} on device {dev}, got {t.dtype} on {t.device}")
+    if shape != (tokens, *inner):
+        raise _invalid(f"{what} is {tuple(shape)}, not {(tokens, *inner)}")
+    n = 1
+    for i in range(len(inner), 0, -1):
+        if shape[i] > 1 and stride[i] != n and tokens:
+            raise _invalid(f"a row of {what} must be contiguous")
+        n *= shape[i]
+    return t.data_ptr(), stride[0] if tokens > 1 else n
+
+
+def _out_like(out, out_dtype, shape, default, device, stream):
+    if out is None:
+        return _fresh(stream, lambda: torch.empty(shape, dtype=out_dtype or default, device=device))
+    if out.shape != shape or (out_dtype is not None and out.dtype != out_dtype):
+        raise _invalid(f"out is {out.dtype} {tuple(out.shape)}, not {tuple(shape)} of the type asked for")
+    return out
+
+
+def short_conv(x: torch.Tensor, weight: torch.Tensor, state: torch.Tensor, batch: StateBatch, bias=None,
+               silu: bool = True, out: torch.Tensor = None, out_dtype=None, flags=None, stream=None) -> torch.Tensor:
+    """The causal convolution of a recurrent layer over each channel's last inputs
+    (ihip_short_conv_dev).  x: tokens x channels (rows of a wider projection as they
+    are), fp32, fp16 or bf16; weight: channels x width fp32, the newest input's last;
+    state: slots x (width - 1) x channels fp32, updated in place.  Returns tokens x
+    channels of out_dtype (default: x's type)."""
+    dev = x.get_device()
+    _same_device(dev, batch)
+    act = _ACT_TYPES.get(x.dtype)
+    if x.dim() != 2 or weight.dim() != 2 or act is None:
+        raise _invalid("x is tokens x channels of fp32, fp16 or bf16, weight channels x width")
+    channels, width = weight.shape
+    step = _slots(state, "state", ("width - 1", "channels"))
+    if state.shape[1:] != (width - 1, channels):
+        raise _invalid(f"state is {tuple(state.shape)}, not slots x {width - 1} x {channels}")
+    if state.get_device() != dev:
+        raise _invalid(f"state must be on device {dev}")
+    xp, xs = _row_step(x, "x", dev, x.dtype, batch.tokens, channels)
+    out = _out_like(out, out_dtype, x.shape, x.dtype, x.device, stream)
+    to = _ACT_TYPES.get(out.dtype)
+    if to is None:
+        raise _invalid("out must be fp32, fp16 or bf16")
+    _launch(dev, stream, lib().ihip_short_conv_dev, xp, act, xs, _at(weight, torch.float32, "weight", dev),
+            _at(bias, torch.float32, "bias", dev, channels), channels, width, int(silu), state.data_ptr(), step,
+            state.shape[0], _at(out, out.dtype, "out", dev), to, batch.ref, _at(flags, torch.int32, "flags", dev, 1))
+    return out
+
+
+class DeltaLayer:
+    """A layer of the gated delta rule (ihip_delta_layer): state (slots x v_heads x
+    k_dim x v_dim fp32, updated in place by gated_delta), the heads of q and k, the
+    heads' decay (at most 0, as a GGUF file's ssm_a) and dt_bias, and the output
+    norm's weights (v_dim) or None.  scale defaults to k_dim ** -0.5."""
+
+    def __init__(self, state: torch.Tensor, k_heads: int, decay: torch.Tensor, dt_bias: torch.Tensor, norm_w=None,
+                 norm_eps: float = 1e-6, l2_eps: float = 1e-6, scale: float = None):
+        step = _slots(state, "state", ("v_heads", "k_dim", "v_dim"))
+        self.slots, self.v_heads, self.k_dim, self.v_dim = state.shape
+        self.k_heads, self.index, self.device = k_heads, state.get_device(), state.device
+        self.state, self.decay, self.dt_bias, self.norm_w = state, decay, dt_bias, norm_w
+        dev = self.index
+        self.struct = _lib.DeltaLayerStruct(
+            state.data_ptr(), step, self.slots, k_heads, self.v_heads, self.k_dim, self.v_dim,
+            _at(decay, torch.float32, "decay", dev, self.v_heads), _at(dt_bias, torch.float32, "dt_bias", dev, self.v_heads),
+            _at(norm_w, torch.float32, "norm_w", dev, self.v_dim), norm_eps, l2_eps,
+            self.k_dim ** -0.5 if scale is None else scale)
+        self.ref = C.byref(self.struct)
+
+
+def delta_workspace(layer: DeltaLayer, batch: StateBatch, dtype):
+    """The workspace of gated_delta for a batch of these sizes with q, k and v of
+    `dtype`, or None where it needs none.  Calls that share one must not overlap."""
+    n = lib().ihip_gated_delta_scratch_bytes(_ACT_TYPES.get(dtype, -1), layer.ref, batch.ref)
+    return torch.empty(n, dtype=torch.uint8, device=layer.device) if n else None
+
+
+def gated_delta(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, a: torch.Tensor, b: torch.Tensor, layer: DeltaLayer,
+                batch: StateBatch, gate=None, out: torch.Tensor = None, out_dtype=None, workspace=None, flags=None,
+                stream=None) -> torch.Tensor:
+    """The gated delta rule over the batch's new tokens (ihip_gated_delta_dev): q, k
+    (tokens x k_heads x k_dim) and v (tokens x v_heads x v_dim) of one type, slices of
+    the short convolution's rows as they are; a, b: tokens x v_heads fp32; gate:
+    tokens x v_heads x v_dim fp32 or None.  The layer's state is updated in place.
+    Returns tokens x v_heads x v_dim of out_dtype (fp32 or q's type, the default)."""
+    dev, T = q.get_device(), batch.tokens
+    _same_device(dev, layer, batch)
+    kind = q.dtype
+    act = _ACT_TYPES.get(kind)
+    if act is None:
+        raise _invalid(f"q, k and v must be fp32, fp16 or bf16, got {kind}")
+    K, H, dk, dv = layer.k_heads, layer.v_heads, layer.k_dim, layer.v_dim
+    qp, qs = _row_step(q, "q", dev, kind, T, K, dk)
+    kp, ks = _row_step(k, "k", dev, kind, T, K, dk)
+    vp, vs = _row_step(v, "v", dev, kind, T, H, dv)
+    ap, as_ = _row_step(a, "a", dev, torch.float32, T, H)
+    bp, bs = _row_step(b, "b", dev, torch.float32, T, H)
+    gp, gs = (None, 0) if gate is None else _row_step(gate, "gate", dev, torch.float32, T, H, dv)
+    out = _out_like(out, out_dtype, v.shape, kind, q.device, stream)
+    to = _ACT_TYPES.get(out.dtype)
+    if to is None:
+        raise _invalid("out must be fp32 or of q's type")
+    if workspace is None:
+        workspace = _fresh_bytes(stream, lib().ihip_gated_delta_scratch_bytes(act, layer.ref, batch.ref), q.device)
+    _launch(dev, stream, lib().ihip_gated_delta_dev, qp, qs, kp, ks, vp, vs, act, ap, as_, bp, bs, gp, gs,
+            _at(out, out.dtype, "out", dev), to, layer.ref, batch.ref, _at(flags, torch.int32, "flags", dev, 1),
+            _at(workspace, torch.uint8, "workspace", dev), 0 if workspace is None else workspace.numel())
+    return out
+
+
+def _fresh_bytes(stream, n, device):
+    return _fresh(stream, lambda: torch.empty(n, dtype=torch.uint8, device=device)) if n else None
+
+
+# ---- the choice of a token --------------------------------------------------------
+def sample_workspace(rows: int, vocab: int, device="cuda"):
+    """The workspace of sample for up to so many rows of so many logits.  Its counts
+    start as zeros, written on the current stream, and every call leaves them so.
+    Calls that share one must not overlap."""
+    n = lib().ihip_sample_scratch_bytes(rows, vocab)
+    if not n:
+        raise _invalid(f"{rows} rows of {vocab} logits")
+    return _counted(n, device, _lib.SAMPLE_COUNT_BYTES)
+
+
+def sample(logits: torch.Tensor, u: torch.Tensor, temperature=None, top_k=None, top_p=None, min_p=None,
+           out: torch.Tensor = None, logprobs=None, flags=None, workspace=None, stream=None) -> torch.Tensor:
+    """A token per row of logits (ihip_sample_dev): rows x vocab of fp32, fp16 or bf16,
+    u (one number in [0, 1) a row) and, one value a row or None, temperature, top_p,
+    min_p (fp32) and top_k (int32), all on the device.  Returns int32 tokens; logprobs
+    (fp32) and flags (int32), where given, are written too."""
+    if logits.dim() != 2:
+        raise _invalid("logits are rows x vocab")
+    kind, dev = _ACT_TYPES.get(logits.dtype), logits.get_device()
+    rows, vocab = logits.shape
+    if kind is None or dev < 0:
+        raise _invalid("logits must be an fp32, fp16 or bf16 device tensor")
+    if rows and vocab > 1 and logits.stride(1) != 1:
+        raise _invalid("a row of logits must be contiguous")
+    if out is None:
+        out = _fresh(stream, lambda: torch.empty(rows, dtype=torch.int32, device=logits.device))
+    if workspace is None:
+        n = lib().ihip_sample_scratch_bytes(rows, vocab)
+        if n:
+            workspace = _fresh(stream, lambda: _counted(n, logits.device, _lib.SAMPLE_COUNT_BYTES))
+    _launch(dev, stream, lib().ihip_sample_dev, logits.data_ptr(), kind, logits.stride(0) if rows > 1 else vocab, rows, vocab,
+            _at(temperature, torch.float32, "temperature", dev, rows), _at(top_k, torch.int32, "top_k", dev, rows),
+            _at(top_p, torch.float32, "top_p", dev, rows), _at(min_p, torch.float32, "min_p", dev, rows),
+            _at(u, torch.float32, "u", dev, rows), _at(out, torch.int32, "out", dev, rows),
+            _at(logprobs, torch.float32, "logprobs", dev, rows), _at(flags, torch.int32, "flags", dev, rows),
+            _at(workspace, torch.uint8, "workspace", dev), 0 if workspace is None else workspace.numel())
+    return out
