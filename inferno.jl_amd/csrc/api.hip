@@ -1891,7 +1891,9 @@ size_t ihip_gated_delta_scratch_bytes(int type, const ihip_delta_layer *layer,
     if (check_layer(layer, &a) != IHIP_OK || check_states(batch, &a.batch) != IHIP_OK || !value_bytes(type) ||
         a.batch.tokens == 0 || a.batch.sequences == 0)
         return 0;
-    return 0;
+    return delta_plan(type == kF32 ? 2 : 1, a.k_heads, a.v_heads, a.k_dim, a.v_dim, a.batch.tokens, a.batch.sequences,
+                      batch->most)
+        .bytes;
 }
 
 int ihip_gated_delta_dev(const void *q, int64_t q_stride, const void *k, int64_t k_stride,
@@ -1937,11 +1939,28 @@ int ihip_gated_delta_dev(const void *q, int64_t q_stride, const void *k, int64_t
     for (const Span &in : ins)
         if (!apart(in, to) || !apart(in, held))
             return fail(IHIP_ERR_INVALID, "out or state overlaps another buffer");
-    (void)workspace, (void)workspace_bytes;
+    d.plan = delta_plan(type == kF32 ? 2 : 1, d.k_heads, d.v_heads, d.k_dim, d.v_dim, T, S, batch->most);
+    if (!grid_fits(d.plan.tiles * d.v_heads))
+        return fail(IHIP_ERR_INVALID, "%lld tokens of %d heads are too many for one call", (long long)T, d.v_heads);
+    if (d.plan.bytes) {
+        const Span work{workspace, d.plan.bytes};
+        if (!workspace || workspace_bytes < d.plan.bytes || !al16(workspace))
+            return fail(IHIP_ERR_INVALID, "the workspace needs %zu bytes, 16-byte aligned", d.plan.bytes);
+        bool free = apart(work, to) && apart(work, held);
+        for (const Span &in : ins)
+            free = free && apart(in, work);
+        if (!free)
+            return fail(IHIP_ERR_INVALID, "the workspace overlaps another buffer");
+    }
     d.q = q, d.k = k, d.v = v, d.type = type, d.q_step = q_stride, d.k_step = k_stride, d.v_step = v_stride;
     d.a = a, d.b = b, d.a_step = a_stride, d.b_step = b_stride, d.gate = gate, d.gate_step = gate_stride;
     d.out = out, d.out_type = out_type, d.flags = flags;
-    hipError_t e = launch_delta_step(d, (hipStream_t)stream);
+    d.few = d.plan.chunks ? (d.plan.steps ? kDeltaStepMost : 0) : -1;
+    d.work = (uint8_t *)workspace;
+    d.raw = out_type == kF32 ? (float *)out : (d.norm_w || gate) ? (float *)(d.work + d.plan.raw) : nullptr;
+    hipError_t e = d.plan.steps ? launch_delta_step(d, (hipStream_t)stream) : hipSuccess;
+    if (e == hipSuccess && d.plan.chunks)
+        e = launch_delta_chunks(d, (hipStream_t)stream);
     if (e != hipSuccess)
         return fail(IHIP_ERR_HIP, "delta rule launch failed: %s", hipGetErrorString(e));
     return IHIP_OK;

@@ -7,6 +7,7 @@
 // index formed from them leaves the buffers.
 #pragma once
 
+#include "gd_plan.h"
 #include "kq_common.h"
 #include "kv_common.h"
 
@@ -14,7 +15,6 @@ namespace ihip {
 
 constexpr int kMaxDeltaDim = 128;            // of a head's keys and values
 constexpr uint32_t kFlagStateSlot = 64;      // IHIP_FLAG_STATE_SLOT
-constexpr int kDeltaChunk = 64;              // tokens of a chunk (gd_chunk.hip)
 
 struct StateBatch {
     const int32_t *starts, *lens, *slots;
@@ -68,11 +68,6 @@ __device__ __forceinline__ GdSeq gd_seq(const StateBatch &b, int pool, int s, ui
 // tile c of sequence s is (start >> shift) + s + c.  As start does not decrease,
 // no two tiles have one number; some numbers have no tile, and they end below
 // gd_tiles(): floor(start / m) + floor((n - 1) / m) <= floor((start + n - 1) / m).
-__host__ __device__ constexpr int64_t gd_tiles(int64_t tokens, int64_t sequences, int shift)
-{
-    return (tokens > 0 ? (tokens - 1) >> shift : 0) + sequences;
-}
-
 __device__ __forceinline__ int gd_base(const StateBatch &b, int shift, int s)
 {
     return (kv_clamp(b.starts[s], 0, b.tokens) >> shift) + s;

@@ -43,7 +43,14 @@ struct DeltaArgs {
     float norm_eps, l2_eps, scale;
     StateBatch batch;
     uint32_t *flags;
+    // sequences that the chunks' kernels leave to the other one: with so many new
+    // tokens, or fewer (the step kernel takes those; all of them where it is negative)
+    int few;
+    uint8_t *work;
+    DeltaPlan plan;
+    float *raw; // outputs before their norm (out itself where that is fp32)
 };
 hipError_t launch_delta_step(const DeltaArgs &a, hipStream_t s);
+hipError_t launch_delta_chunks(const DeltaArgs &a, hipStream_t s);
 
 } // namespace ihip

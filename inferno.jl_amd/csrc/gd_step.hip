@@ -35,7 +35,7 @@ __global__ void __launch_bounds__(STEP_THREADS) k_delta_step(DeltaArgs a)
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int h = blockIdx.x % a.v_heads, s = blockIdx.x / a.v_heads, kh = h / a.group;
     const GdSeq seq = gd_seq(a.batch, a.pool, s, h == 0 ? a.flags : nullptr);
-    if (seq.slot < 0 || seq.n == 0)
+    if (seq.slot < 0 || seq.n == 0 || (a.few >= 0 && seq.n > a.few))
         return;
     const int row0 = R * (lane / CL), col0 = wave * (VD / STEP_WAVES) + 4 * (lane % CL);
     float *state = a.state + seq.slot * a.slot_step + (int64_t)h * a.k_dim * a.v_dim;
