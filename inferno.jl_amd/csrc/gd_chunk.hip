@@ -309,15 +309,34 @@ __device__ __forceinline__ float column_most(float m)
     return fmaxf(m, __shfl_xor(m, 32));
 }
 
-// A workgroup takes NW * 16 columns of one head of one sequence.
+// Every copy but the last N has arrived, every read of LDS is done, in all waves
+template <int N>
+__device__ __forceinline__ void scan_sync()
+{
+    static_assert(N < 64, "vmcnt");
+    __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 0x0070); // vmcnt(N) lgkmcnt(0)
+    lds_barrier();
+}
+
+// A workgroup takes NW * 16 columns of one head of one sequence.  What a chunk reads
+// comes to LDS by direct copies, each operand into the place of the last chunk's as
+// soon as that is read: K is on its way while V' is formed, Q, T, P and V while the
+// state is, K^T meanwhile.
 template <int KD, int PARTS, int NW>
 __global__ void __launch_bounds__(64 * NW) k_delta_scan(DeltaArgs a)
 {
     constexpr int KS = KD / 32;
     constexpr int FRAG = 4 * KS * PARTS * 1024;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[3 * FRAG + 2 * kDeltaTri];
-    __shared__ float fs[kDeltaRows];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, r = lane & 15;
+    constexpr int VB = PARTS > 1 ? 4 : 2; // bytes of a value of V
+    constexpr int VROW = 16 * NW * VB;    // of a row of it
+    // in LDS: K | Q | K^T | T, P | V
+    constexpr int Q_AT = FRAG, KT_AT = 2 * FRAG, T_AT = 3 * FRAG, P_AT = T_AT + kDeltaTri, V_AT = P_AT + kDeltaTri;
+    // 1 KB copies of a wave
+    constexpr int NF = FRAG / 1024 / NW, NT = 2 * kDeltaTri / 1024 / NW, NV = VB;
+    static_assert(NF * NW * 1024 == FRAG && NT * NW * 1024 == 2 * kDeltaTri, "copies are shared evenly");
+    __shared__ __attribute__((aligned(16))) uint8_t lds[V_AT + 64 * VROW];
+    __shared__ __attribute__((aligned(16))) float rows[2][kDeltaRows];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, r = lane & 15;
     // the workgroups of the heads that read one K lie on one XCD (its L2)
     const int blocks = (a.v_dim + 16 * NW - 1) / (16 * NW), each = a.group * blocks;
     const int j = blockIdx.x / 8, u = j / each * 8 + blockIdx.x % 8;
@@ -327,9 +346,40 @@ __global__ void __launch_bounds__(64 * NW) k_delta_scan(DeltaArgs a)
     const GdSeq seq = gd_seq(a.batch, a.pool, s, h == 0 && j % blocks == 0 ? a.flags : nullptr);
     if (seq.slot < 0 || seq.n <= a.few)
         return;
-    const int col = (j % blocks * NW + wave) * 16 + r;
+    const int col0 = j % blocks * NW * 16, col = col0 + wave * 16 + r;
     const bool live = col < a.v_dim;
     float *const state = a.state + seq.slot * a.slot_step + (int64_t)h * a.k_dim * a.v_dim + col;
+
+    const int chunks = (seq.n + 63) / 64, tile0 = gd_base(a.batch, kDeltaShift, s);
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds;
+    const uint32_t rows0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) float *)&rows[0][0];
+    auto kq = [&](int c) { return a.work + ((int64_t)(tile0 + c) * a.k_heads + kh) * 3 * FRAG; };
+    auto unit = [&](int c) { return (int64_t)(tile0 + c) * a.v_heads + h; };
+    auto copy = [&](const uint8_t *from, int to, int n) { // n KB a wave
+        for (int i = 0; i < n; ++i)
+            lds_copy16_at(from, (uint32_t)((wave * n + i) * 1024 + lane * 16), lds0 + to + (wave * n + i) * 1024);
+    };
+    // K and the rows' factors (each wave the same 1 KB, so that all wait alike)
+    auto copy_k = [&](int c) {
+        copy(kq(c), 0, NF);
+        lds_copy16_at(a.work + a.plan.rows + unit(c) * kDeltaRows * 4, lane * 16, rows0 + (c & 1) * kDeltaRows * 4);
+    };
+    auto copy_kt = [&](int c) { copy(kq(c) + FRAG, KT_AT, NF); };
+    auto copy_rest = [&](int c) {
+        copy(kq(c) + 2 * FRAG, Q_AT, NF);
+        copy(a.work + a.plan.tri + unit(c) * 2 * kDeltaTri, T_AT, NT);
+        const int n = min(64, seq.n - 64 * c);
+        // (rows behind the last token and columns behind the last one are read as
+        // others and not used)
+        for (int i = 0; i < NV; ++i) {
+            const int at = ((wave * NV + i) * 64 + lane) * 16, e = at % VROW / VB;
+            const int64_t row = seq.start + 64 * c + min(at / VROW, n - 1);
+            lds_copy16((const uint8_t *)a.v + (row * a.v_step + (int64_t)h * a.v_dim + (col0 + e < a.v_dim ? col0 + e : 0)) * VB,
+                       lds0 + V_AT + (wave * NV + i) * 1024);
+        }
+    };
+    copy_k(0);
+    copy_rest(0);
     gd_f4 S[KD / 16];
 #pragma unroll
     for (int m = 0; m < KD / 16; ++m)
@@ -338,33 +388,10 @@ __global__ void __launch_bounds__(64 * NW) k_delta_scan(DeltaArgs a)
             const int at = 16 * m + 4 * g + i;
             S[m][i] = live && !seq.begins && at < a.k_dim ? state[(int64_t)at * a.v_dim] : 0.0f;
         }
-    const int chunks = (seq.n + 63) / 64, tile0 = gd_base(a.batch, kDeltaShift, s);
     for (int c = 0; c < chunks; ++c) {
-        const int n = min(64, seq.n - 64 * c);
+        const int n = min(64, seq.n - 64 * c), next = min(c + 1, chunks - 1);
         const int64_t first = seq.start + 64 * c;
-        const uint8_t *kq = a.work + ((int64_t)(tile0 + c) * a.k_heads + kh) * 3 * FRAG;
-        const int64_t unit = (int64_t)(tile0 + c) * a.v_heads + h;
-        const uint8_t *tri = a.work + a.plan.tri + unit * 2 * kDeltaTri;
-        const float *f = (const float *)(a.work + a.plan.rows) + unit * kDeltaRows;
-        for (int i = tid * 16; i < 3 * FRAG; i += 64 * NW * 16)
-            *(uint4 *)(lds + i) = *(const uint4 *)(kq + i);
-        for (int i = tid * 16; i < 2 * kDeltaTri; i += 64 * NW * 16)
-            *(uint4 *)(lds + 3 * FRAG + i) = *(const uint4 *)(tri + i);
-        for (int i = tid; i < kDeltaRows; i += 64 * NW)
-            fs[i] = f[i];
-        gd_f4 V[4];
-#pragma unroll
-        for (int m = 0; m < 4; ++m)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int at = 16 * m + 4 * g + i;
-                const int64_t from = (first + at) * a.v_step + (int64_t)h * a.v_dim + col;
-                V[m][i] = 0.0f;
-                if (live && at < n)
-                    V[m][i] = a.type == kF32 ? ((const float *)a.v)[from]
-                            : a.type == kF16 ? (float)((const _Float16 *)a.v)[from] : (float)((const __bf16 *)a.v)[from];
-            }
-        __syncthreads();
+        const float *const fs = rows[c & 1];
         // S as an operand
         float most = 0.0f, to, back;
 #pragma unroll
@@ -377,34 +404,53 @@ __global__ void __launch_bounds__(64 * NW) k_delta_scan(DeltaArgs a)
 #pragma unroll
         for (int k = 0; k < KS; ++k)
             gd_split(__builtin_shufflevector(S[2 * k], S[2 * k + 1], 0, 1, 2, 3, 4, 5, 6, 7), to, shi[k], slo[k]);
+        scan_sync<NF + NT + NV>(); // K is here; K^T is read
+        copy_kt(c);
         gd_f4 ks[4], O[4];
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-            ks[m] = O[m] = gd_f4{};
+            ks[m] = gd_f4{};
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
                 const uint8_t *at = lds + (m * KS + k) * PARTS * 1024 + lane * 16;
-                const gd_h8 kh_ = *(const gd_h8 *)at, qh = *(const gd_h8 *)(at + 2 * FRAG);
-                ks[m] = gd_mfma(kh_, shi[k], ks[m]);
-                ks[m] = gd_mfma(kh_, slo[k], ks[m]);
-                O[m] = gd_mfma(qh, shi[k], O[m]);
-                O[m] = gd_mfma(qh, slo[k], O[m]);
-                if (PARTS > 1) {
+                const gd_h8 kf = *(const gd_h8 *)at;
+                ks[m] = gd_mfma(kf, shi[k], ks[m]);
+                ks[m] = gd_mfma(kf, slo[k], ks[m]);
+                if (PARTS > 1)
                     ks[m] = gd_mfma(*(const gd_h8 *)(at + 1024), shi[k], ks[m]);
-                    O[m] = gd_mfma(*(const gd_h8 *)(at + 2 * FRAG + 1024), shi[k], O[m]);
-                }
+            }
+        }
+        scan_sync<NF>(); // Q, T, P and V are here; K is read
+        copy_k(next);
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+            O[m] = gd_f4{};
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                const uint8_t *at = lds + Q_AT + (m * KS + k) * PARTS * 1024 + lane * 16;
+                const gd_h8 qf = *(const gd_h8 *)at;
+                O[m] = gd_mfma(qf, shi[k], O[m]);
+                O[m] = gd_mfma(qf, slo[k], O[m]);
+                if (PARTS > 1)
+                    O[m] = gd_mfma(*(const gd_h8 *)(at + 1024), shi[k], O[m]);
             }
         }
         // X = V - e^G K S as an operand, V' = T X
         gd_f4 x[4];
         most = 0.0f;
+        const float sback = back;
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-            const gd_f4 fk = *(const gd_f4 *)(fs + 16 * m + 4 * g), fq = *(const gd_f4 *)(fs + 64 + 16 * m + 4 * g);
+            const gd_f4 fk = *(const gd_f4 *)(fs + 16 * m + 4 * g);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                x[m][i] = V[m][i] - fk[i] * (ks[m][i] * back);
-                O[m][i] = fq[i] * (O[m][i] * back);
+                const int at = 16 * m + 4 * g + i;
+                const uint8_t *from = lds + V_AT + at * VROW + (wave * 16 + r) * VB;
+                float v = a.type == kF32 ? *(const float *)from
+                        : a.type == kF16 ? (float)*(const _Float16 *)from : (float)*(const __bf16 *)from;
+                if (!live || at >= n)
+                    v = 0.0f;
+                x[m][i] = v - fk[i] * (ks[m][i] * sback);
                 most = fmaxf(most, fabsf(x[m][i]));
             }
         }
@@ -420,7 +466,7 @@ __global__ void __launch_bounds__(64 * NW) k_delta_scan(DeltaArgs a)
             w[m] = gd_f4{};
 #pragma unroll
             for (int k = 0; k <= m / 2; ++k) {
-                const uint8_t *at = lds + 3 * FRAG + (m < 2 ? m : 2 * m - 2 + k) * 2048 + lane * 16;
+                const uint8_t *at = lds + T_AT + (m < 2 ? m : 2 * m - 2 + k) * 2048 + lane * 16;
                 const gd_h8 th = *(const gd_h8 *)at, tl = *(const gd_h8 *)(at + 1024);
                 w[m] = gd_mfma(th, hi[k], w[m]);
                 w[m] = gd_mfma(th, lo[k], w[m]);
@@ -428,7 +474,7 @@ __global__ void __launch_bounds__(64 * NW) k_delta_scan(DeltaArgs a)
             }
             w[m] = w[m] * back;
         }
-        // O += P V'
+        // O = scale (e^G Q S + P V')
         most = 0.0f;
 #pragma unroll
         for (int m = 0; m < 4; ++m)
@@ -442,10 +488,11 @@ __global__ void __launch_bounds__(64 * NW) k_delta_scan(DeltaArgs a)
         back *= 1.0f / (1 << TOP);
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
+            const gd_f4 fq = *(const gd_f4 *)(fs + 64 + 16 * m + 4 * g);
             gd_f4 y{};
 #pragma unroll
             for (int k = 0; k <= m / 2; ++k) {
-                const uint8_t *at = lds + 3 * FRAG + kDeltaTri + (m < 2 ? m : 2 * m - 2 + k) * 2048 + lane * 16;
+                const uint8_t *at = lds + P_AT + (m < 2 ? m : 2 * m - 2 + k) * 2048 + lane * 16;
                 const gd_h8 th = *(const gd_h8 *)at, tl = *(const gd_h8 *)(at + 1024);
                 y = gd_mfma(th, hi[k], y);
                 y = gd_mfma(th, lo[k], y);
@@ -454,7 +501,7 @@ __global__ void __launch_bounds__(64 * NW) k_delta_scan(DeltaArgs a)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int at = 16 * m + 4 * g + i;
-                const float o = a.scale * fmaf(y[i], back, O[m][i]);
+                const float o = a.scale * fmaf(y[i], back, fq[i] * (O[m][i] * sback));
                 const int64_t where = ((first + at) * a.v_heads + h) * a.v_dim + col;
                 if (live && at < n) {
                     if (a.raw)
@@ -480,12 +527,14 @@ __global__ void __launch_bounds__(64 * NW) k_delta_scan(DeltaArgs a)
         for (int k = 0; k < 2; ++k)
             gd_split(__builtin_shufflevector(w[2 * k], w[2 * k + 1], 0, 1, 2, 3, 4, 5, 6, 7), to, hi[k], lo[k]);
         const float keep = fs[192];
+        scan_sync<NF + 1>(); // K^T is here; Q, T, P and V are read
+        copy_rest(next);
 #pragma unroll
         for (int m = 0; m < KD / 16; ++m) {
             gd_f4 y{};
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                const uint8_t *at = lds + FRAG + (2 * m + k) * PARTS * 1024 + lane * 16;
+                const uint8_t *at = lds + KT_AT + (2 * m + k) * PARTS * 1024 + lane * 16;
                 const gd_h8 kt = *(const gd_h8 *)at;
                 y = gd_mfma(kt, hi[k], y);
                 y = gd_mfma(kt, lo[k], y);
@@ -496,8 +545,8 @@ __global__ void __launch_bounds__(64 * NW) k_delta_scan(DeltaArgs a)
             for (int i = 0; i < 4; ++i)
                 S[m][i] = fmaf(keep, S[m][i], y[i] * back);
         }
-        __syncthreads(); // lds and fs are read
     }
+    __builtin_amdgcn_s_waitcnt(0x0070); // no copy is in flight when the workgroup ends
 #pragma unroll
     for (int m = 0; m < KD / 16; ++m)
 #pragma unroll
@@ -551,7 +600,7 @@ __global__ void __launch_bounds__(NORM_THREADS) k_delta_norm(DeltaArgs a)
 template <int KD, int PARTS>
 void launch(const DeltaArgs &a, hipStream_t s)
 {
-    constexpr int NW = 2;
+    constexpr int NW = 4;
     const unsigned units = (unsigned)(a.plan.tiles * a.v_heads);
     hipLaunchKernelGGL((k_delta_prep<KD, PARTS>), dim3(units), dim3(PREP_THREADS), 0, s, a);
     const unsigned blocks = (unsigned)((a.v_dim + 16 * NW - 1) / (16 * NW)) * (unsigned)a.group;
