@@ -14,7 +14,7 @@
 // Operands are fp16 times a power of two (of a row of K and Q, of a column of S, V and
 // V'), so that the largest value lies in 2^13 .. 2^14: values of F16 and BF16 inputs
 // fit one part exactly down to 2^-27 of their row's largest; fp32 values and
-// everything derived is held in two parts, which leave 2^-22 of a value, and products
+// everything derived are held in two parts, which leave 2^-22 of a value, and products
 // of the two lower parts (2^-22) are not formed.  Sums are fp32.  Rows' factors (unit
 // length, e^G) are applied to the products, in fp32, so that K and Q are shared by the
 // heads that read them.
@@ -38,12 +38,15 @@ __device__ __forceinline__ void gd_power(float x, float &to, float &back)
     back = __uint_as_float((uint32_t)(e - TOP) << 23);
 }
 
-// x * by as one fp16 part, or its rest as the next one too
+// x * by as one fp16 part, and the rest of it, times 2^11, as the next.  (The matrix
+// cores take fp16 values below 2^-14 as zeros: unscaled rests of all but the largest
+// values would be cut, to 2^-16 of a typical state.)
+constexpr float REST = 2048.0f;
 __device__ __forceinline__ void gd_split(gd_f8 x, float by, gd_h8 &hi, gd_h8 &lo)
 {
     x = x * by;
     hi = __builtin_convertvector(x, gd_h8);
-    lo = __builtin_convertvector(x - __builtin_convertvector(hi, gd_f8), gd_h8);
+    lo = __builtin_convertvector((x - __builtin_convertvector(hi, gd_f8)) * REST, gd_h8);
 }
 
 __device__ __forceinline__ gd_f4 gd_mfma(gd_h8 a, gd_h8 b, gd_f4 c)
@@ -207,6 +210,7 @@ __global__ void __launch_bounds__(PREP_THREADS) k_delta_prep(DeltaArgs a)
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
         kk[t] = qk[t] = gd_f4{};
+        gd_f4 krest{}, qrest{};
         if (t > wave)
             continue;
 #pragma unroll
@@ -215,13 +219,18 @@ __global__ void __launch_bounds__(PREP_THREADS) k_delta_prep(DeltaArgs a)
 #pragma unroll
             for (int p = 0; p < PARTS; ++p)
                 b[p] = *(const gd_h8 *)(lds + ((t * KS + i) * PARTS + p) * 1024 + lane * 16);
-#pragma unroll
-            for (int p = 0; p < PARTS; ++p)
-#pragma unroll
-                for (int q = 0; q + p < PARTS; ++q) {
-                    kk[t] = gd_mfma(kf[i][p], b[q], kk[t]);
-                    qk[t] = gd_mfma(qf[i][p], b[q], qk[t]);
-                }
+            kk[t] = gd_mfma(kf[i][0], b[0], kk[t]);
+            qk[t] = gd_mfma(qf[i][0], b[0], qk[t]);
+            if (PARTS > 1) {
+                krest = gd_mfma(kf[i][0], b[PARTS - 1], krest);
+                krest = gd_mfma(kf[i][PARTS - 1], b[0], krest);
+                qrest = gd_mfma(qf[i][0], b[PARTS - 1], qrest);
+                qrest = gd_mfma(qf[i][PARTS - 1], b[0], qrest);
+            }
+        }
+        if (PARTS > 1) {
+            kk[t] += krest * (1.0f / REST);
+            qk[t] += qrest * (1.0f / REST);
         }
     }
     float rqs[4];
@@ -302,43 +311,48 @@ __global__ void __launch_bounds__(PREP_THREADS) k_delta_prep(DeltaArgs a)
 }
 
 // ---- down the chunks ---------------------------------------------------------------
-// The largest |x| of a lane's column (in its 4 lanes)
-__device__ __forceinline__ float column_most(float m)
-{
-    m = fmaxf(m, __shfl_xor(m, 16));
-    return fmaxf(m, __shfl_xor(m, 32));
-}
+constexpr int SCAN_WAVES = 4;
 
-// Every copy but the last N has arrived, every read of LDS is done, in all waves
-template <int N>
+// What a wave reads of a chunk: its 16 rows of K, Q, T and P, its 32 rows of K^T (in
+// steps of columns), the factors of its 16 tokens and their values in its columns.
+template <int KS, int PARTS, int CT>
+struct ScanOps {
+    gd_h8 k[KS][PARTS], q[KS][PARTS], kt[2][2][PARTS], t[2][2], p[2][2];
+    gd_f4 fk, fq, fu;
+    uint32_t v[CT][4]; // as they lie in memory
+    float keep;
+};
+
+// All waves are here, and what they wrote to LDS is
 __device__ __forceinline__ void scan_sync()
 {
-    static_assert(N < 64, "vmcnt");
-    __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 0x0070); // vmcnt(N) lgkmcnt(0)
+    __builtin_amdgcn_s_waitcnt(0xc07f); // lgkmcnt(0); loads stay on their way
     lds_barrier();
 }
 
-// A workgroup takes NW * 16 columns of one head of one sequence.  What a chunk reads
-// comes to LDS by direct copies, each operand into the place of the last chunk's as
-// soon as that is read: K is on its way while V' is formed, Q, T, P and V while the
-// state is, K^T meanwhile.
-template <int KD, int PARTS, int NW>
-__global__ void __launch_bounds__(64 * NW) k_delta_scan(DeltaArgs a)
+// A workgroup takes 16 CT columns of one head of one sequence, each of its waves the
+// tokens 16 w .. 16 w + 15 of a chunk and the rows 32 w .. 32 w + 31 of S (there are
+// KD / 32 such waves).  A wave so reads only its own part of the operands, from memory
+// into registers, a chunk ahead, and the waves exchange S, X, V' and what is written to
+// S as fp16 fragments in LDS, with three barriers a chunk.  Bound by that chain, not by
+// bytes or products: a chunk follows the other.
+//
+// One power of two serves a column for a whole chunk.  k and q have unit length at most,
+// and no token adds more than |v| to the length of a column of S, so |X|, |V'| and the
+// new S lie below 12 max |S| + 66 max |v| (sqrt(128) < 12).  Fragments keep 22 bits of
+// what is over 2^-27 of that.
+template <int KD, int PARTS, int CT>
+__global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
 {
     constexpr int KS = KD / 32;
     constexpr int FRAG = 4 * KS * PARTS * 1024;
-    constexpr int VB = PARTS > 1 ? 4 : 2; // bytes of a value of V
-    constexpr int VROW = 16 * NW * VB;    // of a row of it
-    // in LDS: K | Q | K^T | T, P | V
-    constexpr int Q_AT = FRAG, KT_AT = 2 * FRAG, T_AT = 3 * FRAG, P_AT = T_AT + kDeltaTri, V_AT = P_AT + kDeltaTri;
-    // 1 KB copies of a wave
-    constexpr int NF = FRAG / 1024 / NW, NT = 2 * kDeltaTri / 1024 / NW, NV = VB;
-    static_assert(NF * NW * 1024 == FRAG && NT * NW * 1024 == 2 * kDeltaTri, "copies are shared evenly");
-    __shared__ __attribute__((aligned(16))) uint8_t lds[V_AT + 64 * VROW];
-    __shared__ __attribute__((aligned(16))) float rows[2][kDeltaRows];
+    using Ops = ScanOps<KS, PARTS, CT>;
+    __shared__ __attribute__((aligned(16))) uint8_t sf[CT][KS][2][1024], xf[CT][2][2][1024], wf[CT][2][2][1024], uf[CT][2][2][1024];
+    __shared__ float bounds[SCAN_WAVES][CT][16];
+    __shared__ __attribute__((aligned(16))) float turn[SCAN_WAVES][16][20];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, r = lane & 15;
     // the workgroups of the heads that read one K lie on one XCD (its L2)
-    const int blocks = (a.v_dim + 16 * NW - 1) / (16 * NW), each = a.group * blocks;
+    const int blocks = (a.v_dim + 16 * CT - 1) / (16 * CT), each = a.group * blocks;
     const int j = blockIdx.x / 8, u = j / each * 8 + blockIdx.x % 8;
     if (u >= a.k_heads * a.batch.sequences)
         return;
@@ -346,215 +360,239 @@ __global__ void __launch_bounds__(64 * NW) k_delta_scan(DeltaArgs a)
     const GdSeq seq = gd_seq(a.batch, a.pool, s, h == 0 && j % blocks == 0 ? a.flags : nullptr);
     if (seq.slot < 0 || seq.n <= a.few)
         return;
-    const int col0 = j % blocks * NW * 16, col = col0 + wave * 16 + r;
-    const bool live = col < a.v_dim;
-    float *const state = a.state + seq.slot * a.slot_step + (int64_t)h * a.k_dim * a.v_dim + col;
-
+    const int col0 = j % blocks * CT * 16;
+    float *const state = a.state + seq.slot * a.slot_step + (int64_t)h * a.k_dim * a.v_dim + col0 + r;
     const int chunks = (seq.n + 63) / 64, tile0 = gd_base(a.batch, kDeltaShift, s);
-    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds;
-    const uint32_t rows0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) float *)&rows[0][0];
-    auto kq = [&](int c) { return a.work + ((int64_t)(tile0 + c) * a.k_heads + kh) * 3 * FRAG; };
-    auto unit = [&](int c) { return (int64_t)(tile0 + c) * a.v_heads + h; };
-    auto copy = [&](const uint8_t *from, int to, int n) { // n KB a wave
-        for (int i = 0; i < n; ++i)
-            lds_copy16_at(from, (uint32_t)((wave * n + i) * 1024 + lane * 16), lds0 + to + (wave * n + i) * 1024);
-    };
-    // K and the rows' factors (each wave the same 1 KB, so that all wait alike)
-    auto copy_k = [&](int c) {
-        copy(kq(c), 0, NF);
-        lds_copy16_at(a.work + a.plan.rows + unit(c) * kDeltaRows * 4, lane * 16, rows0 + (c & 1) * kDeltaRows * 4);
-    };
-    auto copy_kt = [&](int c) { copy(kq(c) + FRAG, KT_AT, NF); };
-    auto copy_rest = [&](int c) {
-        copy(kq(c) + 2 * FRAG, Q_AT, NF);
-        copy(a.work + a.plan.tri + unit(c) * 2 * kDeltaTri, T_AT, NT);
-        const int n = min(64, seq.n - 64 * c);
-        // (rows behind the last token and columns behind the last one are read as
-        // others and not used)
-        for (int i = 0; i < NV; ++i) {
-            const int at = ((wave * NV + i) * 64 + lane) * 16, e = at % VROW / VB;
-            const int64_t row = seq.start + 64 * c + min(at / VROW, n - 1);
-            lds_copy16((const uint8_t *)a.v + (row * a.v_step + (int64_t)h * a.v_dim + (col0 + e < a.v_dim ? col0 + e : 0)) * VB,
-                       lds0 + V_AT + (wave * NV + i) * 1024);
-        }
-    };
-    copy_k(0);
-    copy_rest(0);
-    gd_f4 S[KD / 16];
+    const bool half = a.type == kF16, owner = wave < KS;
+    bool live[CT];
 #pragma unroll
-    for (int m = 0; m < KD / 16; ++m)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int at = 16 * m + 4 * g + i;
-            S[m][i] = live && !seq.begins && at < a.k_dim ? state[(int64_t)at * a.v_dim] : 0.0f;
-        }
-    for (int c = 0; c < chunks; ++c) {
-        const int n = min(64, seq.n - 64 * c), next = min(c + 1, chunks - 1);
-        const int64_t first = seq.start + 64 * c;
-        const float *const fs = rows[c & 1];
-        // S as an operand
-        float most = 0.0f, to, back;
-#pragma unroll
-        for (int m = 0; m < KD / 16; ++m)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                most = fmaxf(most, fabsf(S[m][i]));
-        gd_power(column_most(most), to, back);
-        gd_h8 shi[KS], slo[KS];
+    for (int e = 0; e < CT; ++e)
+        live[e] = col0 + 16 * e < a.v_dim;
+
+    auto load = [&](Ops &o, int c) {
+        c = min(c, chunks - 1); // (behind the last chunk: its operands again)
+        const int64_t unit = (int64_t)(tile0 + c) * a.v_heads + h;
+        const uint8_t *const kq = a.work + ((int64_t)(tile0 + c) * a.k_heads + kh) * 3 * FRAG + lane * 16;
+        const uint8_t *const tri = a.work + a.plan.tri + unit * 2 * kDeltaTri + lane * 16;
+        const float *const f = (const float *)(a.work + a.plan.rows) + unit * kDeltaRows;
 #pragma unroll
         for (int k = 0; k < KS; ++k)
-            gd_split(__builtin_shufflevector(S[2 * k], S[2 * k + 1], 0, 1, 2, 3, 4, 5, 6, 7), to, shi[k], slo[k]);
-        scan_sync<NF + NT + NV>(); // K is here; K^T is read
-        copy_kt(c);
-        gd_f4 ks[4], O[4];
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
-            ks[m] = gd_f4{};
+            for (int p = 0; p < PARTS; ++p)
+                o.k[k][p] = *(const gd_h8 *)(kq + ((wave * KS + k) * PARTS + p) * 1024);
+        o.fk = *(const gd_f4 *)(f + 16 * wave + 4 * g);
+        // (rows behind the last token and columns behind the last one: others', not used)
+        const int at0 = 64 * c + 16 * wave + 4 * g;
 #pragma unroll
-            for (int k = 0; k < KS; ++k) {
-                const uint8_t *at = lds + (m * KS + k) * PARTS * 1024 + lane * 16;
-                const gd_h8 kf = *(const gd_h8 *)at;
-                ks[m] = gd_mfma(kf, shi[k], ks[m]);
-                ks[m] = gd_mfma(kf, slo[k], ks[m]);
-                if (PARTS > 1)
-                    ks[m] = gd_mfma(*(const gd_h8 *)(at + 1024), shi[k], ks[m]);
-            }
-        }
-        scan_sync<NF>(); // Q, T, P and V are here; K is read
-        copy_k(next);
-#pragma unroll
-        for (int m = 0; m < 4; ++m) {
-            O[m] = gd_f4{};
-#pragma unroll
-            for (int k = 0; k < KS; ++k) {
-                const uint8_t *at = lds + Q_AT + (m * KS + k) * PARTS * 1024 + lane * 16;
-                const gd_h8 qf = *(const gd_h8 *)at;
-                O[m] = gd_mfma(qf, shi[k], O[m]);
-                O[m] = gd_mfma(qf, slo[k], O[m]);
-                if (PARTS > 1)
-                    O[m] = gd_mfma(*(const gd_h8 *)(at + 1024), shi[k], O[m]);
-            }
-        }
-        // X = V - e^G K S as an operand, V' = T X
-        gd_f4 x[4];
-        most = 0.0f;
-        const float sback = back;
-#pragma unroll
-        for (int m = 0; m < 4; ++m) {
-            const gd_f4 fk = *(const gd_f4 *)(fs + 16 * m + 4 * g);
+        for (int e = 0; e < CT; ++e)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int at = 16 * m + 4 * g + i;
-                const uint8_t *from = lds + V_AT + at * VROW + (wave * 16 + r) * VB;
-                float v = a.type == kF32 ? *(const float *)from
-                        : a.type == kF16 ? (float)*(const _Float16 *)from : (float)*(const __bf16 *)from;
-                if (!live || at >= n)
-                    v = 0.0f;
-                x[m][i] = v - fk[i] * (ks[m][i] * sback);
-                most = fmaxf(most, fabsf(x[m][i]));
+                const int64_t from = (int64_t)(seq.start + min(at0 + i, seq.n - 1)) * a.v_step + (int64_t)h * a.v_dim + col0 +
+                                     (live[e] ? 16 * e : 0) + r;
+                o.v[e][i] = PARTS > 1 ? ((const uint32_t *)a.v)[from] : ((const uint16_t *)a.v)[from];
+            }
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p)
+                o.q[k][p] = *(const gd_h8 *)(kq + 2 * FRAG + ((wave * KS + k) * PARTS + p) * 1024);
+        const int t0 = wave < 2 ? wave : 2 * wave - 2; // this wave's first tile of a triangle
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+            o.t[0][p] = *(const gd_h8 *)(tri + (2 * t0 + p) * 1024);
+            o.p[0][p] = *(const gd_h8 *)(tri + kDeltaTri + (2 * t0 + p) * 1024);
+            if (wave >= 2) {
+                o.t[1][p] = *(const gd_h8 *)(tri + (2 * t0 + 2 + p) * 1024);
+                o.p[1][p] = *(const gd_h8 *)(tri + kDeltaTri + (2 * t0 + 2 + p) * 1024);
             }
         }
-        gd_power(column_most(most), to, back);
-        gd_h8 hi[2], lo[2];
+        o.fq = *(const gd_f4 *)(f + 64 + 16 * wave + 4 * g);
+        o.fu = *(const gd_f4 *)(f + 128 + 16 * wave + 4 * g);
+        o.keep = f[192];
+        if (owner)
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
-            gd_split(__builtin_shufflevector(x[2 * k], x[2 * k + 1], 0, 1, 2, 3, 4, 5, 6, 7), to, hi[k], lo[k]);
-        back *= 1.0f / (1 << TOP);
-        gd_f4 w[4];
+            for (int m = 0; m < 2; ++m)
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
-            w[m] = gd_f4{};
+                for (int k = 0; k < 2; ++k)
 #pragma unroll
-            for (int k = 0; k <= m / 2; ++k) {
-                const uint8_t *at = lds + T_AT + (m < 2 ? m : 2 * m - 2 + k) * 2048 + lane * 16;
-                const gd_h8 th = *(const gd_h8 *)at, tl = *(const gd_h8 *)(at + 1024);
-                w[m] = gd_mfma(th, hi[k], w[m]);
-                w[m] = gd_mfma(th, lo[k], w[m]);
-                w[m] = gd_mfma(tl, hi[k], w[m]);
-            }
-            w[m] = w[m] * back;
-        }
-        // O = scale (e^G Q S + P V')
-        most = 0.0f;
+                    for (int p = 0; p < PARTS; ++p)
+                        o.kt[m][k][p] = *(const gd_h8 *)(kq + FRAG + ((2 * (2 * wave + m) + k) * PARTS + p) * 1024);
+    };
+    auto most4 = [](gd_f4 x) { return fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))); };
+    // four values of a column as half a fragment's 8
+    auto put = [&](uint8_t (*to)[2][1024], gd_f4 x, float by) {
+        typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+        x = x * by;
+        const h4 hi = __builtin_convertvector(x, h4);
+        const h4 lo = __builtin_convertvector((x - __builtin_convertvector(hi, gd_f4)) * REST, h4);
+        *(h4 *)(to[wave / 2][0] + lane * 16 + 8 * (wave & 1)) = hi;
+        *(h4 *)(to[wave / 2][1] + lane * 16 + 8 * (wave & 1)) = lo;
+    };
+
+    gd_f4 S[CT][2];
+    float to_s[CT], back_s[CT];
 #pragma unroll
-        for (int m = 0; m < 4; ++m)
+    for (int e = 0; e < CT; ++e) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                most = fmaxf(most, fabsf(w[m][i]));
-        gd_power(column_most(most), to, back);
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-            gd_split(__builtin_shufflevector(w[2 * k], w[2 * k + 1], 0, 1, 2, 3, 4, 5, 6, 7), to, hi[k], lo[k]);
-        back *= 1.0f / (1 << TOP);
-#pragma unroll
-        for (int m = 0; m < 4; ++m) {
-            const gd_f4 fq = *(const gd_f4 *)(fs + 64 + 16 * m + 4 * g);
-            gd_f4 y{};
-#pragma unroll
-            for (int k = 0; k <= m / 2; ++k) {
-                const uint8_t *at = lds + P_AT + (m < 2 ? m : 2 * m - 2 + k) * 2048 + lane * 16;
-                const gd_h8 th = *(const gd_h8 *)at, tl = *(const gd_h8 *)(at + 1024);
-                y = gd_mfma(th, hi[k], y);
-                y = gd_mfma(th, lo[k], y);
-                y = gd_mfma(tl, hi[k], y);
-            }
+        for (int m = 0; m < 2; ++m)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int at = 16 * m + 4 * g + i;
-                const float o = a.scale * fmaf(y[i], back, fq[i] * (O[m][i] * sback));
-                const int64_t where = ((first + at) * a.v_heads + h) * a.v_dim + col;
-                if (live && at < n) {
-                    if (a.raw)
-                        a.raw[where] = o;
-                    else if (a.out_type == kF16)
-                        ((_Float16 *)a.out)[where] = (_Float16)o;
-                    else
-                        ((__bf16 *)a.out)[where] = (__bf16)o;
-                }
+                const int at = 32 * wave + 16 * m + 4 * g + i;
+                S[e][m][i] = owner && live[e] && !seq.begins && at < a.k_dim ? state[(int64_t)at * a.v_dim + 16 * e] : 0.0f;
             }
-        }
-        // S <- e^G_64 S + K^T (e^(G_64 - G) V')
-        most = 0.0f;
-#pragma unroll
-        for (int m = 0; m < 4; ++m) {
-            w[m] = w[m] * *(const gd_f4 *)(fs + 128 + 16 * m + 4 * g);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                most = fmaxf(most, fabsf(w[m][i]));
-        }
-        gd_power(column_most(most), to, back);
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-            gd_split(__builtin_shufflevector(w[2 * k], w[2 * k + 1], 0, 1, 2, 3, 4, 5, 6, 7), to, hi[k], lo[k]);
-        const float keep = fs[192];
-        scan_sync<NF + 1>(); // K^T is here; Q, T, P and V are read
-        copy_rest(next);
-#pragma unroll
-        for (int m = 0; m < KD / 16; ++m) {
-            gd_f4 y{};
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const uint8_t *at = lds + KT_AT + (2 * m + k) * PARTS * 1024 + lane * 16;
-                const gd_h8 kt = *(const gd_h8 *)at;
-                y = gd_mfma(kt, hi[k], y);
-                y = gd_mfma(kt, lo[k], y);
-                if (PARTS > 1)
-                    y = gd_mfma(*(const gd_h8 *)(at + 1024), hi[k], y);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                S[m][i] = fmaf(keep, S[m][i], y[i] * back);
-        }
+        const float most = gd_max32(gd_max16(fmaxf(most4(S[e][0]), most4(S[e][1]))));
+        if (g == 0)
+            bounds[wave][e][r] = most;
     }
-    __builtin_amdgcn_s_waitcnt(0x0070); // no copy is in flight when the workgroup ends
+    scan_sync();
+    auto widest = [&](int e) {
+        return fmaxf(fmaxf(bounds[0][e][r], bounds[1][e][r]), fmaxf(bounds[2][e][r], bounds[3][e][r]));
+    };
 #pragma unroll
-    for (int m = 0; m < KD / 16; ++m)
+    for (int e = 0; e < CT; ++e)
+        gd_power(widest(e), to_s[e], back_s[e]);
+    scan_sync();
+
+    auto chunk = [&](const Ops &o, int c) {
+        const int n = min(64, seq.n - 64 * c);
+        gd_f4 v[CT];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int at = 16 * m + 4 * g + i;
-            if (live && at < a.k_dim)
-                state[(int64_t)at * a.v_dim] = S[m][i];
+        for (int e = 0; e < CT; ++e) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float x = PARTS > 1 ? __uint_as_float(o.v[e][i]) : half ? h2f(o.v[e][i]) : __uint_as_float(o.v[e][i] << 16);
+                v[e][i] = live[e] && 16 * wave + 4 * g + i < n ? x : 0.0f;
+            }
+            if (owner) {
+                gd_h8 hi, lo;
+                gd_split(__builtin_shufflevector(S[e][0], S[e][1], 0, 1, 2, 3, 4, 5, 6, 7), to_s[e], hi, lo);
+                *(gd_h8 *)(sf[e][wave][0] + lane * 16) = hi;
+                *(gd_h8 *)(sf[e][wave][1] + lane * 16) = lo;
+            }
+            const float most = 12.0f * fmaxf(most4(S[e][0]), most4(S[e][1])) + 66.0f * most4(v[e]);
+            const float all = gd_max32(gd_max16(most));
+            if (g == 0)
+                bounds[wave][e][r] = all;
         }
+        scan_sync();
+        // K S and Q S; X = V - e^G K S
+        gd_f4 qs[CT];
+        float to[CT], back[CT];
+#pragma unroll
+        for (int e = 0; e < CT; ++e) {
+            gd_power(widest(e), to[e], back[e]);
+            gd_h8 hi[KS], lo[KS];
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                hi[k] = *(const gd_h8 *)(sf[e][k][0] + lane * 16);
+                lo[k] = *(const gd_h8 *)(sf[e][k][1] + lane * 16);
+            }
+            gd_f4 x{}, y{}, z{}, w{};
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                x = gd_mfma(o.k[k][0], hi[k], x);
+                y = gd_mfma(o.k[k][0], lo[k], y);
+                if (PARTS > 1)
+                    y = gd_mfma(o.k[k][PARTS - 1], hi[k], y);
+            }
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                z = gd_mfma(o.q[k][0], hi[k], z);
+                w = gd_mfma(o.q[k][0], lo[k], w);
+                if (PARTS > 1)
+                    w = gd_mfma(o.q[k][PARTS - 1], hi[k], w);
+            }
+            put(xf[e], v[e] - o.fk * ((x + y * (1.0f / REST)) * back_s[e]), to[e]);
+            qs[e] = (z + w * (1.0f / REST)) * back_s[e] * o.fq;
+        }
+        scan_sync();
+        // V' = T X, and what is written to S
+#pragma unroll
+        for (int e = 0; e < CT; ++e) {
+            gd_f4 x{}, y{};
+            auto step = [&](int k) {
+                const gd_h8 hi = *(const gd_h8 *)(xf[e][k][0] + lane * 16), lo = *(const gd_h8 *)(xf[e][k][1] + lane * 16);
+                x = gd_mfma(o.t[k][0], hi, x);
+                y = gd_mfma(o.t[k][0], lo, y);
+                y = gd_mfma(o.t[k][1], hi, y);
+            };
+            step(0);
+            if (wave >= 2)
+                step(1);
+            // (still times the column's power of two)
+            const gd_f4 w = (x + y * (1.0f / REST)) * (1.0f / (1 << TOP));
+            put(wf[e], w, 1.0f);
+            put(uf[e], w * o.fu, 1.0f);
+        }
+        scan_sync();
+        // S <- e^G_64 S + K^T (e^(G_64 - G) V');  O = scale (e^G Q S + P V')
+#pragma unroll
+        for (int e = 0; e < CT; ++e) {
+            if (owner) {
+                gd_f4 x[2]{}, y[2]{};
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const gd_h8 hi = *(const gd_h8 *)(uf[e][k][0] + lane * 16), lo = *(const gd_h8 *)(uf[e][k][1] + lane * 16);
+#pragma unroll
+                    for (int m = 0; m < 2; ++m) {
+                        x[m] = gd_mfma(o.kt[m][k][0], hi, x[m]);
+                        y[m] = gd_mfma(o.kt[m][k][0], lo, y[m]);
+                        if (PARTS > 1)
+                            y[m] = gd_mfma(o.kt[m][k][PARTS - 1], hi, y[m]);
+                    }
+                }
+#pragma unroll
+                for (int m = 0; m < 2; ++m)
+                    S[e][m] = S[e][m] * o.keep + (x[m] + y[m] * (1.0f / REST)) * back[e];
+            }
+            gd_f4 x{}, y{};
+            auto step = [&](int k) {
+                const gd_h8 hi = *(const gd_h8 *)(wf[e][k][0] + lane * 16), lo = *(const gd_h8 *)(wf[e][k][1] + lane * 16);
+                x = gd_mfma(o.p[k][0], hi, x);
+                y = gd_mfma(o.p[k][0], lo, y);
+                y = gd_mfma(o.p[k][1], hi, y);
+            };
+            step(0);
+            if (wave >= 2)
+                step(1);
+            const gd_f4 out = a.scale * (qs[e] + (x + y * (1.0f / REST)) * (back[e] * (1.0f / (1 << TOP))));
+            // through LDS, so that a lane stores 4 neighbours
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                turn[wave][4 * g + i][r] = out[i];
+            const gd_f4 flat = *(const gd_f4 *)&turn[wave][lane / 4][4 * (lane % 4)];
+            const int at = 16 * wave + lane / 4;
+            if (live[e] && at < n) {
+                const int64_t where = ((int64_t)(seq.start + 64 * c + at) * a.v_heads + h) * a.v_dim + col0 + 16 * e + 4 * (lane % 4);
+                if (a.raw)
+                    *(gd_f4 *)(a.raw + where) = flat;
+                else
+                    gd_store4(a.out, where, a.out_type, flat);
+            }
+            to_s[e] = to[e], back_s[e] = back[e];
+        }
+    };
+    Ops even, odd;
+    load(even, 0);
+    for (int c = 0; c < chunks; c += 2) {
+        load(odd, c + 1);
+        chunk(even, c);
+        if (c + 1 >= chunks)
+            break;
+        load(even, c + 2);
+        chunk(odd, c + 1);
+    }
+    if (owner)
+#pragma unroll
+        for (int e = 0; e < CT; ++e)
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int at = 32 * wave + 16 * m + 4 * g + i;
+                    if (live[e] && at < a.k_dim)
+                        state[(int64_t)at * a.v_dim + 16 * e] = S[e][m][i];
+                }
 }
 
 // ---- the output norm ---------------------------------------------------------------
@@ -600,12 +638,12 @@ __global__ void __launch_bounds__(NORM_THREADS) k_delta_norm(DeltaArgs a)
 template <int KD, int PARTS>
 void launch(const DeltaArgs &a, hipStream_t s)
 {
-    constexpr int NW = 4;
+    constexpr int CT = 1;
     const unsigned units = (unsigned)(a.plan.tiles * a.v_heads);
     hipLaunchKernelGGL((k_delta_prep<KD, PARTS>), dim3(units), dim3(PREP_THREADS), 0, s, a);
-    const unsigned blocks = (unsigned)((a.v_dim + 16 * NW - 1) / (16 * NW)) * (unsigned)a.group;
+    const unsigned blocks = (unsigned)((a.v_dim + 16 * CT - 1) / (16 * CT)) * (unsigned)a.group;
     const unsigned heads = ((unsigned)(a.k_heads * a.batch.sequences) + 7) / 8 * 8;
-    hipLaunchKernelGGL((k_delta_scan<KD, PARTS, NW>), dim3(heads * blocks), dim3(64 * NW), 0, s, a);
+    hipLaunchKernelGGL((k_delta_scan<KD, PARTS, CT>), dim3(heads * blocks), dim3(64 * SCAN_WAVES), 0, s, a);
     if (a.norm_w || a.gate)
         hipLaunchKernelGGL(k_delta_norm, dim3(units), dim3(NORM_THREADS), 0, s, a);
 }
