@@ -369,12 +369,14 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
     for (int e = 0; e < CT; ++e)
         live[e] = col0 + 16 * e < a.v_dim;
 
-    auto load = [&](Ops &o, int c) {
-        c = min(c, chunks - 1); // (behind the last chunk: its operands again)
-        const int64_t unit = (int64_t)(tile0 + c) * a.v_heads + h;
-        const uint8_t *const kq = a.work + ((int64_t)(tile0 + c) * a.k_heads + kh) * 3 * FRAG + lane * 16;
-        const uint8_t *const tri = a.work + a.plan.tri + unit * 2 * kDeltaTri + lane * 16;
-        const float *const f = (const float *)(a.work + a.plan.rows) + unit * kDeltaRows;
+    // A chunk's operands, in three portions that take turns with the products of the
+    // chunk before: all at once they would hold up the wave while they are issued.
+    // (Behind the last chunk: its operands again.)
+    auto at_kq = [&](int c) { return a.work + ((int64_t)(tile0 + min(c, chunks - 1)) * a.k_heads + kh) * 3 * FRAG + lane * 16; };
+    auto at_unit = [&](int c) { return (int64_t)(tile0 + min(c, chunks - 1)) * a.v_heads + h; };
+    auto load_k = [&](Ops &o, int c) {
+        const uint8_t *const kq = at_kq(c);
+        const float *const f = (const float *)(a.work + a.plan.rows) + at_unit(c) * kDeltaRows;
 #pragma unroll
         for (int k = 0; k < KS; ++k)
 #pragma unroll
@@ -382,7 +384,7 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
                 o.k[k][p] = *(const gd_h8 *)(kq + ((wave * KS + k) * PARTS + p) * 1024);
         o.fk = *(const gd_f4 *)(f + 16 * wave + 4 * g);
         // (rows behind the last token and columns behind the last one: others', not used)
-        const int at0 = 64 * c + 16 * wave + 4 * g;
+        const int at0 = 64 * min(c, chunks - 1) + 16 * wave + 4 * g;
 #pragma unroll
         for (int e = 0; e < CT; ++e)
 #pragma unroll
@@ -391,11 +393,21 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
                                      (live[e] ? 16 * e : 0) + r;
                 o.v[e][i] = PARTS > 1 ? ((const uint32_t *)a.v)[from] : ((const uint16_t *)a.v)[from];
             }
+    };
+    auto load_q = [&](Ops &o, int c) {
+        const uint8_t *const kq = at_kq(c) + 2 * FRAG;
+        const float *const f = (const float *)(a.work + a.plan.rows) + at_unit(c) * kDeltaRows;
 #pragma unroll
         for (int k = 0; k < KS; ++k)
 #pragma unroll
             for (int p = 0; p < PARTS; ++p)
-                o.q[k][p] = *(const gd_h8 *)(kq + 2 * FRAG + ((wave * KS + k) * PARTS + p) * 1024);
+                o.q[k][p] = *(const gd_h8 *)(kq + ((wave * KS + k) * PARTS + p) * 1024);
+        o.fq = *(const gd_f4 *)(f + 64 + 16 * wave + 4 * g);
+        o.fu = *(const gd_f4 *)(f + 128 + 16 * wave + 4 * g);
+        o.keep = f[192];
+    };
+    auto load_rest = [&](Ops &o, int c) {
+        const uint8_t *const tri = a.work + a.plan.tri + at_unit(c) * 2 * kDeltaTri + lane * 16;
         const int t0 = wave < 2 ? wave : 2 * wave - 2; // this wave's first tile of a triangle
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
@@ -406,9 +418,7 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
                 o.p[1][p] = *(const gd_h8 *)(tri + kDeltaTri + (2 * t0 + 2 + p) * 1024);
             }
         }
-        o.fq = *(const gd_f4 *)(f + 64 + 16 * wave + 4 * g);
-        o.fu = *(const gd_f4 *)(f + 128 + 16 * wave + 4 * g);
-        o.keep = f[192];
+        const uint8_t *const kq = at_kq(c) + FRAG;
         if (owner)
 #pragma unroll
             for (int m = 0; m < 2; ++m)
@@ -416,7 +426,7 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
                 for (int k = 0; k < 2; ++k)
 #pragma unroll
                     for (int p = 0; p < PARTS; ++p)
-                        o.kt[m][k][p] = *(const gd_h8 *)(kq + FRAG + ((2 * (2 * wave + m) + k) * PARTS + p) * 1024);
+                        o.kt[m][k][p] = *(const gd_h8 *)(kq + ((2 * (2 * wave + m) + k) * PARTS + p) * 1024);
     };
     auto most4 = [](gd_f4 x) { return fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))); };
     // four values of a column as half a fragment's 8
@@ -453,7 +463,7 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
         gd_power(widest(e), to_s[e], back_s[e]);
     scan_sync();
 
-    auto chunk = [&](const Ops &o, int c) {
+    auto chunk = [&](const Ops &o, Ops &next, int c) {
         const int n = min(64, seq.n - 64 * c);
         gd_f4 v[CT];
 #pragma unroll
@@ -505,6 +515,7 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
             put(xf[e], v[e] - o.fk * ((x + y * (1.0f / REST)) * back_s[e]), to[e]);
             qs[e] = (z + w * (1.0f / REST)) * back_s[e] * o.fq;
         }
+        load_k(next, c + 1);
         scan_sync();
         // V' = T X, and what is written to S
 #pragma unroll
@@ -524,6 +535,7 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
             put(wf[e], w, 1.0f);
             put(uf[e], w * o.fu, 1.0f);
         }
+        load_q(next, c + 1);
         scan_sync();
         // S <- e^G_64 S + K^T (e^(G_64 - G) V');  O = scale (e^G Q S + P V')
 #pragma unroll
@@ -571,16 +583,14 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
             }
             to_s[e] = to[e], back_s[e] = back[e];
         }
+        load_rest(next, c + 1);
     };
     Ops even, odd;
-    load(even, 0);
+    load_k(even, 0), load_q(even, 0), load_rest(even, 0);
     for (int c = 0; c < chunks; c += 2) {
-        load(odd, c + 1);
-        chunk(even, c);
-        if (c + 1 >= chunks)
-            break;
-        load(even, c + 2);
-        chunk(odd, c + 1);
+        chunk(even, odd, c);
+        if (c + 1 < chunks)
+            chunk(odd, even, c + 1);
     }
     if (owner)
 #pragma unroll
