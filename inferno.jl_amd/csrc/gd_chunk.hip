@@ -3,16 +3,16 @@
 // decays up to token i of the chunk, S the state before it, and k, q of unit length,
 //
 //   A_ij = beta_i k_i.k_j e^(G_i - G_j), j < i;      T = (1 + A)^-1 diag(beta)
-//   V' = T (V - e^G K S)                             (what the tokens write)
-//   O = scale (e^G Q S + P V'),                      P_ij = q_i.k_j e^(G_i - G_j), j <= i
-//   S <- e^G_64 S + (e^(G_64 - G) K)^T V'
+//   X = V - e^G K S                                  (what the state does not bring back)
+//   O = scale (e^G Q S + P X),   P = [q_i.k_j e^(G_i - G_j), j <= i] T
+//   S <- e^G_64 S + M X,         M = (e^(G_64 - G) K)^T T
 //
-// T and P do not depend on S: k_delta_prep forms them, and K and Q as matrix operands,
-// for all chunks at once.  k_delta_scan then walks down a sequence's chunks, each wave
-// with 16 columns of S, which do not touch the other columns.
+// P and M do not depend on S: k_delta_prep forms them, and K and Q as matrix operands,
+// for all chunks at once.  k_delta_scan then walks down a sequence's chunks; the columns
+// of S do not touch each other.
 //
-// Operands are fp16 times a power of two (of a row of K and Q, of a column of S, V and
-// V'), so that the largest value lies in 2^13 .. 2^14: values of F16 and BF16 inputs
+// Operands are fp16 times a power of two (of a row of K and Q, of a column of S and
+// X), so that the largest value lies in 2^13 .. 2^14: values of F16 and BF16 inputs
 // fit one part exactly down to 2^-27 of their row's largest; fp32 values and
 // everything derived are held in two parts, which leave 2^-22 of a value, and products
 // of the two lower parts (2^-22) are not formed.  Sums are fp32.  Rows' factors (unit
@@ -57,44 +57,23 @@ __device__ __forceinline__ gd_f4 gd_mfma(gd_h8 a, gd_h8 b, gd_f4 c)
 // Fragments.  A 16-row tile of an operand is stored as the matrix cores take it: for
 // each step of 32 columns, lane (g, r) = (lane / 16, lane % 16) holds of row r the
 // columns 4 g .. 4 g + 3 and 16 + 4 g .. 16 + 4 g + 3, 16 bytes a lane.  These are the
-// rows that a lane holds of two tiles of a product's result, so that results (S, V')
+// rows that a lane holds of two tiles of a product's result, so that results (S, X)
 // are the next product's operands without leaving their registers.
 
 // ---- chunks' operands ------------------------------------------------------------
 constexpr int PREP_THREADS = 256;
 constexpr int TRI = 68; // floats from a row of a 64 x 64 matrix to the next, in LDS
 
-// Lower triangle in LDS, column j times by[j], as fragments of two parts: 6 tiles of
-// 16 x 32 (the others are zeros).  M holds zeros behind the diagonal of those.
-__device__ __forceinline__ void store_tri(const float *M, const float *by, uint8_t *to)
-{
-    const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
-    for (int t = threadIdx.x >> 6; t < 6; t += PREP_THREADS / 64) {
-        const int m = t < 2 ? t : 2 + (t - 2) / 2, k = t < 2 ? 0 : (t - 2) & 1;
-        const int c = 32 * k + 4 * g;
-        const float *row = M + (16 * m + r) * TRI + c;
-        gd_f8 x;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[i] = row[i] * (by ? by[c + i] : 1.0f);
-            x[4 + i] = row[16 + i] * (by ? by[c + 16 + i] : 1.0f);
-        }
-        gd_h8 hi, lo;
-        gd_split(x, (float)(1 << TOP), hi, lo);
-        *(gd_h8 *)(to + (2 * t) * 1024 + lane * 16) = hi;
-        *(gd_h8 *)(to + (2 * t + 1) * 1024 + lane * 16) = lo;
-    }
-}
-
 template <int KD, int PARTS>
 __global__ void __launch_bounds__(PREP_THREADS) k_delta_prep(DeltaArgs a)
 {
     constexpr int KS = KD / 32;               // steps of a row of K
     constexpr int FRAG = 4 * KS * PARTS * 1024; // bytes of K or Q
+    constexpr int MD = KD / 64;               // 16-row tiles of M that a wave forms
     constexpr int MATS = 3 * 64 * TRI * 4;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[FRAG > MATS ? FRAG : MATS];
+    __shared__ __attribute__((aligned(16))) uint8_t lds[FRAG > MATS ? FRAG : MATS], tt[2][6][2][1024];
     __shared__ double G[64];
-    __shared__ float beta[64], rk[64];
+    __shared__ float beta[64], rk[64], fu[64];
     float *const A = (float *)lds, *const T = A + 64 * TRI, *const P = T + 64 * TRI;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, r = lane & 15;
     const int h = blockIdx.x % a.v_heads, tile = blockIdx.x / a.v_heads, kh = h / a.group;
@@ -142,7 +121,8 @@ __global__ void __launch_bounds__(PREP_THREADS) k_delta_prep(DeltaArgs a)
         // (a row's largest value may be as small as 2^-149: its power of two as an
         // exponent, not as a value)
         const int up = most > 0.0f && most < __builtin_inff() ? TOP - ilogbf(most) : 0;
-        const float unit = row < n ? (float)ldexp(1.0 / sqrt(sum + (double)a.l2_eps), -up) : 0.0f;
+        // (a row of zeros stays one)
+        const float unit = row < n && most > 0.0f ? (float)ldexp(1.0 / sqrt(sum + (double)a.l2_eps), -up) : 0.0f;
 #pragma unroll
         for (int i = 0; i < KS; ++i) {
             gd_f8 y;
@@ -160,7 +140,7 @@ __global__ void __launch_bounds__(PREP_THREADS) k_delta_prep(DeltaArgs a)
         else if (g == 0)
             rk[row] = unit;
     }
-    uint8_t *const work = a.work + ((int64_t)tile * a.k_heads + kh) * 3 * FRAG;
+    uint8_t *const work = a.work + ((int64_t)tile * a.k_heads + kh) * 2 * FRAG;
     const bool mine = h % a.group == 0; // this head writes the operands that its group reads
 #pragma unroll
     for (int i = 0; i < KS; ++i)
@@ -170,7 +150,7 @@ __global__ void __launch_bounds__(PREP_THREADS) k_delta_prep(DeltaArgs a)
             *(gd_h8 *)(lds + at) = kf[i][p];
             if (mine) {
                 *(gd_h8 *)(work + at) = kf[i][p];
-                *(gd_h8 *)(work + 2 * FRAG + at) = qf[i][p];
+                *(gd_h8 *)(work + FRAG + at) = qf[i][p];
             }
         }
     // the decays' logarithms, summed in 64 bits: differences of them matter
@@ -188,22 +168,22 @@ __global__ void __launch_bounds__(PREP_THREADS) k_delta_prep(DeltaArgs a)
     }
     __syncthreads();
 
-    // K^T as an operand: rows are K's columns, and tokens its columns
-    if (mine)
-        for (int t = wave; t < KD / 16 * 2; t += PREP_THREADS / 64) {
-            const int m = t / 2, k = t % 2;
+    if (wave == 0)
+        fu[lane] = rk[lane] * expf((float)(G[63] - G[lane]));
+    // this wave's columns of K, with the tokens in steps
+    gd_h8 kt[MD][2][PARTS];
 #pragma unroll
-            for (int p = 0; p < PARTS; ++p) {
-                gd_h8 v;
+    for (int m = 0; m < MD; ++m)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const int token = 4 * g + i % 4, of = 2 * k + i / 4; // of tile `of`
-                    v[i] = *(const _Float16 *)(lds + ((of * KS + m / 2) * PARTS + p) * 1024 + (r / 4 * 16 + token) * 16 +
-                                               (4 * (m & 1) + r % 4) * 2);
+                    const int token = 4 * g + i % 4, of = 2 * k + i / 4, md = MD * wave + m; // of tile `of`
+                    kt[m][k][p][i] = *(const _Float16 *)(lds + ((of * KS + md / 2) * PARTS + p) * 1024 + (r / 4 * 16 + token) * 16 +
+                                                         (4 * (md & 1) + r % 4) * 2);
                 }
-                *(gd_h8 *)(work + FRAG + (t * PARTS + p) * 1024 + lane * 16) = v;
-            }
-        }
 
     // this wave's rows of K K^T and Q K^T
     gd_f4 kk[4], qk[4];
@@ -295,16 +275,94 @@ __global__ void __launch_bounds__(PREP_THREADS) k_delta_prep(DeltaArgs a)
             T[(16 * i + 4 * g + e) * TRI + 16 * j + r] = y[e];
     }
     __syncthreads();
+    // T^T as an operand (16 x 32 tiles on and over its diagonal), its columns once as
+    // they are and once times the factors of what is written to the state.  fu and K's
+    // power of two are 1 together, so fu alone is below 2^-TOP.
+    constexpr float UP = 1 << TOP, BACK = 1.0f / UP;
+    for (int t = wave; t < 6; t += PREP_THREADS / 64) {
+        const int jt = t < 4 ? t / 2 : t - 2, k = t < 4 ? t % 2 : 1, j = 16 * jt + r;
+        gd_f8 x, y;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int at = 32 * k + 4 * g + i % 4 + 16 * (i / 4);
+            x[i] = T[at * TRI + j] * beta[j];
+            y[i] = x[i] * (fu[at] * UP);
+        }
+        gd_h8 hi, lo;
+        gd_split(x, UP, hi, lo);
+        *(gd_h8 *)(tt[0][t][0] + lane * 16) = hi;
+        *(gd_h8 *)(tt[0][t][1] + lane * 16) = lo;
+        gd_split(y, UP, hi, lo);
+        *(gd_h8 *)(tt[1][t][0] + lane * 16) = hi;
+        *(gd_h8 *)(tt[1][t][1] + lane * 16) = lo;
+    }
+    __syncthreads();
+    // P and M, transposed (T^T times the other matrix's transpose), so that a lane holds
+    // the columns of a row that it stores as a fragment
     const int64_t unit = (int64_t)tile * a.v_heads + h;
-    uint8_t *const tri = a.work + a.plan.tri + unit * 2 * kDeltaTri;
-    store_tri(T, beta, tri);
-    store_tri(P, nullptr, tri + kDeltaTri);
+    uint8_t *const to = a.work + a.plan.tri + unit * (kDeltaTri + KD * 256) + lane * 16;
+    auto store = [&](int at, gd_f4 left, gd_f4 right) {
+        gd_h8 hi, lo;
+        gd_split(__builtin_shufflevector(left, right, 0, 1, 2, 3, 4, 5, 6, 7), BACK, hi, lo);
+        *(gd_h8 *)(to + at) = hi;
+        *(gd_h8 *)(to + at + 1024) = lo;
+    };
+    gd_f4 out[4];
+    {
+        gd_h8 hi[2], lo[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const float *from = P + row * TRI + 32 * k + 4 * g;
+            gd_f8 x{};
+            if (k <= wave / 2)
+                x = __builtin_shufflevector(*(const gd_f4 *)from, *(const gd_f4 *)(from + 16), 0, 1, 2, 3, 4, 5, 6, 7);
+            gd_split(x, UP, hi[k], lo[k]);
+        }
+#pragma unroll
+        for (int jt = 0; jt < 4; ++jt) {
+            gd_f4 x{}, y{};
+#pragma unroll
+            for (int k = jt / 2; k < 2; ++k) {
+                if (jt > wave || k > wave / 2)
+                    continue;
+                const uint8_t(*f)[1024] = tt[0][jt < 2 ? 2 * jt + k : 2 + jt];
+                const gd_h8 th = *(const gd_h8 *)(f[0] + lane * 16), tl = *(const gd_h8 *)(f[1] + lane * 16);
+                x = gd_mfma(th, hi[k], x);
+                y = gd_mfma(th, lo[k], y);
+                y = gd_mfma(tl, hi[k], y);
+            }
+            out[jt] = x + y * (1.0f / REST);
+        }
+        const int t0 = wave < 2 ? wave : 2 * wave - 2; // this wave's first tile of a triangle
+        store(2 * t0 * 1024, out[0], out[1]);
+        if (wave >= 2)
+            store((2 * t0 + 2) * 1024, out[2], out[3]);
+    }
+#pragma unroll
+    for (int m = 0; m < MD; ++m) {
+#pragma unroll
+        for (int jt = 0; jt < 4; ++jt) {
+            gd_f4 x{}, y{};
+#pragma unroll
+            for (int k = jt / 2; k < 2; ++k) {
+                const uint8_t(*f)[1024] = tt[1][jt < 2 ? 2 * jt + k : 2 + jt];
+                const gd_h8 th = *(const gd_h8 *)(f[0] + lane * 16), tl = *(const gd_h8 *)(f[1] + lane * 16);
+                x = gd_mfma(th, kt[m][k][0], x);
+                y = gd_mfma(tl, kt[m][k][0], y);
+                if (PARTS > 1)
+                    y = gd_mfma(th, kt[m][k][PARTS - 1], y);
+            }
+            out[jt] = x + y * (1.0f / REST);
+        }
+        const int md = MD * wave + m;
+        store(kDeltaTri + 2 * md * 2048, out[0], out[1]);
+        store(kDeltaTri + (2 * md + 1) * 2048, out[2], out[3]);
+    }
     float *const f = (float *)(a.work + a.plan.rows) + unit * kDeltaRows;
     if (wave == 0) {
-        f[lane] = rk[lane] * expf((float)G[lane]);                // of K S
-        f[128 + lane] = rk[lane] * expf((float)(G[63] - G[lane])); // of what is written
+        f[lane] = rk[lane] * expf((float)G[lane]); // of K S
         if (lane == 0)
-            f[192] = expf((float)G[63]);
+            f[128] = expf((float)G[63]);
     }
     if (g == 0)
         f[64 + row] = rq * expf((float)G[row]); // of Q S
@@ -313,12 +371,12 @@ __global__ void __launch_bounds__(PREP_THREADS) k_delta_prep(DeltaArgs a)
 // ---- down the chunks ---------------------------------------------------------------
 constexpr int SCAN_WAVES = 4;
 
-// What a wave reads of a chunk: its 16 rows of K, Q, T and P, its 32 rows of K^T (in
-// steps of columns), the factors of its 16 tokens and their values in its columns.
+// What a wave reads of a chunk: its 16 rows of K, Q and P, its 32 rows of M, the factors
+// of its 16 tokens and their values in its columns.
 template <int KS, int PARTS, int CT>
 struct ScanOps {
-    gd_h8 k[KS][PARTS], q[KS][PARTS], kt[2][2][PARTS], t[2][2], p[2][2];
-    gd_f4 fk, fq, fu;
+    gd_h8 k[KS][PARTS], q[KS][PARTS], m[2][2][2], p[2][2];
+    gd_f4 fk, fq;
     uint32_t v[CT][4]; // as they lie in memory
     float keep;
 };
@@ -333,12 +391,12 @@ __device__ __forceinline__ void scan_sync()
 // A workgroup takes 16 CT columns of one head of one sequence, each of its waves the
 // tokens 16 w .. 16 w + 15 of a chunk and the rows 32 w .. 32 w + 31 of S (there are
 // KD / 32 such waves).  A wave so reads only its own part of the operands, from memory
-// into registers, a chunk ahead, and the waves exchange S, X, V' and what is written to
-// S as fp16 fragments in LDS, with three barriers a chunk.  Bound by that chain, not by
+// into registers, a chunk ahead, and the waves exchange S and X as fp16 fragments in LDS,
+// with two barriers a chunk.  Bound by that chain, not by
 // bytes or products: a chunk follows the other.
 //
 // One power of two serves a column for a whole chunk.  k and q have unit length at most,
-// and no token adds more than |v| to the length of a column of S, so |X|, |V'| and the
+// and no token adds more than |v| to the length of a column of S, so |X| and the
 // new S lie below 12 max |S| + 66 max |v| (sqrt(128) < 12).  Fragments keep 22 bits of
 // what is over 2^-27 of that.
 template <int KD, int PARTS, int CT>
@@ -346,8 +404,9 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
 {
     constexpr int KS = KD / 32;
     constexpr int FRAG = 4 * KS * PARTS * 1024;
+    constexpr int VB = PARTS > 1 ? 4 : 2; // bytes of a value of V
     using Ops = ScanOps<KS, PARTS, CT>;
-    __shared__ __attribute__((aligned(16))) uint8_t sf[CT][KS][2][1024], xf[CT][2][2][1024], wf[CT][2][2][1024], uf[CT][2][2][1024];
+    __shared__ __attribute__((aligned(16))) uint8_t sf[CT][KS][2][1024], xf[CT][2][2][1024];
     __shared__ float bounds[SCAN_WAVES][CT][16];
     __shared__ __attribute__((aligned(16))) float turn[SCAN_WAVES][16][20];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, r = lane & 15;
@@ -364,6 +423,11 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
     float *const state = a.state + seq.slot * a.slot_step + (int64_t)h * a.k_dim * a.v_dim + col0 + r;
     const int chunks = (seq.n + 63) / 64, tile0 = gd_base(a.batch, kDeltaShift, s);
     const bool half = a.type == kF16, owner = wave < KS;
+    int64_t vat[4]; // of this lane's values of V in a whole chunk
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        vat[i] = ((16 * wave + 4 * g + i) * a.v_step + r) * VB;
+    const int64_t oat = (int64_t)(16 * wave + lane / 4) * a.v_heads * a.v_dim + 4 * (lane % 4);
     bool live[CT];
 #pragma unroll
     for (int e = 0; e < CT; ++e)
@@ -372,7 +436,7 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
     // A chunk's operands, in three portions that take turns with the products of the
     // chunk before: all at once they would hold up the wave while they are issued.
     // (Behind the last chunk: its operands again.)
-    auto at_kq = [&](int c) { return a.work + ((int64_t)(tile0 + min(c, chunks - 1)) * a.k_heads + kh) * 3 * FRAG + lane * 16; };
+    auto at_kq = [&](int c) { return a.work + ((int64_t)(tile0 + min(c, chunks - 1)) * a.k_heads + kh) * 2 * FRAG + lane * 16; };
     auto at_unit = [&](int c) { return (int64_t)(tile0 + min(c, chunks - 1)) * a.v_heads + h; };
     auto load_k = [&](Ops &o, int c) {
         const uint8_t *const kq = at_kq(c);
@@ -384,18 +448,22 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
                 o.k[k][p] = *(const gd_h8 *)(kq + ((wave * KS + k) * PARTS + p) * 1024);
         o.fk = *(const gd_f4 *)(f + 16 * wave + 4 * g);
         // (rows behind the last token and columns behind the last one: others', not used)
-        const int at0 = 64 * min(c, chunks - 1) + 16 * wave + 4 * g;
+        const int at0 = 64 * min(c, chunks - 1);
+        const uint8_t *const v = (const uint8_t *)a.v + ((seq.start + at0) * a.v_step + (int64_t)h * a.v_dim + col0) * VB;
+        const int last = seq.n - 1 - at0;
 #pragma unroll
-        for (int e = 0; e < CT; ++e)
+        for (int i = 0; i < 4; ++i) {
+            const int row = 16 * wave + 4 * g + i;
+            const int64_t from = last >= 63 ? vat[i] : (min(row, last) * a.v_step + r) * VB;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int64_t from = (int64_t)(seq.start + min(at0 + i, seq.n - 1)) * a.v_step + (int64_t)h * a.v_dim + col0 +
-                                     (live[e] ? 16 * e : 0) + r;
-                o.v[e][i] = PARTS > 1 ? ((const uint32_t *)a.v)[from] : ((const uint16_t *)a.v)[from];
+            for (int e = 0; e < CT; ++e) {
+                const uint8_t *at = v + from + (live[e] ? 16 * e * VB : 0);
+                o.v[e][i] = PARTS > 1 ? *(const uint32_t *)at : *(const uint16_t *)at;
             }
+        }
     };
     auto load_q = [&](Ops &o, int c) {
-        const uint8_t *const kq = at_kq(c) + 2 * FRAG;
+        const uint8_t *const kq = at_kq(c) + FRAG;
         const float *const f = (const float *)(a.work + a.plan.rows) + at_unit(c) * kDeltaRows;
 #pragma unroll
         for (int k = 0; k < KS; ++k)
@@ -403,30 +471,25 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
             for (int p = 0; p < PARTS; ++p)
                 o.q[k][p] = *(const gd_h8 *)(kq + ((wave * KS + k) * PARTS + p) * 1024);
         o.fq = *(const gd_f4 *)(f + 64 + 16 * wave + 4 * g);
-        o.fu = *(const gd_f4 *)(f + 128 + 16 * wave + 4 * g);
-        o.keep = f[192];
+        o.keep = f[128];
     };
     auto load_rest = [&](Ops &o, int c) {
-        const uint8_t *const tri = a.work + a.plan.tri + at_unit(c) * 2 * kDeltaTri + lane * 16;
+        const uint8_t *const tri = a.work + a.plan.tri + at_unit(c) * (kDeltaTri + KD * 256) + lane * 16;
         const int t0 = wave < 2 ? wave : 2 * wave - 2; // this wave's first tile of a triangle
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
-            o.t[0][p] = *(const gd_h8 *)(tri + (2 * t0 + p) * 1024);
-            o.p[0][p] = *(const gd_h8 *)(tri + kDeltaTri + (2 * t0 + p) * 1024);
-            if (wave >= 2) {
-                o.t[1][p] = *(const gd_h8 *)(tri + (2 * t0 + 2 + p) * 1024);
-                o.p[1][p] = *(const gd_h8 *)(tri + kDeltaTri + (2 * t0 + 2 + p) * 1024);
-            }
+            o.p[0][p] = *(const gd_h8 *)(tri + (2 * t0 + p) * 1024);
+            if (wave >= 2)
+                o.p[1][p] = *(const gd_h8 *)(tri + (2 * t0 + 2 + p) * 1024);
         }
-        const uint8_t *const kq = at_kq(c) + FRAG;
         if (owner)
 #pragma unroll
             for (int m = 0; m < 2; ++m)
 #pragma unroll
                 for (int k = 0; k < 2; ++k)
 #pragma unroll
-                    for (int p = 0; p < PARTS; ++p)
-                        o.kt[m][k][p] = *(const gd_h8 *)(kq + ((2 * (2 * wave + m) + k) * PARTS + p) * 1024);
+                    for (int p = 0; p < 2; ++p)
+                        o.m[m][k][p] = *(const gd_h8 *)(tri + kDeltaTri + ((2 * (2 * wave + m) + k) * 2 + p) * 1024);
     };
     auto most4 = [](gd_f4 x) { return fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))); };
     // four values of a column as half a fragment's 8
@@ -517,65 +580,47 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
         }
         load_k(next, c + 1);
         scan_sync();
-        // V' = T X, and what is written to S
+        // S <- e^G_64 S + M X;  O = scale (e^G Q S + P X)
 #pragma unroll
         for (int e = 0; e < CT; ++e) {
-            gd_f4 x{}, y{};
-            auto step = [&](int k) {
-                const gd_h8 hi = *(const gd_h8 *)(xf[e][k][0] + lane * 16), lo = *(const gd_h8 *)(xf[e][k][1] + lane * 16);
-                x = gd_mfma(o.t[k][0], hi, x);
-                y = gd_mfma(o.t[k][0], lo, y);
-                y = gd_mfma(o.t[k][1], hi, y);
-            };
-            step(0);
-            if (wave >= 2)
-                step(1);
-            // (still times the column's power of two)
-            const gd_f4 w = (x + y * (1.0f / REST)) * (1.0f / (1 << TOP));
-            put(wf[e], w, 1.0f);
-            put(uf[e], w * o.fu, 1.0f);
-        }
-        load_q(next, c + 1);
-        scan_sync();
-        // S <- e^G_64 S + K^T (e^(G_64 - G) V');  O = scale (e^G Q S + P V')
+            gd_h8 hi[2], lo[2];
 #pragma unroll
-        for (int e = 0; e < CT; ++e) {
+            for (int k = 0; k < 2; ++k) {
+                hi[k] = *(const gd_h8 *)(xf[e][k][0] + lane * 16);
+                lo[k] = *(const gd_h8 *)(xf[e][k][1] + lane * 16);
+            }
+            const float by = back[e] * (1.0f / (1 << TOP));
             if (owner) {
                 gd_f4 x[2]{}, y[2]{};
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const gd_h8 hi = *(const gd_h8 *)(uf[e][k][0] + lane * 16), lo = *(const gd_h8 *)(uf[e][k][1] + lane * 16);
+                for (int k = 0; k < 2; ++k)
 #pragma unroll
                     for (int m = 0; m < 2; ++m) {
-                        x[m] = gd_mfma(o.kt[m][k][0], hi, x[m]);
-                        y[m] = gd_mfma(o.kt[m][k][0], lo, y[m]);
-                        if (PARTS > 1)
-                            y[m] = gd_mfma(o.kt[m][k][PARTS - 1], hi, y[m]);
+                        x[m] = gd_mfma(o.m[m][k][0], hi[k], x[m]);
+                        y[m] = gd_mfma(o.m[m][k][0], lo[k], y[m]);
+                        y[m] = gd_mfma(o.m[m][k][1], hi[k], y[m]);
                     }
-                }
 #pragma unroll
                 for (int m = 0; m < 2; ++m)
-                    S[e][m] = S[e][m] * o.keep + (x[m] + y[m] * (1.0f / REST)) * back[e];
+                    S[e][m] = S[e][m] * o.keep + (x[m] + y[m] * (1.0f / REST)) * by;
             }
             gd_f4 x{}, y{};
-            auto step = [&](int k) {
-                const gd_h8 hi = *(const gd_h8 *)(wf[e][k][0] + lane * 16), lo = *(const gd_h8 *)(wf[e][k][1] + lane * 16);
-                x = gd_mfma(o.p[k][0], hi, x);
-                y = gd_mfma(o.p[k][0], lo, y);
-                y = gd_mfma(o.p[k][1], hi, y);
-            };
-            step(0);
-            if (wave >= 2)
-                step(1);
-            const gd_f4 out = a.scale * (qs[e] + (x + y * (1.0f / REST)) * (back[e] * (1.0f / (1 << TOP))));
+            x = gd_mfma(o.p[0][0], hi[0], x);
+            y = gd_mfma(o.p[0][0], lo[0], y);
+            y = gd_mfma(o.p[0][1], hi[0], y);
+            if (wave >= 2) {
+                x = gd_mfma(o.p[1][0], hi[1], x);
+                y = gd_mfma(o.p[1][0], lo[1], y);
+                y = gd_mfma(o.p[1][1], hi[1], y);
+            }
+            const gd_f4 out = a.scale * (qs[e] + (x + y * (1.0f / REST)) * by);
             // through LDS, so that a lane stores 4 neighbours
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 turn[wave][4 * g + i][r] = out[i];
             const gd_f4 flat = *(const gd_f4 *)&turn[wave][lane / 4][4 * (lane % 4)];
-            const int at = 16 * wave + lane / 4;
-            if (live[e] && at < n) {
-                const int64_t where = ((int64_t)(seq.start + 64 * c + at) * a.v_heads + h) * a.v_dim + col0 + 16 * e + 4 * (lane % 4);
+            if (live[e] && 16 * wave + lane / 4 < n) {
+                const int64_t where = ((seq.start + 64 * (int64_t)c) * a.v_heads + h) * a.v_dim + col0 + 16 * e + oat;
                 if (a.raw)
                     *(gd_f4 *)(a.raw + where) = flat;
                 else
@@ -583,6 +628,7 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
             }
             to_s[e] = to[e], back_s[e] = back[e];
         }
+        load_q(next, c + 1);
         load_rest(next, c + 1);
     };
     Ops even, odd;
