@@ -391,7 +391,7 @@ __device__ __forceinline__ void scan_sync()
 // A workgroup takes 16 CT columns of one head of one sequence, each of its waves the
 // tokens 16 w .. 16 w + 15 of a chunk and the rows 32 w .. 32 w + 31 of S (there are
 // KD / 32 such waves).  A wave so reads only its own part of the operands, from memory
-// into registers, a chunk ahead, and the waves exchange S and X as fp16 fragments in LDS,
+// into registers, two chunks ahead, and the waves exchange S and X as fp16 fragments in LDS,
 // with two barriers a chunk.  Bound by that chain, not by
 // bytes or products: a chunk follows the other.
 //
@@ -433,12 +433,11 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
     for (int e = 0; e < CT; ++e)
         live[e] = col0 + 16 * e < a.v_dim;
 
-    // A chunk's operands, in three portions that take turns with the products of the
-    // chunk before: all at once they would hold up the wave while they are issued.
-    // (Behind the last chunk: its operands again.)
+    // A chunk's operands, in two portions: those of the chunk after the next follow
+    // as soon as their registers are free.  (Behind the last chunk: its operands again.)
     auto at_kq = [&](int c) { return a.work + ((int64_t)(tile0 + min(c, chunks - 1)) * a.k_heads + kh) * 2 * FRAG + lane * 16; };
     auto at_unit = [&](int c) { return (int64_t)(tile0 + min(c, chunks - 1)) * a.v_heads + h; };
-    auto load_k = [&](Ops &o, int c) {
+    auto load_kqv = [&](Ops &o, int c) {
         const uint8_t *const kq = at_kq(c);
         const float *const f = (const float *)(a.work + a.plan.rows) + at_unit(c) * kDeltaRows;
 #pragma unroll
@@ -446,7 +445,13 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
 #pragma unroll
             for (int p = 0; p < PARTS; ++p)
                 o.k[k][p] = *(const gd_h8 *)(kq + ((wave * KS + k) * PARTS + p) * 1024);
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p)
+                o.q[k][p] = *(const gd_h8 *)(kq + FRAG + ((wave * KS + k) * PARTS + p) * 1024);
         o.fk = *(const gd_f4 *)(f + 16 * wave + 4 * g);
+        o.fq = *(const gd_f4 *)(f + 64 + 16 * wave + 4 * g);
         // (rows behind the last token and columns behind the last one: others', not used)
         const int at0 = 64 * min(c, chunks - 1);
         const uint8_t *const v = (const uint8_t *)a.v + ((seq.start + at0) * a.v_step + (int64_t)h * a.v_dim + col0) * VB;
@@ -462,18 +467,8 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
             }
         }
     };
-    auto load_q = [&](Ops &o, int c) {
-        const uint8_t *const kq = at_kq(c) + FRAG;
-        const float *const f = (const float *)(a.work + a.plan.rows) + at_unit(c) * kDeltaRows;
-#pragma unroll
-        for (int k = 0; k < KS; ++k)
-#pragma unroll
-            for (int p = 0; p < PARTS; ++p)
-                o.q[k][p] = *(const gd_h8 *)(kq + ((wave * KS + k) * PARTS + p) * 1024);
-        o.fq = *(const gd_f4 *)(f + 64 + 16 * wave + 4 * g);
-        o.keep = f[128];
-    };
-    auto load_rest = [&](Ops &o, int c) {
+    auto load_pm = [&](Ops &o, int c) {
+        o.keep = ((const float *)(a.work + a.plan.rows) + at_unit(c) * kDeltaRows)[128];
         const uint8_t *const tri = a.work + a.plan.tri + at_unit(c) * (kDeltaTri + KD * 256) + lane * 16;
         const int t0 = wave < 2 ? wave : 2 * wave - 2; // this wave's first tile of a triangle
 #pragma unroll
@@ -526,7 +521,7 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
         gd_power(widest(e), to_s[e], back_s[e]);
     scan_sync();
 
-    auto chunk = [&](const Ops &o, Ops &next, int c) {
+    auto chunk = [&](Ops &o, int c) {
         const int n = min(64, seq.n - 64 * c);
         gd_f4 v[CT];
 #pragma unroll
@@ -578,7 +573,7 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
             put(xf[e], v[e] - o.fk * ((x + y * (1.0f / REST)) * back_s[e]), to[e]);
             qs[e] = (z + w * (1.0f / REST)) * back_s[e] * o.fq;
         }
-        load_k(next, c + 1);
+        load_kqv(o, c + 2);
         scan_sync();
         // S <- e^G_64 S + M X;  O = scale (e^G Q S + P X)
 #pragma unroll
@@ -628,16 +623,18 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
             }
             to_s[e] = to[e], back_s[e] = back[e];
         }
-        load_q(next, c + 1);
-        load_rest(next, c + 1);
+        load_pm(o, c + 2);
     };
     Ops even, odd;
-    load_k(even, 0), load_q(even, 0), load_rest(even, 0);
-    for (int c = 0; c < chunks; c += 2) {
-        chunk(even, odd, c);
-        if (c + 1 < chunks)
-            chunk(odd, even, c + 1);
+    load_kqv(even, 0), load_pm(even, 0);
+    load_kqv(odd, 1), load_pm(odd, 1);
+    int c = 0;
+    for (; c + 1 < chunks; c += 2) { // (no way out between: the operands stay in their registers)
+        chunk(even, c);
+        chunk(odd, c + 1);
     }
+    if (c < chunks)
+        chunk(even, c);
     if (owner)
 #pragma unroll
         for (int e = 0; e < CT; ++e)
