@@ -637,9 +637,8 @@ size_t ihip_gated_delta_scratch_bytes(int type, const ihip_delta_layer *layer,
  * first IHIP_SAMPLE_COUNT_BYTES with zeros once, before its first call; every call
  * leaves them zero again, so that it serves any number of calls of any sizes that it
  * is large enough for.  Calls that share it must not overlap on the GPU.  At most
- * IHIP_SAMPLE_ROWS rows and 2^30 logits a row. */
-#define IHIP_SAMPLE_COUNT_BYTES 65536
-#define IHIP_SAMPLE_ROWS 16384
+ * 2^30 logits a row. */
+#define IHIP_SAMPLE_COUNT_BYTES 16384
 int ihip_sample_dev(const void *logits, int type, int64_t row_stride, int rows, int vocab,
                     const float *temperature, const int32_t *top_k, const float *top_p,
                     const float *min_p, const float *u, int32_t *tokens, float *logprobs,

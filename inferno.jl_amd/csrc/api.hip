@@ -1970,7 +1970,7 @@ int ihip_gated_delta_dev(const void *q, int64_t q_stride, const void *k, int64_t
 
 size_t ihip_sample_scratch_bytes(int rows, int vocab)
 {
-    return rows <= 0 || rows > IHIP_SAMPLE_ROWS || vocab <= 0 || vocab > 1 << 30 ? 0 : IHIP_SAMPLE_COUNT_BYTES;
+    return rows <= 0 || vocab <= 0 || vocab > 1 << 30 ? 0 : sample_plan(rows, vocab).bytes;
 }
 
 int ihip_sample_dev(const void *logits, int type, int64_t row_stride, int rows, int vocab,
@@ -1985,8 +1985,8 @@ int ihip_sample_dev(const void *logits, int type, int64_t row_stride, int rows, 
     const int vb = value_bytes(type);
     if (!vb)
         return fail(IHIP_ERR_INVALID, "type=%d is none of F32, F16, BF16", type);
-    if (rows < 0 || rows > IHIP_SAMPLE_ROWS || vocab < 0 || vocab > 1 << 30)
-        return fail(IHIP_ERR_INVALID, "rows=%d (up to %d), vocab=%d (up to 2^30)", rows, IHIP_SAMPLE_ROWS, vocab);
+    if (rows < 0 || vocab < 0 || vocab > 1 << 30)
+        return fail(IHIP_ERR_INVALID, "rows=%d, vocab=%d (up to 2^30)", rows, vocab);
     if (rows == 0)
         return IHIP_OK;
     if (vocab == 0)
@@ -1997,7 +1997,8 @@ int ihip_sample_dev(const void *logits, int type, int64_t row_stride, int rows, 
         return fail(IHIP_ERR_INVALID, "row_stride=%lld does not hold %d logits", (long long)row_stride, vocab);
     if ((uintptr_t)logits & (uintptr_t)(vb - 1))
         return fail(IHIP_ERR_INVALID, "logits are not aligned to their values");
-    const size_t need = ihip_sample_scratch_bytes(rows, vocab), n = 4 * (size_t)rows;
+    const SamplePlan plan = sample_plan(rows, vocab);
+    const size_t need = plan.bytes, n = 4 * (size_t)rows;
     if (!workspace || workspace_bytes < need || !al16(workspace))
         return fail(IHIP_ERR_INVALID, "the workspace needs %zu bytes, 16-byte aligned", need);
     const Span ins[] = {rows_of(logits, rows, row_stride, vocab, vb), {temperature, temperature ? n : 0}, {top_k, top_k ? n : 0},
@@ -2011,7 +2012,8 @@ int ihip_sample_dev(const void *logits, int type, int64_t row_stride, int rows, 
             if (&p < &o && !apart(p, o))
                 return fail(IHIP_ERR_INVALID, "two outputs, or one and the workspace, overlap");
     }
-    SampleArgs a{logits, type, rows, vocab, row_stride, temperature, top_k, top_p, min_p, u, tokens, logprobs, flags};
+    SampleArgs a{logits, type, rows, vocab, row_stride, temperature, top_k, top_p, min_p, u, tokens, logprobs, flags,
+                 (uint8_t *)workspace, plan, 0};
     hipError_t e = launch_sample(a, (hipStream_t)stream);
     if (e != hipSuccess)
         return fail(IHIP_ERR_HIP, "sampling launch failed: %s", hipGetErrorString(e));

@@ -3,6 +3,7 @@
 #pragma once
 
 #include "gd_common.h"
+#include "sample_plan.h"
 
 namespace ihip {
 
@@ -19,8 +20,11 @@ struct SampleArgs {
     int32_t *tokens;
     float *logprobs;
     uint32_t *flags;
+    uint8_t *work;
+    SamplePlan plan;
+    int row0; // of the launch's rows
 };
-hipError_t launch_sample(const SampleArgs &a, hipStream_t s);
+hipError_t launch_sample(SampleArgs a, hipStream_t s);
 
 struct SampleRow {
     float t, p, min_p, u;
