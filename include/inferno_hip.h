@@ -633,12 +633,9 @@ size_t ihip_gated_delta_scratch_bytes(int type, const ihip_delta_layer *layer,
  * is never chosen.  flags[r] = IHIP_FLAG_NAN / IHIP_FLAG_POSINF where the row holds
  * such a value (the token is then 0 and the logprob NaN), IHIP_FLAG_ALL_NEGINF where
  * every logit is -infinity (the token is 0), else 0.  Everything is device memory.
- * workspace: ihip_sample_scratch_bytes bytes, 16-byte aligned.  The caller fills its
- * first IHIP_SAMPLE_COUNT_BYTES with zeros once, before its first call; every call
- * leaves them zero again, so that it serves any number of calls of any sizes that it
- * is large enough for.  Calls that share it must not overlap on the GPU.  At most
- * 2^30 logits a row. */
-#define IHIP_SAMPLE_COUNT_BYTES 16384
+ * workspace: ihip_sample_scratch_bytes bytes, 16-byte aligned; its contents do not
+ * matter.  Calls that share it must not overlap on the GPU.  At most 2^22 logits a
+ * row. */
 int ihip_sample_dev(const void *logits, int type, int64_t row_stride, int rows, int vocab,
                     const float *temperature, const int32_t *top_k, const float *top_p,
                     const float *min_p, const float *u, int32_t *tokens, float *logprobs,

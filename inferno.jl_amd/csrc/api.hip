@@ -1970,7 +1970,7 @@ int ihip_gated_delta_dev(const void *q, int64_t q_stride, const void *k, int64_t
 
 size_t ihip_sample_scratch_bytes(int rows, int vocab)
 {
-    return rows <= 0 || vocab <= 0 || vocab > 1 << 30 ? 0 : sample_plan(rows, vocab).bytes;
+    return rows <= 0 || vocab <= 0 || vocab > kSampleVocab ? 0 : sample_plan(rows, vocab).bytes;
 }
 
 int ihip_sample_dev(const void *logits, int type, int64_t row_stride, int rows, int vocab,
@@ -1985,8 +1985,9 @@ int ihip_sample_dev(const void *logits, int type, int64_t row_stride, int rows, 
     const int vb = value_bytes(type);
     if (!vb)
         return fail(IHIP_ERR_INVALID, "type=%d is none of F32, F16, BF16", type);
-    if (rows < 0 || vocab < 0 || vocab > 1 << 30)
-        return fail(IHIP_ERR_INVALID, "rows=%d, vocab=%d (up to 2^30)", rows, vocab);
+    if (rows < 0 || vocab < 0 || vocab > kSampleVocab)
+        return fail(IHIP_ERR_INVALID, "rows=%d, vocab=%d (up to 2^22)", rows, vocab);
+    static_assert(kSampleVocab == 1 << 22, "as the interface says");
     if (rows == 0)
         return IHIP_OK;
     if (vocab == 0)

@@ -212,13 +212,16 @@ __device__ void sample_whole_row(const SampleArgs &a, int row, const SampleRow &
 
 
 // ---- rows in slices ------------------------------------------------------------
-// What of a row is zero between calls: the largest logit seen (its key, then ~place),
-// what is not finite, workgroups that have ended, tokens listed.
-struct Record {
-    unsigned long long best;
-    uint32_t flags, ended[2], listed, pad[2];
+// A row's slices go to workgroups all over the chip, and what they find to one that
+// joins them, a launch later (a launch costs what a count of ended workgroups, and
+// reads past the caches, would).
+
+struct Part { // of a slice
+    unsigned long long best; // the largest logit (its key, then ~place)
+    double sum;              // of weights
+    uint32_t flags, pad;
 };
-static_assert(sizeof(Record) == kSampleRecord, "a row's record");
+static_assert(sizeof(Part) == kSamplePart, "a slice's values");
 
 // The prefixes that top-k and top-p keep end within these bins: nothing over bin
 // `whole` is cut, and the tokens of bin k and of bins p_low .. p_high are listed.
@@ -227,74 +230,70 @@ struct Bounds {
     unsigned long long all;            // of all tokens (where top-k is off)
     uint32_t k_count;                  // tokens over bin k
     int k, p_low, p_high, whole;
+    uint32_t listed;                   // tokens
+};
+static_assert(sizeof(Bounds) <= kSampleRecord, "a row's bounds");
+
+__device__ __forceinline__ Part *parts_of(const SampleArgs &a, int rr)
+{
+    return (Part *)a.work + (int64_t)rr * a.plan.slices;
+}
+__device__ __forceinline__ Bounds *bounds_of(const SampleArgs &a, int rr)
+{
+    return (Bounds *)(a.work + a.plan.bounds + (int64_t)rr * kSampleRecord);
+}
+
+template <int TYPE>
+struct LogitOf;
+template <>
+struct LogitOf<kF32> {
+    typedef float T;
+};
+template <>
+struct LogitOf<kF16> {
+    typedef _Float16 T;
+};
+template <>
+struct LogitOf<kBF16> {
+    typedef __bf16 T;
 };
 
-struct Part { // of a slice
-    unsigned long long best;
-    double sum;
-};
+// A thread's N logits of a slice, 4 neighbours at a time, all on their way at once;
+// -infinity behind the row's end.
+template <int TYPE, int N>
+struct Slice {
+    float l[N];
+    int begin, end;
 
-__device__ __forceinline__ Record *record_of(const SampleArgs &a, int r)
-{
-    return (Record *)a.work + r;
-}
-__device__ __forceinline__ unsigned long long agent_load(const unsigned long long *p)
-{
-    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ void agent_store(unsigned long long *p, unsigned long long v)
-{
-    __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-
-__device__ __forceinline__ void agent_clear(uint32_t *p)
-{
-    __hip_atomic_store(p, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-
-// Whether this workgroup is the last of the row's `n` to come here.  What passes
-// between them goes through memory that all of the chip sees (agent_load and _store,
-// atomics); a workgroup counts itself when its stores have arrived, and the last one
-// sets the count to 0 again.
-__device__ __forceinline__ bool last_of(uint32_t *count, int n, int *lds)
-{
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (threadIdx.x == 0)
-        *lds = atomicInc(count, (uint32_t)n - 1) == (uint32_t)n - 1;
-    __syncthreads();
-    return *lds;
-}
-
-// f(logit, index) for this thread's logits of a slice, 4 neighbours a thread at a time
-template <typename F>
-__device__ __forceinline__ void each_logit(const SampleArgs &a, int row, int slice, F f)
-{
-    const int begin = slice * a.plan.per, end = (int)min((int64_t)begin + a.plan.per, (int64_t)a.vocab);
-    const int64_t base = row * a.row_step;
-    const int size = a.type == kF32 ? 4 : 2;
-    const bool wide = (((uintptr_t)a.logits + (uintptr_t)(base * size)) & (uintptr_t)(4 * size - 1)) == 0; // (begin is a multiple of 4)
-    for (int i0 = begin + 4 * (int)threadIdx.x; i0 < end; i0 += 4 * 4 * ROW_THREADS) {
-        // four such groups in flight
-        gd_f4 l[4];
+    __device__ __forceinline__ Slice(const SampleArgs &a, int row, int slice)
+    {
+        typedef typename LogitOf<TYPE>::T T;
+        typedef T T4 __attribute__((ext_vector_type(4)));
+        begin = slice * (N * ROW_THREADS), end = min(begin + N * ROW_THREADS, a.vocab);
+        const T *const p = (const T *)a.logits + row * a.row_step;
+        const bool wide = ((uintptr_t)(p + begin) & (sizeof(T4) - 1)) == 0 && end == begin + N * ROW_THREADS;
+        if (wide) {
+            T4 v[N / 4];
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            const int i = i0 + b * 4 * ROW_THREADS;
-            if (wide && i + 3 < end)
-                l[b] = gd_load4(a.logits, base + i, a.type);
-            else
+            for (int j = 0; j < N; j += 4)
+                v[j / 4] = *(const T4 *)(p + at(j));
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    l[b][e] = i + e < end ? sample_logit(a.logits, base + i + e, a.type) : 0.0f;
+            for (int j = 0; j < N; ++j)
+                l[j] = (float)v[j / 4][j % 4];
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                l[j] = (float)p[min(at(j), a.vocab - 1)];
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                l[j] = at(j) < end ? l[j] : -__builtin_inff();
         }
-#pragma unroll
-        for (int b = 0; b < 4; ++b)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (i0 + b * 4 * ROW_THREADS + e < end)
-                    f(l[b][e], i0 + b * 4 * ROW_THREADS + e);
     }
-}
+    __device__ __forceinline__ int at(int j) const
+    {
+        return begin + (j / 4 * ROW_THREADS + (int)threadIdx.x) * 4 + j % 4;
+    }
+};
 
 // The larger of keys, the lowest place among equal ones
 __device__ __forceinline__ unsigned long long best_of(float l, int at)
@@ -334,16 +333,19 @@ __device__ __forceinline__ double wg_sum(double v, double *part)
     return all;
 }
 
-// Bins by distance from the largest logit: 32 to a factor of 2 in weight down to 2^-32,
-// then 64 to a factor of 2 in distance.  In order of the logits.
+// Bins by distance from the largest logit: 16 to a factor of 2 in weight down to 2^-32,
+// then 32 to a factor of 2 in distance.  In order of the logits.
 __device__ __forceinline__ int bin_of(float l, float most, float rate)
 {
     const float d = (most - l) * rate;
     if (d < 32.0f)
-        return (int)(d * 32.0f);
-    constexpr uint32_t from = 0x42000000u >> 17; // 32
-    return (int)min((__float_as_uint(d) >> 17) - from + 1024u, (uint32_t)(kSampleBins - 1));
+        return (int)(d * 16.0f);
+    constexpr uint32_t from = 0x42000000u >> 18; // 32
+    return (int)min((__float_as_uint(d) >> 18) - from + 512u, (uint32_t)(kSampleBins - 1));
 }
+// From this bin on (over 1150 factors of 2 below the largest) weights are 0 in 64 bits:
+// where top-k's cut falls among them it cuts nothing that counts.
+constexpr int ZERO_BIN = 680;
 __device__ __forceinline__ float bin_rate(float t)
 {
     return fminf(1.44269504f / t, 3e38f);
@@ -357,446 +359,570 @@ __device__ __forceinline__ bool filtered(const SampleRow &r, int vocab, bool &by
 }
 
 // The row's token from its slices' sums: `sum` (this thread's slice's, threads behind
-// the last slice 0) and what a token has to pass to be kept.
+// the last slice 0), `total` (what the logprob is a share of) and the last kept token.
 struct PickLds {
     double part[ROW_WAVES], before;
-    int slice, wat[ROW_WAVES], wlast[ROW_WAVES];
+    int first[ROW_WAVES], last[ROW_WAVES];
 };
-__device__ void pick(const SampleArgs &a, int row, const SampleRow &r, const SampleScale &sc, unsigned long long best, uint32_t fl,
-                     double sum, unsigned long long border, double low, PickLds &lds)
+
+// The first thread for which `yes`, and the last one for which `some` (-1: none).  By
+// ballots: hundreds of atomics to one address would take longer than all the rest.
+__device__ __forceinline__ int2 first_and_last(bool yes, bool some, int *first, int *last)
 {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    double before;
-    const double total = wg_scan(sum, lds.part, before);
-    const double want = sample_u(r.u) * total;
-    // the first slice at which the sums pass it, else the last one that has any
-    if (tid == 0)
-        lds.slice = 0x7fffffff;
+    const int wave = threadIdx.x >> 6;
+    const uint64_t y = __ballot(yes), h = __ballot(some);
     __syncthreads();
-    if (sum > 0.0 && before + sum > want)
-        atomicMin(&lds.slice, tid);
-    __syncthreads();
-    if (lds.slice == 0x7fffffff) {
-        __syncthreads();
-        if (tid == 0)
-            lds.slice = -1;
-        __syncthreads();
-        if (sum > 0.0)
-            atomicMax(&lds.slice, tid);
-        __syncthreads();
+    if ((threadIdx.x & 63) == 0) {
+        first[wave] = y ? 64 * wave + __builtin_ctzll(y) : 0x7fffffff;
+        last[wave] = h ? 64 * wave + 63 - __builtin_clzll(h) : -1;
     }
-    const int slice = max(lds.slice, 0);
-    if (tid == slice)
+    __syncthreads();
+    int2 r = make_int2(0x7fffffff, -1);
+    for (int i = 0; i < ROW_WAVES; ++i) {
+        r.x = min(r.x, first[i]);
+        r.y = max(r.y, last[i]);
+    }
+    return make_int2(r.x == 0x7fffffff ? -1 : r.x, r.y);
+}
+
+// The first thread whose sum passes `want` (the sum of the threads before it is handed
+// on in lds.before), else the last one that has any; -1: none has.
+__device__ __forceinline__ int first_passing(double sum, double before, double want, PickLds &lds)
+{
+    const int2 r = first_and_last(sum > 0.0 && before + sum > want, sum > 0.0, lds.first, lds.last);
+    const int at = r.x >= 0 ? r.x : r.y;
+    if ((int)threadIdx.x == at)
         lds.before = before;
     __syncthreads();
-    double run = lds.before;
-    const int64_t base = row * a.row_step;
-    const int begin = slice * a.plan.per, end = (int)min((int64_t)begin + a.plan.per, (int64_t)a.vocab);
-    int token = (int)~(uint32_t)best;
-    for (int i0 = begin; i0 < end; i0 += 4 * ROW_THREADS) {
-        double m[4], mine = 0.0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int i = i0 + 4 * tid + e;
-            const float l = i < end ? sample_logit(a.logits, base + i, a.type) : -__builtin_inff();
-            const unsigned long long o = best_of(l, i);
-            m[e] = i < end && o >= border ? sample_weight(sc, l) : 0.0;
-            if (m[e] < low && o != best)
-                m[e] = 0.0;
-            mine += m[e];
-        }
-        double ahead;
-        const double all = wg_scan(mine, lds.part, ahead);
-        double upto = run + ahead;
-        int found = 0x7fffffff, last = -1;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            upto += m[e];
-            if (m[e] > 0.0) {
-                last = i0 + 4 * tid + e;
-                if (upto > want && found == 0x7fffffff)
-                    found = last;
-            }
-        }
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            found = min(found, __shfl_xor(found, d));
-            last = max(last, __shfl_xor(last, d));
-        }
-        if (lane == 0)
-            lds.wat[wave] = found, lds.wlast[wave] = last;
-        __syncthreads();
-        for (int i = 0; i < ROW_WAVES; ++i) {
-            found = min(found, lds.wat[i]);
-            last = max(last, lds.wlast[i]);
-        }
-        if (last >= 0)
-            token = last;
-        if (found != 0x7fffffff) {
-            token = found;
-            break;
-        }
-        run += all;
-        __syncthreads();
-    }
-    if (tid == 0)
-        sample_done(a, row, fl, token, log(sample_weight(sc, sample_logit(a.logits, base + token, a.type)) / total));
+    return at;
 }
 
-// Whether the row's token needs no sums: what is not finite, or the greedy choice
-__device__ __forceinline__ bool settled(const SampleArgs &a, int row, const SampleRow &r, unsigned long long best, uint32_t fl)
+__device__ void pick(const SampleArgs &a, int row, const SampleRow &r, const SampleScale &sc, unsigned long long best, uint32_t fl,
+                     double sum, double total, unsigned long long border, double low, PickLds &lds)
 {
-    if (!(fl & (kSampleNan | kSamplePosInf)) && (fl & kSampleFinite) && r.t > 0.0f)
-        return false;
-    if (threadIdx.x == 0 && a.tokens)
-        sample_done(a, row, fl, (fl & kSampleFinite) ? (int)~(uint32_t)best : 0, 0.0);
-    return true;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int64_t base = row * a.row_step;
+    // what token i counts
+    auto weight = [&](int i, float l) {
+        const unsigned long long o = best_of(l, i);
+        const double w = o >= border ? sample_weight(sc, l) : 0.0;
+        return w < low && o != best ? 0.0 : w;
+    };
+    // the slice, then the thread's share of it, then the token
+    double before;
+    const double want = sample_u(r.u) * wg_scan(sum, lds.part, before);
+    const int slice = max(first_passing(sum, before, want, lds), 0);
+    double run = lds.before;
+    const int share = a.plan.per / ROW_THREADS; // neighbours
+    const int begin = slice * a.plan.per, end = min(begin + a.plan.per, a.vocab);
+    sum = 0.0;
+    for (int e0 = 0; e0 < share; e0 += 8) {
+        float l[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            l[e] = sample_logit(a.logits, base + min(begin + tid * share + e0 + e, end - 1), a.type);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int i = begin + tid * share + e0 + e;
+            sum += i < end ? weight(i, l[e]) : 0.0;
+        }
+    }
+    wg_scan(sum, lds.part, before);
+    const int owner = first_passing(sum, run + before, want, lds);
+    if (tid >= 64)
+        return;
+    run = lds.before;
+    const int i = begin + max(owner, 0) * share + lane;
+    const float l = sample_logit(a.logits, base + min(i, end - 1), a.type);
+    const double w = owner >= 0 && lane < share && i < end ? weight(i, l) : 0.0;
+    double upto = w;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const double up = __shfl_up(upto, d);
+        upto += lane >= d ? up : 0.0;
+    }
+    const uint64_t has = __ballot(w > 0.0), passed = __ballot(w > 0.0 && run + upto > want);
+    const int at = passed ? __builtin_ctzll(passed) : has ? 63 - __builtin_clzll(has) : -1;
+    if (lane == max(at, 0)) // (no kept token: the likeliest)
+        sample_done(a, row, fl, at < 0 ? (int)~(uint32_t)best : i, at < 0 ? 0.0 : log(w / total));
 }
 
-// Without filters, one launch: a slice's largest logit, then its weights relative to
-// that (the slice's second reading comes from the caches); the row's last workgroup
-// joins the slices and looks the token up in the one where it lies.
-__global__ void __launch_bounds__(ROW_THREADS) k_sample_plain(SampleArgs a)
+// Whether the row's weights matter: it is finite, and not for the greedy choice
+__device__ __forceinline__ bool weighed(float t, uint32_t fl)
+{
+    return !(fl & (kSampleNan | kSamplePosInf)) && (fl & kSampleFinite) && t > 0.0f;
+}
+__device__ __forceinline__ void settle(const SampleArgs &a, int row, unsigned long long best, uint32_t fl)
+{
+    if (threadIdx.x == 0)
+        sample_done(a, row, fl, (fl & kSampleFinite) ? (int)~(uint32_t)best : 0, 0.0);
+}
+
+// A slice's largest logit, and what is not finite in it
+template <typename S>
+__device__ __forceinline__ void slice_best(const S &x, unsigned long long &best, uint32_t &fl, unsigned long long *wbest, uint32_t *wfl)
+{
+    constexpr int N = (int)(sizeof x.l / 4);
+    float most = -__builtin_inff();
+    bool nan = false;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        most = fmaxf(most, x.l[j]);
+        nan |= x.l[j] != x.l[j];
+    }
+    int at = 0x7fffffff;
+#pragma unroll
+    for (int j = N - 1; j >= 0; --j)
+        at = x.l[j] == most ? x.at(j) : at;
+    fl = (nan ? kSampleNan : 0) | sample_flags(most);
+    best = best_of(most, at);
+    wg_best(best, fl, wbest, wfl);
+}
+
+// A row's largest logit and flags, from its slices'
+__device__ __forceinline__ void row_best(const SampleArgs &a, int rr, unsigned long long &best, uint32_t &fl, unsigned long long *wbest,
+                                         uint32_t *wfl)
+{
+    best = 0, fl = 0;
+    if ((int)threadIdx.x < a.plan.slices) {
+        const Part p = parts_of(a, rr)[threadIdx.x];
+        best = p.best, fl = p.flags;
+    }
+    wg_best(best, fl, wbest, wfl);
+}
+
+// Every slice's largest logit and, without filters, its weights relative to that.
+template <int TYPE, int N, bool SUMS>
+__global__ void __launch_bounds__(ROW_THREADS) k_sample_best(SampleArgs a)
 {
     __shared__ unsigned long long wbest[ROW_WAVES];
     __shared__ uint32_t wfl[ROW_WAVES];
     __shared__ double part[ROW_WAVES];
-    __shared__ PickLds lds;
-    __shared__ int lds_last;
-    const int slice = blockIdx.x % a.plan.slices, rr = blockIdx.x / a.plan.slices, row = a.row0 + rr, tid = threadIdx.x;
-    const SampleRow r = sample_row(a, row);
-    unsigned long long best = 0;
-    uint32_t fl = 0;
-    each_logit(a, row, slice, [&](float l, int i) {
-        fl |= sample_flags(l);
-        const unsigned long long o = best_of(l, i);
-        best = o > best ? o : best;
-    });
-    wg_best(best, fl, wbest, wfl);
+    const int slice = blockIdx.x % a.plan.slices, rr = blockIdx.x / a.plan.slices, row = a.row0 + rr;
+    const Slice<TYPE, N> x(a, row, slice);
+    unsigned long long best;
+    uint32_t fl;
+    slice_best(x, best, fl, wbest, wfl);
     double sum = 0.0;
-    if ((fl & kSampleFinite) && !(fl & (kSampleNan | kSamplePosInf)) && r.t > 0.0f) {
-        const SampleScale sc = sample_scale(r.t, sample_value((uint32_t)(best >> 32)), a.vocab);
-        each_logit(a, row, slice, [&](float l, int) { sum += sample_weight(sc, l); });
-        sum = wg_sum(sum, part);
+    if (SUMS) {
+        const float t = a.temperature ? a.temperature[row] : 1.0f;
+        if (weighed(t, fl)) {
+            const SampleScale sc = sample_scale(t, sample_value((uint32_t)(best >> 32)), a.vocab);
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                sum += sample_weight(sc, x.l[j]);
+            sum = wg_sum(sum, part);
+        }
     }
-    Record *const rec = record_of(a, rr);
-    Part *const parts = (Part *)(a.work + a.plan.parts) + (int64_t)rr * a.plan.slices;
-    if (tid == 0) {
-        agent_store(&parts[slice].best, best);
-        agent_store((unsigned long long *)&parts[slice].sum, __double_as_longlong(sum));
-        atomicOr(&rec->flags, fl);
-    }
-    if (!last_of(&rec->ended[0], a.plan.slices, &lds_last))
-        return;
-    unsigned long long mine = 0;
-    sum = 0.0;
-    if (tid < a.plan.slices) {
-        mine = agent_load(&parts[tid].best);
-        sum = __longlong_as_double(agent_load((unsigned long long *)&parts[tid].sum));
-    }
-    best = mine;
-    fl = __hip_atomic_load(&rec->flags, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    wg_best(best, fl, wbest, wfl);
-    if (tid == 0)
-        agent_clear(&rec->flags);
-    if (settled(a, row, r, best, fl))
-        return;
-    const SampleScale sc = sample_scale(r.t, sample_value((uint32_t)(best >> 32)), a.vocab);
-    if (sum > 0.0)
-        sum *= sample_weight(sc, sample_value((uint32_t)(mine >> 32)));
-    pick(a, row, r, sc, best, fl, sum, 0, 0.0, lds);
+    if (threadIdx.x == 0)
+        parts_of(a, rr)[slice] = Part{best, sum, fl, 0};
 }
 
-// With filters: the rows' largest logits (and empty bins for the next launch) ...
-__global__ void __launch_bounds__(ROW_THREADS) k_sample_best(SampleArgs a, int bins)
+// Without filters: the slices joined, and the token looked up in the one where it lies.
+__global__ void __launch_bounds__(ROW_THREADS) k_sample_join(SampleArgs a)
 {
     __shared__ unsigned long long wbest[ROW_WAVES];
     __shared__ uint32_t wfl[ROW_WAVES];
-    const int slice = blockIdx.x % a.plan.slices, rr = blockIdx.x / a.plan.slices;
-    if (bins) {
-        uint32_t *const b = (uint32_t *)(a.work + a.plan.bins + (int64_t)rr * kSampleBins * 12);
-        for (int i = slice * ROW_THREADS + threadIdx.x; i < kSampleBins * 3; i += a.plan.slices * ROW_THREADS)
-            b[i] = 0;
+    __shared__ PickLds lds;
+    const int rr = blockIdx.x, row = a.row0 + rr, tid = threadIdx.x;
+    const SampleRow r = sample_row(a, row);
+    unsigned long long best;
+    uint32_t fl;
+    row_best(a, rr, best, fl, wbest, wfl);
+    if (!weighed(r.t, fl)) {
+        settle(a, row, best, fl);
+        return;
     }
-    unsigned long long best = 0;
-    uint32_t fl = 0;
-    each_logit(a, a.row0 + rr, slice, [&](float l, int i) {
-        fl |= sample_flags(l);
-        const unsigned long long o = best_of(l, i);
-        best = o > best ? o : best;
-    });
-    wg_best(best, fl, wbest, wfl);
-    if (threadIdx.x == 0) {
-        atomicMax(&record_of(a, rr)->best, best);
-        atomicOr(&record_of(a, rr)->flags, fl);
+    const SampleScale sc = sample_scale(r.t, sample_value((uint32_t)(best >> 32)), a.vocab);
+    double sum = 0.0;
+    if (tid < a.plan.slices) {
+        const Part p = parts_of(a, rr)[tid];
+        sum = p.sum > 0.0 ? p.sum * sample_weight(sc, sample_value((uint32_t)(p.best >> 32))) : 0.0;
     }
+    pick(a, row, r, sc, best, fl, sum, wg_sum(sum, lds.part), 0, 0.0, lds);
 }
 
-// ... the tokens and weights of every bin, and from them the bins in which the kept
-// prefixes end ...
+// With top-k or top-p: the tokens and weights of every bin of a slice ...
+template <int TYPE, int N>
 __global__ void __launch_bounds__(ROW_THREADS) k_sample_bins(SampleArgs a)
 {
     __shared__ unsigned long long mass[kSampleBins];
     __shared__ uint32_t count[kSampleBins];
-    __shared__ unsigned long long part[ROW_WAVES];
-    __shared__ int lds_last, ends[3];
-    __shared__ unsigned long long over[2];
+    __shared__ unsigned long long wbest[ROW_WAVES];
+    __shared__ uint32_t wfl[ROW_WAVES];
     const int slice = blockIdx.x % a.plan.slices, rr = blockIdx.x / a.plan.slices, row = a.row0 + rr, tid = threadIdx.x;
     const SampleRow r = sample_row(a, row);
-    Record *const rec = record_of(a, rr);
-    const uint32_t fl = rec->flags;
     bool by_k, by_p;
-    if ((fl & (kSampleNan | kSamplePosInf)) || !(fl & kSampleFinite) || !(r.t > 0.0f) || !filtered(r, a.vocab, by_k, by_p))
+    if (!filtered(r, a.vocab, by_k, by_p) || !(r.t > 0.0f))
         return;
+    const Slice<TYPE, N> x(a, row, slice);
     for (int i = tid; i < kSampleBins; i += ROW_THREADS)
         mass[i] = 0, count[i] = 0;
-    __syncthreads();
-    const float most = sample_value((uint32_t)(rec->best >> 32)), rate = bin_rate(r.t);
+    unsigned long long best;
+    uint32_t fl;
+    row_best(a, rr, best, fl, wbest, wfl);
+    if (!weighed(r.t, fl))
+        return;
+    const float most = sample_value((uint32_t)(best >> 32)), rate = bin_rate(r.t);
     const SampleScale sc = sample_scale(r.t, most, a.vocab);
-    each_logit(a, row, slice, [&](float l, int) {
-        const int b = bin_of(l, most, rate);
-        if (by_k)
+    // (the last bin, of tokens that a grammar rules out, is counted apart: its atomics
+    // would all have one address)
+    uint32_t far = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const int b = bin_of(x.l[j], most, rate);
+        if (x.at(j) >= x.end)
+            continue;
+        far += b == kSampleBins - 1;
+        if (by_k && b < kSampleBins - 1)
             atomicAdd(&count[b], 1u);
-        if (by_p)
-            atomicAdd(&mass[b], (unsigned long long)sample_mass(sc, l));
-    });
+        if (by_p) {
+            const unsigned long long m = sample_mass(sc, x.l[j]);
+            if (m)
+                atomicAdd(&mass[b], m);
+        }
+    }
+    if (by_k && far)
+        atomicAdd(&count[kSampleBins - 1], far);
     __syncthreads();
-    unsigned long long *const all_mass = (unsigned long long *)(a.work + a.plan.bins + (int64_t)rr * kSampleBins * 12);
+    unsigned long long *const all_mass =
+        (unsigned long long *)(a.work + a.plan.bins + ((int64_t)rr * a.plan.slices + slice) * (kSampleBins * 12));
     uint32_t *const all_count = (uint32_t *)(all_mass + kSampleBins);
     for (int i = tid; i < kSampleBins; i += ROW_THREADS) {
-        if (mass[i])
-            atomicAdd(&all_mass[i], mass[i]);
-        if (count[i])
-            atomicAdd(&all_count[i], count[i]);
+        if (by_p)
+            all_mass[i] = mass[i];
+        if (by_k)
+            all_count[i] = count[i];
     }
-    if (!last_of(&rec->ended[0], a.plan.slices, &lds_last))
+}
+
+// ... summed over the slices, 64 bins a workgroup: one workgroup alone would wait for
+// hundreds of KB (38 slices: 20 us) ...
+constexpr int MERGE_BINS = 64;
+__global__ void __launch_bounds__(ROW_THREADS) k_sample_merge(SampleArgs a)
+{
+    __shared__ unsigned long long mass[ROW_WAVES][MERGE_BINS];
+    __shared__ uint32_t count[ROW_WAVES][MERGE_BINS];
+    constexpr int BLOCKS = kSampleBins / MERGE_BINS;
+    const int rr = blockIdx.x / BLOCKS, row = a.row0 + rr, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int bin = blockIdx.x % BLOCKS * MERGE_BINS + lane;
+    const SampleRow r = sample_row(a, row);
+    bool by_k, by_p;
+    if (!filtered(r, a.vocab, by_k, by_p) || !(r.t > 0.0f))
         return;
-    // 4 neighbouring bins a thread
-    constexpr int E = kSampleBins / ROW_THREADS;
-    unsigned long long m[E], c[E], before_m, before_c, sum_m = 0, sum_c = 0;
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-        m[i] = agent_load(&all_mass[E * tid + i]);
-        c[i] = __hip_atomic_load(&all_count[E * tid + i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        sum_m += m[i], sum_c += c[i];
+    // (a row that is not weighed has no bins: what lies there is summed and not looked at)
+    const uint8_t *const bins = a.work + a.plan.bins + (int64_t)rr * a.plan.slices * (kSampleBins * 12);
+    unsigned long long m = 0;
+    uint32_t c = 0;
+#pragma unroll 4
+    for (int q = wave; q < a.plan.slices; q += ROW_WAVES) {
+        const uint8_t *const from = bins + (int64_t)q * (kSampleBins * 12);
+        m += ((const unsigned long long *)from)[bin];
+        c += ((const uint32_t *)(from + kSampleBins * 8))[bin];
     }
-    const unsigned long long all = wg_scan(sum_m, part, before_m);
-    wg_scan(sum_c, part, before_c);
+    mass[wave][lane] = m, count[wave][lane] = c;
+    __syncthreads();
+    if (wave)
+        return;
+#pragma unroll
+    for (int w = 1; w < ROW_WAVES; ++w)
+        m += mass[w][lane], c += count[w][lane];
+    uint8_t *const to = a.work + a.plan.merged + (int64_t)rr * (kSampleBins * 12);
+    ((unsigned long long *)to)[bin] = by_p ? m : 0;
+    ((uint32_t *)(to + kSampleBins * 8))[bin] = by_k ? c : 0;
+}
+
+// ... from them the bins in which the kept prefixes end ...
+__global__ void __launch_bounds__(ROW_THREADS) k_sample_bounds(SampleArgs a)
+{
+    __shared__ unsigned long long mass[kSampleBins];
+    __shared__ uint32_t wfl[ROW_WAVES];
+    __shared__ unsigned long long part[ROW_WAVES], over[2];
+    __shared__ int ends[3];
+    constexpr int E = kSampleBins / ROW_THREADS; // neighbouring bins to a thread
+    static_assert(E == 2, "loaded as pairs");
+    const int rr = blockIdx.x, row = a.row0 + rr, tid = threadIdx.x;
+    const SampleRow r = sample_row(a, row);
+    bool by_k, by_p;
+    if (!filtered(r, a.vocab, by_k, by_p) || !(r.t > 0.0f))
+        return;
+    unsigned long long best;
+    uint32_t fl;
+    row_best(a, rr, best, fl, part, wfl);
+    if (!weighed(r.t, fl))
+        return;
+    const uint8_t *const bins = a.work + a.plan.merged + (int64_t)rr * (kSampleBins * 12);
+    const ulonglong2 mv = ((const ulonglong2 *)bins)[tid];
+    const uint2 cv = ((const uint2 *)(bins + kSampleBins * 8))[tid];
+    const unsigned long long m[E]{mv.x, mv.y}, c[E]{cv.x, cv.y};
+    unsigned long long before_m, before_c;
+    mass[E * tid] = m[0], mass[E * tid + 1] = m[1];
     if (tid < 3)
         ends[tid] = kSampleBins;
-    __syncthreads();
+    const unsigned long long all = wg_scan(m[0] + m[1], part, before_m);
+    wg_scan(c[0] + c[1], part, before_c);
     Bounds bo{};
     bo.all = all, bo.k = bo.p_low = bo.p_high = bo.whole = kSampleBins;
     if (by_k) {
-        unsigned long long upto = before_c;
+        unsigned long long upto = before_c, upto_m = before_m;
 #pragma unroll
         for (int i = 0; i < E; ++i) {
-            if (c[i] && upto < (unsigned long long)r.k && upto + c[i] >= (unsigned long long)r.k) { // (one bin of one thread)
-                ends[0] = E * tid + i;
-                over[0] = upto;
-                over[1] = before_m;
-                for (int e = 0; e < i; ++e)
-                    over[1] += m[e];
-            }
-            upto += c[i];
+            if (upto < (unsigned long long)r.k && upto + c[i] >= (unsigned long long)r.k) // (one bin of one thread)
+                ends[0] = E * tid + i, over[0] = upto, over[1] = upto_m;
+            upto += c[i], upto_m += m[i];
         }
         __syncthreads();
-        bo.k = bo.whole = ends[0], bo.k_count = (uint32_t)over[0], bo.k_over = over[1];
+        by_k = ends[0] < ZERO_BIN;
+        if (by_k)
+            bo.k = bo.whole = ends[0], bo.k_count = (uint32_t)over[0], bo.k_over = over[1];
     }
+    __syncthreads(); // over is read
     if (by_p) {
-        // weights that top-k leaves: between those over bin k and those down to it
-        const unsigned long long in_k = by_k ? agent_load(&all_mass[min(bo.k, kSampleBins - 1)]) : 0;
-        const double least = (double)fmaxf(r.p, 0.0f) * (double)(by_k ? bo.k_over : all);
-        const double largest = (double)fmaxf(r.p, 0.0f) * (double)(by_k ? bo.k_over + in_k : all);
+        // p of the weights that top-k leaves, which lie between those over bin k and
+        // those down to it
+        const double p = (double)fmaxf(r.p, 0.0f);
+        const double least = p * (double)(by_k ? bo.k_over : all);
+        const double largest = p * (double)(by_k ? bo.k_over + mass[bo.k] : all);
+        // the first bin with weights down to which they reach it
         unsigned long long upto = before_m;
 #pragma unroll
         for (int i = 0; i < E; ++i) {
-            if (m[i] && (double)(upto + m[i]) >= least)
-                atomicMin(&ends[1], E * tid + i);
-            if (m[i] && (double)(upto + m[i]) >= largest)
-                atomicMin(&ends[2], E * tid + i);
+            const unsigned long long prior = upto;
             upto += m[i];
+            if (m[i] && (double)upto >= least && (prior == 0 || (double)prior < least))
+                ends[1] = E * tid + i, over[0] = prior;
+            if (m[i] && (double)upto >= largest && (prior == 0 || (double)prior < largest))
+                ends[2] = E * tid + i;
         }
         __syncthreads();
-        bo.p_low = bo.whole = ends[1], bo.p_high = ends[2];
-        upto = before_m;
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-            if (E * tid + i == ends[1])
-                over[0] = upto;
-            upto += m[i];
-        }
-        __syncthreads();
-        bo.p_over = over[0];
+        bo.p_low = bo.whole = ends[1], bo.p_high = ends[2], bo.p_over = over[0];
     }
     if (tid == 0)
-        ((Bounds *)(a.work + a.plan.bounds))[rr] = bo;
+        *bounds_of(a, rr) = bo;
 }
 
-// ... and the tokens in those bins, and the weights of the ones over them.  The row's
-// last workgroup resolves the former and picks the token.
+// ... and the tokens in those bins, and the weights of the ones over them.  BINS: some
+// row has them; else (min-p alone) nothing is listed.
+template <int TYPE, int N, bool BINS>
+__global__ void __launch_bounds__(ROW_THREADS) k_sample_list(SampleArgs a)
+{
+    __shared__ unsigned long long mine[BINS ? kSampleList : 1];
+    __shared__ unsigned long long wbest[ROW_WAVES];
+    __shared__ uint32_t wfl[ROW_WAVES], listed, first;
+    __shared__ double part[ROW_WAVES];
+    const int slice = blockIdx.x % a.plan.slices, rr = blockIdx.x / a.plan.slices, row = a.row0 + rr, tid = threadIdx.x;
+    const SampleRow r = sample_row(a, row);
+    if (!(r.t > 0.0f))
+        return;
+    const Slice<TYPE, N> x(a, row, slice);
+    if (tid == 0)
+        listed = 0;
+    unsigned long long best;
+    uint32_t fl;
+    row_best(a, rr, best, fl, wbest, wfl);
+    if (!weighed(r.t, fl))
+        return;
+    const float most = sample_value((uint32_t)(best >> 32)), rate = bin_rate(r.t);
+    const SampleScale sc = sample_scale(r.t, most, a.vocab);
+    const double low = r.min_p > 0.0f ? (double)r.min_p : 0.0;
+    bool by_k = false, by_p = false;
+    int k = kSampleBins, p_low = kSampleBins, p_high = kSampleBins, whole = kSampleBins;
+    if (BINS && filtered(r, a.vocab, by_k, by_p)) {
+        const Bounds *const bo = bounds_of(a, rr);
+        k = bo->k, p_low = bo->p_low, p_high = bo->p_high, whole = bo->whole;
+    }
+    double sum = 0.0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const int b = BINS ? bin_of(x.l[j], most, rate) : 0;
+        if (b < whole) {
+            const double w = sample_weight(sc, x.l[j]);
+            sum += w >= low || best_of(x.l[j], x.at(j)) == best ? w : 0.0;
+        } else if (BINS && (b == k || (b >= p_low && b <= p_high)) && x.at(j) < x.end) {
+            const uint32_t n = atomicAdd(&listed, 1u);
+            if (n < (uint32_t)kSampleList)
+                mine[n] = best_of(x.l[j], x.at(j));
+        }
+    }
+    sum = wg_sum(sum, part);
+    if (tid == 0)
+        parts_of(a, rr)[slice].sum = sum;
+    if (!BINS || listed == 0)
+        return;
+    if (tid == 0)
+        first = atomicAdd(&bounds_of(a, rr)->listed, listed);
+    __syncthreads();
+    unsigned long long *const list = (unsigned long long *)(a.work + a.plan.list) + (int64_t)rr * kSampleList;
+    for (uint32_t i = tid; i < listed && first + i < (uint32_t)kSampleList; i += ROW_THREADS)
+        list[first + i] = mine[i];
+}
+
+// ... which are put in order and cut; then the token.
 struct ListLds {
-    unsigned long long order[kSampleList], mass[kSampleList];
+    unsigned long long order[kSampleList], mass[kSampleSlices];
 };
-__global__ void __launch_bounds__(ROW_THREADS) k_sample_pick(SampleArgs a, int bins)
+__global__ void __launch_bounds__(ROW_THREADS) k_sample_pick(SampleArgs a)
 {
     __shared__ union {
         ListLds list;
         RowLds row;
     } u;
     __shared__ PickLds lds;
-    __shared__ double part[ROW_WAVES];
-    __shared__ unsigned long long upart[ROW_WAVES], border;
-    __shared__ int lds_last;
-    const int slice = blockIdx.x % a.plan.slices, rr = blockIdx.x / a.plan.slices, row = a.row0 + rr, tid = threadIdx.x;
+    __shared__ unsigned long long upart[ROW_WAVES];
+    __shared__ uint32_t wfl[ROW_WAVES];
+    __shared__ int first_k, kept;
+    const int rr = blockIdx.x, row = a.row0 + rr, tid = threadIdx.x;
     const SampleRow r = sample_row(a, row);
-    Record *const rec = record_of(a, rr);
-    Part *const parts = (Part *)(a.work + a.plan.parts) + (int64_t)rr * a.plan.slices;
-    unsigned long long *const list = (unsigned long long *)(a.work + a.plan.list) + (int64_t)rr * kSampleList;
-    const uint32_t fl = rec->flags;
-    const unsigned long long best = rec->best;
-    const float most = sample_value((uint32_t)(best >> 32)), rate = bin_rate(r.t);
-    const bool sums = !(fl & (kSampleNan | kSamplePosInf)) && (fl & kSampleFinite) && r.t > 0.0f;
-    bool by_k = false, by_p = false;
+    bool by_k, by_p;
     Bounds bo{};
-    bo.k = bo.p_low = bo.p_high = bo.whole = kSampleBins;
-    if (sums && bins && filtered(r, a.vocab, by_k, by_p))
-        bo = ((const Bounds *)(a.work + a.plan.bounds))[rr];
+    const bool cut_row = filtered(r, a.vocab, by_k, by_p);
+    if (cut_row)
+        bo = *bounds_of(a, rr); // (not looked at where the row is not weighed)
+    double sum = tid < a.plan.slices ? parts_of(a, rr)[tid].sum : 0.0;
+    unsigned long long best;
+    uint32_t fl;
+    row_best(a, rr, best, fl, upart, wfl);
+    if (!weighed(r.t, fl)) {
+        settle(a, row, best, fl);
+        return;
+    }
+    const float most = sample_value((uint32_t)(best >> 32)), rate = bin_rate(r.t);
     const SampleScale sc = sample_scale(r.t, most, a.vocab);
     const double low = r.min_p > 0.0f ? (double)r.min_p : 0.0;
-    if (sums) {
-        double sum = 0.0;
-        each_logit(a, row, slice, [&](float l, int i) {
-            const int b = bin_of(l, most, rate);
-            const unsigned long long o = best_of(l, i);
-            if (b < bo.whole) {
-                const double w = sample_weight(sc, l);
-                sum += w >= low || o == best ? w : 0.0;
-            } else if (b == bo.k || (b >= bo.p_low && b <= bo.p_high)) {
-                const uint32_t n = atomicAdd(&rec->listed, 1u);
-                if (n < (uint32_t)kSampleList)
-                    agent_store(&list[n], o);
-            }
-        });
-        sum = wg_sum(sum, part);
-        if (tid == 0)
-            agent_store((unsigned long long *)&parts[slice].sum, __double_as_longlong(sum));
-    }
-    if (!last_of(&rec->ended[1], a.plan.slices, &lds_last))
-        return;
-    const int n = (int)__hip_atomic_load(&rec->listed, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __syncthreads();
-    if (tid == 0) {
-        agent_store(&rec->best, 0);
-        agent_clear(&rec->flags);
-        agent_clear(&rec->listed);
-    }
-    if (settled(a, row, r, best, fl))
-        return;
+    const int n = (int)bo.listed;
     if (n > kSampleList) {
         sample_whole_row(a, row, r, (uint32_t)(best >> 32), (int)~(uint32_t)best, fl, u.row);
         return;
     }
-    double sum = tid < a.plan.slices ? __longlong_as_double(agent_load((unsigned long long *)&parts[tid].sum)) : 0.0;
+    double total = wg_sum(sum, lds.part);
     unsigned long long from = 0; // the last kept token, in the order of best_of
-    if (by_k || by_p) {
+    if (cut_row && bo.whole < kSampleBins) {
+        // the listed tokens in order, the first first; 0 behind them
+        const unsigned long long *const list = (const unsigned long long *)(a.work + a.plan.list) + (int64_t)rr * kSampleList;
+        int size = 2;
+        while (size < n)
+            size *= 2;
+        unsigned long long *const order = u.list.order;
+        for (int i = tid; i < size; i += ROW_THREADS)
+            order[i] = i < n ? list[i] : 0;
+        for (int i = tid; i < kSampleSlices; i += ROW_THREADS)
+            u.list.mass[i] = 0;
+        __syncthreads();
+        for (int run = 2; run <= size; run *= 2)
+            for (int d = run / 2; d > 0; d /= 2) {
+                for (int p = tid; p < size / 2; p += ROW_THREADS) {
+                    const int i = 2 * p - (p & (d - 1)), j = i + d;
+                    const unsigned long long x = order[i], y = order[j];
+                    if ((x < y) == ((i & run) == 0))
+                        order[i] = y, order[j] = x;
+                }
+                __syncthreads();
+            }
+        // neighbours to a thread; the weights of those before
         constexpr int E = kSampleList / ROW_THREADS;
-        for (int i = tid; i < n; i += ROW_THREADS) {
-            const unsigned long long o = agent_load(&list[i]);
-            u.list.order[i] = o;
-            u.list.mass[i] = by_p ? sample_mass(sc, sample_value((uint32_t)(o >> 32))) : 0;
-        }
-        if (tid == 0)
-            border = ~0ull;
-        __syncthreads();
-        unsigned long long total = bo.all; // weights that top-k leaves
-        if (by_k) {
-            // the listed tokens of bin k by their places among them
-            unsigned long long kept = 0, before;
-            for (int e = 0; e < E; ++e) {
-                const int i = tid + e * ROW_THREADS;
-                if (i >= n)
-                    break;
-                const unsigned long long o = u.list.order[i];
-                if (bin_of(sample_value((uint32_t)(o >> 32)), most, rate) != bo.k)
-                    continue;
-                uint32_t rank = bo.k_count;
-                for (int j = 0; j < n; ++j) {
-                    const unsigned long long p = u.list.order[j];
-                    rank += p > o && bin_of(sample_value((uint32_t)(p >> 32)), most, rate) == bo.k;
-                }
-                if (rank < (uint32_t)r.k) {
-                    kept += u.list.mass[i];
-                    atomicMin(&border, o);
-                }
-            }
-            total = bo.k_over + wg_scan(kept, upart, before);
-            __syncthreads();
-            from = border;
-        }
-        if (by_p) {
-            const double want = (double)fmaxf(r.p, 0.0f) * (double)total;
-            __syncthreads();
-            if (tid == 0)
-                border = ~0ull;
-            __syncthreads();
-            for (int e = 0; e < E; ++e) {
-                const int i = tid + e * ROW_THREADS;
-                if (i >= n)
-                    break;
-                const unsigned long long o = u.list.order[i];
-                unsigned long long over = bo.p_over;
-                for (int j = 0; j < n; ++j)
-                    over += u.list.order[j] > o ? u.list.mass[j] : 0;
-                if (o >= from && ((double)over < want || o == best))
-                    atomicMin(&border, o);
-            }
-            __syncthreads();
-            from = border;
-        }
-        // the kept ones' weights, in order, to their slices
-        __syncthreads();
+        unsigned long long o[E], m[E], mine = 0, before = 0;
+#pragma unroll
         for (int e = 0; e < E; ++e) {
-            const int i = tid + e * ROW_THREADS;
-            if (i >= n)
-                break;
-            const unsigned long long o = u.list.order[i];
-            int rank = 0;
-            for (int j = 0; j < n; ++j)
-                rank += u.list.order[j] > o;
-            u.list.mass[rank] = o; // (mass is read)
+            o[e] = E * tid + e < n ? order[E * tid + e] : 0;
+            m[e] = by_p && o[e] ? sample_mass(sc, sample_value((uint32_t)(o[e] >> 32))) : 0;
+            mine += m[e];
         }
+        int cut = n; // kept by top-k: those before it
+        unsigned long long left = bo.all;
+        if (bo.k < kSampleBins) {
+            // (bin k's tokens are the last ones)
+            int ahead = 0;
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                ahead += o[e] && bin_of(sample_value((uint32_t)(o[e] >> 32)), most, rate) != bo.k;
+            const int2 at = first_and_last(false, ahead > 0, lds.first, lds.last);
+            if (tid == max(at.y, 0))
+                first_k = at.y < 0 ? 0 : E * tid + ahead;
+            __syncthreads();
+            cut = first_k + (r.k - (int)bo.k_count);
+            unsigned long long in_k = 0;
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                in_k += E * tid + e >= first_k && E * tid + e < cut ? m[e] : 0;
+            left = bo.k_over + wg_scan(in_k, upart, before);
+        }
+        wg_scan(mine, upart, before);
+        const double want = (double)fmaxf(r.p, 0.0f) * (double)left;
+        unsigned long long over = bo.p_over + before;
+        int last = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            if (o[e] && E * tid + e < cut && (!by_p || (double)over < want || o[e] == best))
+                last = E * tid + e + 1;
+            over += m[e];
+        }
+        const int2 at = first_and_last(false, last > 0, lds.first, lds.last);
+        if (tid == max(at.y, 0))
+            kept = last;
         __syncthreads();
-        if (tid < a.plan.slices)
-            for (int i = 0; i < n; ++i) {
-                const unsigned long long o = u.list.mass[i];
-                if (o < from)
-                    break;
-                if ((int)(~(uint32_t)o / (uint32_t)a.plan.per) == tid) {
-                    const double w = sample_weight(sc, sample_value((uint32_t)(o >> 32)));
-                    sum += w >= low || o == best ? w : 0.0;
-                }
+        from = kept ? order[kept - 1] : best;
+        double w = 0.0;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (E * tid + e < kept) {
+                double x = sample_weight(sc, sample_value((uint32_t)(o[e] >> 32)));
+                x = x >= low || o[e] == best ? x : 0.0;
+                w += x;
+                // (to their slices as whole numbers: in any order)
+                if (x > 0.0)
+                    atomicAdd(&u.list.mass[~(uint32_t)o[e] / (uint32_t)a.plan.per], (unsigned long long)rint(ldexp(x, sc.bits)));
             }
+        total += wg_sum(w, lds.part);
+        if (tid < a.plan.slices)
+            sum += ldexp((double)u.list.mass[tid], -sc.bits);
     }
-    pick(a, row, r, sc, best, fl, sum, from, low, lds);
+    pick(a, row, r, sc, best, fl, sum, total, from, low, lds);
+}
+
+template <int TYPE, int N>
+void launch(const SampleArgs &a, unsigned rows, hipStream_t s)
+{
+    const dim3 slices(rows * (unsigned)a.plan.slices), threads(ROW_THREADS);
+    const bool bins = a.top_k || a.top_p;
+    if (!bins && !a.min_p) {
+        hipLaunchKernelGGL((k_sample_best<TYPE, N, true>), slices, threads, 0, s, a);
+        hipLaunchKernelGGL(k_sample_join, dim3(rows), threads, 0, s, a);
+        return;
+    }
+    hipLaunchKernelGGL((k_sample_best<TYPE, N, false>), slices, threads, 0, s, a);
+    if (bins) {
+        hipLaunchKernelGGL((k_sample_bins<TYPE, N>), slices, threads, 0, s, a);
+        hipLaunchKernelGGL(k_sample_merge, dim3(rows * (kSampleBins / MERGE_BINS)), threads, 0, s, a);
+        hipLaunchKernelGGL(k_sample_bounds, dim3(rows), threads, 0, s, a);
+        hipLaunchKernelGGL((k_sample_list<TYPE, N, true>), slices, threads, 0, s, a);
+    } else {
+        hipLaunchKernelGGL((k_sample_list<TYPE, N, false>), slices, threads, 0, s, a);
+    }
+    hipLaunchKernelGGL(k_sample_pick, dim3(rows), threads, 0, s, a);
+}
+
+template <int TYPE>
+void launch(const SampleArgs &a, unsigned rows, hipStream_t s)
+{
+    if (a.plan.per == kSampleWide)
+        launch<TYPE, kSampleWide / ROW_THREADS>(a, rows, s);
+    else
+        launch<TYPE, kSampleNarrow / ROW_THREADS>(a, rows, s);
 }
 
 } // namespace
 
 hipError_t launch_sample(SampleArgs a, hipStream_t s)
 {
-    const bool bins = a.top_k || a.top_p;
     const int rows = a.rows;
     for (a.row0 = 0; a.row0 < rows; a.row0 += a.plan.rows) {
-        const dim3 grid((unsigned)((rows - a.row0 < a.plan.rows ? rows - a.row0 : a.plan.rows) * a.plan.slices));
-        if (!bins && !a.min_p) {
-            hipLaunchKernelGGL(k_sample_plain, grid, dim3(ROW_THREADS), 0, s, a);
-            continue;
-        }
-        hipLaunchKernelGGL(k_sample_best, grid, dim3(ROW_THREADS), 0, s, a, (int)bins);
-        if (bins)
-            hipLaunchKernelGGL(k_sample_bins, grid, dim3(ROW_THREADS), 0, s, a);
-        hipLaunchKernelGGL(k_sample_pick, grid, dim3(ROW_THREADS), 0, s, a, (int)bins);
+        const unsigned n = (unsigned)(rows - a.row0 < a.plan.rows ? rows - a.row0 : a.plan.rows);
+        if (a.type == kF32)
+            launch<kF32>(a, n, s);
+        else if (a.type == kF16)
+            launch<kF16>(a, n, s);
+        else
+            launch<kBF16>(a, n, s);
     }
     return hipGetLastError();
 }

@@ -76,13 +76,15 @@ __device__ __forceinline__ SampleScale sample_scale(float t, float most, int voc
     return SampleScale{1.4426950408889634074 / (double)t, (double)most, min(46, 62 - (32 - __builtin_clz(vocab)))};
 }
 
-// 2^x for x <= 0: 2^f, |f| <= 1/2, by its series, whose rest is below 2^-52
+// 2^x for x <= 0: 2^f, |f| <= 1/2, by its series, whose rest is below 2^-47; 0 from
+// 2^-1075 on
 __device__ __forceinline__ double sample_exp2(double x)
 {
+    x = fmax(x, -1100.0);
     const double n = rint(x), f = x - n;
     constexpr double L = 0.69314718055994530942;
     // L^i / i!
-    constexpr double c[13] = {1.0,
+    constexpr double c[12] = {1.0,
                               L,
                               L * L / 2,
                               L * L * L / 6,
@@ -93,18 +95,18 @@ __device__ __forceinline__ double sample_exp2(double x)
                               L * L * L * L * L * L * L * L / 40320,
                               L * L * L * L * L * L * L * L * L / 362880,
                               L * L * L * L * L * L * L * L * L * L / 3628800,
-                              L * L * L * L * L * L * L * L * L * L * L / 39916800,
-                              L * L * L * L * L * L * L * L * L * L * L * L / 479001600};
-    double y = c[12];
+                              L * L * L * L * L * L * L * L * L * L * L / 39916800};
+    double y = c[11];
 #pragma unroll
-    for (int i = 11; i >= 0; --i)
+    for (int i = 10; i >= 0; --i)
         y = fma(y, f, c[i]);
-    return ldexp(y, (int)fmax(n, -2000.0));
+    return ldexp(y, (int)n);
 }
 
+// (-infinity, and a rate of 0 times it, become -1100)
 __device__ __forceinline__ double sample_weight(const SampleScale &s, float l)
 {
-    return l == -__builtin_inff() ? 0.0 : sample_exp2(s.rate * ((double)l - s.most));
+    return sample_exp2(s.rate * ((double)l - s.most));
 }
 
 __device__ __forceinline__ uint64_t sample_mass(const SampleScale &s, float l)

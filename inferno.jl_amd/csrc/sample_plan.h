@@ -9,37 +9,36 @@
 namespace ihip {
 
 constexpr int kSampleThreads = 512;
-constexpr int kSampleBins = 2048;
-constexpr int kSampleList = 2048;  // tokens at a boundary that are resolved in LDS
-constexpr int kSampleRows = 512;   // rows of a launch
-constexpr int kSampleRecord = 32;  // bytes of a row that are zero between calls
-constexpr int kSampleSlices = 512; // of a row, at most
+constexpr int kSampleBins = 1024;
+constexpr int kSampleList = 4096;   // tokens at a boundary that are resolved in LDS
+constexpr int kSampleRows = 256;    // rows of a launch
+constexpr int kSampleRecord = 64;   // bytes of a row's bounds
+constexpr int kSamplePart = 24;     // bytes of a slice's values
+constexpr int kSampleSlices = 512;  // of a row, at most
+constexpr int kSampleWide = 8192;   // logits of a slice (a thread's are in registers),
+constexpr int kSampleNarrow = 4096; // and where those would leave CUs idle
+constexpr int64_t kSampleVocab = (int64_t)kSampleWide * kSampleSlices;
 
 struct SamplePlan {
     int per, slices; // logits of a slice; slices of a row
     int rows;        // of a launch
-    // offsets of the slices' values, the rows' bounds, their bins (weights, then
-    // counts) and the tokens at their boundaries
-    size_t parts, bounds, bins, list, bytes;
+    // offsets of the rows' bounds (behind the slices' values), the slices' and the
+    // rows' bins (weights, then counts) and the tokens at the rows' boundaries
+    size_t bounds, bins, merged, list, bytes;
 };
 
 inline SamplePlan sample_plan(int rows, int vocab)
 {
     SamplePlan p{};
-    // Slices of 16384 logits, or of 4096 where those would leave CUs idle (151936
-    // logits: from 26 rows on; us, either side of it to be measured beside the kernels)
-    const int64_t wide = 16384, narrow = 4096;
-    int64_t per = rows * ((vocab + wide - 1) / wide) >= 256 ? wide : narrow;
-    while ((vocab + per - 1) / per > kSampleSlices)
-        per *= 2;
-    p.per = (int)per;
-    p.slices = (int)((vocab + per - 1) / per);
+    const int64_t wide = (vocab + kSampleWide - 1) / kSampleWide, narrow = (vocab + kSampleNarrow - 1) / kSampleNarrow;
+    p.per = rows * wide >= 256 || narrow > kSampleSlices ? kSampleWide : kSampleNarrow;
+    p.slices = (int)(p.per == kSampleWide ? wide : narrow);
     p.rows = rows < kSampleRows ? rows : kSampleRows;
-    const size_t n = (size_t)p.rows;
-    p.parts = (size_t)kSampleRows * kSampleRecord;
-    p.bounds = p.parts + n * (size_t)p.slices * 16;
-    p.bins = p.bounds + n * 64;
-    p.list = p.bins + n * kSampleBins * 12;
+    const size_t n = (size_t)p.rows, all = n * (size_t)p.slices;
+    p.bounds = (all * kSamplePart + 63) / 64 * 64;
+    p.bins = p.bounds + n * kSampleRecord;
+    p.merged = p.bins + all * kSampleBins * 12;
+    p.list = p.merged + n * kSampleBins * 12;
     p.bytes = p.list + n * kSampleList * 8;
     return p;
 }

@@ -546,10 +546,10 @@ def rope_kv(q: torch.Tensor, k, v, turns: torch.Tensor, cache: KVCache, batch: K
     return out
 
 
-def _counted(n: int, device, front: int = _lib.ATTN_COUNT_BYTES):
-    """n bytes whose front, the counts of a call's parts, is zero."""
+def _counted(n: int, device):
+    """n bytes whose front, the counts of attn_paged's parts, is zero."""
     t = torch.empty(n, dtype=torch.uint8, device=device)
-    t[:front].zero_()
+    t[:_lib.ATTN_COUNT_BYTES].zero_()
     return t
 
 
@@ -798,13 +798,12 @@ def _fresh_bytes(stream, n, device):
 
 # ---- the choice of a token --------------------------------------------------------
 def sample_workspace(rows: int, vocab: int, device="cuda"):
-    """The workspace of sample for up to so many rows of so many logits.  Its counts
-    start as zeros, written on the current stream, and every call leaves them so.
-    Calls that share one must not overlap."""
+    """The workspace of sample for rows x vocab logits.  Calls that share one must not
+    overlap."""
     n = lib().ihip_sample_scratch_bytes(rows, vocab)
     if not n:
         raise _invalid(f"{rows} rows of {vocab} logits")
-    return _counted(n, device, _lib.SAMPLE_COUNT_BYTES)
+    return torch.empty(n, dtype=torch.uint8, device=device)
 
 
 def sample(logits: torch.Tensor, u: torch.Tensor, temperature=None, top_k=None, top_p=None, min_p=None,
@@ -824,9 +823,7 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=None, top_k=None, 
     if out is None:
         out = _fresh(stream, lambda: torch.empty(rows, dtype=torch.int32, device=logits.device))
     if workspace is None:
-        n = lib().ihip_sample_scratch_bytes(rows, vocab)
-        if n:
-            workspace = _fresh(stream, lambda: _counted(n, logits.device, _lib.SAMPLE_COUNT_BYTES))
+        workspace = _fresh_bytes(stream, lib().ihip_sample_scratch_bytes(rows, vocab), logits.device)
     _launch(dev, stream, lib().ihip_sample_dev, logits.data_ptr(), kind, logits.stride(0) if rows > 1 else vocab, rows, vocab,
             _at(temperature, torch.float32, "temperature", dev, rows), _at(top_k, torch.int32, "top_k", dev, rows),
             _at(top_p, torch.float32, "top_p", dev, rows), _at(min_p, torch.float32, "min_p", dev, rows),
