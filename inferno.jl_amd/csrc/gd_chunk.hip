@@ -410,6 +410,8 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
     __shared__ float bounds[SCAN_WAVES][CT][16];
     __shared__ __attribute__((aligned(16))) float turn[SCAN_WAVES][16][20];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, r = lane & 15;
+    if (a.flags && blockIdx.x == 0 && !a.plan.steps)
+        gd_report(a.batch, a.flags);
     // the workgroups of the heads that read one K lie on one XCD (its L2)
     const int blocks = (a.v_dim + 16 * CT - 1) / (16 * CT), each = a.group * blocks;
     const int j = blockIdx.x / 8, u = j / each * 8 + blockIdx.x % 8;

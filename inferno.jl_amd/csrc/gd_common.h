@@ -51,16 +51,22 @@ __device__ __forceinline__ GdSeq gd_seq(const StateBatch &b, int pool, int s, ui
     for (int e = threadIdx.x & 63; e < s; e += 64)
         twice |= b.slots[e] == q.slot && gd_rows(b, e).y > 0;
     const bool bad = (unsigned)q.slot >= (unsigned)pool || __ballot(twice);
-    if (flags && threadIdx.x == 0) {
-        uint32_t f = bad && q.n > 0 ? kFlagStateSlot : 0;
-        if (b.starts[s] != q.start || b.starts[s + 1] != q.start + q.n || len < q.n)
-            f |= kFlagKvLength;
-        if (f)
-            atomicOr(flags, f);
-    }
+    if (flags && threadIdx.x == 0 && bad && q.n > 0)
+        atomicOr(flags, kFlagStateSlot);
     if (bad)
         q.slot = -1;
     return q;
+}
+
+// Reports the sequences whose rows had to be cut, or that have more new tokens than
+// tokens.  One workgroup of a call calls it.
+__device__ __forceinline__ void gd_report(const StateBatch &b, uint32_t *flags)
+{
+    for (int s = threadIdx.x; s < b.sequences; s += blockDim.x) {
+        const int2 r = gd_rows(b, s);
+        if (b.starts[s] != r.x || b.starts[s + 1] != r.x + r.y || (b.lens && b.lens[s] < r.y))
+            atomicOr(flags, kFlagKvLength);
+    }
 }
 
 // The tiles of 2^shift rows that the sequences' rows are taken in are numbered so

@@ -21,6 +21,8 @@ constexpr int CONV_AHEAD = 8; // tokens whose values are on their way at once
 template <int W>
 __global__ void __launch_bounds__(CONV_THREADS) k_short_conv(ConvArgs a)
 {
+    if (a.flags && blockIdx.x == 0 && blockIdx.y == 0)
+        gd_report(a.batch, a.flags);
     int c = 0;
     const int s = gd_find(a.batch, CONV_SHIFT, (int)blockIdx.x, c);
     if (s < 0)

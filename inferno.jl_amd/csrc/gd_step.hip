@@ -34,6 +34,8 @@ __global__ void __launch_bounds__(STEP_THREADS) k_delta_step(DeltaArgs a)
     __shared__ float alpha[STEP_TOKENS], beta[STEP_TOKENS], qk[STEP_TOKENS], squares[STEP_TOKENS][STEP_WAVES];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int h = blockIdx.x % a.v_heads, s = blockIdx.x / a.v_heads, kh = h / a.group;
+    if (a.flags && blockIdx.x == 0)
+        gd_report(a.batch, a.flags);
     const GdSeq seq = gd_seq(a.batch, a.pool, s, h == 0 ? a.flags : nullptr);
     if (seq.slot < 0 || seq.n == 0 || (a.few >= 0 && seq.n > a.few))
         return;
