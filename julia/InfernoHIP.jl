@@ -601,6 +601,7 @@ module Device
 export gemv!, gemv_add!, gemv_norm!, dequantize!, rmsnorm!, gate_up_swiglu!, lm_head_argmax_norm!
 export register_group, weight_bytes
 export rope_turns, rope_kv!, attn_paged!, attn_paged_scratch_bytes, kv_fork!, kv_compact!, kv_copy!
+export short_conv!, gated_delta!, gated_delta_scratch_bytes, sample!, sample_scratch_bytes
 
 import ..InfernoHIP: LIBIHIP, check, require, ArgmaxWorkspace, token_ptr, flags_ptr, read_token
 
@@ -933,6 +934,120 @@ function kv_copy!(cache::KVCache, copies::Ptr{Int32}, n::Integer; layers::Intege
                 (Ref{KVCache}, Cint, Int64, Ptr{Int32}, Cint, Ptr{Int32}, Ptr{UInt32}, Ptr{Cvoid}),
                 Ref(cache), layers, layer_stride, copies, n, count, flags, stream))
     return nothing
+end
+
+"""
+The sequences of a call on layers that keep a state (`ihip_state_batch`): device
+arrays of Int32 -- `q_starts` (sequences + 1 row offsets from 0), `kv_lens` (all
+tokens of each, or C_NULL: every sequence goes on) and `slots` (from 0) -- the
+rows, and the most new tokens of a sequence (0: not known).
+"""
+struct StateBatch
+    q_starts::Ptr{Int32}
+    kv_lens::Ptr{Int32}
+    slots::Ptr{Int32}
+    sequences::Cint
+    tokens::Cint
+    most::Cint
+end
+
+"""
+A layer of the gated delta rule (`ihip_delta_layer`, device memory): `state` is
+`slots` slots of v_heads x k_dim x v_dim floats (Julia arrays of size (v_dim,
+k_dim, v_heads, slots)), `decay` a GGUF file's ssm_a.
+"""
+struct DeltaLayer
+    state::Ptr{Float32}
+    slot_stride::Int64
+    slots::Cint
+    k_heads::Cint
+    v_heads::Cint
+    k_dim::Cint
+    v_dim::Cint
+    decay::Ptr{Float32}
+    dt_bias::Ptr{Float32}
+    norm_w::Ptr{Float32}
+    norm_eps::Cfloat
+    l2_eps::Cfloat
+    scale::Cfloat
+end
+
+"""
+    short_conv!(out, out_type, x, x_type, x_stride, w, channels, width, state, slot_stride, slots, batch;
+                bias, silu, flags, stream)
+
+The causal convolution of a recurrent layer over each channel's last inputs
+(src/ModelCPU.jl:511-759); `state` keeps the last width - 1 of every slot.
+"""
+function short_conv!(out::Ptr{Cvoid}, out_type::Integer, x::Ptr{Cvoid}, x_type::Integer, x_stride::Integer,
+                     w::Ptr{Float32}, channels::Integer, width::Integer, state::Ptr{Float32},
+                     slot_stride::Integer, slots::Integer, batch::StateBatch;
+                     bias::Ptr{Float32} = Ptr{Float32}(C_NULL), silu::Bool = true,
+                     flags::Ptr{UInt32} = Ptr{UInt32}(C_NULL), stream::Ptr{Cvoid} = C_NULL)
+    require()
+    check(ccall((:ihip_short_conv_dev, LIBIHIP), Cint,
+                (Ptr{Cvoid}, Cint, Int64, Ptr{Float32}, Ptr{Float32}, Cint, Cint, Cint, Ptr{Float32},
+                 Int64, Cint, Ptr{Cvoid}, Cint, Ref{StateBatch}, Ptr{UInt32}, Ptr{Cvoid}),
+                x, x_type, x_stride, w, bias, channels, width, silu ? 1 : 0, state, slot_stride, slots,
+                out, out_type, Ref(batch), flags, stream))
+    return out
+end
+
+"""Workspace of `gated_delta!` for a batch of these sizes."""
+gated_delta_scratch_bytes(type::Integer, layer::DeltaLayer, batch::StateBatch) =
+    Int(ccall((:ihip_gated_delta_scratch_bytes, LIBIHIP), Csize_t,
+              (Cint, Ref{DeltaLayer}, Ref{StateBatch}), type, Ref(layer), Ref(batch)))
+
+"""
+    gated_delta!(out, out_type, q, q_stride, k, k_stride, v, v_stride, type, a, a_stride, b, b_stride,
+                 layer, batch; gate, gate_stride, flags, workspace, workspace_bytes, stream)
+
+The gated delta rule over the batch's new tokens (src/ModelCPU.jl:511-759), with
+the unit length of q and k, decay and write strength from their projections a
+and b, and the output norm and gate.  q, k, v: rows of `short_conv!`'s output.
+"""
+function gated_delta!(out::Ptr{Cvoid}, out_type::Integer, q::Ptr{Cvoid}, q_stride::Integer, k::Ptr{Cvoid},
+                      k_stride::Integer, v::Ptr{Cvoid}, v_stride::Integer, type::Integer,
+                      a::Ptr{Float32}, a_stride::Integer, b::Ptr{Float32}, b_stride::Integer,
+                      layer::DeltaLayer, batch::StateBatch;
+                      gate::Ptr{Float32} = Ptr{Float32}(C_NULL), gate_stride::Integer = 0,
+                      flags::Ptr{UInt32} = Ptr{UInt32}(C_NULL), workspace::Ptr{Cvoid} = C_NULL,
+                      workspace_bytes::Integer = 0, stream::Ptr{Cvoid} = C_NULL)
+    require()
+    check(ccall((:ihip_gated_delta_dev, LIBIHIP), Cint,
+                (Ptr{Cvoid}, Int64, Ptr{Cvoid}, Int64, Ptr{Cvoid}, Int64, Cint, Ptr{Float32}, Int64,
+                 Ptr{Float32}, Int64, Ptr{Float32}, Int64, Ptr{Cvoid}, Cint, Ref{DeltaLayer},
+                 Ref{StateBatch}, Ptr{UInt32}, Ptr{Cvoid}, Csize_t, Ptr{Cvoid}),
+                q, q_stride, k, k_stride, v, v_stride, type, a, a_stride, b, b_stride, gate, gate_stride,
+                out, out_type, Ref(layer), Ref(batch), flags, workspace, workspace_bytes, stream))
+    return out
+end
+
+"""Workspace of `sample!` for so many rows of so many logits."""
+sample_scratch_bytes(rows::Integer, vocab::Integer) =
+    Int(ccall((:ihip_sample_scratch_bytes, LIBIHIP), Csize_t, (Cint, Cint), rows, vocab))
+
+"""
+    sample!(tokens, logits, type, row_stride, rows, vocab, u, workspace, workspace_bytes;
+            temperature, top_k, top_p, min_p, logprobs, flags, stream)
+
+A token (from 0) per row of logits by the given numbers `u` in [0, 1), as
+softmax_sample (src/CommonOps.jl:172) does for one: temperature, top-k, top-p
+and min-p of each row (C_NULL: 1, and no filter).
+"""
+function sample!(tokens::Ptr{Int32}, logits::Ptr{Cvoid}, type::Integer, row_stride::Integer, rows::Integer,
+                 vocab::Integer, u::Ptr{Float32}, workspace::Ptr{Cvoid}, workspace_bytes::Integer;
+                 temperature::Ptr{Float32} = Ptr{Float32}(C_NULL),
+                 top_k::Ptr{Int32} = Ptr{Int32}(C_NULL), top_p::Ptr{Float32} = Ptr{Float32}(C_NULL),
+                 min_p::Ptr{Float32} = Ptr{Float32}(C_NULL), logprobs::Ptr{Float32} = Ptr{Float32}(C_NULL),
+                 flags::Ptr{UInt32} = Ptr{UInt32}(C_NULL), stream::Ptr{Cvoid} = C_NULL)
+    require()
+    check(ccall((:ihip_sample_dev, LIBIHIP), Cint,
+                (Ptr{Cvoid}, Cint, Int64, Cint, Cint, Ptr{Float32}, Ptr{Int32}, Ptr{Float32}, Ptr{Float32},
+                 Ptr{Float32}, Ptr{Int32}, Ptr{Float32}, Ptr{UInt32}, Ptr{Cvoid}, Csize_t, Ptr{Cvoid}),
+                logits, type, row_stride, rows, vocab, temperature, top_k, top_p, min_p, u, tokens, logprobs,
+                flags, workspace, workspace_bytes, stream))
+    return tokens
 end
 
 end # module Device
