@@ -64,9 +64,10 @@ __device__ __forceinline__ gd_f4 gd_mfma(gd_h8 a, gd_h8 b, gd_f4 c)
 constexpr int PREP_THREADS = 256;
 constexpr int TRI = 68; // floats from a row of a 64 x 64 matrix to the next, in LDS
 
-template <int KD, int PARTS>
+template <int TYPE, int KD>
 __global__ void __launch_bounds__(PREP_THREADS) k_delta_prep(DeltaArgs a)
 {
+    constexpr int PARTS = TYPE == kF32 ? 2 : 1;
     constexpr int KS = KD / 32;               // steps of a row of K
     constexpr int FRAG = 4 * KS * PARTS * 1024; // bytes of K or Q
     constexpr int MD = KD / 64;               // 16-row tiles of M that a wave forms
@@ -91,27 +92,28 @@ __global__ void __launch_bounds__(PREP_THREADS) k_delta_prep(DeltaArgs a)
     const int row = 16 * wave + r;
     gd_h8 kf[KS][PARTS], qf[KS][PARTS];
     float rq = 0.0f;
+    // (behind the last token and the last column: others' values, not used)
+    typename GdType<TYPE>::T4 raw[2][2 * KS];
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
-        const void *src = which ? a.q : a.k;
-        const int64_t at = (first + row) * (which ? a.q_step : a.k_step) + (int64_t)kh * a.k_dim + 4 * g;
+        const int64_t at = (first + min(row, n - 1)) * (which ? a.q_step : a.k_step) + (int64_t)kh * a.k_dim;
+#pragma unroll
+        for (int i = 0; i < 2 * KS; ++i)
+            raw[which][i] = gd_raw4<TYPE>(which ? a.q : a.k, at + (16 * i + 4 * g < a.k_dim ? 16 * i + 4 * g : 0));
+    }
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
         gd_f8 x[KS];
         double sum = 0.0;
         float most = 0.0f;
 #pragma unroll
-        for (int i = 0; i < KS; ++i) {
+        for (int i = 0; i < 2 * KS; ++i) {
+            const gd_f4 v = row < n && 16 * i + 4 * g < a.k_dim ? gd_wide(raw[which][i]) : gd_f4{};
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const int e = 32 * i + 16 * half;
-                gd_f4 v{};
-                if (row < n && e + 4 * g < a.k_dim)
-                    v = gd_load4(src, at + e, a.type);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    x[i][4 * half + j] = v[j];
-                    sum += (double)v[j] * v[j];
-                    most = fmaxf(most, fabsf(v[j]));
-                }
+            for (int j = 0; j < 4; ++j) {
+                x[i / 2][4 * (i & 1) + j] = v[j];
+                sum += (double)v[j] * v[j];
+                most = fmaxf(most, fabsf(v[j]));
             }
         }
         sum += __shfl_xor(sum, 16);
@@ -399,9 +401,10 @@ __device__ __forceinline__ void scan_sync()
 // and no token adds more than |v| to the length of a column of S, so |X| and the
 // new S lie below 12 max |S| + 66 max |v| (sqrt(128) < 12).  Fragments keep 22 bits of
 // what is over 2^-27 of that.
-template <int KD, int PARTS, int CT>
+template <int TYPE, int KD, int CT>
 __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
 {
+    constexpr int PARTS = TYPE == kF32 ? 2 : 1;
     constexpr int KS = KD / 32;
     constexpr int FRAG = 4 * KS * PARTS * 1024;
     constexpr int VB = PARTS > 1 ? 4 : 2; // bytes of a value of V
@@ -424,7 +427,7 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
     const int col0 = j % blocks * CT * 16;
     float *const state = a.state + seq.slot * a.slot_step + (int64_t)h * a.k_dim * a.v_dim + col0 + r;
     const int chunks = (seq.n + 63) / 64, tile0 = gd_base(a.batch, kDeltaShift, s);
-    const bool half = a.type == kF16, owner = wave < KS;
+    const bool owner = wave < KS;
     int64_t vat[4]; // of this lane's values of V in a whole chunk
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -530,7 +533,7 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
         for (int e = 0; e < CT; ++e) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float x = PARTS > 1 ? __uint_as_float(o.v[e][i]) : half ? h2f(o.v[e][i]) : __uint_as_float(o.v[e][i] << 16);
+                const float x = TYPE == kF32 ? __uint_as_float(o.v[e][i]) : TYPE == kF16 ? h2f(o.v[e][i]) : __uint_as_float(o.v[e][i] << 16);
                 v[e][i] = live[e] && 16 * wave + 4 * g + i < n ? x : 0.0f;
             }
             if (owner) {
@@ -690,27 +693,30 @@ __global__ void __launch_bounds__(NORM_THREADS) k_delta_norm(DeltaArgs a)
     }
 }
 
-template <int KD, int PARTS>
+template <int TYPE, int KD>
 void launch(const DeltaArgs &a, hipStream_t s)
 {
     constexpr int CT = 1;
     const unsigned units = (unsigned)(a.plan.tiles * a.v_heads);
-    hipLaunchKernelGGL((k_delta_prep<KD, PARTS>), dim3(units), dim3(PREP_THREADS), 0, s, a);
+    hipLaunchKernelGGL((k_delta_prep<TYPE, KD>), dim3(units), dim3(PREP_THREADS), 0, s, a);
     const unsigned blocks = (unsigned)((a.v_dim + 16 * CT - 1) / (16 * CT)) * (unsigned)a.group;
     const unsigned heads = ((unsigned)(a.k_heads * a.batch.sequences) + 7) / 8 * 8;
-    hipLaunchKernelGGL((k_delta_scan<KD, PARTS, CT>), dim3(heads * blocks), dim3(64 * SCAN_WAVES), 0, s, a);
+    hipLaunchKernelGGL((k_delta_scan<TYPE, KD, CT>), dim3(heads * blocks), dim3(64 * SCAN_WAVES), 0, s, a);
     if (a.norm_w || a.gate)
         hipLaunchKernelGGL(k_delta_norm, dim3(units), dim3(NORM_THREADS), 0, s, a);
+}
+
+template <int TYPE>
+void launch(const DeltaArgs &a, hipStream_t s)
+{
+    a.k_dim <= 64 ? launch<TYPE, 64>(a, s) : launch<TYPE, 128>(a, s);
 }
 
 } // namespace
 
 hipError_t launch_delta_chunks(const DeltaArgs &a, hipStream_t s)
 {
-    if (a.type == kF32)
-        a.k_dim <= 64 ? launch<64, 2>(a, s) : launch<128, 2>(a, s);
-    else
-        a.k_dim <= 64 ? launch<64, 1>(a, s) : launch<128, 1>(a, s);
+    a.type == kF32 ? launch<kF32>(a, s) : a.type == kF16 ? launch<kF16>(a, s) : launch<kBF16>(a, s);
     return hipGetLastError();
 }
 

@@ -102,19 +102,35 @@ typedef float gd_f4 __attribute__((ext_vector_type(4)));
 typedef _Float16 gd_h4 __attribute__((ext_vector_type(4)));
 typedef __bf16 gd_b4 __attribute__((ext_vector_type(4)));
 
-__device__ __forceinline__ int gd_bytes(int type)
+// Values of one type, 1 or 4 neighbours, as they lie in memory and as fp32.  The type is
+// the kernels' parameter: looked at beside every load, it would have each of them wait
+// for the one before.
+template <int TYPE>
+struct GdType;
+template <>
+struct GdType<kF32> {
+    typedef float T;
+    typedef gd_f4 T4;
+};
+template <>
+struct GdType<kF16> {
+    typedef _Float16 T;
+    typedef gd_h4 T4;
+};
+template <>
+struct GdType<kBF16> {
+    typedef __bf16 T;
+    typedef gd_b4 T4;
+};
+template <int TYPE>
+__device__ __forceinline__ typename GdType<TYPE>::T4 gd_raw4(const void *base, int64_t at)
 {
-    return type == kF32 ? 4 : 2;
+    return *(const typename GdType<TYPE>::T4 *)((const typename GdType<TYPE>::T *)base + at);
 }
-
-// 4 neighbours, exactly
-__device__ __forceinline__ gd_f4 gd_load4(const void *base, int64_t at, int type)
+template <typename T4>
+__device__ __forceinline__ gd_f4 gd_wide(T4 v)
 {
-    if (type == kF32)
-        return *(const gd_f4 *)((const float *)base + at);
-    if (type == kF16)
-        return __builtin_convertvector(*(const gd_h4 *)((const _Float16 *)base + at), gd_f4);
-    return __builtin_convertvector(*(const gd_b4 *)((const __bf16 *)base + at), gd_f4);
+    return __builtin_convertvector(v, gd_f4);
 }
 
 // 4 neighbours, rounded once to the type they are kept in (to nearest)

@@ -18,7 +18,7 @@ constexpr int CONV_AHEAD = 8; // tokens whose values are on their way at once
 // inputs in registers, so that a tile reads W - 1 rows twice and everything else
 // once.  A sequence's first tile alone reads and writes its state (the new one is
 // read from x, wherever its tile is), and in one thread, so no tile waits for another.
-template <int W>
+template <int TYPE, int W>
 __global__ void __launch_bounds__(CONV_THREADS) k_short_conv(ConvArgs a)
 {
     if (a.flags && blockIdx.x == 0 && blockIdx.y == 0)
@@ -35,13 +35,18 @@ __global__ void __launch_bounds__(CONV_THREADS) k_short_conv(ConvArgs a)
     gd_f4 win[W]; // the last W - 1 inputs, then the token's own
     const int t0 = c << CONV_SHIFT, t1 = min(t0 + (1 << CONV_SHIFT), q.n);
     const int64_t row0 = (int64_t)q.start * a.x_step + ch;
+    if (c > 0) {
 #pragma unroll
-    for (int j = 0; j < W - 1; ++j) {
-        win[j] = gd_f4{};
-        if (c > 0)
-            win[j] = gd_load4(a.x, row0 + (t0 - (W - 1) + j) * a.x_step, a.x_type);
-        else if (!q.begins)
-            win[j] = *(const gd_f4 *)(state + (int64_t)j * a.channels);
+        for (int j = 0; j < W - 1; ++j)
+            win[j] = gd_wide(gd_raw4<TYPE>(a.x, row0 + (t0 - (W - 1) + j) * a.x_step));
+    } else {
+#pragma unroll
+        for (int j = 0; j < W - 1; ++j)
+            win[j] = gd_f4{};
+        if (!q.begins)
+#pragma unroll
+            for (int j = 0; j < W - 1; ++j)
+                win[j] = *(const gd_f4 *)(state + (int64_t)j * a.channels);
     }
     float w[4][W];
 #pragma unroll
@@ -58,7 +63,7 @@ __global__ void __launch_bounds__(CONV_THREADS) k_short_conv(ConvArgs a)
             const int t = q.n - (W - 1) + j;
             gd_f4 v{};
             if (t >= 0)
-                v = gd_load4(a.x, row0 + t * a.x_step, a.x_type);
+                v = gd_wide(gd_raw4<TYPE>(a.x, row0 + t * a.x_step));
             else
 #pragma unroll
                 for (int i = 0; i < W - 1; ++i)
@@ -68,16 +73,15 @@ __global__ void __launch_bounds__(CONV_THREADS) k_short_conv(ConvArgs a)
         }
     }
     for (int t = t0; t < t1; t += CONV_AHEAD) {
-        gd_f4 x[CONV_AHEAD];
+        typename GdType<TYPE>::T4 x[CONV_AHEAD]; // (behind the last token: it again)
 #pragma unroll
         for (int i = 0; i < CONV_AHEAD; ++i)
-            if (t + i < t1)
-                x[i] = gd_load4(a.x, row0 + (t + i) * a.x_step, a.x_type);
+            x[i] = gd_raw4<TYPE>(a.x, row0 + min(t + i, t1 - 1) * a.x_step);
 #pragma unroll
         for (int i = 0; i < CONV_AHEAD; ++i) {
             if (t + i >= t1)
                 break;
-            win[W - 1] = x[i];
+            win[W - 1] = gd_wide(x[i]);
             gd_f4 y = bias;
 #pragma unroll
             for (int j = 0; j < W; ++j)
@@ -96,16 +100,15 @@ __global__ void __launch_bounds__(CONV_THREADS) k_short_conv(ConvArgs a)
     }
 }
 
-} // namespace
-
-hipError_t launch_short_conv(const ConvArgs &a, hipStream_t s)
+template <int TYPE>
+hipError_t launch(const ConvArgs &a, hipStream_t s)
 {
     const dim3 grid((unsigned)gd_tiles(a.batch.tokens, a.batch.sequences, CONV_SHIFT),
                     (unsigned)((a.channels / 4 + CONV_THREADS - 1) / CONV_THREADS));
     switch (a.width) {
 #define IHIP_CONV(W)                                                                           \
     case W:                                                                                    \
-        hipLaunchKernelGGL(k_short_conv<W>, grid, dim3(CONV_THREADS), 0, s, a);                \
+        hipLaunchKernelGGL((k_short_conv<TYPE, W>), grid, dim3(CONV_THREADS), 0, s, a);        \
         break;
         IHIP_CONV(2) IHIP_CONV(3) IHIP_CONV(4) IHIP_CONV(5) IHIP_CONV(6) IHIP_CONV(7) IHIP_CONV(8)
 #undef IHIP_CONV
@@ -113,6 +116,13 @@ hipError_t launch_short_conv(const ConvArgs &a, hipStream_t s)
         return hipErrorInvalidValue;
     }
     return hipGetLastError();
+}
+
+} // namespace
+
+hipError_t launch_short_conv(const ConvArgs &a, hipStream_t s)
+{
+    return a.x_type == kF32 ? launch<kF32>(a, s) : a.x_type == kF16 ? launch<kF16>(a, s) : launch<kBF16>(a, s);
 }
 
 } // namespace ihip

@@ -22,7 +22,7 @@ constexpr int STEP_TOKENS = 16; // whose q, k and o a workgroup holds in LDS at 
 // holds 4 columns of R rows, a product with S is summed over the wave's row groups by
 // lane moves, and the tokens follow each other without a barrier.  Bound by the
 // state's bytes for a batch, by three loads that wait for each other for one sequence.
-template <int KD, int VD>
+template <int TYPE, int KD, int VD>
 __global__ void __launch_bounds__(STEP_THREADS) k_delta_step(DeltaArgs a)
 {
     constexpr int CL = VD / 4 / STEP_WAVES; // lanes side by side over a wave's columns
@@ -58,18 +58,19 @@ __global__ void __launch_bounds__(STEP_THREADS) k_delta_step(DeltaArgs a)
         for (int t = wave; t < n; t += STEP_WAVES) {
             const int64_t qa = (first + t) * a.q_step + (int64_t)kh * a.k_dim, ka = (first + t) * a.k_step + (int64_t)kh * a.k_dim;
             constexpr int E = KD / 64;
+            typedef typename GdType<TYPE>::T T;
             float x[E], y[E];
             double xx = 0.0, yy = 0.0, xy = 0.0;
+            T xr[E], yr[E];
 #pragma unroll
             for (int i = 0; i < E; ++i) {
-                const int e = lane * E + i;
-                x[i] = y[i] = 0.0f;
-                if (e < a.k_dim) {
-                    x[i] = a.type == kF32 ? ((const float *)a.q)[qa + e]
-                         : a.type == kF16 ? (float)((const _Float16 *)a.q)[qa + e] : (float)((const __bf16 *)a.q)[qa + e];
-                    y[i] = a.type == kF32 ? ((const float *)a.k)[ka + e]
-                         : a.type == kF16 ? (float)((const _Float16 *)a.k)[ka + e] : (float)((const __bf16 *)a.k)[ka + e];
-                }
+                const int e = min(lane * E + i, a.k_dim - 1);
+                xr[i] = ((const T *)a.q)[qa + e], yr[i] = ((const T *)a.k)[ka + e];
+            }
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                const bool in = lane * E + i < a.k_dim;
+                x[i] = in ? (float)xr[i] : 0.0f, y[i] = in ? (float)yr[i] : 0.0f;
                 xx += (double)x[i] * x[i], yy += (double)y[i] * y[i], xy += (double)x[i] * y[i];
             }
             const double rq = 1.0 / sqrt(gd_wave_sum(xx) + (double)a.l2_eps), rk = 1.0 / sqrt(gd_wave_sum(yy) + (double)a.l2_eps);
@@ -88,7 +89,7 @@ __global__ void __launch_bounds__(STEP_THREADS) k_delta_step(DeltaArgs a)
         }
         __syncthreads();
         for (int t = 0; t < n; ++t) {
-            const gd_f4 v = col0 < a.v_dim ? gd_load4(a.v, (first + t) * a.v_step + (int64_t)h * a.v_dim + col0, a.type) : gd_f4{};
+            const gd_f4 v = col0 < a.v_dim ? gd_wide(gd_raw4<TYPE>(a.v, (first + t) * a.v_step + (int64_t)h * a.v_dim + col0)) : gd_f4{};
             float k[R];
             gd_f4 kS{}, qS{};
 #pragma unroll
@@ -166,20 +167,26 @@ __global__ void __launch_bounds__(STEP_THREADS) k_delta_step(DeltaArgs a)
             *(gd_f4 *)(state + (row0 + i) * a.v_dim + col0) = S[i];
 }
 
-} // namespace
-
-hipError_t launch_delta_step(const DeltaArgs &a, hipStream_t s)
+template <int TYPE>
+void launch(const DeltaArgs &a, hipStream_t s)
 {
     const dim3 grid((unsigned)a.batch.sequences * (unsigned)a.v_heads);
     const bool k64 = a.k_dim <= 64, v64 = a.v_dim <= 64;
     if (k64 && v64)
-        hipLaunchKernelGGL((k_delta_step<64, 64>), grid, dim3(STEP_THREADS), 0, s, a);
+        hipLaunchKernelGGL((k_delta_step<TYPE, 64, 64>), grid, dim3(STEP_THREADS), 0, s, a);
     else if (k64)
-        hipLaunchKernelGGL((k_delta_step<64, 128>), grid, dim3(STEP_THREADS), 0, s, a);
+        hipLaunchKernelGGL((k_delta_step<TYPE, 64, 128>), grid, dim3(STEP_THREADS), 0, s, a);
     else if (v64)
-        hipLaunchKernelGGL((k_delta_step<128, 64>), grid, dim3(STEP_THREADS), 0, s, a);
+        hipLaunchKernelGGL((k_delta_step<TYPE, 128, 64>), grid, dim3(STEP_THREADS), 0, s, a);
     else
-        hipLaunchKernelGGL((k_delta_step<128, 128>), grid, dim3(STEP_THREADS), 0, s, a);
+        hipLaunchKernelGGL((k_delta_step<TYPE, 128, 128>), grid, dim3(STEP_THREADS), 0, s, a);
+}
+
+} // namespace
+
+hipError_t launch_delta_step(const DeltaArgs &a, hipStream_t s)
+{
+    a.type == kF32 ? launch<kF32>(a, s) : a.type == kF16 ? launch<kF16>(a, s) : launch<kBF16>(a, s);
     return hipGetLastError();
 }
 
