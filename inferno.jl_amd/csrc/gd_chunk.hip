@@ -49,6 +49,12 @@ __device__ __forceinline__ void gd_split(gd_f8 x, float by, gd_h8 &hi, gd_h8 &lo
     lo = __builtin_convertvector((x - __builtin_convertvector(hi, gd_f8)) * REST, gd_h8);
 }
 
+// 2^x, x <= 0 (nothing below 2^-126); without a branch
+__device__ __forceinline__ float gd_exp2(double x)
+{
+    return __builtin_amdgcn_exp2f((float)x);
+}
+
 __device__ __forceinline__ gd_f4 gd_mfma(gd_h8 a, gd_h8 b, gd_f4 c)
 {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -71,11 +77,15 @@ __global__ void __launch_bounds__(PREP_THREADS) k_delta_prep(DeltaArgs a)
     constexpr int KS = KD / 32;               // steps of a row of K
     constexpr int FRAG = 4 * KS * PARTS * 1024; // bytes of K or Q
     constexpr int MD = KD / 64;               // 16-row tiles of M that a wave forms
-    constexpr int MATS = 3 * 64 * TRI * 4;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[FRAG > MATS ? FRAG : MATS], tt[2][6][2][1024];
+    // K; then A and its inverse T; then P and T as an operand.  (42 KB: three workgroups
+    // a compute unit.  With each in its own place, 78 KB, there are two.)
+    constexpr int MAT = 64 * TRI * 4, TT = 2 * 6 * 2 * 1024;
+    static_assert(MAT <= TT && FRAG <= MAT + TT, "");
+    __shared__ __attribute__((aligned(16))) uint8_t lds[MAT + TT];
     __shared__ double G[64];
     __shared__ float beta[64], rk[64], fu[64];
-    float *const A = (float *)lds, *const T = A + 64 * TRI, *const P = T + 64 * TRI;
+    float *const A = (float *)lds, *const P = A, *const T = (float *)(lds + MAT);
+    uint8_t(*const tt)[6][2][1024] = (uint8_t(*)[6][2][1024])(lds + MAT);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, r = lane & 15;
     const int h = blockIdx.x % a.v_heads, tile = blockIdx.x / a.v_heads, kh = h / a.group;
     int c = 0;
@@ -155,10 +165,10 @@ __global__ void __launch_bounds__(PREP_THREADS) k_delta_prep(DeltaArgs a)
                 *(gd_h8 *)(work + FRAG + at) = qf[i][p];
             }
         }
-    // the decays' logarithms, summed in 64 bits: differences of them matter
+    // the decays' logarithms, of base 2, summed in 64 bits: differences of them matter
     double sum = 0.0;
     if (lane < n)
-        sum = (double)gd_log_decay(a.decay[h], a.a[(first + lane) * a.a_step + h], a.dt_bias[h]);
+        sum = (double)gd_log_decay(a.decay[h], a.a[(first + lane) * a.a_step + h], a.dt_bias[h]) * 1.4426950408889634;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
         const double up = __shfl_up(sum, d);
@@ -171,7 +181,7 @@ __global__ void __launch_bounds__(PREP_THREADS) k_delta_prep(DeltaArgs a)
     __syncthreads();
 
     if (wave == 0)
-        fu[lane] = rk[lane] * expf((float)(G[63] - G[lane]));
+        fu[lane] = rk[lane] * gd_exp2(G[63] - G[lane]);
     // this wave's columns of K, with the tokens in steps
     gd_h8 kt[MD][2][PARTS];
 #pragma unroll
@@ -228,9 +238,9 @@ __global__ void __launch_bounds__(PREP_THREADS) k_delta_prep(DeltaArgs a)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int at = 16 * wave + 4 * g + i;
-            const float fade = j <= at ? expf((float)(G[at] - G[j])) * rk[j] : 0.0f;
+            const float fade = gd_exp2(j <= at ? G[at] - G[j] : 0.0) * rk[j];
             A[at * TRI + j] = j < at ? beta[at] * rk[at] * fade * kk[t][i] : 0.0f;
-            P[at * TRI + j] = j <= at ? rqs[i] * fade * qk[t][i] : 0.0f;
+            qk[t][i] = j <= at ? rqs[i] * fade * qk[t][i] : 0.0f;
             if (t != wave)
                 T[at * TRI + j] = 0.0f;
         }
@@ -281,7 +291,12 @@ __global__ void __launch_bounds__(PREP_THREADS) k_delta_prep(DeltaArgs a)
     // they are and once times the factors of what is written to the state.  fu and K's
     // power of two are 1 together, so fu alone is below 2^-TOP.
     constexpr float UP = 1 << TOP, BACK = 1.0f / UP;
-    for (int t = wave; t < 6; t += PREP_THREADS / 64) {
+    gd_h8 to_t[2][2], to_f[2][2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const int t = wave + 4 * u;
+        if (t >= 6)
+            continue;
         const int jt = t < 4 ? t / 2 : t - 2, k = t < 4 ? t % 2 : 1, j = 16 * jt + r;
         gd_f8 x, y;
 #pragma unroll
@@ -290,14 +305,26 @@ __global__ void __launch_bounds__(PREP_THREADS) k_delta_prep(DeltaArgs a)
             x[i] = T[at * TRI + j] * beta[j];
             y[i] = x[i] * (fu[at] * UP);
         }
-        gd_h8 hi, lo;
-        gd_split(x, UP, hi, lo);
-        *(gd_h8 *)(tt[0][t][0] + lane * 16) = hi;
-        *(gd_h8 *)(tt[0][t][1] + lane * 16) = lo;
-        gd_split(y, UP, hi, lo);
-        *(gd_h8 *)(tt[1][t][0] + lane * 16) = hi;
-        *(gd_h8 *)(tt[1][t][1] + lane * 16) = lo;
+        gd_split(x, UP, to_t[u][0], to_t[u][1]);
+        gd_split(y, UP, to_f[u][0], to_f[u][1]);
     }
+    __syncthreads(); // A and T are read
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+            const int t = wave + 4 * u;
+            if (t >= 6)
+                continue;
+            *(gd_h8 *)(tt[0][t][p] + lane * 16) = to_t[u][p];
+            *(gd_h8 *)(tt[1][t][p] + lane * 16) = to_f[u][p];
+        }
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+        if (t <= (wave | 1))
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                P[(16 * wave + 4 * g + i) * TRI + 16 * t + r] = qk[t][i];
     __syncthreads();
     // P and M, transposed (T^T times the other matrix's transpose), so that a lane holds
     // the columns of a row that it stores as a fragment
@@ -362,12 +389,12 @@ __global__ void __launch_bounds__(PREP_THREADS) k_delta_prep(DeltaArgs a)
     }
     float *const f = (float *)(a.work + a.plan.rows) + unit * kDeltaRows;
     if (wave == 0) {
-        f[lane] = rk[lane] * expf((float)G[lane]); // of K S
+        f[lane] = rk[lane] * gd_exp2(G[lane]); // of K S
         if (lane == 0)
-            f[128] = expf((float)G[63]);
+            f[128] = gd_exp2(G[63]);
     }
     if (g == 0)
-        f[64 + row] = rq * expf((float)G[row]); // of Q S
+        f[64 + row] = rq * gd_exp2(G[row]); // of Q S
 }
 
 // ---- down the chunks ---------------------------------------------------------------
