@@ -397,8 +397,11 @@ __device__ __forceinline__ int first_passing(double sum, double before, double w
     return at;
 }
 
+// (The slice comes to its threads through LDS: read as neighbours to a thread, it costs a
+// cache line a logit, 4 us of 12.)
+constexpr int STAGED = kSampleWide + kSampleWide / 16;
 __device__ void pick(const SampleArgs &a, int row, const SampleRow &r, const SampleScale &sc, unsigned long long best, uint32_t fl,
-                     double sum, double total, unsigned long long border, double low, PickLds &lds)
+                     double sum, double total, unsigned long long border, double low, PickLds &lds, float *staged)
 {
     const int tid = threadIdx.x, lane = tid & 63;
     const int64_t base = row * a.row_step;
@@ -413,28 +416,42 @@ __device__ void pick(const SampleArgs &a, int row, const SampleRow &r, const Sam
     const double want = sample_u(r.u) * wg_scan(sum, lds.part, before);
     const int slice = max(first_passing(sum, before, want, lds), 0);
     double run = lds.before;
+    constexpr int MOST = kSampleWide / ROW_THREADS;
     const int share = a.plan.per / ROW_THREADS; // neighbours
     const int begin = slice * a.plan.per, end = min(begin + a.plan.per, a.vocab);
-    sum = 0.0;
-    for (int e0 = 0; e0 < share; e0 += 8) {
-        float l[8];
+    {
+        // (one look at the type for all loads: beside each, they would wait for each other)
+        uint32_t bits[MOST];
+        if (a.type == kF32) {
+            const uint32_t *const l = (const uint32_t *)a.logits + base;
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            l[e] = sample_logit(a.logits, base + min(begin + tid * share + e0 + e, end - 1), a.type);
+            for (int e = 0; e < MOST; ++e)
+                bits[e] = l[min(begin + e * ROW_THREADS + tid, end - 1)];
+        } else {
+            const uint16_t *const l = (const uint16_t *)a.logits + base;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int i = begin + tid * share + e0 + e;
-            sum += i < end ? weight(i, l[e]) : 0.0;
+            for (int e = 0; e < MOST; ++e)
+                bits[e] = l[min(begin + e * ROW_THREADS + tid, end - 1)];
         }
+#pragma unroll
+        for (int e = 0; e < MOST; ++e)
+            staged[e * ROW_THREADS + tid + (e * ROW_THREADS + tid) / 16] =
+                a.type == kF32 ? __uint_as_float(bits[e]) : a.type == kF16 ? h2f(bits[e]) : __uint_as_float(bits[e] << 16);
+    }
+    __syncthreads();
+    sum = 0.0;
+#pragma unroll 4
+    for (int e = 0; e < share; ++e) {
+        const int i = tid * share + e;
+        sum += begin + i < end ? weight(begin + i, staged[i + i / 16]) : 0.0;
     }
     wg_scan(sum, lds.part, before);
     const int owner = first_passing(sum, run + before, want, lds);
     if (tid >= 64)
         return;
     run = lds.before;
-    const int i = begin + max(owner, 0) * share + lane;
-    const float l = sample_logit(a.logits, base + min(i, end - 1), a.type);
-    const double w = owner >= 0 && lane < share && i < end ? weight(i, l) : 0.0;
+    const int in = max(owner, 0) * share + min(lane, share - 1), i = begin + in;
+    const double w = owner >= 0 && lane < share && i < end ? weight(i, staged[in + in / 16]) : 0.0;
     double upto = w;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
@@ -524,6 +541,7 @@ __global__ void __launch_bounds__(ROW_THREADS) k_sample_join(SampleArgs a)
     __shared__ unsigned long long wbest[ROW_WAVES];
     __shared__ uint32_t wfl[ROW_WAVES];
     __shared__ PickLds lds;
+    __shared__ float staged[STAGED];
     const int rr = blockIdx.x, row = a.row0 + rr, tid = threadIdx.x;
     const SampleRow r = sample_row(a, row);
     unsigned long long best;
@@ -539,7 +557,7 @@ __global__ void __launch_bounds__(ROW_THREADS) k_sample_join(SampleArgs a)
         const Part p = parts_of(a, rr)[tid];
         sum = p.sum > 0.0 ? p.sum * sample_weight(sc, sample_value((uint32_t)(p.best >> 32))) : 0.0;
     }
-    pick(a, row, r, sc, best, fl, sum, wg_sum(sum, lds.part), 0, 0.0, lds);
+    pick(a, row, r, sc, best, fl, sum, wg_sum(sum, lds.part), 0, 0.0, lds, staged);
 }
 
 // With top-k or top-p: the tokens and weights of every bin of a slice ...
@@ -759,13 +777,14 @@ __global__ void __launch_bounds__(ROW_THREADS) k_sample_list(SampleArgs a)
 
 // ... which are put in order and cut; then the token.
 struct ListLds {
-    unsigned long long order[kSampleList], mass[kSampleSlices];
+    unsigned long long order[kSampleList], masses[kSampleList], mass[kSampleSlices];
 };
 __global__ void __launch_bounds__(ROW_THREADS) k_sample_pick(SampleArgs a)
 {
     __shared__ union {
         ListLds list;
         RowLds row;
+        float staged[STAGED]; // (the list is used up by then)
     } u;
     __shared__ PickLds lds;
     __shared__ unsigned long long upart[ROW_WAVES];
@@ -773,12 +792,15 @@ __global__ void __launch_bounds__(ROW_THREADS) k_sample_pick(SampleArgs a)
     __shared__ int first_k, kept;
     const int rr = blockIdx.x, row = a.row0 + rr, tid = threadIdx.x;
     const SampleRow r = sample_row(a, row);
-    bool by_k, by_p;
-    Bounds bo{};
-    const bool cut_row = filtered(r, a.vocab, by_k, by_p);
-    if (cut_row)
-        bo = *bounds_of(a, rr); // (not looked at where the row is not weighed)
+    // (loaded together, before it is known whether they are looked at)
+    const unsigned long long *const list = (const unsigned long long *)(a.work + a.plan.list) + (int64_t)rr * kSampleList;
+    const unsigned long long early = list[tid];
+    Bounds bo = *bounds_of(a, rr);
     double sum = tid < a.plan.slices ? parts_of(a, rr)[tid].sum : 0.0;
+    bool by_k, by_p;
+    const bool cut_row = filtered(r, a.vocab, by_k, by_p);
+    if (!cut_row)
+        bo.listed = 0;
     unsigned long long best;
     uint32_t fl;
     row_best(a, rr, best, fl, upart, wfl);
@@ -798,13 +820,12 @@ __global__ void __launch_bounds__(ROW_THREADS) k_sample_pick(SampleArgs a)
     unsigned long long from = 0; // the last kept token, in the order of best_of
     if (cut_row && bo.whole < kSampleBins) {
         // the listed tokens in order, the first first; 0 behind them
-        const unsigned long long *const list = (const unsigned long long *)(a.work + a.plan.list) + (int64_t)rr * kSampleList;
         int size = 2;
         while (size < n)
             size *= 2;
         unsigned long long *const order = u.list.order;
         for (int i = tid; i < size; i += ROW_THREADS)
-            order[i] = i < n ? list[i] : 0;
+            order[i] = i < n ? (i < ROW_THREADS ? early : list[i]) : 0;
         for (int i = tid; i < kSampleSlices; i += ROW_THREADS)
             u.list.mass[i] = 0;
         __syncthreads();
@@ -819,42 +840,42 @@ __global__ void __launch_bounds__(ROW_THREADS) k_sample_pick(SampleArgs a)
                 __syncthreads();
             }
         // neighbours to a thread; the weights of those before
-        constexpr int E = kSampleList / ROW_THREADS;
-        unsigned long long o[E], m[E], mine = 0, before = 0;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            o[e] = E * tid + e < n ? order[E * tid + e] : 0;
-            m[e] = by_p && o[e] ? sample_mass(sc, sample_value((uint32_t)(o[e] >> 32))) : 0;
-            mine += m[e];
-        }
+        const int each = (n + ROW_THREADS - 1) / ROW_THREADS, at0 = each * tid, at1 = min(at0 + each, n);
+        unsigned long long *const masses = u.list.masses;
+        unsigned long long mine = 0, before = 0;
+        if (by_p)
+#pragma unroll 1
+            for (int i = at0; i < at1; ++i)
+                mine += masses[i] = sample_mass(sc, sample_value((uint32_t)(order[i] >> 32)));
         int cut = n; // kept by top-k: those before it
         unsigned long long left = bo.all;
         if (bo.k < kSampleBins) {
             // (bin k's tokens are the last ones)
             int ahead = 0;
-#pragma unroll
-            for (int e = 0; e < E; ++e)
-                ahead += o[e] && bin_of(sample_value((uint32_t)(o[e] >> 32)), most, rate) != bo.k;
+#pragma unroll 1
+            for (int i = at0; i < at1; ++i)
+                ahead += bin_of(sample_value((uint32_t)(order[i] >> 32)), most, rate) != bo.k;
             const int2 at = first_and_last(false, ahead > 0, lds.first, lds.last);
             if (tid == max(at.y, 0))
-                first_k = at.y < 0 ? 0 : E * tid + ahead;
+                first_k = at.y < 0 ? 0 : at0 + ahead;
             __syncthreads();
             cut = first_k + (r.k - (int)bo.k_count);
             unsigned long long in_k = 0;
-#pragma unroll
-            for (int e = 0; e < E; ++e)
-                in_k += E * tid + e >= first_k && E * tid + e < cut ? m[e] : 0;
+            if (by_p)
+#pragma unroll 1
+                for (int i = max(at0, first_k); i < min(at1, cut); ++i)
+                    in_k += masses[i];
             left = bo.k_over + wg_scan(in_k, upart, before);
         }
         wg_scan(mine, upart, before);
         const double want = (double)fmaxf(r.p, 0.0f) * (double)left;
         unsigned long long over = bo.p_over + before;
         int last = 0;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            if (o[e] && E * tid + e < cut && (!by_p || (double)over < want || o[e] == best))
-                last = E * tid + e + 1;
-            over += m[e];
+#pragma unroll 1
+        for (int i = at0; i < min(at1, cut); ++i) {
+            if (!by_p || (double)over < want || order[i] == best)
+                last = i + 1;
+            over += by_p ? masses[i] : 0;
         }
         const int2 at = first_and_last(false, last > 0, lds.first, lds.last);
         if (tid == max(at.y, 0))
@@ -862,21 +883,20 @@ __global__ void __launch_bounds__(ROW_THREADS) k_sample_pick(SampleArgs a)
         __syncthreads();
         from = kept ? order[kept - 1] : best;
         double w = 0.0;
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-            if (E * tid + e < kept) {
-                double x = sample_weight(sc, sample_value((uint32_t)(o[e] >> 32)));
-                x = x >= low || o[e] == best ? x : 0.0;
-                w += x;
-                // (to their slices as whole numbers: in any order)
-                if (x > 0.0)
-                    atomicAdd(&u.list.mass[~(uint32_t)o[e] / (uint32_t)a.plan.per], (unsigned long long)rint(ldexp(x, sc.bits)));
-            }
+#pragma unroll 1
+        for (int i = at0; i < min(at1, kept); ++i) {
+            double x = sample_weight(sc, sample_value((uint32_t)(order[i] >> 32)));
+            x = x >= low || order[i] == best ? x : 0.0;
+            w += x;
+            // (to their slices as whole numbers: in any order)
+            if (x > 0.0)
+                atomicAdd(&u.list.mass[~(uint32_t)order[i] / (uint32_t)a.plan.per], (unsigned long long)rint(ldexp(x, sc.bits)));
+        }
         total += wg_sum(w, lds.part);
         if (tid < a.plan.slices)
             sum += ldexp((double)u.list.mass[tid], -sc.bits);
     }
-    pick(a, row, r, sc, best, fl, sum, total, from, low, lds);
+    pick(a, row, r, sc, best, fl, sum, total, from, low, lds, u.staged);
 }
 
 template <int TYPE, int N>
