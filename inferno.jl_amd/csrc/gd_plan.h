@@ -10,7 +10,6 @@ namespace ihip {
 
 constexpr int kDeltaChunk = 64;  // tokens of a chunk
 constexpr int kDeltaShift = 6;
-constexpr int kDeltaStepMost = 16; // new tokens up to which a sequence goes a token at a time
 constexpr int kDeltaTri = 6 * 2 * 1024; // a 64 x 64 lower triangle: 6 tiles of 16 x 32 in two fp16 parts
 constexpr int kDeltaRows = 192;  // floats of a chunk's row factors
 
@@ -20,8 +19,23 @@ constexpr int64_t gd_tiles(int64_t tokens, int64_t sequences, int shift)
     return (tokens > 0 ? (tokens - 1) >> shift : 0) + sequences;
 }
 
+// New tokens up to which a sequence goes a token at a time.  A token costs the step
+// kernel 1.4 us whatever the batch, until that fills the chip; a chunk costs its
+// kernels the same with few tokens as with 64, and every chunk of the batch adds to it.
+// Measured on sequences of equally many tokens, 32 heads of 128 x 128 in bf16, the two are even
+// at 11 tokens for one sequence (12: 24.7 us by steps, 23.1 by chunks; 8: 18.3, 22.4), 17 for
+// two (16: 28.9, 30.6; 20: 34.9, 31.6), 28 for four (24: 39.5, 44.3; 32: 49.6, 45.4) and 41
+// for eight (32: 54.8, 69.3; 48: 79.7, 71.8).  Beyond 32 is left to the chunks: of a
+// batch of many lengths the step kernel's time is the longest one's.
+constexpr int delta_few(int v_heads, int64_t sequences)
+{
+    const int64_t few = sequences * v_heads / 4;
+    return few < 10 ? 10 : few > 32 ? 32 : (int)few;
+}
+
 struct DeltaPlan {
-    bool chunks;     // some sequence may have more new tokens than kDeltaStepMost
+    int few;         // delta_few
+    bool chunks;     // some sequence may have more new tokens
     bool steps;      // some may have fewer beside it
     int64_t tiles;   // numbers of chunks
     int frag;        // bytes of a chunk's K or Q of one head
@@ -34,7 +48,8 @@ inline DeltaPlan delta_plan(int parts, int k_heads, int v_heads, int k_dim, int 
 {
     DeltaPlan p{};
     const int64_t longest = most > 0 && most < tokens ? most : tokens;
-    p.chunks = longest > kDeltaStepMost;
+    p.few = delta_few(v_heads, sequences);
+    p.chunks = longest > p.few;
     p.steps = !p.chunks || sequences > 1;
     if (!p.chunks)
         return p;

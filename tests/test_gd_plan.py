@@ -57,10 +57,11 @@ def test_areas_of_the_delta_rule(lib):
         parts, k_heads, group = rng.choice([1, 2]), rng.randint(1, 20), rng.randint(1, 5)
         dk, dv = 16 * rng.randint(1, 8), 16 * rng.randint(1, 8)
         tokens, sequences = int(2 ** rng.uniform(0, 14)), rng.randint(1, 80)
-        most = rng.choice([0, 1, 16, 17, tokens])
+        few = min(max(sequences * k_heads * group // 4, 10), 32)
+        most = rng.choice([0, 1, 10, 11, few, few + 1, tokens])
         p = delta(lib, parts, k_heads, k_heads * group, dk, dv, tokens, sequences, most)
         longest = min(most or tokens, tokens)
-        assert bool(p["chunks"]) == (longest > 16) and bool(p["steps"]) == (longest <= 16 or sequences > 1)
+        assert bool(p["chunks"]) == (longest > few) and bool(p["steps"]) == (longest <= few or sequences > 1)
         if not p["chunks"]:
             assert p["bytes"] == 0
             continue

@@ -117,6 +117,14 @@ def test_epilogues(kind, gate, norm):
         c.check(c.run(), c.plain())
 
 
+@pytest.mark.parametrize("H", [1, 6, 16])
+def test_lengths_beside_the_ones_that_go_a_token_at_a_time(H):
+    """Up to 10 tokens where heads and sequences are few, up to 32 where they are many."""
+    new = [9, 10, 11, 12, 15, 16, 31, 32, 33, 34]
+    c = Case(H, new, [i % 2 == 0 for i in range(len(new))], K=1, H=H, dk=64, dv=32)
+    c.check(c.run(), c.plain())
+
+
 @pytest.mark.parametrize("most", [1, 4, 16, 17, 200, 1 << 20])
 def test_any_hint_gives_the_same_results(most):
     """`most` chooses kernels; the states of either way are the same to rounding."""
