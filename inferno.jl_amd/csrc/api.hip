@@ -1955,7 +1955,7 @@ int ihip_gated_delta_dev(const void *q, int64_t q_stride, const void *k, int64_t
     d.q = q, d.k = k, d.v = v, d.type = type, d.q_step = q_stride, d.k_step = k_stride, d.v_step = v_stride;
     d.a = a, d.b = b, d.a_step = a_stride, d.b_step = b_stride, d.gate = gate, d.gate_step = gate_stride;
     d.out = out, d.out_type = out_type, d.flags = flags;
-    d.few = d.plan.chunks ? (d.plan.steps ? d.plan.few : 0) : -1;
+    d.few = d.plan.chunks ? d.plan.few : -1;
     d.work = (uint8_t *)workspace;
     d.raw = out_type == kF32 ? (float *)out : (d.norm_w || gate) ? (float *)(d.work + d.plan.raw) : nullptr;
     hipError_t e = d.plan.steps ? launch_delta_step(d, (hipStream_t)stream) : hipSuccess;

@@ -19,23 +19,31 @@ constexpr int64_t gd_tiles(int64_t tokens, int64_t sequences, int shift)
     return (tokens > 0 ? (tokens - 1) >> shift : 0) + sequences;
 }
 
-// New tokens up to which a sequence goes a token at a time.  A token costs the step
+// New tokens up to which a batch goes a token at a time, all of it.  A token costs the step
 // kernel 1.4 us whatever the batch, until that fills the chip; a chunk costs its
 // kernels the same with few tokens as with 64, and every chunk of the batch adds to it.
 // Measured on sequences of equally many tokens, 32 heads of 128 x 128 in bf16, the two are even
 // at 11 tokens for one sequence (12: 24.7 us by steps, 23.1 by chunks; 8: 18.3, 22.4), 17 for
 // two (16: 28.9, 30.6; 20: 34.9, 31.6), 28 for four (24: 39.5, 44.3; 32: 49.6, 45.4) and 41
-// for eight (32: 54.8, 69.3; 48: 79.7, 71.8).  Beyond 32 is left to the chunks: of a
-// batch of many lengths the step kernel's time is the longest one's.
+// for eight (32: 54.8, 69.3; 48: 79.7, 71.8).
 constexpr int delta_few(int v_heads, int64_t sequences)
 {
     const int64_t few = sequences * v_heads / 4;
     return few < 10 ? 10 : few > 32 ? 32 : (int)few;
 }
 
+// Beside longer sequences, the step kernel comes before the chunks' and lasts as long as
+// its longest sequence, and chunks that do not fill the chip are next to free: there
+// only a few tokens go by steps (sequences of 22, 8, 135, 5 and 72 tokens, 24 heads of
+// 64 x 64: 30.0 us with up to 4, 36.0 with up to 10, 47 with up to 30).
+constexpr int delta_few_beside(int v_heads, int64_t sequences)
+{
+    return sequences * v_heads < 256 ? 4 : 10;
+}
+
 struct DeltaPlan {
-    int few;         // delta_few
-    bool chunks;     // some sequence may have more new tokens
+    int few;         // new tokens up to which a sequence goes a token at a time, where others take chunks
+    bool chunks;     // some sequence may have more new tokens than delta_few
     bool steps;      // some may have fewer beside it
     int64_t tiles;   // numbers of chunks
     int frag;        // bytes of a chunk's K or Q of one head
@@ -48,9 +56,9 @@ inline DeltaPlan delta_plan(int parts, int k_heads, int v_heads, int k_dim, int 
 {
     DeltaPlan p{};
     const int64_t longest = most > 0 && most < tokens ? most : tokens;
-    p.few = delta_few(v_heads, sequences);
-    p.chunks = longest > p.few;
+    p.chunks = longest > delta_few(v_heads, sequences);
     p.steps = !p.chunks || sequences > 1;
+    p.few = p.steps ? delta_few_beside(v_heads, sequences) : 0;
     if (!p.chunks)
         return p;
     p.tiles = gd_tiles(tokens, sequences, kDeltaShift);

@@ -119,10 +119,11 @@ def test_epilogues(kind, gate, norm):
 
 @pytest.mark.parametrize("H", [1, 6, 16])
 def test_lengths_beside_the_ones_that_go_a_token_at_a_time(H):
-    """Up to 10 tokens where heads and sequences are few, up to 32 where they are many."""
-    new = [9, 10, 11, 12, 15, 16, 31, 32, 33, 34]
-    c = Case(H, new, [i % 2 == 0 for i in range(len(new))], K=1, H=H, dk=64, dv=32)
-    c.check(c.run(), c.plain())
+    """Up to 4 or 10 beside longer ones; alone up to 10 to 32, by the numbers of heads and sequences."""
+    for new in ([3, 4, 5, 33] * 5, [9, 10, 11, 12, 15, 16, 31, 32, 33, 34], [9, 10, 1], [9, 1, 11], [32, 31, 9, 10, 11, 1, 2, 8], [33, 32]):
+        c = Case(H, new, [i % 2 == 0 for i in range(len(new))], K=1, H=H, dk=64, dv=32)
+        c.check(c.run(), c.plain())
+        c.check(c.run(most=max(new)), c.plain())
 
 
 @pytest.mark.parametrize("most", [1, 4, 16, 17, 200, 1 << 20])
@@ -221,7 +222,7 @@ def test_a_nan_stays_in_its_head_and_sequence(new):
     where = c.starts[1] + new[1] - 1  # the second sequence's last token, first head of v
     c.qkv[where, 2 * c.K * 64 + 3] = float("nan")
     out, state, _ = c.run()
-    chunk = c.starts[1] + (new[1] - 1) // 64 * 64 if new[1] > 16 else where
+    chunk = c.starts[1] + (new[1] - 1) // 64 * 64  # (the 64 that go together share it)
     assert gd_plain.off(out[:chunk], y[:chunk]) <= gd_plain.NEAR
     assert gd_plain.off(out[:, 1:], y[:, 1:]) <= gd_plain.NEAR
     assert bool(torch.isnan(out[where, 0, 3])) and bool(torch.isnan(state[c.slots[1], 0, :, 3]).all())
