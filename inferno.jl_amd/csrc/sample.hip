@@ -564,8 +564,11 @@ __global__ void __launch_bounds__(ROW_THREADS) k_sample_join(SampleArgs a)
 template <int TYPE, int N>
 __global__ void __launch_bounds__(ROW_THREADS) k_sample_bins(SampleArgs a)
 {
-    __shared__ unsigned long long mass[kSampleBins];
-    __shared__ uint32_t count[kSampleBins];
+    // (bins in two copies, by lane, where neighbouring tokens' atomics meet less often: 61
+    // rows 18.9 us, one copy 21.6, four 19.6)
+    constexpr int COPIES = 2;
+    __shared__ unsigned long long mass[COPIES * kSampleBins];
+    __shared__ uint32_t count[COPIES * kSampleBins];
     __shared__ unsigned long long wbest[ROW_WAVES];
     __shared__ uint32_t wfl[ROW_WAVES];
     const int slice = blockIdx.x % a.plan.slices, rr = blockIdx.x / a.plan.slices, row = a.row0 + rr, tid = threadIdx.x;
@@ -574,8 +577,9 @@ __global__ void __launch_bounds__(ROW_THREADS) k_sample_bins(SampleArgs a)
     if (!filtered(r, a.vocab, by_k, by_p) || !(r.t > 0.0f))
         return;
     const Slice<TYPE, N> x(a, row, slice);
-    for (int i = tid; i < kSampleBins; i += ROW_THREADS)
+    for (int i = tid; i < COPIES * kSampleBins; i += ROW_THREADS)
         mass[i] = 0, count[i] = 0;
+    const int copy = tid % COPIES;
     unsigned long long best;
     uint32_t fl;
     row_best(a, rr, best, fl, wbest, wfl);
@@ -593,24 +597,29 @@ __global__ void __launch_bounds__(ROW_THREADS) k_sample_bins(SampleArgs a)
             continue;
         far += b == kSampleBins - 1;
         if (by_k && b < kSampleBins - 1)
-            atomicAdd(&count[b], 1u);
+            atomicAdd(&count[b * COPIES + copy], 1u);
         if (by_p) {
             const unsigned long long m = sample_mass(sc, x.l[j]);
             if (m)
-                atomicAdd(&mass[b], m);
+                atomicAdd(&mass[b * COPIES + copy], m);
         }
     }
     if (by_k && far)
-        atomicAdd(&count[kSampleBins - 1], far);
+        atomicAdd(&count[(kSampleBins - 1) * COPIES + copy], far);
     __syncthreads();
     unsigned long long *const all_mass =
         (unsigned long long *)(a.work + a.plan.bins + ((int64_t)rr * a.plan.slices + slice) * (kSampleBins * 12));
     uint32_t *const all_count = (uint32_t *)(all_mass + kSampleBins);
     for (int i = tid; i < kSampleBins; i += ROW_THREADS) {
+        unsigned long long m = 0;
+        uint32_t c = 0;
+#pragma unroll
+        for (int k = 0; k < COPIES; ++k)
+            m += mass[i * COPIES + k], c += count[i * COPIES + k];
         if (by_p)
-            all_mass[i] = mass[i];
+            all_mass[i] = m;
         if (by_k)
-            all_count[i] = count[i];
+            all_count[i] = c;
     }
 }
 
