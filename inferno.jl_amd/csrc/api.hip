@@ -697,6 +697,9 @@ bool in_pools(const KvCache &c, const void *p, size_t bytes)
 // A launch of `units` workgroups fits a grid.
 bool grid_fits(int64_t units) { return units <= (int64_t)INT32_MAX; }
 
+// A launch of `units` workgroups of 256 threads does: those are counted in 32 bits.
+bool threads_fit(int64_t units) { return units < 1 << 24; }
+
 // ---- layers that keep a state ---------------------------------------------------
 int check_states(const ihip_state_batch *b, StateBatch *out)
 {
@@ -1863,6 +1866,8 @@ int ihip_short_conv_dev(const void *x, int x_type, int64_t x_stride, const float
         return IHIP_OK; // (an empty buffer has no address to check)
     if (!x || !w || !state || !out)
         return fail(IHIP_ERR_INVALID, "null pointer");
+    if (!threads_fit(gd_tiles(T, a.batch.sequences, kConvShift)))
+        return fail(IHIP_ERR_INVALID, "%lld tokens of %d sequences are too many for one call", (long long)T, a.batch.sequences);
     if (!step_fits(x_stride, channels, T, 8))
         return fail(IHIP_ERR_INVALID, "x_stride=%lld is no multiple of 8 that holds %d channels", (long long)x_stride, channels);
     if (!al16(x) || !al16(w) || !al16(bias) || !al16(state) || !al16(out))
@@ -1925,7 +1930,8 @@ int ihip_gated_delta_dev(const void *q, int64_t q_stride, const void *k, int64_t
         return fail(IHIP_ERR_INVALID, "a stride does not hold a token's heads, or is no multiple of 8 (q, k, v) or 4 (gate)");
     if (!al16(q) || !al16(k) || !al16(v) || !al16(gate) || !al16(out) || ((uintptr_t)a & 3) || ((uintptr_t)b & 3))
         return fail(IHIP_ERR_INVALID, "a pointer is not 16-byte aligned (a, b: 4)");
-    if (!grid_fits((T + S) * d.v_heads) || T * vw > INT64_MAX / 8)
+    // (of a head's columns 16 a workgroup: up to 8, and the sequences' heads in eights)
+    if (!threads_fit((S + 8) * d.v_heads * 8) || !threads_fit(gd_tiles(T, S, kDeltaShift) * d.v_heads))
         return fail(IHIP_ERR_INVALID, "%lld tokens and %lld sequences of %d heads are too many for one call", (long long)T,
                     (long long)S, d.v_heads);
     const Span to = rows_of(out, T, vw, vw, value_bytes(out_type));
@@ -1940,8 +1946,6 @@ int ihip_gated_delta_dev(const void *q, int64_t q_stride, const void *k, int64_t
         if (!apart(in, to) || !apart(in, held))
             return fail(IHIP_ERR_INVALID, "out or state overlaps another buffer");
     d.plan = delta_plan(type == kF32 ? 2 : 1, d.k_heads, d.v_heads, d.k_dim, d.v_dim, T, S, batch->most);
-    if (!grid_fits(d.plan.tiles * d.v_heads))
-        return fail(IHIP_ERR_INVALID, "%lld tokens of %d heads are too many for one call", (long long)T, d.v_heads);
     if (d.plan.bytes) {
         const Span work{workspace, d.plan.bytes};
         if (!workspace || workspace_bytes < d.plan.bytes || !al16(workspace))

@@ -8,8 +8,8 @@
 
 namespace ihip {
 
-constexpr int kDeltaChunk = 64;  // tokens of a chunk
-constexpr int kDeltaShift = 6;
+constexpr int kDeltaShift = 6;  // a chunk is 64 tokens
+constexpr int kConvShift = 5;   // a tile of the short convolution is 32
 constexpr int kDeltaTri = 6 * 2 * 1024; // a 64 x 64 lower triangle: 6 tiles of 16 x 32 in two fp16 parts
 constexpr int kDeltaRows = 192;  // floats of a chunk's row factors
 

@@ -113,6 +113,14 @@ def test_rows_of_no_logits_are_an_error_of_their_own():
     assert sample(vocab=0) == _lib.IHIP_ERR_EMPTY and said()
 
 
+def test_more_workgroups_than_a_launch_has():
+    for b in (batch(sequences=1 << 24), batch(tokens=(1 << 30) - 1), batch(sequences=1 << 29)):
+        assert conv(b) == _lib.IHIP_ERR_INVALID and b"too many" in said()
+        assert delta(b) == _lib.IHIP_ERR_INVALID and b"too many" in said()
+    b = batch(sequences=1 << 19)  # 4 heads, up to 8 workgroups a head
+    assert delta(b) == _lib.IHIP_ERR_INVALID and b"too many" in said()
+
+
 def test_nothing_to_do_needs_no_buffers():
     for b in (batch(tokens=0, q_starts=None, slots=None, kv_lens=None), batch(sequences=0, q_starts=None, slots=None)):
         assert conv(b, x=None, w=None, state=None, out=None) == _lib.IHIP_OK
