@@ -70,6 +70,12 @@ __device__ __forceinline__ gd_f4 gd_mfma(gd_h8 a, gd_h8 b, gd_f4 c)
 constexpr int PREP_THREADS = 256;
 constexpr int TRI = 68; // floats from a row of a 64 x 64 matrix to the next, in LDS
 
+// A workgroup takes a chunk of a head of v; a wave 16 of its rows.  k's and q's products
+// and P and M are on the fp16 matrix cores, the inverse in fp32: 16 x 16 blocks on the diagonal
+// by substitution, the ones below from those on the fp32 matrix cores.  Heads that share
+// K and Q form them again each (their rows are in L2), and one writes them.  8192 tokens of 32
+// heads of 128 on 16, bf16: 107 us for 67 MB in and 252 out (P and M 185 of them), 3.0 TB/s;
+// 163 with two workgroups a CU instead of three and loads that wait for each other.
 template <int TYPE, int KD>
 __global__ void __launch_bounds__(PREP_THREADS) k_delta_prep(DeltaArgs a)
 {
@@ -421,8 +427,12 @@ __device__ __forceinline__ void scan_sync()
 // tokens 16 w .. 16 w + 15 of a chunk and the rows 32 w .. 32 w + 31 of S (there are
 // KD / 32 such waves).  A wave so reads only its own part of the operands, from memory
 // into registers, two chunks ahead, and the waves exchange S and X as fp16 fragments in LDS,
-// with two barriers a chunk.  Bound by that chain, not by
-// bytes or products: a chunk follows the other.
+// with two barriers a chunk.  Bound by that chain, as a chunk follows the other: 8192
+// tokens of 32 heads of 128 x 128 take 282 us, 2.2 a chunk on every CU, of which the
+// products, exchanges and barriers alone are 1.2 and the operands' way (76 KB a chunk and CU)
+// adds 0.6 from L2 and 0.4 from further away.  (One chunk ahead 322, three 274, with registers that
+// let one workgroup on a CU where sequences would give it two; 32 columns a workgroup, which halves
+// the bytes and the CUs in use, 385.)
 //
 // One power of two serves a column for a whole chunk.  k and q have unit length at most,
 // and no token adds more than |v| to the length of a column of S, so |X| and the
@@ -683,7 +693,9 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
 // ---- the output norm ---------------------------------------------------------------
 constexpr int NORM_THREADS = 256;
 
-// raw -> out: 32 lanes a row of a head (4 columns each), 64 rows of a sequence.
+// raw -> out: 32 lanes a row of a head (4 columns each), 64 rows of a sequence.  (The
+// scan's workgroups hold 16 columns each and no row's norm.)  Bound by bytes: 8192 tokens of
+// 32 heads of 128, raw and gate fp32, bf16 out: 75 us for 336 MB, 4.5 TB/s.
 __global__ void __launch_bounds__(NORM_THREADS) k_delta_norm(DeltaArgs a)
 {
     int c = 0;

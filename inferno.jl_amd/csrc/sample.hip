@@ -214,7 +214,12 @@ __device__ void sample_whole_row(const SampleArgs &a, int row, const SampleRow &
 // ---- rows in slices ------------------------------------------------------------
 // A row's slices go to workgroups all over the chip, and what they find to one that
 // joins them, a launch later (a launch costs what a count of ended workgroups, and
-// reads past the caches, would).
+// reads past the caches, would).  One row of 151936 fp32 logits, us: best 3.2, bins 6, merge 3.2,
+// bounds 4.3, list 5.8, pick 12; bound by these launches and the loads and sums that
+// follow each other in them (the logits are 0.1 at the rate of reads).  61 rows of bf16
+// with mixed filters: 6.4, 18.9, 4.7, 4.6, 14.9, 24.5; bound by atomics to shared bins,
+// 64-bit weights and the longest of the rows' lists.  256 rows of fp32 without filters: best 50
+// (156 MB, 3.1 TB/s: 20 operations in 64 bits a weight beside its load), join 12.
 
 struct Part { // of a slice
     unsigned long long best; // the largest logit (its key, then ~place)
