@@ -1866,7 +1866,8 @@ int ihip_short_conv_dev(const void *x, int x_type, int64_t x_stride, const float
         return IHIP_OK; // (an empty buffer has no address to check)
     if (!x || !w || !state || !out)
         return fail(IHIP_ERR_INVALID, "null pointer");
-    if (!threads_fit(gd_tiles(T, a.batch.sequences, kConvShift)))
+    a.shift = conv_shift(T, a.batch.sequences, channels);
+    if (!threads_fit(gd_tiles(T, a.batch.sequences, a.shift)))
         return fail(IHIP_ERR_INVALID, "%lld tokens of %d sequences are too many for one call", (long long)T, a.batch.sequences);
     if (!step_fits(x_stride, channels, T, 8))
         return fail(IHIP_ERR_INVALID, "x_stride=%lld is no multiple of 8 that holds %d channels", (long long)x_stride, channels);

@@ -26,7 +26,7 @@ __global__ void __launch_bounds__(CONV_THREADS) k_short_conv(ConvArgs a)
     if (a.flags && blockIdx.x == 0 && blockIdx.y == 0)
         gd_report(a.batch, a.flags);
     int c = 0;
-    const int s = gd_find(a.batch, kConvShift, (int)blockIdx.x, c);
+    const int s = gd_find(a.batch, a.shift, (int)blockIdx.x, c);
     if (s < 0)
         return;
     const GdSeq q = gd_seq(a.batch, a.pool, s, c == 0 && blockIdx.y == 0 ? a.flags : nullptr);
@@ -35,7 +35,7 @@ __global__ void __launch_bounds__(CONV_THREADS) k_short_conv(ConvArgs a)
         return;
     float *state = a.state + q.slot * a.slot_step + ch;
     gd_f4 win[W]; // the last W - 1 inputs, then the token's own
-    const int t0 = c << kConvShift, t1 = min(t0 + (1 << kConvShift), q.n);
+    const int t0 = c << a.shift, t1 = min(t0 + (1 << a.shift), q.n);
     const int64_t row0 = (int64_t)q.start * a.x_step + ch;
     if (c > 0) {
 #pragma unroll
@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(CONV_THREADS) k_short_conv(ConvArgs a)
 template <int TYPE>
 hipError_t launch(const ConvArgs &a, hipStream_t s)
 {
-    const dim3 grid((unsigned)gd_tiles(a.batch.tokens, a.batch.sequences, kConvShift),
+    const dim3 grid((unsigned)gd_tiles(a.batch.tokens, a.batch.sequences, a.shift),
                     (unsigned)((a.channels / 4 + CONV_THREADS - 1) / CONV_THREADS));
     switch (a.width) {
 #define IHIP_CONV(W)                                                                           \

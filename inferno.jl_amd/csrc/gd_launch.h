@@ -14,6 +14,7 @@ struct ConvArgs {
     int64_t x_step; // elements from one token to the next
     const float *w, *bias;
     int channels, width, silu;
+    int shift; // a tile has 2^shift tokens
     float *state;
     int64_t slot_step; // floats from one slot to the next
     int pool;

@@ -9,7 +9,6 @@
 namespace ihip {
 
 constexpr int kDeltaShift = 6;  // a chunk is 64 tokens
-constexpr int kConvShift = 5;   // a tile of the short convolution is 32
 constexpr int kDeltaTri = 6 * 2 * 1024; // a 64 x 64 lower triangle: 6 tiles of 16 x 32 in two fp16 parts
 constexpr int kDeltaRows = 192;  // floats of a chunk's row factors
 
@@ -39,6 +38,14 @@ constexpr int delta_few(int v_heads, int64_t sequences)
 constexpr int delta_few_beside(int v_heads, int64_t sequences)
 {
     return sequences * v_heads < 256 ? 4 : 10;
+}
+
+// Tokens of a tile of the short convolution, as a power of two: 32, or 16 where those are
+// fewer than 4 workgroups to a CU (1024 channels each).  Measured, us with 16 | 32: 2146 tokens of
+// 2560 channels 14.3 | 17.7, 8192 of 8192 100.9 | 94.8 (a tile reads width - 1 rows twice).
+constexpr int conv_shift(int64_t tokens, int64_t sequences, int channels)
+{
+    return gd_tiles(tokens, sequences, 5) * ((channels + 1023) / 1024) < 1024 ? 4 : 5;
 }
 
 struct DeltaPlan {

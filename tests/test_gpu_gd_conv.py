@@ -63,6 +63,13 @@ def test_lengths_and_types(W, act, out_type):
     check(case(W, new, [i % 3 == 0 for i in range(len(new))], 1032, W, TYPES[act], TYPES[out_type], W % 2 == 0, first=3, pad=5))
 
 
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+def test_tiles_of_32_tokens(act):
+    """From 1024 workgroups on; fewer take tiles of 16."""
+    new = [15, 16, 17, 1, 31, 32, 33, 0, 32768, 65]
+    check(case(21, new, [i % 2 == 0 for i in range(len(new))], 24, 4, TYPES[act], TYPES[act], True, first=2, pad=3))
+
+
 @pytest.mark.parametrize("W", [5, 6, 7])
 def test_other_widths_and_no_silu(W):
     check(case(W, [1, 70, W - 2], [False, True, False], 40, W, F32, F32, True), silu=False)
