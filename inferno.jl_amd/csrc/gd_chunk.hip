@@ -428,7 +428,7 @@ __device__ __forceinline__ void scan_sync()
 // KD / 32 such waves).  A wave so reads only its own part of the operands, from memory
 // into registers, two chunks ahead, and the waves exchange S and X as fp16 fragments in LDS,
 // with two barriers a chunk.  Bound by that chain, as a chunk follows the other: 8192
-// tokens of 32 heads of 128 x 128 take 282 us, 2.2 a chunk on every CU, of which the
+// tokens of 32 heads of 128 x 128 take 286 us, 2.2 a chunk on every CU, of which the
 // products, exchanges and barriers alone are 1.2 and the operands' way (76 KB a chunk and CU)
 // adds 0.6 from L2 and 0.4 from further away.  (One chunk ahead 322, three 274, with registers that
 // let one workgroup on a CU where sequences would give it two; 32 columns a workgroup, which halves

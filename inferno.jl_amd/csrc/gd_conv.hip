@@ -17,7 +17,7 @@ constexpr int CONV_AHEAD = 8; // tokens whose values are on their way at once
 // inputs in registers, so that a tile reads W - 1 rows twice and everything else
 // once.  A sequence's first tile alone reads and writes its state (the new one is
 // read from x, wherever its tile is), and in one thread, so no tile waits for another.
-// Bound by bytes: 8192 tokens of 8192 channels, fp32 in and bf16 out, 91 us (4.4 TB/s;
+// Bound by bytes: 8192 tokens of 8192 channels, fp32 in and bf16 out, 93 to 96 us (4.2 to 4.3 TB/s;
 // 103 with the type looked at beside every load, which then wait for each other); one
 // token of 6144 channels 4.1, its launch and two rounds of loads.
 template <int TYPE, int W>

@@ -21,8 +21,8 @@ constexpr int STEP_TOKENS = 16; // whose q, k and o a workgroup holds in LDS at 
 // columns of S do not touch each other, so a wave has VD / 4 of them to itself: a lane
 // holds 4 columns of R rows, a product with S is summed over the wave's row groups by
 // lane moves, and the tokens follow each other without a barrier.  Bound by the
-// state's bytes for a batch (61 tokens, 32 heads of 128 x 128: 64 to 67 us for 260 MB, 3.9
-// to 4.1 TB/s), by loads that wait for each other for one sequence (8.7 us), and by
+// state's bytes for a batch (61 tokens, 32 heads of 128 x 128: 66 to 68 us for 260 MB, 3.8
+// to 3.9 TB/s), by loads that wait for each other for one sequence (8.7 us), and by
 // the chain of a token's sums for several (1.4 us a token).
 template <int TYPE, int KD, int VD>
 __global__ void __launch_bounds__(STEP_THREADS) k_delta_step(DeltaArgs a)
