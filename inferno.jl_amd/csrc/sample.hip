@@ -217,9 +217,9 @@ __device__ void sample_whole_row(const SampleArgs &a, int row, const SampleRow &
 // reads past the caches, would).  One row of 151936 fp32 logits, us: best 3.2, bins 6, merge 3.2,
 // bounds 4.3, list 5.8, pick 12; bound by these launches and the loads and sums that
 // follow each other in them (the logits are 0.1 at the rate of reads).  61 rows of bf16
-// with mixed filters: 6.4, 18.9, 4.7, 4.6, 14.9, 24.5; bound by atomics to shared bins,
-// 64-bit weights and the longest of the rows' lists.  256 rows of fp32 without filters: best 50
-// (156 MB, 3.1 TB/s: 20 operations in 64 bits a weight beside its load), join 12.
+// with mixed filters: 6.7, 17.5, 4.4, 4.6, 15, 24.3; bound by atomics to shared bins,
+// 64-bit weights and the longest of the rows' lists.  256 rows of fp32 without filters: best 46
+// (156 MB, 3.4 TB/s: 16 operations in 64 bits a weight beside its load), join 12.
 
 struct Part { // of a slice
     unsigned long long best; // the largest logit (its key, then ~place)
@@ -522,6 +522,8 @@ __global__ void __launch_bounds__(ROW_THREADS) k_sample_best(SampleArgs a)
     __shared__ double part[ROW_WAVES];
     const int slice = blockIdx.x % a.plan.slices, rr = blockIdx.x / a.plan.slices, row = a.row0 + rr;
     const Slice<TYPE, N> x(a, row, slice);
+    if (SUMS)
+        sample_fill_table();
     unsigned long long best;
     uint32_t fl;
     slice_best(x, best, fl, wbest, wfl);
@@ -549,6 +551,7 @@ __global__ void __launch_bounds__(ROW_THREADS) k_sample_join(SampleArgs a)
     __shared__ float staged[STAGED];
     const int rr = blockIdx.x, row = a.row0 + rr, tid = threadIdx.x;
     const SampleRow r = sample_row(a, row);
+    sample_fill_table();
     unsigned long long best;
     uint32_t fl;
     row_best(a, rr, best, fl, wbest, wfl);
@@ -570,7 +573,7 @@ template <int TYPE, int N>
 __global__ void __launch_bounds__(ROW_THREADS) k_sample_bins(SampleArgs a)
 {
     // (bins in two copies, by lane, where neighbouring tokens' atomics meet less often: 61
-    // rows 18.9 us, one copy 21.6, four 19.6)
+    // rows 18.9 us, one copy 21.6, four 19.6, with weights of six operations more)
     constexpr int COPIES = 2;
     __shared__ unsigned long long mass[COPIES * kSampleBins];
     __shared__ uint32_t count[COPIES * kSampleBins];
@@ -582,6 +585,7 @@ __global__ void __launch_bounds__(ROW_THREADS) k_sample_bins(SampleArgs a)
     if (!filtered(r, a.vocab, by_k, by_p) || !(r.t > 0.0f))
         return;
     const Slice<TYPE, N> x(a, row, slice);
+    sample_fill_table();
     for (int i = tid; i < COPIES * kSampleBins; i += ROW_THREADS)
         mass[i] = 0, count[i] = 0;
     const int copy = tid % COPIES;
@@ -747,6 +751,7 @@ __global__ void __launch_bounds__(ROW_THREADS) k_sample_list(SampleArgs a)
     if (!(r.t > 0.0f))
         return;
     const Slice<TYPE, N> x(a, row, slice);
+    sample_fill_table();
     if (tid == 0)
         listed = 0;
     unsigned long long best;
@@ -815,6 +820,7 @@ __global__ void __launch_bounds__(ROW_THREADS) k_sample_pick(SampleArgs a)
     const bool cut_row = filtered(r, a.vocab, by_k, by_p);
     if (!cut_row)
         bo.listed = 0;
+    sample_fill_table();
     unsigned long long best;
     uint32_t fl;
     row_best(a, rr, best, fl, upart, wfl);

@@ -64,7 +64,7 @@ __device__ __forceinline__ uint32_t sample_flags(float l)
     return l != l ? kSampleNan : l == __builtin_inff() ? kSamplePosInf : l == -__builtin_inff() ? 0 : kSampleFinite;
 }
 
-// w = 2^(rate (l - most)), and as a whole number of units of which 2^bits make 1, so
+// w = 2^(rate (l - most) / 32), and as a whole number of units of which 2^bits make 1, so
 // that a row's sums fit 63 bits.
 struct SampleScale {
     double rate, most;
@@ -73,40 +73,45 @@ struct SampleScale {
 
 __device__ __forceinline__ SampleScale sample_scale(float t, float most, int vocab)
 {
-    return SampleScale{1.4426950408889634074 / (double)t, (double)most, min(46, 62 - (32 - __builtin_clz(vocab)))};
+    return SampleScale{32 * 1.4426950408889634074 / (double)t, (double)most, min(46, 62 - (32 - __builtin_clz(vocab)))};
 }
 
-// 2^x for x <= 0: 2^f, |f| <= 1/2, by its series, whose rest is below 2^-47; 0 from
-// 2^-1075 on
-__device__ __forceinline__ double sample_exp2(double x)
+// 2^(i / 32), in every workgroup's LDS; filled before its first barrier
+__device__ __forceinline__ double *sample_table()
 {
-    x = fmax(x, -1100.0);
-    const double n = rint(x), f = x - n;
-    constexpr double L = 0.69314718055994530942;
+    __shared__ double table[32];
+    return table;
+}
+__device__ __forceinline__ void sample_fill_table()
+{
+    if (threadIdx.x < 32)
+        sample_table()[threadIdx.x] = exp2((double)threadIdx.x / 32);
+}
+
+// 2^(x / 32) for x <= 0: x to the nearest whole number, whose power of two is in the
+// table, and the rest, |f| <= 1/2, by the series of 2^(f / 32), whose own rest is below 2^-48.
+// 0 from 2^-1075 on.  (Without the table the series takes six operations more, of 20 in 64
+// bits: sums of 256 rows of 151936 logits 50 us, 46 with it.)
+__device__ __forceinline__ double sample_exp2_32(double x)
+{
+    x = fmax(x, -1100.0 * 32);
+    constexpr double WHOLE = 6755399441055744.0; // 1.5 * 2^52: a sum with it is whole
+    const double s = x + WHOLE, f = x - (s - WHOLE);
+    const int n = (int)(uint32_t)__double_as_longlong(s);
+    constexpr double L = 0.69314718055994530942 / 32;
     // L^i / i!
-    constexpr double c[12] = {1.0,
-                              L,
-                              L * L / 2,
-                              L * L * L / 6,
-                              L * L * L * L / 24,
-                              L * L * L * L * L / 120,
-                              L * L * L * L * L * L / 720,
-                              L * L * L * L * L * L * L / 5040,
-                              L * L * L * L * L * L * L * L / 40320,
-                              L * L * L * L * L * L * L * L * L / 362880,
-                              L * L * L * L * L * L * L * L * L * L / 3628800,
-                              L * L * L * L * L * L * L * L * L * L * L / 39916800};
-    double y = c[11];
+    constexpr double c[6] = {1.0, L, L * L / 2, L * L * L / 6, L * L * L * L / 24, L * L * L * L * L / 120};
+    double y = c[5];
 #pragma unroll
-    for (int i = 10; i >= 0; --i)
+    for (int i = 4; i >= 0; --i)
         y = fma(y, f, c[i]);
-    return ldexp(y, (int)n);
+    return ldexp(y * sample_table()[n & 31], n >> 5);
 }
 
 // (-infinity, and a rate of 0 times it, become -1100)
 __device__ __forceinline__ double sample_weight(const SampleScale &s, float l)
 {
-    return sample_exp2(s.rate * ((double)l - s.most));
+    return sample_exp2_32(s.rate * ((double)l - s.most));
 }
 
 __device__ __forceinline__ uint64_t sample_mass(const SampleScale &s, float l)
