@@ -408,11 +408,11 @@ constexpr int SCAN_WAVES = 4;
 
 // What a wave reads of a chunk: its 16 rows of K, Q and P, its 32 rows of M, the factors
 // of its 16 tokens and their values in its columns.
-template <int KS, int PARTS, int CT>
+template <int KS, int PARTS>
 struct ScanOps {
     gd_h8 k[KS][PARTS], q[KS][PARTS], m[2][2][2], p[2][2];
     gd_f4 fk, fq;
-    uint32_t v[CT][4]; // as they lie in memory
+    uint32_t v[4]; // as they lie in memory
     float keep;
 };
 
@@ -423,7 +423,7 @@ __device__ __forceinline__ void scan_sync()
     lds_barrier();
 }
 
-// A workgroup takes 16 CT columns of one head of one sequence, each of its waves the
+// A workgroup takes 16 columns of one head of one sequence, each of its waves the
 // tokens 16 w .. 16 w + 15 of a chunk and the rows 32 w .. 32 w + 31 of S (there are
 // KD / 32 such waves).  A wave so reads only its own part of the operands, from memory
 // into registers, two chunks ahead, and the waves exchange S and X as fp16 fragments in LDS,
@@ -438,22 +438,22 @@ __device__ __forceinline__ void scan_sync()
 // and no token adds more than |v| to the length of a column of S, so |X| and the
 // new S lie below 12 max |S| + 66 max |v| (sqrt(128) < 12).  Fragments keep 22 bits of
 // what is over 2^-27 of that.
-template <int TYPE, int KD, int CT>
+template <int TYPE, int KD>
 __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
 {
     constexpr int PARTS = TYPE == kF32 ? 2 : 1;
     constexpr int KS = KD / 32;
     constexpr int FRAG = 4 * KS * PARTS * 1024;
     constexpr int VB = PARTS > 1 ? 4 : 2; // bytes of a value of V
-    using Ops = ScanOps<KS, PARTS, CT>;
-    __shared__ __attribute__((aligned(16))) uint8_t sf[CT][KS][2][1024], xf[CT][2][2][1024];
-    __shared__ float bounds[SCAN_WAVES][CT][16];
+    using Ops = ScanOps<KS, PARTS>;
+    __shared__ __attribute__((aligned(16))) uint8_t sf[KS][2][1024], xf[2][2][1024];
+    __shared__ float bounds[SCAN_WAVES][16];
     __shared__ __attribute__((aligned(16))) float turn[SCAN_WAVES][16][20];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, r = lane & 15;
     if (a.flags && blockIdx.x == 0 && !a.plan.steps)
         gd_report(a.batch, a.flags);
     // the workgroups of the heads that read one K lie on one XCD (its L2)
-    const int blocks = (a.v_dim + 16 * CT - 1) / (16 * CT), each = a.group * blocks;
+    const int blocks = a.v_dim / 16, each = a.group * blocks;
     const int j = blockIdx.x / 8, u = j / each * 8 + blockIdx.x % 8;
     if (u >= a.k_heads * a.batch.sequences)
         return;
@@ -461,7 +461,7 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
     const GdSeq seq = gd_seq(a.batch, a.pool, s, h == 0 && j % blocks == 0 ? a.flags : nullptr);
     if (seq.slot < 0 || seq.n <= a.few)
         return;
-    const int col0 = j % blocks * CT * 16;
+    const int col0 = j % blocks * 16;
     float *const state = a.state + seq.slot * a.slot_step + (int64_t)h * a.k_dim * a.v_dim + col0 + r;
     const int chunks = (seq.n + 63) / 64, tile0 = gd_base(a.batch, kDeltaShift, s);
     const bool owner = wave < KS;
@@ -470,10 +470,6 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
     for (int i = 0; i < 4; ++i)
         vat[i] = ((16 * wave + 4 * g + i) * a.v_step + r) * VB;
     const int64_t oat = (int64_t)(16 * wave + lane / 4) * a.v_heads * a.v_dim + 4 * (lane % 4);
-    bool live[CT];
-#pragma unroll
-    for (int e = 0; e < CT; ++e)
-        live[e] = col0 + 16 * e < a.v_dim;
 
     // A chunk's operands, in two portions: those of the chunk after the next follow
     // as soon as their registers are free.  (Behind the last chunk: its operands again.)
@@ -494,19 +490,15 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
                 o.q[k][p] = *(const gd_h8 *)(kq + FRAG + ((wave * KS + k) * PARTS + p) * 1024);
         o.fk = *(const gd_f4 *)(f + 16 * wave + 4 * g);
         o.fq = *(const gd_f4 *)(f + 64 + 16 * wave + 4 * g);
-        // (rows behind the last token and columns behind the last one: others', not used)
+        // (rows behind the last token: others', not used)
         const int at0 = 64 * min(c, chunks - 1);
         const uint8_t *const v = (const uint8_t *)a.v + ((seq.start + at0) * a.v_step + (int64_t)h * a.v_dim + col0) * VB;
         const int last = seq.n - 1 - at0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int row = 16 * wave + 4 * g + i;
-            const int64_t from = last >= 63 ? vat[i] : (min(row, last) * a.v_step + r) * VB;
-#pragma unroll
-            for (int e = 0; e < CT; ++e) {
-                const uint8_t *at = v + from + (live[e] ? 16 * e * VB : 0);
-                o.v[e][i] = PARTS > 1 ? *(const uint32_t *)at : *(const uint16_t *)at;
-            }
+            const uint8_t *const at = v + (last >= 63 ? vat[i] : (min(row, last) * a.v_step + r) * VB);
+            o.v[i] = PARTS > 1 ? *(const uint32_t *)at : *(const uint16_t *)at;
         }
     };
     auto load_pm = [&](Ops &o, int c) {
@@ -539,63 +531,54 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
         *(h4 *)(to[wave / 2][1] + lane * 16 + 8 * (wave & 1)) = lo;
     };
 
-    gd_f4 S[CT][2];
-    float to_s[CT], back_s[CT];
+    gd_f4 S[2];
+    float to_s, back_s;
 #pragma unroll
-    for (int e = 0; e < CT; ++e) {
+    for (int m = 0; m < 2; ++m)
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int at = 32 * wave + 16 * m + 4 * g + i;
-                S[e][m][i] = owner && live[e] && !seq.begins && at < a.k_dim ? state[(int64_t)at * a.v_dim + 16 * e] : 0.0f;
-            }
-        const float most = gd_max32(gd_max16(fmaxf(most4(S[e][0]), most4(S[e][1]))));
-        if (g == 0)
-            bounds[wave][e][r] = most;
-    }
+        for (int i = 0; i < 4; ++i) {
+            const int at = 32 * wave + 16 * m + 4 * g + i;
+            S[m][i] = owner && !seq.begins && at < a.k_dim ? state[(int64_t)at * a.v_dim] : 0.0f;
+        }
+    const float most = gd_max32(gd_max16(fmaxf(most4(S[0]), most4(S[1]))));
+    if (g == 0)
+        bounds[wave][r] = most;
     scan_sync();
-    auto widest = [&](int e) {
-        return fmaxf(fmaxf(bounds[0][e][r], bounds[1][e][r]), fmaxf(bounds[2][e][r], bounds[3][e][r]));
+    auto widest = [&]() {
+        return fmaxf(fmaxf(bounds[0][r], bounds[1][r]), fmaxf(bounds[2][r], bounds[3][r]));
     };
-#pragma unroll
-    for (int e = 0; e < CT; ++e)
-        gd_power(widest(e), to_s[e], back_s[e]);
+    gd_power(widest(), to_s, back_s);
     scan_sync();
 
     auto chunk = [&](Ops &o, int c) {
         const int n = min(64, seq.n - 64 * c);
-        gd_f4 v[CT];
+        gd_f4 v;
 #pragma unroll
-        for (int e = 0; e < CT; ++e) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float x = TYPE == kF32 ? __uint_as_float(o.v[e][i]) : TYPE == kF16 ? h2f(o.v[e][i]) : __uint_as_float(o.v[e][i] << 16);
-                v[e][i] = live[e] && 16 * wave + 4 * g + i < n ? x : 0.0f;
-            }
-            if (owner) {
-                gd_h8 hi, lo;
-                gd_split(__builtin_shufflevector(S[e][0], S[e][1], 0, 1, 2, 3, 4, 5, 6, 7), to_s[e], hi, lo);
-                *(gd_h8 *)(sf[e][wave][0] + lane * 16) = hi;
-                *(gd_h8 *)(sf[e][wave][1] + lane * 16) = lo;
-            }
-            const float most = 12.0f * fmaxf(most4(S[e][0]), most4(S[e][1])) + 66.0f * most4(v[e]);
-            const float all = gd_max32(gd_max16(most));
-            if (g == 0)
-                bounds[wave][e][r] = all;
+        for (int i = 0; i < 4; ++i) {
+            const float x = TYPE == kF32 ? __uint_as_float(o.v[i]) : TYPE == kF16 ? h2f(o.v[i]) : __uint_as_float(o.v[i] << 16);
+            v[i] = 16 * wave + 4 * g + i < n ? x : 0.0f;
         }
+        if (owner) {
+            gd_h8 hi, lo;
+            gd_split(__builtin_shufflevector(S[0], S[1], 0, 1, 2, 3, 4, 5, 6, 7), to_s, hi, lo);
+            *(gd_h8 *)(sf[wave][0] + lane * 16) = hi;
+            *(gd_h8 *)(sf[wave][1] + lane * 16) = lo;
+        }
+        const float most = 12.0f * fmaxf(most4(S[0]), most4(S[1])) + 66.0f * most4(v);
+        const float all = gd_max32(gd_max16(most));
+        if (g == 0)
+            bounds[wave][r] = all;
         scan_sync();
         // K S and Q S; X = V - e^G K S
-        gd_f4 qs[CT];
-        float to[CT], back[CT];
-#pragma unroll
-        for (int e = 0; e < CT; ++e) {
-            gd_power(widest(e), to[e], back[e]);
+        gd_f4 qs;
+        float to, back;
+        gd_power(widest(), to, back);
+        {
             gd_h8 hi[KS], lo[KS];
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
-                hi[k] = *(const gd_h8 *)(sf[e][k][0] + lane * 16);
-                lo[k] = *(const gd_h8 *)(sf[e][k][1] + lane * 16);
+                hi[k] = *(const gd_h8 *)(sf[k][0] + lane * 16);
+                lo[k] = *(const gd_h8 *)(sf[k][1] + lane * 16);
             }
             gd_f4 x{}, y{}, z{}, w{};
 #pragma unroll
@@ -612,59 +595,56 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
                 if (PARTS > 1)
                     w = gd_mfma(o.q[k][PARTS - 1], hi[k], w);
             }
-            put(xf[e], v[e] - o.fk * ((x + y * (1.0f / REST)) * back_s[e]), to[e]);
-            qs[e] = (z + w * (1.0f / REST)) * back_s[e] * o.fq;
+            put(xf, v - o.fk * ((x + y * (1.0f / REST)) * back_s), to);
+            qs = (z + w * (1.0f / REST)) * back_s * o.fq;
         }
         load_kqv(o, c + 2);
         scan_sync();
         // S <- e^G_64 S + M X;  O = scale (e^G Q S + P X)
+        gd_h8 hi[2], lo[2];
 #pragma unroll
-        for (int e = 0; e < CT; ++e) {
-            gd_h8 hi[2], lo[2];
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                hi[k] = *(const gd_h8 *)(xf[e][k][0] + lane * 16);
-                lo[k] = *(const gd_h8 *)(xf[e][k][1] + lane * 16);
-            }
-            const float by = back[e] * (1.0f / (1 << TOP));
-            if (owner) {
-                gd_f4 x[2]{}, y[2]{};
-#pragma unroll
-                for (int k = 0; k < 2; ++k)
-#pragma unroll
-                    for (int m = 0; m < 2; ++m) {
-                        x[m] = gd_mfma(o.m[m][k][0], hi[k], x[m]);
-                        y[m] = gd_mfma(o.m[m][k][0], lo[k], y[m]);
-                        y[m] = gd_mfma(o.m[m][k][1], hi[k], y[m]);
-                    }
-#pragma unroll
-                for (int m = 0; m < 2; ++m)
-                    S[e][m] = S[e][m] * o.keep + (x[m] + y[m] * (1.0f / REST)) * by;
-            }
-            gd_f4 x{}, y{};
-            x = gd_mfma(o.p[0][0], hi[0], x);
-            y = gd_mfma(o.p[0][0], lo[0], y);
-            y = gd_mfma(o.p[0][1], hi[0], y);
-            if (wave >= 2) {
-                x = gd_mfma(o.p[1][0], hi[1], x);
-                y = gd_mfma(o.p[1][0], lo[1], y);
-                y = gd_mfma(o.p[1][1], hi[1], y);
-            }
-            const gd_f4 out = a.scale * (qs[e] + (x + y * (1.0f / REST)) * by);
-            // through LDS, so that a lane stores 4 neighbours
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                turn[wave][4 * g + i][r] = out[i];
-            const gd_f4 flat = *(const gd_f4 *)&turn[wave][lane / 4][4 * (lane % 4)];
-            if (live[e] && 16 * wave + lane / 4 < n) {
-                const int64_t where = ((seq.start + 64 * (int64_t)c) * a.v_heads + h) * a.v_dim + col0 + 16 * e + oat;
-                if (a.raw)
-                    *(gd_f4 *)(a.raw + where) = flat;
-                else
-                    gd_store4(a.out, where, a.out_type, flat);
-            }
-            to_s[e] = to[e], back_s[e] = back[e];
+        for (int k = 0; k < 2; ++k) {
+            hi[k] = *(const gd_h8 *)(xf[k][0] + lane * 16);
+            lo[k] = *(const gd_h8 *)(xf[k][1] + lane * 16);
         }
+        const float by = back * (1.0f / (1 << TOP));
+        if (owner) {
+            gd_f4 x[2]{}, y[2]{};
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int m = 0; m < 2; ++m) {
+                    x[m] = gd_mfma(o.m[m][k][0], hi[k], x[m]);
+                    y[m] = gd_mfma(o.m[m][k][0], lo[k], y[m]);
+                    y[m] = gd_mfma(o.m[m][k][1], hi[k], y[m]);
+                }
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+                S[m] = S[m] * o.keep + (x[m] + y[m] * (1.0f / REST)) * by;
+        }
+        gd_f4 x{}, y{};
+        x = gd_mfma(o.p[0][0], hi[0], x);
+        y = gd_mfma(o.p[0][0], lo[0], y);
+        y = gd_mfma(o.p[0][1], hi[0], y);
+        if (wave >= 2) {
+            x = gd_mfma(o.p[1][0], hi[1], x);
+            y = gd_mfma(o.p[1][0], lo[1], y);
+            y = gd_mfma(o.p[1][1], hi[1], y);
+        }
+        const gd_f4 out = a.scale * (qs + (x + y * (1.0f / REST)) * by);
+        // through LDS, so that a lane stores 4 neighbours
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            turn[wave][4 * g + i][r] = out[i];
+        const gd_f4 flat = *(const gd_f4 *)&turn[wave][lane / 4][4 * (lane % 4)];
+        if (16 * wave + lane / 4 < n) {
+            const int64_t where = ((seq.start + 64 * (int64_t)c) * a.v_heads + h) * a.v_dim + col0 + oat;
+            if (a.raw)
+                *(gd_f4 *)(a.raw + where) = flat;
+            else
+                gd_store4(a.out, where, a.out_type, flat);
+        }
+        to_s = to, back_s = back;
         load_pm(o, c + 2);
     };
     Ops even, odd;
@@ -679,15 +659,13 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
         chunk(even, c);
     if (owner)
 #pragma unroll
-        for (int e = 0; e < CT; ++e)
+        for (int m = 0; m < 2; ++m)
 #pragma unroll
-            for (int m = 0; m < 2; ++m)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int at = 32 * wave + 16 * m + 4 * g + i;
-                    if (live[e] && at < a.k_dim)
-                        state[(int64_t)at * a.v_dim + 16 * e] = S[e][m][i];
-                }
+            for (int i = 0; i < 4; ++i) {
+                const int at = 32 * wave + 16 * m + 4 * g + i;
+                if (at < a.k_dim)
+                    state[(int64_t)at * a.v_dim] = S[m][i];
+            }
 }
 
 // ---- the output norm ---------------------------------------------------------------
@@ -735,12 +713,11 @@ __global__ void __launch_bounds__(NORM_THREADS) k_delta_norm(DeltaArgs a)
 template <int TYPE, int KD>
 void launch(const DeltaArgs &a, hipStream_t s)
 {
-    constexpr int CT = 1;
     const unsigned units = (unsigned)(a.plan.tiles * a.v_heads);
     hipLaunchKernelGGL((k_delta_prep<TYPE, KD>), dim3(units), dim3(PREP_THREADS), 0, s, a);
-    const unsigned blocks = (unsigned)((a.v_dim + 16 * CT - 1) / (16 * CT)) * (unsigned)a.group;
+    const unsigned blocks = (unsigned)(a.v_dim / 16) * (unsigned)a.group;
     const unsigned heads = ((unsigned)(a.k_heads * a.batch.sequences) + 7) / 8 * 8;
-    hipLaunchKernelGGL((k_delta_scan<TYPE, KD, CT>), dim3(heads * blocks), dim3(64 * SCAN_WAVES), 0, s, a);
+    hipLaunchKernelGGL((k_delta_scan<TYPE, KD>), dim3(heads * blocks), dim3(64 * SCAN_WAVES), 0, s, a);
     if (a.norm_w || a.gate)
         hipLaunchKernelGGL(k_delta_norm, dim3(units), dim3(NORM_THREADS), 0, s, a);
 }
