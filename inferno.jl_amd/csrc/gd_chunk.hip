@@ -11,13 +11,19 @@
 // for all chunks at once.  k_delta_scan then walks down a sequence's chunks; the columns
 // of S do not touch each other.
 //
-// Operands are fp16 times a power of two (of a row of K and Q, of a column of S and
-// X), so that the largest value lies in 2^13 .. 2^14: values of F16 and BF16 inputs
-// fit one part exactly down to 2^-27 of their row's largest; fp32 values and
-// everything derived are held in two parts, which leave 2^-22 of a value, and products
+// A chunk's tokens may be of any sizes beside each other: a quiet token before a loud one, a
+// loud one that is forgotten before a quiet one, a head that hardly writes.  So X, T, P
+// and M are operands of three bf16 parts, which have 24 bits and the exponents of fp32; of
+// the products of their parts those below 2^-24 are not formed.  (In two fp16 parts with a
+// power of two for a chunk, rows 10^7 below the largest lost their last bits, and 10^9 all.)
+// A product with S sums over all of a row of K or Q and a column of S, so what is small
+// beside the row's or the column's largest value counts as little there as in fp32: those
+// operands are fp16 times a power of two, the largest in 2^13 .. 2^14.  Values of F16 and
+// BF16 inputs fit one such part exactly down to 2^-27 of their row's largest, and to 2^-38 of
+// that below; fp32 ones and S are held in two, which leave 2^-22 of a value, and products
 // of the two lower parts (2^-22) are not formed.  Sums are fp32.  Rows' factors (unit
-// length, e^G) are applied to the products, in fp32, so that K and Q are shared by the
-// heads that read them.
+// length, e^G) are applied to the products, in fp32, so that K and Q are shared by the heads
+// that read them.
 #include "gd_launch.h"
 
 namespace ihip {
@@ -25,9 +31,10 @@ namespace ihip {
 namespace {
 
 typedef _Float16 gd_h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 gd_b8 __attribute__((ext_vector_type(8)));
 typedef float gd_f8 __attribute__((ext_vector_type(8)));
 
-constexpr int TOP = 13; // operands' largest values have this binary exponent
+constexpr int TOP = 13; // fp16 operands' largest values have this binary exponent
 
 // 2^(TOP - exponent of x), and its inverse; x >= 0.  (Below 2^-113 of nothing; an
 // infinity or NaN is left one.)
@@ -38,15 +45,38 @@ __device__ __forceinline__ void gd_power(float x, float &to, float &back)
     back = __uint_as_float((uint32_t)(e - TOP) << 23);
 }
 
-// x * by as one fp16 part, and the rest of it, times 2^11, as the next.  (The matrix
-// cores take fp16 values below 2^-14 as zeros: unscaled rests of all but the largest
-// values would be cut, to 2^-16 of a typical state.)
+// x * by as one fp16 part, and the rest of it, times 2^11, as the next: where the first is one of
+// fp16's subnormal values, the rest still has bits below it.
 constexpr float REST = 2048.0f;
 __device__ __forceinline__ void gd_split(gd_f8 x, float by, gd_h8 &hi, gd_h8 &lo)
 {
     x = x * by;
     hi = __builtin_convertvector(x, gd_h8);
     lo = __builtin_convertvector((x - __builtin_convertvector(hi, gd_f8)) * REST, gd_h8);
+}
+
+// x as three bf16 parts, each the nearest of what the ones before leave.  (In pairs, as the
+// conversion takes them: 5.5 operations a value.)
+template <typename F, typename B>
+__device__ __forceinline__ void gd_split3(F x, B (&part)[3])
+{
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    constexpr int PAIRS = sizeof(F) / 8;
+    typedef uint32_t Pairs __attribute__((ext_vector_type(PAIRS)));
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        Pairs u;
+#pragma unroll
+        for (int j = 0; j < PAIRS; ++j) {
+            u[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){x[2 * j], x[2 * j + 1]}, b2));
+            if (i < 2) {
+                x[2 * j] -= __uint_as_float(u[j] << 16);
+                x[2 * j + 1] -= __uint_as_float(u[j] & 0xffff0000u);
+            }
+        }
+        part[i] = __builtin_bit_cast(B, u);
+    }
 }
 
 // 2^x, x <= 0 (nothing below 2^-126); without a branch
@@ -59,22 +89,41 @@ __device__ __forceinline__ gd_f4 gd_mfma(gd_h8 a, gd_h8 b, gd_f4 c)
 {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
+__device__ __forceinline__ gd_f4 gd_mfma(gd_b8 a, gd_b8 b, gd_f4 c)
+{
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// x + rest += the product of operands in 3 and N bf16 parts: x of the first ones, rest of the
+// others whose sizes are over 2^-24 of that
+template <int N>
+__device__ __forceinline__ void gd_dot(const gd_b8 (&a)[3], const gd_b8 (&b)[N], gd_f4 &x, gd_f4 &rest)
+{
+    x = gd_mfma(a[0], b[0], x);
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            if (i + j == 1 || i + j == 2)
+                rest = gd_mfma(a[i], b[j], rest);
+}
 
 // Fragments.  A 16-row tile of an operand is stored as the matrix cores take it: for
 // each step of 32 columns, lane (g, r) = (lane / 16, lane % 16) holds of row r the
 // columns 4 g .. 4 g + 3 and 16 + 4 g .. 16 + 4 g + 3, 16 bytes a lane.  These are the
 // rows that a lane holds of two tiles of a product's result, so that results (S, X)
-// are the next product's operands without leaving their registers.
+// are the next product's operands without leaving their registers.  P and M, which come out
+// of fp32 sums, lie as two such planes of 4 fp32 values a lane.
 
 // ---- chunks' operands ------------------------------------------------------------
 constexpr int PREP_THREADS = 256;
 constexpr int TRI = 68; // floats from a row of a 64 x 64 matrix to the next, in LDS
 
 // A workgroup takes a chunk of a head of v; a wave 16 of its rows.  k's and q's products
-// and P and M are on the fp16 matrix cores, the inverse in fp32: 16 x 16 blocks on the diagonal
-// by substitution, the ones below from those on the fp32 matrix cores.  Heads that share
+// are on the fp16 matrix cores, P and M on the bf16 ones, the inverse in fp32: 16 x 16 blocks on
+// the diagonal by substitution, the ones below from those on the fp32 matrix cores.  Heads that share
 // K and Q form them again each (their rows are in L2), and one writes them.  8192 tokens of 32
-// heads of 128 on 16, bf16: 107 us for 67 MB in and 252 out (P and M 185 of them), 3.0 TB/s;
+// heads of 128 on 16, bf16: 105 us for 67 MB in and 253 out (P and M 185 of them), 3.0 TB/s;
 // 163 with two workgroups a CU instead of three and loads that wait for each other.
 template <int TYPE, int KD>
 __global__ void __launch_bounds__(PREP_THREADS) k_delta_prep(DeltaArgs a)
@@ -83,15 +132,16 @@ __global__ void __launch_bounds__(PREP_THREADS) k_delta_prep(DeltaArgs a)
     constexpr int KS = KD / 32;               // steps of a row of K
     constexpr int FRAG = 4 * KS * PARTS * 1024; // bytes of K or Q
     constexpr int MD = KD / 64;               // 16-row tiles of M that a wave forms
-    // K; then A and its inverse T; then P and T as an operand.  (42 KB: three workgroups
-    // a compute unit.  With each in its own place, 78 KB, there are two.)
-    constexpr int MAT = 64 * TRI * 4, TT = 2 * 6 * 2 * 1024;
-    static_assert(MAT <= TT && FRAG <= MAT + TT, "");
-    __shared__ __attribute__((aligned(16))) uint8_t lds[MAT + TT];
+    // bf16 parts of a value of K
+    constexpr int BF = TYPE == kF32 ? 3 : TYPE == kF16 ? 2 : 1;
+    // K; then A (P in its place) and its inverse T; then T as two operands
+    constexpr int MAT = 64 * TRI * 4, TT = 6 * 3 * 1024;
+    static_assert(MAT <= TT && FRAG <= 2 * TT, "");
+    __shared__ __attribute__((aligned(16))) uint8_t lds[2 * TT];
     __shared__ double G[64];
     __shared__ float beta[64], rk[64], fu[64];
-    float *const A = (float *)lds, *const P = A, *const T = (float *)(lds + MAT);
-    uint8_t(*const tt)[6][2][1024] = (uint8_t(*)[6][2][1024])(lds + MAT);
+    float *const A = (float *)lds, *const P = A, *const T = (float *)(lds + TT);
+    uint8_t(*const tt)[6][3][1024] = (uint8_t(*)[6][3][1024])lds;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, r = lane & 15;
     const int h = blockIdx.x % a.v_heads, tile = blockIdx.x / a.v_heads, kh = h / a.group;
     int c = 0;
@@ -189,19 +239,29 @@ __global__ void __launch_bounds__(PREP_THREADS) k_delta_prep(DeltaArgs a)
     if (wave == 0)
         fu[lane] = rk[lane] * gd_exp2(G[63] - G[lane]);
     // this wave's columns of K, with the tokens in steps
-    gd_h8 kt[MD][2][PARTS];
+    gd_b8 kt[MD][2][BF];
 #pragma unroll
     for (int m = 0; m < MD; ++m)
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
+        for (int k = 0; k < 2; ++k) {
+            gd_f8 x;
 #pragma unroll
-            for (int p = 0; p < PARTS; ++p)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int token = 4 * g + i % 4, of = 2 * k + i / 4, md = MD * wave + m; // of tile `of`
-                    kt[m][k][p][i] = *(const _Float16 *)(lds + ((of * KS + md / 2) * PARTS + p) * 1024 + (r / 4 * 16 + token) * 16 +
-                                                         (4 * (md & 1) + r % 4) * 2);
-                }
+            for (int i = 0; i < 8; ++i) {
+                const int token = 4 * g + i % 4, of = 2 * k + i / 4, md = MD * wave + m; // of tile `of`
+                const uint8_t *const at =
+                    lds + (of * KS + md / 2) * PARTS * 1024 + (r / 4 * 16 + token) * 16 + (4 * (md & 1) + r % 4) * 2;
+                x[i] = (float)*(const _Float16 *)at;
+                if (PARTS > 1)
+                    x[i] = fmaf((float)*(const _Float16 *)(at + 1024), 1.0f / REST, x[i]);
+            }
+            if constexpr (BF == 3) {
+                gd_split3(x, kt[m][k]);
+            } else {
+                kt[m][k][0] = __builtin_convertvector(x, gd_b8);
+                if constexpr (BF == 2)
+                    kt[m][k][1] = __builtin_convertvector(x - __builtin_convertvector(kt[m][k][0], gd_f8), gd_b8);
+            }
+        }
 
     // this wave's rows of K K^T and Q K^T
     gd_f4 kk[4], qk[4];
@@ -292,12 +352,27 @@ __global__ void __launch_bounds__(PREP_THREADS) k_delta_prep(DeltaArgs a)
         for (int e = 0; e < 4; ++e)
             T[(16 * i + 4 * g + e) * TRI + 16 * j + r] = y[e];
     }
-    __syncthreads();
+    __syncthreads(); // A is read, T written
+    // P by rows, as an operand of this wave alone
+    gd_b8 pf[2][3];
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+        if (t <= (wave | 1))
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                P[(16 * wave + 4 * g + i) * TRI + 16 * t + r] = qk[t][i];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const float *from = P + row * TRI + 32 * k + 4 * g;
+        gd_f8 x{};
+        if (k <= wave / 2)
+            x = __builtin_shufflevector(*(const gd_f4 *)from, *(const gd_f4 *)(from + 16), 0, 1, 2, 3, 4, 5, 6, 7);
+        gd_split3(x, pf[k]);
+    }
     // T^T as an operand (16 x 32 tiles on and over its diagonal), its columns once as
-    // they are and once times the factors of what is written to the state.  fu and K's
-    // power of two are 1 together, so fu alone is below 2^-TOP.
-    constexpr float UP = 1 << TOP, BACK = 1.0f / UP;
-    gd_h8 to_t[2][2], to_f[2][2];
+    // they are and once times the factors of what is written to the state
+    gd_b8 to[2][2][3];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
         const int t = wave + 4 * u;
@@ -309,70 +384,54 @@ __global__ void __launch_bounds__(PREP_THREADS) k_delta_prep(DeltaArgs a)
         for (int i = 0; i < 8; ++i) {
             const int at = 32 * k + 4 * g + i % 4 + 16 * (i / 4);
             x[i] = T[at * TRI + j] * beta[j];
-            y[i] = x[i] * (fu[at] * UP);
+            y[i] = x[i] * fu[at];
         }
-        gd_split(x, UP, to_t[u][0], to_t[u][1]);
-        gd_split(y, UP, to_f[u][0], to_f[u][1]);
+        gd_split3(x, to[0][u]);
+        gd_split3(y, to[1][u]);
     }
-    __syncthreads(); // A and T are read
+    __syncthreads(); // P and T are read
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int p = 0; p < 2; ++p) {
+        for (int p = 0; p < 3; ++p) {
             const int t = wave + 4 * u;
             if (t >= 6)
                 continue;
-            *(gd_h8 *)(tt[0][t][p] + lane * 16) = to_t[u][p];
-            *(gd_h8 *)(tt[1][t][p] + lane * 16) = to_f[u][p];
+            *(gd_b8 *)(tt[0][t][p] + lane * 16) = to[0][u][p];
+            *(gd_b8 *)(tt[1][t][p] + lane * 16) = to[1][u][p];
         }
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-        if (t <= (wave | 1))
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                P[(16 * wave + 4 * g + i) * TRI + 16 * t + r] = qk[t][i];
     __syncthreads();
     // P and M, transposed (T^T times the other matrix's transpose), so that a lane holds
     // the columns of a row that it stores as a fragment
     const int64_t unit = (int64_t)tile * a.v_heads + h;
-    uint8_t *const to = a.work + a.plan.tri + unit * (kDeltaTri + KD * 256) + lane * 16;
-    auto store = [&](int at, gd_f4 left, gd_f4 right) {
-        gd_h8 hi, lo;
-        gd_split(__builtin_shufflevector(left, right, 0, 1, 2, 3, 4, 5, 6, 7), BACK, hi, lo);
-        *(gd_h8 *)(to + at) = hi;
-        *(gd_h8 *)(to + at + 1024) = lo;
+    uint8_t *const tri = a.work + a.plan.tri + unit * (kDeltaTri + KD * 256) + lane * 16;
+    auto store = [&](int n, gd_f4 left, gd_f4 right) { // the n-th tile of P and M
+        *(gd_f4 *)(tri + n * 2048) = left;
+        *(gd_f4 *)(tri + n * 2048 + 1024) = right;
+    };
+    auto load = [&](int which, int jt, int k, gd_b8(&part)[3]) {
+#pragma unroll
+        for (int p = 0; p < 3; ++p)
+            part[p] = *(const gd_b8 *)(tt[which][jt < 2 ? 2 * jt + k : 2 + jt][p] + lane * 16);
     };
     gd_f4 out[4];
-    {
-        gd_h8 hi[2], lo[2];
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const float *from = P + row * TRI + 32 * k + 4 * g;
-            gd_f8 x{};
-            if (k <= wave / 2)
-                x = __builtin_shufflevector(*(const gd_f4 *)from, *(const gd_f4 *)(from + 16), 0, 1, 2, 3, 4, 5, 6, 7);
-            gd_split(x, UP, hi[k], lo[k]);
+    for (int jt = 0; jt < 4; ++jt) {
+        gd_f4 x{}, y{};
+#pragma unroll
+        for (int k = jt / 2; k < 2; ++k) {
+            if (jt > wave || k > wave / 2)
+                continue;
+            gd_b8 t[3];
+            load(0, jt, k, t);
+            gd_dot(t, pf[k], x, y);
         }
-#pragma unroll
-        for (int jt = 0; jt < 4; ++jt) {
-            gd_f4 x{}, y{};
-#pragma unroll
-            for (int k = jt / 2; k < 2; ++k) {
-                if (jt > wave || k > wave / 2)
-                    continue;
-                const uint8_t(*f)[1024] = tt[0][jt < 2 ? 2 * jt + k : 2 + jt];
-                const gd_h8 th = *(const gd_h8 *)(f[0] + lane * 16), tl = *(const gd_h8 *)(f[1] + lane * 16);
-                x = gd_mfma(th, hi[k], x);
-                y = gd_mfma(th, lo[k], y);
-                y = gd_mfma(tl, hi[k], y);
-            }
-            out[jt] = x + y * (1.0f / REST);
-        }
-        const int t0 = wave < 2 ? wave : 2 * wave - 2; // this wave's first tile of a triangle
-        store(2 * t0 * 1024, out[0], out[1]);
-        if (wave >= 2)
-            store((2 * t0 + 2) * 1024, out[2], out[3]);
+        out[jt] = x + y;
     }
+    const int t0 = wave < 2 ? wave : 2 * wave - 2; // this wave's first tile of a triangle
+    store(t0, out[0], out[1]);
+    if (wave >= 2)
+        store(t0 + 1, out[2], out[3]);
 #pragma unroll
     for (int m = 0; m < MD; ++m) {
 #pragma unroll
@@ -380,24 +439,22 @@ __global__ void __launch_bounds__(PREP_THREADS) k_delta_prep(DeltaArgs a)
             gd_f4 x{}, y{};
 #pragma unroll
             for (int k = jt / 2; k < 2; ++k) {
-                const uint8_t(*f)[1024] = tt[1][jt < 2 ? 2 * jt + k : 2 + jt];
-                const gd_h8 th = *(const gd_h8 *)(f[0] + lane * 16), tl = *(const gd_h8 *)(f[1] + lane * 16);
-                x = gd_mfma(th, kt[m][k][0], x);
-                y = gd_mfma(tl, kt[m][k][0], y);
-                if (PARTS > 1)
-                    y = gd_mfma(th, kt[m][k][PARTS - 1], y);
+                gd_b8 t[3];
+                load(1, jt, k, t);
+                gd_dot(t, kt[m][k], x, y);
             }
-            out[jt] = x + y * (1.0f / REST);
+            out[jt] = x + y;
         }
         const int md = MD * wave + m;
-        store(kDeltaTri + 2 * md * 2048, out[0], out[1]);
-        store(kDeltaTri + (2 * md + 1) * 2048, out[2], out[3]);
+        store(6 + 2 * md, out[0], out[1]);
+        store(6 + 2 * md + 1, out[2], out[3]);
     }
     float *const f = (float *)(a.work + a.plan.rows) + unit * kDeltaRows;
     if (wave == 0) {
         f[lane] = rk[lane] * gd_exp2(G[lane]); // of K S
+        f[128 + lane] = beta[lane] * gd_exp2(G[63] - G[lane]); // of what a token adds to S
         if (lane == 0)
-            f[128] = gd_exp2(G[63]);
+            f[192] = gd_exp2(G[63]);
     }
     if (g == 0)
         f[64 + row] = rq * gd_exp2(G[row]); // of Q S
@@ -410,8 +467,9 @@ constexpr int SCAN_WAVES = 4;
 // of its 16 tokens and their values in its columns.
 template <int KS, int PARTS>
 struct ScanOps {
-    gd_h8 k[KS][PARTS], q[KS][PARTS], m[2][2][2], p[2][2];
-    gd_f4 fk, fq;
+    gd_h8 k[KS][PARTS], q[KS][PARTS];
+    gd_f4 m[2][2][2], p[2][2]; // in fp32
+    gd_f4 fk, fq, fs;
     uint32_t v[4]; // as they lie in memory
     float keep;
 };
@@ -426,18 +484,19 @@ __device__ __forceinline__ void scan_sync()
 // A workgroup takes 16 columns of one head of one sequence, each of its waves the
 // tokens 16 w .. 16 w + 15 of a chunk and the rows 32 w .. 32 w + 31 of S (there are
 // KD / 32 such waves).  A wave so reads only its own part of the operands, from memory
-// into registers, two chunks ahead, and the waves exchange S and X as fp16 fragments in LDS,
-// with two barriers a chunk.  Bound by that chain, as a chunk follows the other: 8192
-// tokens of 32 heads of 128 x 128 take 286 us, 2.2 a chunk on every CU, of which the
-// products, exchanges and barriers alone are 1.2 and the operands' way (76 KB a chunk and CU)
-// adds 0.6 from L2 and 0.4 from further away.  (One chunk ahead 322, three 274, with registers that
-// let one workgroup on a CU where sequences would give it two; 32 columns a workgroup, which halves
-// the bytes and the CUs in use, 385.)
+// into registers, two chunks ahead, and the waves exchange S and X as fragments in LDS,
+// with two barriers a chunk.  Bound by that chain, as a chunk follows the other, and by the
+// operands' way: 8192 tokens of 32 heads of 128 x 128 take 286 us, 2.2 a chunk of 76 KB on every CU
+// (35 KB a microsecond).  (In a form with half the products, which took as long, products, exchanges and
+// barriers alone were 1.2 a chunk, and the operands added 0.6 from L2 and 0.4 from further away; one
+// chunk ahead was 322, three 274; 32 columns a workgroup, which halves the bytes and the CUs in
+// use, 385.  M and P in parts as they are stored, half as many bytes again: 354.)
 //
-// One power of two serves a column for a whole chunk.  k and q have unit length at most,
-// and no token adds more than |v| to the length of a column of S, so |X| and the
-// new S lie below 12 max |S| + 66 max |v| (sqrt(128) < 12).  Fragments keep 22 bits of
-// what is over 2^-27 of that.
+// A column of S has a power of two for every chunk, from a bound that no token passes: k and q
+// have unit length at most, a token adds no more than beta |v| to a column's length, and
+// all of it fades, so that S after a chunk lies below 12 e^G_64 max |S| + 66 max(e^(G_64 - G) beta
+// |v|) (sqrt(128) < 12).  Values down to 2^-27 of that keep 22 bits, and smaller ones
+// 2^-49 of it.
 template <int TYPE, int KD>
 __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
 {
@@ -446,7 +505,7 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
     constexpr int FRAG = 4 * KS * PARTS * 1024;
     constexpr int VB = PARTS > 1 ? 4 : 2; // bytes of a value of V
     using Ops = ScanOps<KS, PARTS>;
-    __shared__ __attribute__((aligned(16))) uint8_t sf[KS][2][1024], xf[2][2][1024];
+    __shared__ __attribute__((aligned(16))) uint8_t sf[KS][2][1024], xf[2][3][1024];
     __shared__ float bounds[SCAN_WAVES][16];
     __shared__ __attribute__((aligned(16))) float turn[SCAN_WAVES][16][20];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, r = lane & 15;
@@ -458,12 +517,14 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
     if (u >= a.k_heads * a.batch.sequences)
         return;
     const int s = u / a.k_heads, kh = u % a.k_heads, h = kh * a.group + j % each / blocks;
-    const GdSeq seq = gd_seq(a.batch, a.pool, s, h == 0 && j % blocks == 0 ? a.flags : nullptr);
+    GdSeq seq = gd_seq(a.batch, a.pool, s, h == 0 && j % blocks == 0 ? a.flags : nullptr);
     if (seq.slot < 0 || seq.n <= a.few)
         return;
+    // (one value a workgroup, and so one address a chunk for what all lanes read beside each other)
+    seq.start = __builtin_amdgcn_readfirstlane(seq.start), seq.n = __builtin_amdgcn_readfirstlane(seq.n);
     const int col0 = j % blocks * 16;
     float *const state = a.state + seq.slot * a.slot_step + (int64_t)h * a.k_dim * a.v_dim + col0 + r;
-    const int chunks = (seq.n + 63) / 64, tile0 = gd_base(a.batch, kDeltaShift, s);
+    const int chunks = (seq.n + 63) / 64, tile0 = (seq.start >> kDeltaShift) + s;
     const bool owner = wave < KS;
     int64_t vat[4]; // of this lane's values of V in a whole chunk
 #pragma unroll
@@ -471,25 +532,28 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
         vat[i] = ((16 * wave + 4 * g + i) * a.v_step + r) * VB;
     const int64_t oat = (int64_t)(16 * wave + lane / 4) * a.v_heads * a.v_dim + 4 * (lane % 4);
 
-    // A chunk's operands, in two portions: those of the chunk after the next follow
-    // as soon as their registers are free.  (Behind the last chunk: its operands again.)
-    auto at_kq = [&](int c) { return a.work + ((int64_t)(tile0 + min(c, chunks - 1)) * a.k_heads + kh) * 2 * FRAG + lane * 16; };
+    // A chunk's operands: those of the chunk after the next follow one by one, as soon as
+    // their registers are free.  Loads that follow each other hold the wave up; between the
+    // products they do not (8192 tokens 359 us of scan with the loads of K and Q, and of M
+    // and P, together, 286 so).  (Behind the last chunk: its operands again.)
+    const uint32_t mine = lane * 16;
+    auto at_kq = [&](int c) { return a.work + ((int64_t)(tile0 + min(c, chunks - 1)) * a.k_heads + kh) * 2 * FRAG; };
     auto at_unit = [&](int c) { return (int64_t)(tile0 + min(c, chunks - 1)) * a.v_heads + h; };
-    auto load_kqv = [&](Ops &o, int c) {
-        const uint8_t *const kq = at_kq(c);
+    auto load_key = [&](Ops &o, int c, int k) {
+        const uint8_t *const kq = at_kq(c) + (wave * KS + k) * PARTS * 1024;
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) {
+            o.k[k][p] = *(const gd_h8 *)(kq + p * 1024 + mine);
+            o.q[k][p] = *(const gd_h8 *)(kq + FRAG + p * 1024 + mine);
+        }
+    };
+    auto load_rows = [&](Ops &o, int c) {
         const float *const f = (const float *)(a.work + a.plan.rows) + at_unit(c) * kDeltaRows;
-#pragma unroll
-        for (int k = 0; k < KS; ++k)
-#pragma unroll
-            for (int p = 0; p < PARTS; ++p)
-                o.k[k][p] = *(const gd_h8 *)(kq + ((wave * KS + k) * PARTS + p) * 1024);
-#pragma unroll
-        for (int k = 0; k < KS; ++k)
-#pragma unroll
-            for (int p = 0; p < PARTS; ++p)
-                o.q[k][p] = *(const gd_h8 *)(kq + FRAG + ((wave * KS + k) * PARTS + p) * 1024);
-        o.fk = *(const gd_f4 *)(f + 16 * wave + 4 * g);
-        o.fq = *(const gd_f4 *)(f + 64 + 16 * wave + 4 * g);
+        const uint32_t at = 16 * wave + 4 * g;
+        o.fk = *(const gd_f4 *)(f + at);
+        o.fq = *(const gd_f4 *)(f + 64 + at);
+        o.fs = *(const gd_f4 *)(f + 128 + at);
+        o.keep = f[192];
         // (rows behind the last token: others', not used)
         const int at0 = 64 * min(c, chunks - 1);
         const uint8_t *const v = (const uint8_t *)a.v + ((seq.start + at0) * a.v_step + (int64_t)h * a.v_dim + col0) * VB;
@@ -501,35 +565,34 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
             o.v[i] = PARTS > 1 ? *(const uint32_t *)at : *(const uint16_t *)at;
         }
     };
-    auto load_pm = [&](Ops &o, int c) {
-        o.keep = ((const float *)(a.work + a.plan.rows) + at_unit(c) * kDeltaRows)[128];
-        const uint8_t *const tri = a.work + a.plan.tri + at_unit(c) * (kDeltaTri + KD * 256) + lane * 16;
-        const int t0 = wave < 2 ? wave : 2 * wave - 2; // this wave's first tile of a triangle
+    auto at_tri = [&](int c) { return a.work + a.plan.tri + at_unit(c) * (kDeltaTri + KD * 256); };
+    auto load_tile = [&](gd_f4(&to)[2], int c, int n) { // the n-th of P and M
+        const uint8_t *const from = at_tri(c) + n * 2048;
+        to[0] = *(const gd_f4 *)(from + mine);
+        to[1] = *(const gd_f4 *)(from + 1024 + mine);
+    };
+    const int p0 = wave < 2 ? wave : 2 * wave - 2; // this wave's first tile of P
+    auto load_p = [&](Ops &o, int c) {
+        load_tile(o.p[0], c, p0);
+        if (wave >= 2)
+            load_tile(o.p[1], c, p0 + 1);
+    };
+    auto load_m = [&](Ops &o, int c, int m, int k) { load_tile(o.m[m][k], c, 6 + 2 * (2 * wave + m) + k); };
+    auto load_all = [&](Ops &o, int c) {
 #pragma unroll
-        for (int p = 0; p < 2; ++p) {
-            o.p[0][p] = *(const gd_h8 *)(tri + (2 * t0 + p) * 1024);
-            if (wave >= 2)
-                o.p[1][p] = *(const gd_h8 *)(tri + (2 * t0 + 2 + p) * 1024);
-        }
+        for (int k = 0; k < KS; ++k)
+            load_key(o, c, k);
+        load_rows(o, c);
+        load_p(o, c);
         if (owner)
 #pragma unroll
             for (int m = 0; m < 2; ++m)
 #pragma unroll
                 for (int k = 0; k < 2; ++k)
-#pragma unroll
-                    for (int p = 0; p < 2; ++p)
-                        o.m[m][k][p] = *(const gd_h8 *)(tri + kDeltaTri + ((2 * (2 * wave + m) + k) * 2 + p) * 1024);
+                    load_m(o, c, m, k);
     };
+    auto wide = [](const gd_f4 (&half)[2]) { return __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7); };
     auto most4 = [](gd_f4 x) { return fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))); };
-    // four values of a column as half a fragment's 8
-    auto put = [&](uint8_t (*to)[2][1024], gd_f4 x, float by) {
-        typedef _Float16 h4 __attribute__((ext_vector_type(4)));
-        x = x * by;
-        const h4 hi = __builtin_convertvector(x, h4);
-        const h4 lo = __builtin_convertvector((x - __builtin_convertvector(hi, gd_f4)) * REST, h4);
-        *(h4 *)(to[wave / 2][0] + lane * 16 + 8 * (wave & 1)) = hi;
-        *(h4 *)(to[wave / 2][1] + lane * 16 + 8 * (wave & 1)) = lo;
-    };
 
     gd_f4 S[2];
     float to_s, back_s;
@@ -549,6 +612,14 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
     };
     gd_power(widest(), to_s, back_s);
     scan_sync();
+    auto put_s = [&]() { // S as a fragment
+        gd_h8 hi, lo;
+        gd_split(__builtin_shufflevector(S[0], S[1], 0, 1, 2, 3, 4, 5, 6, 7), to_s, hi, lo);
+        *(gd_h8 *)(sf[wave][0] + lane * 16) = hi;
+        *(gd_h8 *)(sf[wave][1] + lane * 16) = lo;
+    };
+    if (owner)
+        put_s();
 
     auto chunk = [&](Ops &o, int c) {
         const int n = min(64, seq.n - 64 * c);
@@ -558,80 +629,71 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
             const float x = TYPE == kF32 ? __uint_as_float(o.v[i]) : TYPE == kF16 ? h2f(o.v[i]) : __uint_as_float(o.v[i] << 16);
             v[i] = 16 * wave + 4 * g + i < n ? x : 0.0f;
         }
-        if (owner) {
-            gd_h8 hi, lo;
-            gd_split(__builtin_shufflevector(S[0], S[1], 0, 1, 2, 3, 4, 5, 6, 7), to_s, hi, lo);
-            *(gd_h8 *)(sf[wave][0] + lane * 16) = hi;
-            *(gd_h8 *)(sf[wave][1] + lane * 16) = lo;
-        }
-        const float most = 12.0f * fmaxf(most4(S[0]), most4(S[1])) + 66.0f * most4(v);
+        const float most = 12.0f * o.keep * fmaxf(most4(S[0]), most4(S[1])) + 66.0f * most4(v * o.fs);
         const float all = gd_max32(gd_max16(most));
         if (g == 0)
             bounds[wave][r] = all;
         scan_sync();
         // K S and Q S; X = V - e^G K S
         gd_f4 qs;
-        float to, back;
-        gd_power(widest(), to, back);
+        const float next = widest(), keep = o.keep;
         {
-            gd_h8 hi[KS], lo[KS];
-#pragma unroll
-            for (int k = 0; k < KS; ++k) {
-                hi[k] = *(const gd_h8 *)(sf[k][0] + lane * 16);
-                lo[k] = *(const gd_h8 *)(sf[k][1] + lane * 16);
-            }
             gd_f4 x{}, y{}, z{}, w{};
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
-                x = gd_mfma(o.k[k][0], hi[k], x);
-                y = gd_mfma(o.k[k][0], lo[k], y);
-                if (PARTS > 1)
-                    y = gd_mfma(o.k[k][PARTS - 1], hi[k], y);
+                const gd_h8 hi = *(const gd_h8 *)(sf[k][0] + lane * 16), lo = *(const gd_h8 *)(sf[k][1] + lane * 16);
+                x = gd_mfma(o.k[k][0], hi, x);
+                y = gd_mfma(o.k[k][0], lo, y);
+                z = gd_mfma(o.q[k][0], hi, z);
+                w = gd_mfma(o.q[k][0], lo, w);
+                if (PARTS > 1) {
+                    y = gd_mfma(o.k[k][PARTS - 1], hi, y);
+                    w = gd_mfma(o.q[k][PARTS - 1], hi, w);
+                }
+                load_key(o, c + 2, k);
             }
+            gd_b4 part[3]; // half a fragment
+            gd_split3(v - o.fk * ((x + y * (1.0f / REST)) * back_s), part);
 #pragma unroll
-            for (int k = 0; k < KS; ++k) {
-                z = gd_mfma(o.q[k][0], hi[k], z);
-                w = gd_mfma(o.q[k][0], lo[k], w);
-                if (PARTS > 1)
-                    w = gd_mfma(o.q[k][PARTS - 1], hi[k], w);
-            }
-            put(xf, v - o.fk * ((x + y * (1.0f / REST)) * back_s), to);
+            for (int p = 0; p < 3; ++p)
+                *(gd_b4 *)(xf[wave / 2][p] + lane * 16 + 8 * (wave & 1)) = part[p];
             qs = (z + w * (1.0f / REST)) * back_s * o.fq;
         }
-        load_kqv(o, c + 2);
+        load_rows(o, c + 2);
         scan_sync();
         // S <- e^G_64 S + M X;  O = scale (e^G Q S + P X)
-        gd_h8 hi[2], lo[2];
+        gd_b8 xp[2][3];
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            hi[k] = *(const gd_h8 *)(xf[k][0] + lane * 16);
-            lo[k] = *(const gd_h8 *)(xf[k][1] + lane * 16);
-        }
-        const float by = back * (1.0f / (1 << TOP));
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int p = 0; p < 3; ++p)
+                xp[k][p] = *(const gd_b8 *)(xf[k][p] + lane * 16);
+        gd_power(next, to_s, back_s);
         if (owner) {
             gd_f4 x[2]{}, y[2]{};
 #pragma unroll
             for (int k = 0; k < 2; ++k)
 #pragma unroll
                 for (int m = 0; m < 2; ++m) {
-                    x[m] = gd_mfma(o.m[m][k][0], hi[k], x[m]);
-                    y[m] = gd_mfma(o.m[m][k][0], lo[k], y[m]);
-                    y[m] = gd_mfma(o.m[m][k][1], hi[k], y[m]);
+                    gd_b8 part[3];
+                    gd_split3(wide(o.m[m][k]), part);
+                    gd_dot(part, xp[k], x[m], y[m]);
+                    load_m(o, c + 2, m, k);
                 }
 #pragma unroll
             for (int m = 0; m < 2; ++m)
-                S[m] = S[m] * o.keep + (x[m] + y[m] * (1.0f / REST)) * by;
+                S[m] = S[m] * keep + (x[m] + y[m]);
+            put_s();
         }
         gd_f4 x{}, y{};
-        x = gd_mfma(o.p[0][0], hi[0], x);
-        y = gd_mfma(o.p[0][0], lo[0], y);
-        y = gd_mfma(o.p[0][1], hi[0], y);
-        if (wave >= 2) {
-            x = gd_mfma(o.p[1][0], hi[1], x);
-            y = gd_mfma(o.p[1][0], lo[1], y);
-            y = gd_mfma(o.p[1][1], hi[1], y);
-        }
-        const gd_f4 out = a.scale * (qs + (x + y * (1.0f / REST)) * by);
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+            if (k == 0 || wave >= 2) {
+                gd_b8 part[3];
+                gd_split3(wide(o.p[k]), part);
+                gd_dot(part, xp[k], x, y);
+            }
+        const gd_f4 out = a.scale * (qs + (x + y));
         // through LDS, so that a lane stores 4 neighbours
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -644,12 +706,10 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
             else
                 gd_store4(a.out, where, a.out_type, flat);
         }
-        to_s = to, back_s = back;
-        load_pm(o, c + 2);
+        load_p(o, c + 2);
     };
     Ops even, odd;
-    load_kqv(even, 0), load_pm(even, 0);
-    load_kqv(odd, 1), load_pm(odd, 1);
+    load_all(even, 0), load_all(odd, 1);
     int c = 0;
     for (; c + 1 < chunks; c += 2) { // (no way out between: the operands stay in their registers)
         chunk(even, c);

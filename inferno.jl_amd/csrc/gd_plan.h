@@ -9,8 +9,8 @@
 namespace ihip {
 
 constexpr int kDeltaShift = 6;  // a chunk is 64 tokens
-constexpr int kDeltaTri = 6 * 2 * 1024; // a 64 x 64 lower triangle: 6 tiles of 16 x 32 in two fp16 parts
-constexpr int kDeltaRows = 192;  // floats of a chunk's row factors
+constexpr int kDeltaTri = 6 * 2 * 1024; // a 64 x 64 lower triangle: 6 tiles of 16 x 32 fp32 values
+constexpr int kDeltaRows = 256;  // floats of a chunk's row factors
 
 // Numbers of tiles of 2^shift rows that sequences of `tokens` rows in all can have.
 constexpr int64_t gd_tiles(int64_t tokens, int64_t sequences, int shift)
