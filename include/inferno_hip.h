@@ -588,7 +588,7 @@ typedef struct ihip_delta_layer {
 } ihip_delta_layer;
 
 /* For every new token of a sequence and every head, with S the head's state,
- *   q^ = q / sqrt(|q|^2 + l2_eps), k^ alike,  beta = sigmoid(b),
+ *   q^ = q / sqrt(|q|^2 + l2_eps), k^ alike (zeros stay zeros),  beta = sigmoid(b),
  *   S <- exp(decay * softplus(a + dt_bias)) S;  S <- S + beta k^ (v - k^T S)^T;
  *   o = scale * q^T S
  * and out = o, divided by sqrt(mean(o^2) + norm_eps) and times norm_w where that is

@@ -75,7 +75,9 @@ __global__ void __launch_bounds__(STEP_THREADS) k_delta_step(DeltaArgs a)
                 x[i] = in ? (float)xr[i] : 0.0f, y[i] = in ? (float)yr[i] : 0.0f;
                 xx += (double)x[i] * x[i], yy += (double)y[i] * y[i], xy += (double)x[i] * y[i];
             }
-            const double rq = 1.0 / sqrt(gd_wave_sum(xx) + (double)a.l2_eps), rk = 1.0 / sqrt(gd_wave_sum(yy) + (double)a.l2_eps);
+            xx = gd_wave_sum(xx) + (double)a.l2_eps, yy = gd_wave_sum(yy) + (double)a.l2_eps;
+            // (a row of zeros stays one, without an eps too)
+            const double rq = xx == 0.0 ? 0.0 : 1.0 / sqrt(xx), rk = yy == 0.0 ? 0.0 : 1.0 / sqrt(yy);
             xy = gd_wave_sum(xy);
 #pragma unroll
             for (int i = 0; i < E; ++i) {

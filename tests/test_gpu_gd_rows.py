@@ -148,3 +148,16 @@ def test_fades(kind, total, new):
         if at is not None:
             c.a[at] = -total
         check(c)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("new", [[9], [100], [100, 3]])
+def test_rows_of_zeros_without_an_eps(kind, new):
+    """A row of zeros stays one where l2_eps is 0 too, by steps and in chunks."""
+    c = Case(17, new, [False] * len(new), dk=64, dv=32, kind=TYPES[kind], out=F32, gate=False, norm=False)
+    K = c.K * 64
+    c.qkv[2, :K] = 0
+    c.qkv[4, K:2 * K] = 0
+    c.qkv[-1, :2 * K] = 0
+    # (as the definition's limit: 0 / sqrt(0 + 1e-300), which changes no other row in 64 bits)
+    c.check(c.run(l2_eps=0.0), c.plain(l2_eps=1e-300))
