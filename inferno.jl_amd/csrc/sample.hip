@@ -164,7 +164,7 @@ __device__ void sample_whole_row(const SampleArgs &a, int row, const SampleRow &
                 if (k == border)
                     keep = rank++ < ties;
                 m[j] = keep && t0 + 4 * tid + j < a.vocab ? sample_weight(sc, l[j]) : 0.0;
-                if (m[j] < low && k != best)
+                if (m[j] < low && t0 + 4 * tid + j != at)
                     m[j] = 0.0;
                 sum += m[j];
             }
