@@ -342,7 +342,7 @@ __device__ __forceinline__ double wg_sum(double v, double *part)
 // then 32 to a factor of 2 in distance.  In order of the logits.
 __device__ __forceinline__ int bin_of(float l, float most, float rate)
 {
-    const float d = (most - l) * rate;
+    const float d = fmaf(-0.5f, l, 0.5f * most) * rate; // (halves: the difference of two logits may pass the range)
     if (d < 32.0f)
         return (int)(d * 16.0f);
     constexpr uint32_t from = 0x42000000u >> 18; // 32
@@ -351,9 +351,9 @@ __device__ __forceinline__ int bin_of(float l, float most, float rate)
 // From this bin on (over 1150 factors of 2 below the largest) weights are 0 in 64 bits:
 // where top-k's cut falls among them it cuts nothing that counts.
 constexpr int ZERO_BIN = 680;
-__device__ __forceinline__ float bin_rate(float t)
+__device__ __forceinline__ float bin_rate(float t) // of half a difference
 {
-    return fminf(1.44269504f / t, 3e38f);
+    return fminf(2 * 1.44269504f / t, 3e38f);
 }
 
 __device__ __forceinline__ bool filtered(const SampleRow &r, int vocab, bool &by_k, bool &by_p)
