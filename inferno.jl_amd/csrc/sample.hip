@@ -908,9 +908,11 @@ __global__ void __launch_bounds__(ROW_THREADS) k_sample_pick(SampleArgs a)
             double x = sample_weight(sc, sample_value((uint32_t)(order[i] >> 32)));
             x = x >= low || order[i] == best ? x : 0.0;
             w += x;
-            // (to their slices as whole numbers: in any order)
+            // (to their slices as whole numbers: in any order.  Where the last kept token is
+            // asked for, a slice with one is not to look empty.)
             if (x > 0.0)
-                atomicAdd(&u.list.mass[~(uint32_t)order[i] / (uint32_t)a.plan.per], (unsigned long long)rint(ldexp(x, sc.bits)));
+                atomicAdd(&u.list.mass[~(uint32_t)order[i] / (uint32_t)a.plan.per],
+                          (unsigned long long)fmax(rint(ldexp(x, sc.bits)), r.u >= 1.0f ? 1.0 : 0.0));
         }
         total += wg_sum(w, lds.part);
         if (tid < a.plan.slices)

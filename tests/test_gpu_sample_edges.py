@@ -33,3 +33,14 @@ def test_logits_whose_differences_pass_the_range(t):
     check(x, u, [t] * 6, [2000, 500, 40, 1600, 2500, 1400])
     check(x, u, [t] * 6, None, [0.99, 0.9, 0.9999, 0.999, 0.7, 0.5])
     check(x, u, [t] * 6, [1600] * 6, [0.999] * 6)
+
+
+@pytest.mark.parametrize("u", [1.0, 7.0])
+def test_the_last_kept_token_hardly_weighs(u):
+    """Where no sum passes u of all, the last kept token is taken, also one of 2^-65 of the weights in a slice of its own."""
+    x = torch.full((3, 20000), -100.0)
+    x[:, 3] = 0.0
+    x[0, 19000], x[1, 9000], x[2, 100] = -45.0, -45.0, -45.0
+    check(x, [u] * 3, [1.0] * 3, [2] * 3)
+    check(x, [u] * 3, [1.0] * 3, [3] * 3, [1.0] * 3)
+    check(x, [u] * 3, [1.0] * 3)
