@@ -634,8 +634,8 @@ size_t ihip_gated_delta_scratch_bytes(int type, const ihip_delta_layer *layer,
  * such a value (the token is then 0 and the logprob NaN), IHIP_FLAG_ALL_NEGINF where
  * every logit is -infinity (the token is 0), else 0.  Everything is device memory.
  * workspace: ihip_sample_scratch_bytes bytes, 16-byte aligned; its contents do not
- * matter.  Calls that share it must not overlap on the GPU.  At most 2^22 logits a
- * row. */
+ * matter, and one that does for so many rows and logits does for fewer.  Calls that
+ * share it must not overlap on the GPU.  At most 2^22 logits a row. */
 int ihip_sample_dev(const void *logits, int type, int64_t row_stride, int rows, int vocab,
                     const float *temperature, const int32_t *top_k, const float *top_p,
                     const float *min_p, const float *u, int32_t *tokens, float *logprobs,

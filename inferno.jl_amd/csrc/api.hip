@@ -1975,7 +1975,7 @@ int ihip_gated_delta_dev(const void *q, int64_t q_stride, const void *k, int64_t
 
 size_t ihip_sample_scratch_bytes(int rows, int vocab)
 {
-    return rows <= 0 || vocab <= 0 || vocab > kSampleVocab ? 0 : sample_plan(rows, vocab).bytes;
+    return rows <= 0 || vocab <= 0 || vocab > kSampleVocab ? 0 : sample_scratch(rows, vocab);
 }
 
 int ihip_sample_dev(const void *logits, int type, int64_t row_stride, int rows, int vocab,

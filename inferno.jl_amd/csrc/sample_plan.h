@@ -27,6 +27,17 @@ struct SamplePlan {
     size_t bounds, bins, merged, list, bytes;
 };
 
+// The areas of `all` slices in p.rows rows
+inline void sample_areas(SamplePlan &p, size_t all)
+{
+    const size_t n = (size_t)p.rows;
+    p.bounds = (all * kSamplePart + 63) / 64 * 64;
+    p.bins = p.bounds + n * kSampleRecord;
+    p.merged = p.bins + all * kSampleBins * 12;
+    p.list = p.merged + n * kSampleBins * 12;
+    p.bytes = p.list + n * kSampleList * 8;
+}
+
 inline SamplePlan sample_plan(int rows, int vocab)
 {
     SamplePlan p{};
@@ -36,13 +47,21 @@ inline SamplePlan sample_plan(int rows, int vocab)
     p.per = rows * wide >= 512 || narrow > kSampleSlices ? kSampleWide : kSampleNarrow;
     p.slices = (int)(p.per == kSampleWide ? wide : narrow);
     p.rows = rows < kSampleRows ? rows : kSampleRows;
-    const size_t n = (size_t)p.rows, all = n * (size_t)p.slices;
-    p.bounds = (all * kSamplePart + 63) / 64 * 64;
-    p.bins = p.bounds + n * kSampleRecord;
-    p.merged = p.bins + all * kSampleBins * 12;
-    p.list = p.merged + n * kSampleBins * 12;
-    p.bytes = p.list + n * kSampleList * 8;
+    sample_areas(p, (size_t)p.rows * (size_t)p.slices);
     return p;
+}
+
+// Bytes that do for these rows and logits and for every call of no more of either.  Fewer rows, or
+// logits, may have more slices, as theirs are narrow: rows * wide < 512 then, and narrow <= 2
+// wide, so that there are at most 1022 of those.
+inline size_t sample_scratch(int rows, int vocab)
+{
+    const int64_t wide = (vocab + kSampleWide - 1) / kSampleWide, narrow = (vocab + kSampleNarrow - 1) / kSampleNarrow;
+    SamplePlan p{};
+    p.rows = rows < kSampleRows ? rows : kSampleRows;
+    const int64_t narrows = p.rows * narrow < 1022 ? p.rows * narrow : 1022;
+    sample_areas(p, (size_t)(p.rows * wide > narrows ? p.rows * wide : narrows));
+    return p.bytes;
 }
 
 } // namespace ihip
