@@ -611,7 +611,8 @@ int ihip_gated_delta_dev(const void *q, int64_t q_stride, const void *k, int64_t
                          uint32_t *flags, void *workspace, size_t workspace_bytes,
                          ihip_stream stream);
 /* From the sizes alone (of the layer and the batch, `most` among them), for any
- * contents of the batch's arrays. */
+ * contents of the batch's arrays, and enough for every batch of no more tokens,
+ * sequences and `most` (where that is 0, the tokens count as it). */
 size_t ihip_gated_delta_scratch_bytes(int type, const ihip_delta_layer *layer,
                                       const ihip_state_batch *batch);
 

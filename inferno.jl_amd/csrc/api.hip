@@ -1897,9 +1897,8 @@ size_t ihip_gated_delta_scratch_bytes(int type, const ihip_delta_layer *layer,
     if (check_layer(layer, &a) != IHIP_OK || check_states(batch, &a.batch) != IHIP_OK || !value_bytes(type) ||
         a.batch.tokens == 0 || a.batch.sequences == 0)
         return 0;
-    return delta_plan(type == kF32 ? 2 : 1, a.k_heads, a.v_heads, a.k_dim, a.v_dim, a.batch.tokens, a.batch.sequences,
-                      batch->most)
-        .bytes;
+    return delta_scratch(type == kF32 ? 2 : 1, a.k_heads, a.v_heads, a.k_dim, a.v_dim, a.batch.tokens, a.batch.sequences,
+                         batch->most);
 }
 
 int ihip_gated_delta_dev(const void *q, int64_t q_stride, const void *k, int64_t k_stride,

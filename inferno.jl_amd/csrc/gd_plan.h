@@ -57,17 +57,16 @@ struct DeltaPlan {
     size_t tri, rows, raw, bytes; // offsets (K and Q first; P and M, factors, raw outputs) and the size
 };
 
-// parts: fp16 values that a value of K or Q is held in (2 for fp32, else 1)
-inline DeltaPlan delta_plan(int parts, int k_heads, int v_heads, int k_dim, int v_dim, int64_t tokens, int64_t sequences,
-                            int most)
+// The longest sequence that a batch may have
+constexpr int64_t delta_longest(int64_t tokens, int most)
 {
-    DeltaPlan p{};
-    const int64_t longest = most > 0 && most < tokens ? most : tokens;
-    p.chunks = longest > delta_few(v_heads, sequences);
-    p.steps = !p.chunks || sequences > 1;
-    p.few = p.steps ? delta_few_beside(v_heads, sequences) : 0;
-    if (!p.chunks)
-        return p;
+    return most > 0 && most < tokens ? most : tokens;
+}
+
+// The areas of chunks in the workspace.  parts: fp16 values that a value of K or Q is held in (2
+// for fp32, else 1)
+inline void delta_areas(DeltaPlan &p, int parts, int k_heads, int v_heads, int k_dim, int v_dim, int64_t tokens, int64_t sequences)
+{
     p.tiles = gd_tiles(tokens, sequences, kDeltaShift);
     const int padded = k_dim <= 64 ? 64 : 128;
     p.frag = padded * 128 * parts;
@@ -75,7 +74,29 @@ inline DeltaPlan delta_plan(int parts, int k_heads, int v_heads, int k_dim, int 
     p.rows = p.tri + (size_t)p.tiles * (size_t)v_heads * (size_t)(kDeltaTri + padded * 256);
     p.raw = p.rows + (size_t)p.tiles * (size_t)v_heads * kDeltaRows * 4;
     p.bytes = p.raw + (parts == 1 ? (size_t)tokens * (size_t)v_heads * (size_t)v_dim * 4 : 0);
+}
+
+inline DeltaPlan delta_plan(int parts, int k_heads, int v_heads, int k_dim, int v_dim, int64_t tokens, int64_t sequences,
+                            int most)
+{
+    DeltaPlan p{};
+    p.chunks = delta_longest(tokens, most) > delta_few(v_heads, sequences);
+    p.steps = !p.chunks || sequences > 1;
+    p.few = p.steps ? delta_few_beside(v_heads, sequences) : 0;
+    if (p.chunks)
+        delta_areas(p, parts, k_heads, v_heads, k_dim, v_dim, tokens, sequences);
     return p;
+}
+
+// Bytes that do for a batch of these sizes and for every one of no more tokens, sequences and
+// `most`: fewer sequences go in chunks at lengths at which more of them go by steps.
+inline size_t delta_scratch(int parts, int k_heads, int v_heads, int k_dim, int v_dim, int64_t tokens, int64_t sequences,
+                            int most)
+{
+    DeltaPlan p{};
+    if (delta_longest(tokens, most) > delta_few(v_heads, 1))
+        delta_areas(p, parts, k_heads, v_heads, k_dim, v_dim, tokens, sequences);
+    return p.bytes;
 }
 
 } // namespace ihip
