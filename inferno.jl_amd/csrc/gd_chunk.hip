@@ -749,14 +749,9 @@ __global__ void __launch_bounds__(NORM_THREADS) k_delta_norm(DeltaArgs a)
         const int64_t row = seq.start + t, at = (row * a.v_heads + h) * a.v_dim + e;
         gd_f4 o = live ? *(const gd_f4 *)(a.raw + at) : gd_f4{};
         if (a.norm_w) {
-            float sum = (o.x * o.x + o.y * o.y) + (o.z * o.z + o.w * o.w);
-            sum = gd_add_dpp<0xb1>(sum);
-            sum = gd_add_dpp<0x4e>(sum);
-            sum = gd_add_dpp<0x141>(sum);
-            sum = gd_add_dpp<0x140>(sum);
-            sum = gd_add16(sum);
+            o = gd_rms<32>(o, a.v_dim, a.norm_eps);
             if (live)
-                o = o * (1.0f / sqrtf(sum / (float)a.v_dim + a.norm_eps)) * *(const gd_f4 *)(a.norm_w + e);
+                o = o * *(const gd_f4 *)(a.norm_w + e);
         }
         if (!live)
             continue;

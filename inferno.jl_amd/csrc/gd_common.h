@@ -185,6 +185,38 @@ __device__ __forceinline__ double gd_wave_sum(double v)
     return v;
 }
 
+// A head's outputs of a token, LANES (16 or 32) neighbouring lanes with 4 each (zeros behind the
+// last column), divided by sqrt(their mean square + eps).  The squares of fp32 values pass its
+// range: they are formed of values times a power of two that makes the largest one 1 to 2.
+// Smaller ones than 1 stay as they are, where eps is over all that their squares could lose.
+template <int LANES>
+__device__ __forceinline__ gd_f4 gd_rms(gd_f4 o, int v_dim, float eps)
+{
+    // (the order of whole numbers is that of their sizes)
+    uint32_t most = max(max(__float_as_uint(fabsf(o.x)), __float_as_uint(fabsf(o.y))),
+                        max(__float_as_uint(fabsf(o.z)), __float_as_uint(fabsf(o.w))));
+    most = dpp_max_u32<0xb1, 0xf>(most);  // quad_perm [1,0,3,2]
+    most = dpp_max_u32<0x4e, 0xf>(most);  // quad_perm [2,3,0,1]
+    most = dpp_max_u32<0x141, 0xf>(most); // row_half_mirror
+    most = dpp_max_u32<0x140, 0xf>(most); // row_mirror
+    if (LANES == 32) {
+        const auto both = __builtin_amdgcn_permlane16_swap(most, most, false, false);
+        most = max(both[0], both[1]);
+    }
+    const int e = max((int)(most >> 23) - 127, eps > 0x1p-100f ? 0 : -100);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        o[i] = ldexpf(o[i], -e);
+    float sum = (o.x * o.x + o.y * o.y) + (o.z * o.z + o.w * o.w);
+    sum = gd_add_dpp<0xb1>(sum);
+    sum = gd_add_dpp<0x4e>(sum);
+    sum = gd_add_dpp<0x141>(sum);
+    sum = gd_add_dpp<0x140>(sum);
+    if (LANES == 32)
+        sum = gd_add16(sum);
+    return o * (1.0f / sqrtf(sum / (float)v_dim + ldexpf(eps, -2 * e)));
+}
+
 // A token's decay, in logarithms: decay * softplus(a + dt_bias).  A rate above 0 would
 // let the state grow without bound and is taken as 0; below e^-10000 nothing is left
 // in any type, and sums of such logarithms still hold their differences in 64 bits.

@@ -33,7 +33,7 @@ __global__ void __launch_bounds__(STEP_THREADS) k_delta_step(DeltaArgs a)
     constexpr int PAD = R + 4;              // (row groups apart in LDS)
     __shared__ __attribute__((aligned(16))) float qs[STEP_TOKENS][RG * PAD], ks[STEP_TOKENS][RG * PAD];
     __shared__ __attribute__((aligned(16))) float os[STEP_TOKENS][VD];
-    __shared__ float alpha[STEP_TOKENS], beta[STEP_TOKENS], qk[STEP_TOKENS], squares[STEP_TOKENS][STEP_WAVES];
+    __shared__ float alpha[STEP_TOKENS], beta[STEP_TOKENS], qk[STEP_TOKENS];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int h = blockIdx.x % a.v_heads, s = blockIdx.x / a.v_heads, kh = h / a.group;
     if (a.flags && blockIdx.x == 0)
@@ -123,12 +123,10 @@ __global__ void __launch_bounds__(STEP_THREADS) k_delta_step(DeltaArgs a)
             }
             const float al = alpha[t], be = beta[t], w = qk[t];
             gd_f4 d, o;
-            float sum = 0.0f;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 d[e] = be * (v[e] - al * kS[e]);
                 o[e] = a.scale * fmaf(w, d[e], al * qS[e]);
-                sum += o[e] * o[e];
             }
 #pragma unroll
             for (int i = 0; i < R; ++i)
@@ -137,25 +135,17 @@ __global__ void __launch_bounds__(STEP_THREADS) k_delta_step(DeltaArgs a)
                     S[i][e] = fmaf(k[i], d[e], al * S[i][e]);
             if (lane < CL)
                 *(gd_f4 *)&os[t][col0] = o;
-            if (a.norm_w) { // (columns behind v_dim hold zeros)
-                sum = gd_add_dpp<0x4e>(gd_add_dpp<0xb1>(sum)); // quad_perm [1,0,3,2], [2,3,0,1]
-                if (CL == 8)
-                    sum = gd_add_dpp<0x141>(sum); // row_half_mirror
-                if (lane == 0)
-                    squares[t][wave] = sum;
-            }
         }
         __syncthreads();
         for (int i = tid; i < n * (VD / 4); i += STEP_THREADS) {
             const int t = i / (VD / 4), e0 = 4 * (i % (VD / 4));
+            gd_f4 o = *(const gd_f4 *)&os[t][e0]; // (columns behind v_dim hold zeros)
+            if (a.norm_w)
+                o = gd_rms<VD / 4>(o, a.v_dim, a.norm_eps);
             if (e0 >= a.v_dim)
                 continue;
-            gd_f4 o = *(const gd_f4 *)&os[t][e0];
-            if (a.norm_w) {
-                const float ss = (squares[t][0] + squares[t][1]) + (squares[t][2] + squares[t][3]);
-                const float r = 1.0f / sqrtf(ss / (float)a.v_dim + a.norm_eps);
-                o = o * r * *(const gd_f4 *)(a.norm_w + e0);
-            }
+            if (a.norm_w)
+                o = o * *(const gd_f4 *)(a.norm_w + e0);
             if (a.gate) {
                 const gd_f4 z = *(const gd_f4 *)(a.gate + (first + t) * a.gate_step + (int64_t)h * a.v_dim + e0);
 #pragma unroll

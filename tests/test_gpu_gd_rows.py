@@ -161,3 +161,12 @@ def test_rows_of_zeros_without_an_eps(kind, new):
     c.qkv[-1, :2 * K] = 0
     # (as the definition's limit: 0 / sqrt(0 + 1e-300), which changes no other row in 64 bits)
     c.check(c.run(l2_eps=0.0), c.plain(l2_eps=1e-300))
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("size,eps", [(1e24, 1e-6), (1e33, 1e-6), (1e33, 0.0), (1e-24, 0.0), (1e-33, 1e-38)])
+@pytest.mark.parametrize("new,dv", [([6], 64), ([6], 112), ([100], 64), ([100, 3], 112)])
+def test_norms_of_rows_of_any_size(kind, size, eps, new, dv):
+    """Squares of the outputs pass fp32's range, at either end; the norm is the definition's."""
+    c = Case(23, new, [False] * len(new), dk=64, dv=dv, kind=TYPES[kind], out=F32, size=size)
+    c.check(c.run(norm_eps=eps), c.plain(eps=eps))
