@@ -41,6 +41,8 @@ def bounds(c):
     alpha, beta = torch.exp(g), torch.sigmoid(c.b.double())
     rows, last = torch.zeros(v.shape, dtype=torch.float64), {}
     for n, begin, slot, at in zip(c.new, c.begins, c.slots, c.starts):
+        if n == 0:
+            continue
         env = torch.zeros(H, v.shape[2], dtype=torch.float64) if begin else c.state[slot].double().norm(dim=1)
         D, most = torch.zeros_like(env), env
         for t in range(at, at + n):
@@ -71,6 +73,7 @@ def check(c, **kw):
         tol = tol * by.abs().amax(-1)
     # the norm's, the gate's and the type's own roundings
     tol = tol + (16 * 2.0 ** -24 + (0 if out.dtype == F32 else gd_plain.HALF_STEP[out.dtype])) * want.norm(dim=-1)
+    tol = tol + gd_plain.LEAST[out.dtype] * want.shape[-1] ** 0.5  # (half a step of subnormal outputs)
     off = (out.double() - want).norm(dim=-1)
     worst = (off / tol.clamp(min=1e-300))[live]
     assert bool((off <= tol)[live].all()), (float(worst.max()), (worst == worst.max()).nonzero()[0].tolist())
