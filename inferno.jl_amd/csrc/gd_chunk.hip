@@ -48,11 +48,12 @@ __device__ __forceinline__ void gd_power(float x, float &to, float &back)
 // x * by as one fp16 part, and the rest of it, times 2^11, as the next: where the first is one of
 // fp16's subnormal values, the rest still has bits below it.
 constexpr float REST = 2048.0f;
-__device__ __forceinline__ void gd_split(gd_f8 x, float by, gd_h8 &hi, gd_h8 &lo)
+template <typename F, typename H>
+__device__ __forceinline__ void gd_split(F x, float by, H &hi, H &lo)
 {
     x = x * by;
-    hi = __builtin_convertvector(x, gd_h8);
-    lo = __builtin_convertvector((x - __builtin_convertvector(hi, gd_f8)) * REST, gd_h8);
+    hi = __builtin_convertvector(x, H);
+    lo = __builtin_convertvector((x - __builtin_convertvector(hi, F)) * REST, H);
 }
 
 // x as three bf16 parts, each the nearest of what the ones before leave.  (In pairs, as the
@@ -463,12 +464,12 @@ __global__ void __launch_bounds__(PREP_THREADS) k_delta_prep(DeltaArgs a)
 // ---- down the chunks ---------------------------------------------------------------
 constexpr int SCAN_WAVES = 4;
 
-// What a wave reads of a chunk: its 16 rows of K, Q and P, its 32 rows of M, the factors
+// What a wave reads of a chunk: its 16 rows of K, Q and P, its 16 MT rows of M, the factors
 // of its 16 tokens and their values in its columns.
-template <int KS, int PARTS>
+template <int KS, int MT, int PARTS>
 struct ScanOps {
     gd_h8 k[KS][PARTS], q[KS][PARTS];
-    gd_f4 m[2][2][2], p[2][2]; // in fp32
+    gd_f4 m[MT][2][2], p[2][2]; // in fp32
     gd_f4 fk, fq, fs;
     uint32_t v[4]; // as they lie in memory
     float keep;
@@ -482,15 +483,16 @@ __device__ __forceinline__ void scan_sync()
 }
 
 // A workgroup takes 16 columns of one head of one sequence, each of its waves the
-// tokens 16 w .. 16 w + 15 of a chunk and the rows 32 w .. 32 w + 31 of S (there are
-// KD / 32 such waves).  A wave so reads only its own part of the operands, from memory
+// tokens 16 w .. 16 w + 15 of a chunk and KD / 4 rows of S.  A wave so reads only its own part of the operands, from memory
 // into registers, two chunks ahead, and the waves exchange S and X as fragments in LDS,
 // with two barriers a chunk.  Bound by that chain, as a chunk follows the other, and by the
 // operands' way: 8192 tokens of 32 heads of 128 x 128 take 286 us, 2.2 a chunk of 76 KB on every CU
 // (35 KB a microsecond).  (In a form with half the products, which took as long, products, exchanges and
 // barriers alone were 1.2 a chunk, and the operands added 0.6 from L2 and 0.4 from further away; one
 // chunk ahead was 322, three 274; 32 columns a workgroup, which halves the bytes and the CUs in
-// use, 385.  M and P in parts as they are stored, half as many bytes again: 354.)
+// use, 385.  M and P in parts as they are stored, half as many bytes again: 354.)  Heads up to 64 wide
+// have half the rows of S a wave, and registers for two workgroups a CU: 24 heads of 3 sequences of
+// 22 to 135 tokens and 2 shorter ones 9.9 us (two waves with 32 rows each: 16.3).
 //
 // A column of S has a power of two for every chunk, from a bound that no token passes: k and q
 // have unit length at most, a token adds no more than beta |v| to a column's length, and
@@ -501,10 +503,10 @@ template <int TYPE, int KD>
 __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
 {
     constexpr int PARTS = TYPE == kF32 ? 2 : 1;
-    constexpr int KS = KD / 32;
+    constexpr int KS = KD / 32, MT = KD / 64; // steps of a row of K; 16-row tiles of S that a wave has
     constexpr int FRAG = 4 * KS * PARTS * 1024;
     constexpr int VB = PARTS > 1 ? 4 : 2; // bytes of a value of V
-    using Ops = ScanOps<KS, PARTS>;
+    using Ops = ScanOps<KS, MT, PARTS>;
     __shared__ __attribute__((aligned(16))) uint8_t sf[KS][2][1024], xf[2][3][1024];
     __shared__ float bounds[SCAN_WAVES][16];
     __shared__ __attribute__((aligned(16))) float turn[SCAN_WAVES][16][20];
@@ -525,7 +527,6 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
     const int col0 = j % blocks * 16;
     float *const state = a.state + seq.slot * a.slot_step + (int64_t)h * a.k_dim * a.v_dim + col0 + r;
     const int chunks = (seq.n + 63) / 64, tile0 = (seq.start >> kDeltaShift) + s;
-    const bool owner = wave < KS;
     int64_t vat[4]; // of this lane's values of V in a whole chunk
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -577,33 +578,33 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
         if (wave >= 2)
             load_tile(o.p[1], c, p0 + 1);
     };
-    auto load_m = [&](Ops &o, int c, int m, int k) { load_tile(o.m[m][k], c, 6 + 2 * (2 * wave + m) + k); };
+    auto load_m = [&](Ops &o, int c, int m, int k) { load_tile(o.m[m][k], c, 6 + 2 * (MT * wave + m) + k); };
     auto load_all = [&](Ops &o, int c) {
 #pragma unroll
         for (int k = 0; k < KS; ++k)
             load_key(o, c, k);
         load_rows(o, c);
         load_p(o, c);
-        if (owner)
 #pragma unroll
-            for (int m = 0; m < 2; ++m)
+        for (int m = 0; m < MT; ++m)
 #pragma unroll
-                for (int k = 0; k < 2; ++k)
-                    load_m(o, c, m, k);
+            for (int k = 0; k < 2; ++k)
+                load_m(o, c, m, k);
     };
     auto wide = [](const gd_f4 (&half)[2]) { return __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7); };
     auto most4 = [](gd_f4 x) { return fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))); };
 
-    gd_f4 S[2];
+    gd_f4 S[MT];
     float to_s, back_s;
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int at = 32 * wave + 16 * m + 4 * g + i;
-            S[m][i] = owner && !seq.begins && at < a.k_dim ? state[(int64_t)at * a.v_dim] : 0.0f;
+            const int at = 16 * (MT * wave + m) + 4 * g + i;
+            S[m][i] = !seq.begins && at < a.k_dim ? state[(int64_t)at * a.v_dim] : 0.0f;
         }
-    const float most = gd_max32(gd_max16(fmaxf(most4(S[0]), most4(S[1]))));
+    auto most_s = [&]() { return MT > 1 ? fmaxf(most4(S[0]), most4(S[MT - 1])) : most4(S[0]); };
+    const float most = gd_max32(gd_max16(most_s()));
     if (g == 0)
         bounds[wave][r] = most;
     scan_sync();
@@ -612,14 +613,21 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
     };
     gd_power(widest(), to_s, back_s);
     scan_sync();
-    auto put_s = [&]() { // S as a fragment
-        gd_h8 hi, lo;
-        gd_split(__builtin_shufflevector(S[0], S[1], 0, 1, 2, 3, 4, 5, 6, 7), to_s, hi, lo);
-        *(gd_h8 *)(sf[wave][0] + lane * 16) = hi;
-        *(gd_h8 *)(sf[wave][1] + lane * 16) = lo;
+    // S as a fragment, or half of one
+    auto put_s = [&]() {
+        if constexpr (MT > 1) {
+            gd_h8 hi, lo;
+            gd_split(wide(S), to_s, hi, lo);
+            *(gd_h8 *)(sf[wave][0] + lane * 16) = hi;
+            *(gd_h8 *)(sf[wave][1] + lane * 16) = lo;
+        } else {
+            gd_h4 hi, lo;
+            gd_split(S[0], to_s, hi, lo);
+            *(gd_h4 *)(sf[wave / 2][0] + lane * 16 + 8 * (wave & 1)) = hi;
+            *(gd_h4 *)(sf[wave / 2][1] + lane * 16 + 8 * (wave & 1)) = lo;
+        }
     };
-    if (owner)
-        put_s();
+    put_s();
 
     auto chunk = [&](Ops &o, int c) {
         const int n = min(64, seq.n - 64 * c);
@@ -629,7 +637,7 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
             const float x = TYPE == kF32 ? __uint_as_float(o.v[i]) : TYPE == kF16 ? h2f(o.v[i]) : __uint_as_float(o.v[i] << 16);
             v[i] = 16 * wave + 4 * g + i < n ? x : 0.0f;
         }
-        const float most = 12.0f * o.keep * fmaxf(most4(S[0]), most4(S[1])) + 66.0f * most4(v * o.fs);
+        const float most = 12.0f * o.keep * most_s() + 66.0f * most4(v * o.fs);
         const float all = gd_max32(gd_max16(most));
         if (g == 0)
             bounds[wave][r] = all;
@@ -669,19 +677,19 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
             for (int p = 0; p < 3; ++p)
                 xp[k][p] = *(const gd_b8 *)(xf[k][p] + lane * 16);
         gd_power(next, to_s, back_s);
-        if (owner) {
-            gd_f4 x[2]{}, y[2]{};
+        {
+            gd_f4 x[MT]{}, y[MT]{};
 #pragma unroll
             for (int k = 0; k < 2; ++k)
 #pragma unroll
-                for (int m = 0; m < 2; ++m) {
+                for (int m = 0; m < MT; ++m) {
                     gd_b8 part[3];
                     gd_split3(wide(o.m[m][k]), part);
                     gd_dot(part, xp[k], x[m], y[m]);
                     load_m(o, c + 2, m, k);
                 }
 #pragma unroll
-            for (int m = 0; m < 2; ++m)
+            for (int m = 0; m < MT; ++m)
                 S[m] = S[m] * keep + (x[m] + y[m]);
             put_s();
         }
@@ -717,15 +725,14 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
     }
     if (c < chunks)
         chunk(even, c);
-    if (owner)
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int at = 32 * wave + 16 * m + 4 * g + i;
-                if (at < a.k_dim)
-                    state[(int64_t)at * a.v_dim] = S[m][i];
-            }
+        for (int i = 0; i < 4; ++i) {
+            const int at = 16 * (MT * wave + m) + 4 * g + i;
+            if (at < a.k_dim)
+                state[(int64_t)at * a.v_dim] = S[m][i];
+        }
 }
 
 // ---- the output norm ---------------------------------------------------------------
