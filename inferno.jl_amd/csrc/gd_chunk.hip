@@ -717,7 +717,9 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
         load_p(o, c + 2);
     };
     Ops even, odd;
-    load_all(even, 0), load_all(odd, 1);
+    load_all(even, 0);
+    if (chunks > 1)
+        load_all(odd, 1);
     int c = 0;
     for (; c + 1 < chunks; c += 2) { // (no way out between: the operands stay in their registers)
         chunk(even, c);
