@@ -551,7 +551,10 @@ int ihip_kv_copy_dev(const ihip_kv_cache *cache, int layers, int64_t layer_strid
  * written.  Rows before the first sequence's and behind the last one's are not
  * written either.  Flags as for the paged cache.
  * most: the most new tokens that a sequence has, or 0 where that is not known.
- * It only helps to choose kernels: results are right with any value. */
+ * It only helps to choose kernels: results are right with any value.  Where it is
+ * not given, the rows might all be one sequence's, and the gated delta rule lays out
+ * and launches for that too (61 single tokens, 32 heads of 128 x 128: 55 us with
+ * most 1, 109 with 0). */
 typedef struct ihip_state_batch {
     const int32_t *q_starts; /* sequences + 1 */
     const int32_t *kv_lens;  /* sequences, or NULL */
@@ -574,8 +577,9 @@ int ihip_short_conv_dev(const void *x, int x_type, int64_t x_stride, const float
                         const ihip_state_batch *batch, uint32_t *flags, ihip_stream stream);
 
 /* A layer of the gated delta rule: k_heads heads of q and k, v_heads (a multiple
- * of them) of v, head h reading q and k head h / (v_heads / k_heads); k_dim and
- * v_dim multiples of 16, at most 128.  state: `slots` slots of v_heads x k_dim x
+ * of them) of v, head h reading q and k head h / (v_heads / k_heads) (heads of v in
+ * another order, as h mod k_heads, are put into this one at load, with their rows of
+ * state, decay, dt_bias, a, b and gate); k_dim and v_dim multiples of 16, at most 128.  state: `slots` slots of v_heads x k_dim x
  * v_dim floats, slot_stride floats apart (a multiple of 4).  decay (v_heads floats,
  * at most 0, as a GGUF file's ssm_a; a higher one counts as 0), dt_bias (v_heads),
  * norm_w (v_dim, or NULL: no norm). */
@@ -597,7 +601,9 @@ typedef struct ihip_delta_layer {
  * convolution's output is passed as three offsets into it; a, b: rows of v_heads
  * floats; gate: rows of v_heads * v_dim floats (stride a multiple of 4) or NULL; out:
  * tokens x v_heads x v_dim of out_type, which is F32 or the type of q, k and v.
- * States and F32 outputs carry fp32's accuracy; F16 and BF16 outputs are rounded once.
+ * States and F32 outputs carry fp32's accuracy, every token by itself, whatever the sizes
+ * of the ones beside it (fp32 q and k, and the states that they are multiplied with, count
+ * with 22 bits in sequences of many tokens); F16 and BF16 outputs are rounded once.
  * A value that is not finite may reach every output of its head from 64 tokens before
  * it on.  Buffers are 16-byte aligned (a and b 4), out overlaps no input.
  * workspace: ihip_gated_delta_scratch_bytes bytes, 16-byte aligned, NULL where that
@@ -630,8 +636,10 @@ size_t ihip_gated_delta_scratch_bytes(int type, const ihip_delta_layer *layer,
  * and logprobs[r] the logarithm of its share of that sum.  T = 0 (or below) is the
  * greedy choice: the lowest index of the largest logit, with logprob 0.  temperature,
  * top_k, top_p, min_p (one value a row) may be NULL: 1, and no filter; logprobs and
- * flags may be NULL.  Weights and sums are formed in 64 bits.  A logit of -infinity
- * is never chosen.  flags[r] = IHIP_FLAG_NAN / IHIP_FLAG_POSINF where the row holds
+ * flags may be NULL.  Weights are formed and summed in 64 bits; where the prefix that
+ * top-k or top-p keeps ends, as whole numbers of 2^-46 of the largest weight (2^-44 for
+ * 151936 logits), whose sums do not depend on an order.  A logit of -infinity is
+ * never chosen.  flags[r] = IHIP_FLAG_NAN / IHIP_FLAG_POSINF where the row holds
  * such a value (the token is then 0 and the logprob NaN), IHIP_FLAG_ALL_NEGINF where
  * every logit is -infinity (the token is 0), else 0.  Everything is device memory.
  * workspace: ihip_sample_scratch_bytes bytes, 16-byte aligned; its contents do not

@@ -483,16 +483,16 @@ __device__ __forceinline__ void scan_sync()
 }
 
 // A workgroup takes 16 columns of one head of one sequence, each of its waves the
-// tokens 16 w .. 16 w + 15 of a chunk and KD / 4 rows of S.  A wave so reads only its own part of the operands, from memory
-// into registers, two chunks ahead, and the waves exchange S and X as fragments in LDS,
-// with two barriers a chunk.  Bound by that chain, as a chunk follows the other, and by the
+// tokens 16 w .. 16 w + 15 of a chunk and KD / 4 rows of S.  A wave so reads only its own
+// part of the operands, from memory into registers, two chunks ahead, and the waves exchange
+// S and X as fragments in LDS, with two barriers a chunk.  Bound by that chain, as a chunk follows the other, and by the
 // operands' way: 8192 tokens of 32 heads of 128 x 128 take 286 us, 2.2 a chunk of 76 KB on every CU
 // (35 KB a microsecond).  (In a form with half the products, which took as long, products, exchanges and
 // barriers alone were 1.2 a chunk, and the operands added 0.6 from L2 and 0.4 from further away; one
 // chunk ahead was 322, three 274; 32 columns a workgroup, which halves the bytes and the CUs in
-// use, 385.  M and P in parts as they are stored, half as many bytes again: 354.)  Heads up to 64 wide
-// have half the rows of S a wave, and registers for two workgroups a CU: 24 heads of 3 sequences of
-// 22 to 135 tokens and 2 shorter ones 9.9 us (two waves with 32 rows each: 16.3).
+// use, 385.)  Heads up to 64 wide have half the rows of S a wave, and registers for two workgroups a
+// CU: 24 heads of 3 sequences of 22 to 135 tokens and 2 shorter ones 9.9 us (two waves with 32 rows
+// each: 16.3).
 //
 // A column of S has a power of two for every chunk, from a bound that no token passes: k and q
 // have unit length at most, a token adds no more than beta |v| to a column's length, and

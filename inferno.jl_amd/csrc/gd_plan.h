@@ -21,10 +21,9 @@ constexpr int64_t gd_tiles(int64_t tokens, int64_t sequences, int shift)
 // New tokens up to which a batch goes a token at a time, all of it.  A token costs the step
 // kernel 1.4 us whatever the batch, until that fills the chip; a chunk costs its
 // kernels the same with few tokens as with 64, and every chunk of the batch adds to it.
-// Measured on sequences of equally many tokens, 32 heads of 128 x 128 in bf16, the two are even
-// at 11 tokens for one sequence (12: 24.7 us by steps, 23.1 by chunks; 8: 18.3, 22.4), 17 for
-// two (16: 28.9, 30.6; 20: 34.9, 31.6), 28 for four (24: 39.5, 44.3; 32: 49.6, 45.4) and 41
-// for eight (32: 54.8, 69.3; 48: 79.7, 71.8).
+// Measured on sequences of equally many tokens, 32 heads of 128 x 128 in bf16 with norm and gate, us by
+// steps | chunks: one of 8 18.3 | 23.4, of 12 24.5 | 24.6; two of 16 28.8 | 32.4, of 20 35.1 | 33.4; four of 24
+// 44.8 | 43.7, of 32 58.8 | 44.8 (the rule is late there); eight of 32 60.9 | 68.0, of 48 85.6 | 72.1.
 constexpr int delta_few(int v_heads, int64_t sequences)
 {
     const int64_t few = sequences * v_heads / 4;
@@ -34,7 +33,7 @@ constexpr int delta_few(int v_heads, int64_t sequences)
 // Beside longer sequences, the step kernel comes before the chunks' and lasts as long as
 // its longest sequence, and chunks that do not fill the chip are next to free: there
 // only a few tokens go by steps (sequences of 22, 8, 135, 5 and 72 tokens, 24 heads of
-// 64 x 64: 30.0 us with up to 4, 36.0 with up to 10, 47 with up to 30).
+// 64 x 64: 27.1 us with up to 4, 35.8 with up to 10, 49.5 with up to 30).
 constexpr int delta_few_beside(int v_heads, int64_t sequences)
 {
     return sequences * v_heads < 256 ? 4 : 10;

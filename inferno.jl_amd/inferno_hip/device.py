@@ -649,7 +649,8 @@ class StateBatch:
     device tensors q_starts (sequences + 1), slots (sequences) and, where some begin
     with the call, kv_lens (sequences: all their tokens), and the rows of the call.
     Their contents may change between calls, also under a captured graph.  most: the
-    most new tokens of a sequence (a help in the choice of kernels; 0: not known)."""
+    most new tokens of a sequence, 1 in a decode step (a help in the choice of kernels; 0:
+    not known, and then a decode step is launched as the prompt that it might be)."""
 
     def __init__(self, q_starts: torch.Tensor, slots: torch.Tensor, tokens: int, kv_lens=None, most: int = 0):
         n, self.index = slots.numel(), slots.get_device()
@@ -753,8 +754,9 @@ class DeltaLayer:
 
 
 def delta_workspace(layer: DeltaLayer, batch: StateBatch, dtype):
-    """The workspace of gated_delta for a batch of these sizes with q, k and v of
-    `dtype`, or None where it needs none.  Calls that share one must not overlap."""
+    """The workspace of gated_delta for a batch of these sizes, or of smaller ones, with
+    q, k and v of `dtype`, or None where it needs none.  Calls that share one must not
+    overlap."""
     n = lib().ihip_gated_delta_scratch_bytes(_ACT_TYPES.get(dtype, -1), layer.ref, batch.ref)
     return torch.empty(n, dtype=torch.uint8, device=layer.device) if n else None
 
@@ -798,8 +800,8 @@ def _fresh_bytes(stream, n, device):
 
 # ---- the choice of a token --------------------------------------------------------
 def sample_workspace(rows: int, vocab: int, device="cuda"):
-    """The workspace of sample for rows x vocab logits.  Calls that share one must not
-    overlap."""
+    """The workspace of sample for rows x vocab logits, or fewer.  Calls that share one
+    must not overlap."""
     n = lib().ihip_sample_scratch_bytes(rows, vocab)
     if not n:
         raise _invalid(f"{rows} rows of {vocab} logits")

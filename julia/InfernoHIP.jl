@@ -940,7 +940,7 @@ end
 The sequences of a call on layers that keep a state (`ihip_state_batch`): device
 arrays of Int32 -- `q_starts` (sequences + 1 row offsets from 0), `kv_lens` (all
 tokens of each, or C_NULL: every sequence goes on) and `slots` (from 0) -- the
-rows, and the most new tokens of a sequence (0: not known).
+rows, and the most new tokens of a sequence (1 in a decode step; 0: not known).
 """
 struct StateBatch
     q_starts::Ptr{Int32}
@@ -993,7 +993,7 @@ function short_conv!(out::Ptr{Cvoid}, out_type::Integer, x::Ptr{Cvoid}, x_type::
     return out
 end
 
-"""Workspace of `gated_delta!` for a batch of these sizes."""
+"""Workspace of `gated_delta!` for a batch of these sizes, or of smaller ones."""
 gated_delta_scratch_bytes(type::Integer, layer::DeltaLayer, batch::StateBatch) =
     Int(ccall((:ihip_gated_delta_scratch_bytes, LIBIHIP), Csize_t,
               (Cint, Ref{DeltaLayer}, Ref{StateBatch}), type, Ref(layer), Ref(batch)))
@@ -1023,7 +1023,7 @@ function gated_delta!(out::Ptr{Cvoid}, out_type::Integer, q::Ptr{Cvoid}, q_strid
     return out
 end
 
-"""Workspace of `sample!` for so many rows of so many logits."""
+"""Workspace of `sample!` for so many rows of so many logits, or fewer."""
 sample_scratch_bytes(rows::Integer, vocab::Integer) =
     Int(ccall((:ihip_sample_scratch_bytes, LIBIHIP), Csize_t, (Cint, Cint), rows, vocab))
 
