@@ -36,13 +36,14 @@ typedef float gd_f8 __attribute__((ext_vector_type(8)));
 
 constexpr int TOP = 13; // fp16 operands' largest values have this binary exponent
 
-// 2^(TOP - exponent of x), and its inverse; x >= 0.  (Below 2^-113 of nothing; an
-// infinity or NaN is left one.)
+// 2^(TOP - exponent of x), and what a product of such a value with a row of K or Q takes back
+// of it, and of the row's own 2^TOP, before anything else, so that it does not pass the range;
+// x >= 0.  (Below 2^-100 of nothing; an infinity or NaN is left one.)
 __device__ __forceinline__ void gd_power(float x, float &to, float &back)
 {
-    const int e = max((int)(__float_as_uint(x) >> 23), 127 - 113);
+    const int e = max((int)(__float_as_uint(x) >> 23), 127 - 100);
     to = __uint_as_float((uint32_t)(254 + TOP - e) << 23);
-    back = __uint_as_float((uint32_t)(e - TOP) << 23);
+    back = __uint_as_float((uint32_t)(e - 2 * TOP) << 23);
 }
 
 // x * by as one fp16 part, and the rest of it, times 2^11, as the next: where the first is one of
@@ -118,6 +119,7 @@ __device__ __forceinline__ void gd_dot(const gd_b8 (&a)[3], const gd_b8 (&b)[N],
 
 // ---- chunks' operands ------------------------------------------------------------
 constexpr int PREP_THREADS = 256;
+constexpr float LEAST = 0x1p-90f; // of a chunk's fades in the bound on the next S
 constexpr int TRI = 68; // floats from a row of a 64 x 64 matrix to the next, in LDS
 
 // A workgroup takes a chunk of a head of v; a wave 16 of its rows.  k's and q's products
@@ -450,15 +452,16 @@ __global__ void __launch_bounds__(PREP_THREADS) k_delta_prep(DeltaArgs a)
         store(6 + 2 * md, out[0], out[1]);
         store(6 + 2 * md + 1, out[2], out[3]);
     }
+    constexpr float UP = 1 << TOP; // (the rows' own, which the scan takes back first)
     float *const f = (float *)(a.work + a.plan.rows) + unit * kDeltaRows;
     if (wave == 0) {
-        f[lane] = rk[lane] * gd_exp2(G[lane]); // of K S
-        f[128 + lane] = beta[lane] * gd_exp2(G[63] - G[lane]); // of what a token adds to S
+        f[lane] = rk[lane] * UP * gd_exp2(G[lane]); // of K S
+        f[128 + lane] = fmaxf(beta[lane] * gd_exp2(G[63] - G[lane]), LEAST); // of what a token adds to S
         if (lane == 0)
             f[192] = gd_exp2(G[63]);
     }
     if (g == 0)
-        f[64 + row] = rq * gd_exp2(G[row]); // of Q S
+        f[64 + row] = rq * UP * gd_exp2(G[row]); // of Q S
 }
 
 // ---- down the chunks ---------------------------------------------------------------
@@ -498,7 +501,9 @@ __device__ __forceinline__ void scan_sync()
 // have unit length at most, a token adds no more than beta |v| to a column's length, and
 // all of it fades, so that S after a chunk lies below 12 e^G_64 max |S| + 66 max(e^(G_64 - G) beta
 // |v|) (sqrt(128) < 12).  Values down to 2^-27 of that keep 22 bits, and smaller ones
-// 2^-49 of it.
+// 2^-49 of it.  No fade counts as less than 2^-90 in it, so X is below 2^90 of it: where it is
+// under 2^-60, X is lifted by 2^24, as the third parts of values under 2^-109 would have no
+// room in bf16's exponents.
 template <int TYPE, int KD>
 __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
 {
@@ -637,7 +642,7 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
             const float x = TYPE == kF32 ? __uint_as_float(o.v[i]) : TYPE == kF16 ? h2f(o.v[i]) : __uint_as_float(o.v[i] << 16);
             v[i] = 16 * wave + 4 * g + i < n ? x : 0.0f;
         }
-        const float most = 12.0f * o.keep * most_s() + 66.0f * most4(v * o.fs);
+        const float most = 12.0f * fmaxf(o.keep, LEAST) * most_s() + 66.0f * most4(v * o.fs);
         const float all = gd_max32(gd_max16(most));
         if (g == 0)
             bounds[wave][r] = all;
@@ -645,6 +650,7 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
         // K S and Q S; X = V - e^G K S
         gd_f4 qs;
         const float next = widest(), keep = o.keep;
+        const float lift = next < 0x1p-60f ? 0x1p24f : 1.0f, sink = next < 0x1p-60f ? 0x1p-24f : 1.0f;
         {
             gd_f4 x{}, y{}, z{}, w{};
 #pragma unroll
@@ -661,7 +667,7 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
                 load_key(o, c + 2, k);
             }
             gd_b4 part[3]; // half a fragment
-            gd_split3(v - o.fk * ((x + y * (1.0f / REST)) * back_s), part);
+            gd_split3(v * lift - o.fk * ((x + y * (1.0f / REST)) * (back_s * lift)), part);
 #pragma unroll
             for (int p = 0; p < 3; ++p)
                 *(gd_b4 *)(xf[wave / 2][p] + lane * 16 + 8 * (wave & 1)) = part[p];
@@ -690,7 +696,7 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
                 }
 #pragma unroll
             for (int m = 0; m < MT; ++m)
-                S[m] = S[m] * keep + (x[m] + y[m]);
+                S[m] = S[m] * keep + (x[m] + y[m]) * sink;
             put_s();
         }
         gd_f4 x{}, y{};
@@ -701,7 +707,7 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES) k_delta_scan(DeltaArgs a)
                 gd_split3(wide(o.p[k]), part);
                 gd_dot(part, xp[k], x, y);
             }
-        const gd_f4 out = a.scale * (qs + (x + y));
+        const gd_f4 out = a.scale * qs + (a.scale * sink) * (x + y);
         // through LDS, so that a lane stores 4 neighbours
 #pragma unroll
         for (int i = 0; i < 4; ++i)

@@ -173,3 +173,13 @@ def test_norms_of_rows_of_any_size(kind, size, eps, new, dv):
     """Squares of the outputs pass fp32's range, at either end; the norm is the definition's."""
     c = Case(23, new, [False] * len(new), dk=64, dv=dv, kind=TYPES[kind], out=F32, size=size)
     c.check(c.run(norm_eps=eps), c.plain(eps=eps))
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("norm", [False, True])
+@pytest.mark.parametrize("size", [1e35, 1e-35])
+@pytest.mark.parametrize("new", [[6], [150]])
+def test_values_near_the_ends_of_the_range(kind, norm, size, new):
+    """States and values of 10^35, whose products with keys of any scale do not pass fp32's range on the way, and 10^-35."""
+    c = Case(29, new, [False], dk=128, dv=32, kind=TYPES[kind], out=F32, gate=False, norm=norm, size=size)
+    check(c)
